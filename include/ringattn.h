@@ -294,6 +294,105 @@ int ringattn_ring_attention_noalloc(const void* q, const void* k, const void* v,
 size_t ringattn_noalloc_scratch_bytes(void);
 
 /*
+ * ---- Serving from a paged K/V cache ----------------------------------------------------------
+ * What follows the prefill of a long context: the K and V rows of many sequences lie in a pool of pages, every call
+ * brings some new tokens of each, and attention runs from the new tokens over the cached ones.  No counterpart in the reference, which
+ * has no cache.  A plan (head counts, type, mask; workspace, allocated once) serves any number of calls, one at a time like every plan;
+ * its calls may be recorded into graphs of the caller's, and lengths, starts and page table are read on the device at every replay.
+ *
+ * The calls of one step of a serving loop, in order: ringattn_paged_append, ringattn_paged_fwd, and for a cache that is to
+ * be kept within bounds ringattn_paged_weights, and now and then ringattn_paged_evict.
+ */
+typedef struct ringattn_paged_params {
+  int dim;               /* 64 or 128 */
+  int heads;
+  int kv_heads;          /* 0 or `heads`: one per query head; else a divisor of heads, as in ringattn_params */
+  int dtype;             /* RINGATTN_DTYPE_* of Q, K, V and O */
+  float softmax_scale;   /* logit scale; <= 0 selects 1/sqrt(dim) */
+  int page_size;         /* tokens of a page: 16, 32, 64, ... 1024 */
+  int max_batch;         /* sequences of a call at most: up to 4096 */
+  int max_tokens;        /* new tokens of a call at most, all sequences together */
+  int causal;            /* 1: a new token sees the tokens up to itself; 0: every cached token (a cache that holds another part of the
+                            sequence: see RINGATTN_FLAG_PAGED_PARTIALS) */
+  int window;            /* 0: no limit.  w > 0 (causal only): a token sees the last w tokens up to itself ... */
+  int sinks;             /* ... and, with a window, the first `sinks` tokens of the sequence (up to itself) */
+  int flags;             /* RINGATTN_FLAG_PAGED_PARTIALS */
+} ringattn_paged_params;
+
+#define RINGATTN_FLAG_PAGED_PARTIALS 1 /* O is written as fp32, a partial for ringattn_merge: a sequence whose cache is spread
+                                          over several pools (or GPUs) is attended pool by pool and merged by the LSEs */
+
+typedef struct ringattn_paged_plan ringattn_paged_plan;
+
+/*
+ * The sequences of a call.  k, v: a pool [pages, kv_heads, page_size, dim] in any order of memory that keeps a row of dim together
+ * (strides in elements, multiples of 8; both pools alike).  The int arrays lie on the device.  Token j of sequence b is row
+ * j mod page_size of page page_table[b * table_stride + j / page_size].  An entry outside [0, pages) is a page that is not
+ * there: its tokens are hidden from every query, weigh nothing, and are neither written nor moved (pages that lie behind
+ * a window may be given away).  Lengths are held to what the table has room for, starts to the call's tokens.  Pages may be
+ * shared between sequences for reading; a page that is written belongs to one sequence.
+ */
+typedef struct ringattn_paged_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, token_stride;
+  int pages;
+  int table_pages;          /* entries of the table per sequence */
+  int64_t table_stride;     /* ints from a sequence's entries to the next one's */
+  const int* page_table;    /* [batch, table_pages] */
+  const int* kv_lens;       /* [batch] tokens of the sequence in the cache, the new ones of this call among them, as its last */
+  const int* q_starts;      /* [batch + 1] ascending: the new tokens of sequence b are rows [q_starts[b], q_starts[b + 1]) of q,
+                               k_new and v_new; rows behind the last sequence are left as they were (not read by ringattn_paged_evict) */
+  int batch;
+} ringattn_paged_cache;
+
+/* Bytes of device workspace a plan needs (sums of rows whose keys are shared out to several workgroups); 0 if the parameters are invalid. */
+size_t ringattn_paged_workspace_bytes(const ringattn_paged_params* params);
+/* As ringattn_plan_create and ringattn_plan_destroy. */
+int ringattn_paged_plan_create(const ringattn_paged_params* params, void* workspace, size_t workspace_bytes, ringattn_paged_plan** plan_out);
+int ringattn_paged_plan_destroy(ringattn_paged_plan* plan);
+
+/*
+ * New K and V rows into the cache: row t of k_new and v_new [tokens, kv_heads, dim] (by strides, in elements) becomes the token of
+ * its sequence that kv_lens and q_starts say.  scores (may be NULL): the accumulated weights of ringattn_paged_weights; those of
+ * the new tokens are set to 0.
+ */
+int ringattn_paged_append(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* k_new, const void* v_new, int tokens,
+                          int64_t token_stride, int64_t head_stride, float* scores, void* stream);
+
+/*
+ * Attention of the new tokens over the cache (which holds their own K and V rows already).  New token i of n of a sequence of L tokens
+ * is its token p = L - n + i and sees token j iff 0 <= j <= p (causal; else j < L), and, with a window, j > p - window or
+ * j < sinks.  A query that sees nothing gets O = 0 and LSE = -inf.
+ *   q   : [tokens, heads, dim] by strides (elements, multiples of 8)
+ *   out : the same shape, by strides of its own; fp32 with RINGATTN_FLAG_PAGED_PARTIALS (strides multiples of 4)
+ *   lse : [heads, tokens] fp32, natural log
+ */
+int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
+                       int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* stream);
+
+/*
+ * Attention weight that the cached tokens have drawn: scores[page, kv head, row] += sum over the new tokens and the query heads of
+ * the KV head of exp(scale q k - lse), for what ringattn_paged_fwd with the same cache, q and plan sees; lse as it wrote it (rows
+ * of -inf weigh nothing).  scores: [pages, kv_heads, page_size] fp32.  cache->v is not read and may be NULL.  A page that
+ * several sequences share gets the weights of one of them.
+ */
+int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
+                           int64_t q_head_stride, const float* lse, float* scores, void* stream);
+
+/*
+ * Keeps `budget` tokens of every sequence, for each KV head its own: the first keep_first, the last keep_last, and of those between
+ * them the ones with the largest scores (of equal ones the earliest; a NaN, and a token whose page is not there, counts as -inf).  Their K and V rows and scores are copied, in
+ * their order, to the pages of kept_table ([batch, kept_pages] by rows of kept_stride ints, entries of the same pools; kept_pages *
+ * page_size >= budget), which share no page with page_table.  A sequence of no more than `budget` tokens is copied whole.
+ *   kept      : [batch, kv_heads, budget] the places (in page_table) of the kept tokens, -1 behind the last
+ *   kept_lens : [batch] min(kv_lens, budget): the kv_lens that go with kept_table
+ * To the calls above the kept tokens are the tokens of the sequence: causality and windows count them, not what lay between them.
+ */
+int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, float* scores, const int* kept_table, int kept_pages,
+                         int64_t kept_stride, int budget, int keep_first, int keep_last, int* kept, int* kept_lens, void* stream);
+
+/*
  * Seeded input generator -- the counterpart of fillWithNum / initQKV
  * (csrc/ring_attention.cu:731-748), which fill a host buffer and copy it to the
  * device.  Writes n values of N(0, sigma^2), rounded to nearest-even into `dtype`,

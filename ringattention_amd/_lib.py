@@ -42,6 +42,22 @@ class RingattnWorkItem(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("q_start", "q_len", "kv_start", "kv_len", "diag_off", "slot")]
 
 
+class RingattnPagedParams(ctypes.Structure):
+    """struct ringattn_paged_params."""
+    _fields_ = [("dim", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("softmax_scale", ctypes.c_float)] + [(n, ctypes.c_int) for n in (
+                    "page_size", "max_batch", "max_tokens", "causal", "window", "sinks", "flags")]
+
+
+class RingattnPagedCache(ctypes.Structure):
+    """struct ringattn_paged_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("pages", ctypes.c_int), ("table_pages", ctypes.c_int), ("table_stride", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("batch", ctypes.c_int)]
+
+
+_cache_p = ctypes.POINTER(RingattnPagedCache)
+
 SYMBOLS = {
     "ringattn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RingattnParams)]),
     "ringattn_plan_create": (ctypes.c_int, [ctypes.POINTER(RingattnParams), ctypes.c_void_p, ctypes.c_size_t,
@@ -67,6 +83,18 @@ SYMBOLS = {
                                                                                ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                                                ctypes.c_int, ctypes.c_float, ctypes.c_void_p]),
     "ringattn_noalloc_scratch_bytes": (ctypes.c_size_t, []),
+    "ringattn_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RingattnPagedParams)]),
+    "ringattn_paged_plan_create": (ctypes.c_int, [ctypes.POINTER(RingattnPagedParams), ctypes.c_void_p, ctypes.c_size_t,
+                                                  ctypes.POINTER(ctypes.c_void_p)]),
+    "ringattn_paged_plan_destroy": (ctypes.c_int, [ctypes.c_void_p]),
+    "ringattn_paged_append": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                             ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_paged_fwd": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_paged_weights": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_paged_evict": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_fill_normal": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64,
                                             ctypes.c_int64, ctypes.c_double]),
     "ringattn_fill_reference_pattern": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int]),

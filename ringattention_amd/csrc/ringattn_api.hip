@@ -964,6 +964,8 @@ int launch_regions(const ringattn_plan* pl, int first, int count, int max_len, i
 
 }  // namespace
 
+int ringattn::hip_failed(hipError_t e) { return hip_fail(e); }
+
 extern "C" {
 
 size_t ringattn_workspace_bytes(const ringattn_params* params) {

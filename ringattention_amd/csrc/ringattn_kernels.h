@@ -172,4 +172,7 @@ hipError_t launch_split_columns(const BlockArgs& a, unsigned grid, int dtype, in
 hipError_t launch_pair(BlockArgs a, int dtype, int dim, hipStream_t stream);
 hipError_t launch_merge(const MergeArgs& a, int dtype, int dim, hipStream_t stream);
 
+// RINGATTN_ERR_HIP, the error kept for ringattn_last_hip_error
+int hip_failed(hipError_t e);
+
 }  // namespace ringattn

@@ -1,0 +1,231 @@
+// Serving from a paged K/V cache: launch arguments, and what the kernels share -- which sequence a workgroup has, which rows and keys
+// of it, and where those lie.
+//
+// A call has a ragged batch: sequence b has `L` tokens in the cache, the last `n` of them new, and its queries are n x group rows
+// for each KV head (row r: new token r / group, query head r mod group of the KV head's group), so that a K/V tile is read once
+// for all heads of a group.  Lengths, starts and page table lie on the device and may change between two replays of a captured launch:
+// the host knows only how many sequences and new tokens there can be, lays a grid that suffices for any lengths, and every
+// workgroup finds its place from the lengths themselves (find_place).
+#pragma once
+#include "ringattn_device.h"
+
+namespace ringattn {
+namespace paged {
+
+constexpr int kKeyTile = 32;      // keys of a tile
+constexpr int kFewRows = 32;      // query rows of a workgroup of paged_split_kernel
+constexpr int kMaxBatch = 4096;   // sequences of a call
+
+struct Cache {
+  char* k;              // [pages, kv_heads, page, D] by strides
+  char* v;
+  int64_t page_stride, head_stride;  // bytes
+  int token_stride;                  // bytes
+  int pages;            // of the pool: an entry of the table outside [0, pages) is a page that is not there
+  const int* table;     // [batch, table_pages]
+  int64_t table_stride;
+  int table_pages, page_shift;
+  const int* lens;      // [batch] tokens in the cache, the new ones among them
+  const int* starts;    // [batch + 1] first new token of a sequence among all new ones
+  int batch, tokens;    // sequences; new tokens at most (rows of q)
+};
+
+struct AttendArgs {
+  Cache c;
+  const char* q;
+  char* out;
+  float* lse;             // [heads, tokens]
+  float* part_o;          // [slots, rows of a tile, D]
+  float2* part_s;         // [slots, rows of a tile]: reference (log2 units), sum
+  int64_t q_ts, q_hs, o_ts, o_hs;  // bytes between tokens, between heads
+  int kv_heads, group;
+  Divisor by_group, by_kv_heads;
+  float scale_log2;
+  int causal, window, sinks;
+  int out_fp32;
+  int rows_above, rows_upto;  // a launch has the sequences with rows_above < rows <= rows_upto
+  float workgroups;           // the key tiles of a launch are shared out to about so many workgroups
+  int least_tiles;            // ... of so many key tiles at least
+};
+
+struct Seq {
+  int len, start, n;
+};
+static __device__ __forceinline__ int clamped(int x, int lo, int hi) { return min(max(x, lo), hi); }
+// Lengths are data: whatever they hold, nothing outside the tensors is touched.
+static __device__ __forceinline__ Seq seq_of(const Cache& c, int b) {
+  Seq s;
+  s.len = clamped(c.lens[b], 0, c.table_pages << c.page_shift);
+  s.start = clamped(c.starts[b], 0, c.tokens);
+  s.n = clamped(c.starts[b + 1], s.start, c.tokens) - s.start;
+  return s;
+}
+
+// The key tiles that rows of the new tokens [i0, i1] of a sequence see: `sink_tiles` first ones and those from `sink_tiles + skip` on, `count`
+// in all.  Tile u of them is tile u or u + skip of the sequence.
+struct Keys {
+  int sink_tiles, skip, count;
+};
+static __device__ __forceinline__ Keys keys_of(const Seq& s, int i0, int i1, int causal, int window, int sinks) {
+  const int before = s.len - s.n;  // tokens that were there (negative: queries that see nothing)
+  const int end = causal ? min(s.len, before + i1 + 1) : s.len;
+  Keys k{0, 0, 0};
+  if (end <= 0) return k;
+  const int tiles = (end + kKeyTile - 1) / kKeyTile;
+  if (window > 0) {
+    const int low = max(0, before + i0 + 1 - window);
+    k.sink_tiles = (min(sinks, end) + kKeyTile - 1) / kKeyTile;
+    k.skip = max(0, min(low / kKeyTile, tiles) - k.sink_tiles);
+  }
+  k.count = tiles - k.skip;
+  return k;
+}
+
+// What a sequence brings to a launch: row tiles, and the most key tiles that one of them sees.
+template <int ROWS> static __device__ __forceinline__ void load_of(const AttendArgs& a, const Seq& s, int& tiles, int& keys) {
+  const int rows = s.n * a.group;
+  tiles = rows > a.rows_above && rows <= a.rows_upto ? (rows + ROWS - 1) / ROWS : 0;
+  keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks).count;
+  if (a.window > 0) {  // a row tile sees no more than its own window, wherever that begins, and the first tokens
+    const int most = (a.window + ROWS - 1 + kKeyTile - 1) / kKeyTile + 1 + (a.sinks + kKeyTile - 1) / kKeyTile;
+    keys = min(keys, most);
+  }
+}
+
+// The shares that a launch cuts the key tiles of a row tile into: so many that the whole launch makes about a.workgroups
+// workgroups, each of a.least_tiles tiles at least.
+static __device__ __forceinline__ int splits_of(const AttendArgs& a, int keys, float share) {
+  return max(1, (int)ceilf(keys / fmaxf(share, (float)a.least_tiles)));
+}
+
+template <class T> static __device__ __forceinline__ T wave_sum(T x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+static __device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+struct Place {
+  Seq s;
+  int b;
+  int tile, split, splits;  // row tile, which share of its key tiles of how many
+  int slot;                 // where the partial of the row tile's first share lies (splits > 1)
+};
+// The place-th unit of work of a KV head.  MERGE: units are row tiles whose keys were shared out; else the shares themselves.  Every
+// wave works it out for itself, a lane a sequence, so that there is no barrier.  False beyond the last.
+template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
+  const int lane = threadIdx.x & 63;
+  float total = 0.f;
+  for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
+    float work = 0.f;
+    if (b0 + lane < a.c.batch) {
+      int tiles, keys;
+      load_of<ROWS>(a, seq_of(a.c, b0 + lane), tiles, keys);
+      work = (float)tiles * (float)keys;
+    }
+    total += wave_sum(work);
+  }
+  const float share = total * a.kv_heads / a.workgroups;
+  int before = 0, slots_before = 0;
+  for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
+    Seq s{0, 0, 0};
+    int tiles = 0, splits = 1;
+    if (b0 + lane < a.c.batch) {
+      int keys;
+      s = seq_of(a.c, b0 + lane);
+      load_of<ROWS>(a, s, tiles, keys);
+      splits = splits_of(a, keys, share);
+    }
+    const int slots = splits > 1 ? tiles * splits : 0;
+    const int units = MERGE ? (splits > 1 ? tiles : 0) : tiles * splits;
+    const int upto = wave_scan(units, lane), slots_upto = wave_scan(slots, lane);
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(before + upto > place);
+    if (beyond) {
+      const int l = __builtin_ctzll(beyond);
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      p.s = Seq{of(s.len), of(s.start), of(s.n)};
+      p.b = b0 + l;
+      p.splits = of(splits);
+      const int r = place - (before + of(upto) - of(units));
+      const int first = slots_before + of(slots_upto) - of(slots);
+      p.tile = MERGE ? r : r / p.splits;
+      p.split = MERGE ? 0 : r - p.tile * p.splits;
+      p.slot = first + p.tile * p.splits;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+    slots_before += __builtin_amdgcn_readlane(slots_upto, 63);
+  }
+  return false;
+}
+
+// Byte offset of row `key` of a page's KV head from the start of the pool.
+static __device__ __forceinline__ int64_t page_row(const Cache& c, int page, int head, int key) {
+  return page * c.page_stride + head * c.head_stride + (int64_t)(key & ((1 << c.page_shift) - 1)) * c.token_stride;
+}
+
+// O = acc / l and the LSE of row r of a sequence's KV head, eight columns of it.
+template <int DT>
+static __device__ __forceinline__ void store_row(const AttendArgs& a, const Seq& s, int head, int r, int c8, float (&o)[8], float top, float l) {
+  const int token = quotient(r, a.by_group), q_head = head * a.group + r - token * a.group;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] *= inv;
+  char* to = a.out + (s.start + token) * a.o_ts + q_head * a.o_hs;
+  if (a.out_fp32) {
+    *(f32x4*)(to + c8 * 32) = f32x4{o[0], o[1], o[2], o[3]};
+    *(f32x4*)(to + c8 * 32 + 16) = f32x4{o[4], o[5], o[6], o[7]};
+  } else {
+    Store8<DT>::st(to + c8 * 16, o);
+  }
+  if (c8 == 0) a.lse[(int64_t)q_head * a.c.tokens + s.start + token] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
+hipError_t launch_paged_merge(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
+
+struct AppendArgs {
+  Cache c;
+  const char* k;
+  const char* v;
+  int64_t ts, hs;  // bytes between tokens, between heads
+  float* scores;   // [pages, kv_heads, page] or NULL
+  int kv_heads;
+};
+hipError_t launch_paged_append(const AppendArgs& a, int dim, hipStream_t stream);
+
+struct WeightsArgs {
+  Cache c;
+  const char* q;
+  const float* lse;  // [heads, tokens]
+  float* scores;     // [pages, kv_heads, page]
+  int64_t q_ts, q_hs;
+  int kv_heads, group;
+  Divisor by_group;
+  float scale_log2;
+  int causal, window, sinks;
+};
+hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream);
+
+struct EvictArgs {
+  Cache c;
+  float* scores;         // [pages, kv_heads, page]
+  const int* kept_table; // [batch, kept pages]
+  int64_t kept_stride;
+  int kept_pages;
+  int budget, first, last;
+  int* kept;       // [batch, kv_heads, budget]
+  int* kept_lens;  // [batch]
+  int kv_heads;
+};
+hipError_t launch_paged_evict(const EvictArgs& a, int dim, hipStream_t stream);
+
+}  // namespace paged
+}  // namespace ringattn

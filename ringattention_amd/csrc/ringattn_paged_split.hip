@@ -1,0 +1,449 @@
+// gfx950 (CDNA4) kernels: attention of few new tokens over a paged cache, and the merge of what its workgroups leave.
+//
+//   paged_split_kernel : 32 query rows (tokens x heads of a group) of one KV head of a sequence, and a share of the key tiles that
+//       they see.  Its eight waves take the share's 32-key tiles in turn, each with a softmax state of its own, as in
+//       ring_split_kernel: S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMAs, K and V HBM -> LDS -> fragments without a barrier, one
+//       buffer of each per wave; the states meet in LDS at the end.
+//   paged_merge_kernel : O and LSE of a row whose keys went to several workgroups: logsumexp of their sums, in the order of the
+//       shares (the algebra of merge_kernel on sums that were not normalised).
+//
+// A row of few has nothing to reuse: every K and V row is read once from memory for the rows of a group, so that memory is what bounds it, and
+// that wants all compute units to be reading.  The key tiles of a launch are shared out to workgroups in even shares
+// (splits_of), whatever the lengths of its sequences.
+#include "ringattn_paged.h"
+
+namespace ringattn {
+namespace paged {
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void paged_split_kernel(const AttendArgs a) {
+  using E = Elem<DT>;
+  constexpr int WAVES = 8, BM = kFewRows, BN = kKeyTile;
+  constexpr int ROWB = D * 2, TILE = BN * ROWB, CPR = D / 8;
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int PIECES = TILE / 1024;     // 1 KB wave-loads per tile
+  constexpr int HALF = PIECES / 2;        // ... per 16 keys, which always lie in one page
+  constexpr int WREG = 2 * TILE;          // LDS of a wave: a K and a V tile; at the end its acc-O
+  static_assert(WREG >= BM * D * 4, "acc-O of a wave as fp32 takes the place of its tiles");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * WREG];
+  __shared__ float2 stat[WAVES][BM];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+
+  Place p;
+  const int unit = quotient(blockIdx.x, a.by_kv_heads);
+  const int head = blockIdx.x - unit * a.kv_heads;
+  if (!find_place<BM, false>(a, unit, p)) return;
+  const int rows = p.s.n * a.group;
+  const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
+  const int i0 = quotient(r0, a.by_group), i1 = quotient(r_last, a.by_group);
+  const Keys keys = keys_of(p.s, i0, i1, a.causal, a.window, a.sinks);
+  const int u_begin = (int)((int64_t)p.split * keys.count / p.splits), u_end = (int)((int64_t)(p.split + 1) * keys.count / p.splits);
+
+  // this lane's row: its token, its head, its position; rows beyond the range read the last valid one
+  const int row = min(r0 + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
+  const int before = p.s.len - p.s.n;
+  const int lim = a.causal ? min(p.s.len, before + token + 1) : p.s.len;           // keys below it are visible ...
+  const int low = a.window > 0 ? before + token - a.window : -1;                   // ... if they are above this one, or sinks
+  // of all rows of the tile
+  const int lim_all = a.causal ? min(p.s.len, before + i0 + 1) : p.s.len, low_any = a.window > 0 ? before + i1 - a.window : -1;
+
+  s16x8 qf[KS];
+  {
+    const char* qrow = a.q + (p.s.start + token) * a.q_ts + q_head * a.q_hs + h * 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(qrow + ks * 32);
+  }
+
+  unsigned char* my = smem + wave * WREG;
+  const unsigned my_lds = lds_offset(smem) + wave * WREG;
+  int koff[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  int voff[DB];
+  {
+    const int s = lane & 15, g1 = (lane >> 4) & 1;
+    const int row8 = 4 * h + (s >> 2);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int c = 2 * (2 * db + g1) + ((s & 3) >> 1);
+      voff[db] = TILE + row8 * ROWB + ((c ^ v_swizzle<D>(row8)) << 4) + ((s & 1) << 3);
+    }
+  }
+  // Offsets of this lane's 16 bytes of the pieces of 16 keys; a load's own offset moves both ends, and the cache's rows may lie further
+  // apart than those in LDS: the difference is in the offsets.
+  int goff_k[HALF], goff_v[HALF];
+#pragma unroll
+  for (int j = 0; j < HALF; ++j) {
+    const int r = 1024 / ROWB * j + lane / CPR;
+    goff_k[j] = r * a.c.token_stride - 1024 * j + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
+    goff_v[j] = r * a.c.token_stride - 1024 * j + (((lane % CPR) ^ v_swizzle<D>(r)) << 4);
+  }
+  auto load_half = [&](const char* base, unsigned dst, const int (&goff)[HALF]) {
+    if constexpr (HALF == 4)
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+          "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(
+              __builtin_amdgcn_readfirstlane(dst)),
+          "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base)
+          : "m0");
+    else
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(
+                       __builtin_amdgcn_readfirstlane(dst)),
+                   "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)
+                   : "m0");
+  };
+
+  // ---- the tiles of this wave: u_begin + wave, + 8, ...; a lane holds the pages of one of the next 64 of them (16 keys and the 16 behind
+  // them), -1 where there is none
+  const int* table = a.c.table + (int64_t)p.b * a.c.table_stride;
+  auto real_tile = [&](int u) { return u < keys.sink_tiles ? u : u + keys.skip; };
+  int page0, page1, first_held = 0;
+  auto hold_pages = [&](int u) {
+    first_held = u;
+    const int mine = u + WAVES * lane;
+    page0 = page1 = -1;
+    if (mine < u_end) {
+      const int key = real_tile(mine) * BN;
+      const int e0 = key >> a.c.page_shift, e1 = (key + 16) >> a.c.page_shift;
+      page0 = table[e0];
+      page1 = e1 == e0 ? page0 : e1 < a.c.table_pages ? table[e1] : -1;
+      if ((unsigned)page0 >= (unsigned)a.c.pages) page0 = -1;
+      if ((unsigned)page1 >= (unsigned)a.c.pages) page1 = -1;
+    }
+  };
+  struct Tile {
+    int key;             // its first key
+    int gone;            // bit 0, 1: the page of its first, second 16 keys is not there (page 0 is read in its place, and hidden)
+    int64_t at0, at1;
+  };
+  auto tile_at = [&](int u) {
+    if (u - first_held >= 64 * WAVES) hold_pages(u);
+    Tile x;
+    x.key = real_tile(u) * BN;
+    const int l = (u - first_held) / WAVES;
+    const int e0 = __builtin_amdgcn_readlane(page0, l), e1 = __builtin_amdgcn_readlane(page1, l);
+    x.gone = (e0 < 0 ? 1 : 0) | (e1 < 0 ? 2 : 0);
+    x.at0 = page_row(a.c, max(e0, 0), head, x.key);
+    x.at1 = page_row(a.c, max(e1, 0), head, x.key + 16);
+    return x;
+  };
+  auto issue = [&](const char* pool, const Tile& x, unsigned dst, const int (&goff)[HALF]) {
+    load_half(pool + x.at0, dst, goff);
+    load_half(pool + x.at1, dst + TILE / 2, goff);
+  };
+  auto issue_k = [&](const Tile& x) { issue(a.c.k, x, my_lds, goff_k); };
+  auto issue_v = [&](const Tile& x) { issue(a.c.v, x, my_lds + TILE, goff_v); };
+
+  float m = -INFINITY, ms = kNoReference, ls[4] = {0.f, 0.f, 0.f, 0.f};
+  f32x16 oacc[DB], sacc;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+  s16x8 pf[2];
+  float sums[4];
+  // P = exp2(S k2 - m k2); the sums from the unrounded values, the operands of the next product rounded to the storage type: 2^-9 (bf16)
+  // or 2^-12 (fp16) of a probability on average, no more than the output's own rounding
+  auto exponentials = [&]() {
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      typename E::vec8 pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], a.scale_log2, -ms));
+        sums[e & 3] = t2 == 0 && e < 4 ? x : sums[e & 3] + x;
+        pv[e] = (typename E::type)x;
+      }
+      pf[t2] = __builtin_bit_cast(s16x8, pv);
+    }
+  };
+  auto move_reference = [&]() {
+    float m0 = m, m1 = m;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      m0 = fmaxf(fmaxf(m0, sacc[e]), sacc[e + 1]);
+      m1 = fmaxf(fmaxf(m1, sacc[e + 2]), sacc[e + 3]);
+    }
+    m = cross_half_max(fmaxf(m0, m1));
+    const float cs = (m == -INFINITY) ? kNoReference : m * a.scale_log2;
+    const float alpha = __builtin_amdgcn_exp2f(ms - cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ls[i] *= alpha;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
+    ms = cs;
+  };
+  auto hidden = [&](const Tile& x, int e, int hh) {  // of accumulator e of a lane of half hh: is its key hidden from this lane's row?
+    const int key = x.key + 8 * (e >> 2) + (e & 3) + 4 * hh;
+    return key >= lim || (key <= low && key >= a.sinks) || (x.gone >> (e >> 3) & 1);
+  };
+
+  int u = u_begin + wave;
+  bool more = u < u_end;
+  Tile cur{}, nxt{};
+  if (more) {
+    hold_pages(u);
+    cur = tile_at(u);
+    issue_k(cur);
+    issue_v(cur);
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // retire the Q loads with a wait the compiler can see (and the first tiles)
+  for (int pass = 1; more; pass = 0) {  // pass: 1 while there is no reference to take exponentials against
+    u += WAVES;
+    more = u < u_end;
+    if (more) nxt = tile_at(u);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");  // K is in, V may still be on its way
+    {
+      s16x8 kfr[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kfr[ks] = *(const s16x8*)(my + koff[ks]);
+      // the fragments are in registers: the K buffer takes the next tile
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) issue_k(nxt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
+    }
+    const bool masked = cur.key + BN > lim_all || (cur.key <= low_any && cur.key + BN > a.sinks) || cur.gone;
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (hidden(cur, e, h)) sacc[e] = -INFINITY;
+    }
+    // exponentials against the reference as it stands; the row maximum is only looked at when a sum of four of them is above
+    // 2^14 (or not a number)
+#pragma unroll 1
+    for (;; pass = 1) {
+      if (pass) move_reference();
+      exponentials();
+      const bool large = !(fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3])) <= 16384.f);
+      if (pass || __builtin_amdgcn_ballot_w64(large) == 0) break;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ls[i] += sums[i];
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");  // V is in
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where a masked tile's V holds such a value, the
+    // product is taken key by key, over the visible ones.
+    bool odd = false;
+    if (masked) {
+      unsigned top = 0;
+#pragma unroll 1
+      for (int i = 0; i < TILE / 1024; ++i) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 x = *(const u32x4*)(my + TILE + 1024 * i + 16 * lane);
+        constexpr unsigned kExp = DT == 0 ? 0x7c007c00u : 0x7f807f80u, kOne = DT == 0 ? 0x04000400u : 0x00800080u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top |= (x[e] & kExp) + kOne;  // an exponent of ones carries into the sign's place
+      }
+      odd = __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) != 0;
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int e = 0; e < 16; ++e) {
+        typedef typename E::type T;
+        float mine = 0.f;
+#pragma unroll
+        for (int f = 0; f < 16; ++f) {
+          const float x = (float)__builtin_bit_cast(typename E::vec8, pf[f >> 3])[f & 7];
+          mine = e == f ? x : mine;
+        }
+        float other0 = mine, other1 = mine;
+        swap_halves(other0, other1);  // other0: the lower half's, other1: the upper half's
+#pragma unroll 1
+        for (int hh = 0; hh < 2; ++hh) {
+          if (hidden(cur, e, hh)) continue;
+          const float w = hh ? other1 : other0;
+          const int key = 8 * (e >> 2) + (e & 3) + 4 * hh;
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const typename E::vec4 x = *(const typename E::vec4*)(my + TILE + key * ROWB + (((4 * db + q4) ^ v_swizzle<D>(key)) << 4) + 8 * h);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) oacc[db][4 * q4 + i] = __builtin_fmaf(w, (float)(T)x[i], oacc[db][4 * q4 + i]);
+            }
+        }
+      }
+    } else {
+      constexpr int AHEAD = 2;  // fragments read ahead of the MFMA that consumes one
+      s16x8 vfr[2 * DB];
+      auto read_v = [&](int f) {
+        if (f >= 2 * DB) return;
+        const unsigned char* vrow = my + 16 * (f / DB) * ROWB + voff[f % DB];
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vrow));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vrow + 8 * ROWB));
+        vfr[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+#pragma unroll
+      for (int f = 0; f < AHEAD; ++f) read_v(f);
+#pragma unroll
+      for (int f = 0; f < 2 * DB; ++f) {
+        read_v(f + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        oacc[f % DB] = E::mma(vfr[f], pf[f / DB], oacc[f % DB]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue_v(nxt);
+    cur = nxt;
+  }
+
+  // This wave's state where the workgroup can read it: acc-O as fp32 over its own tiles, 16-byte chunk c of row n at chunk c ^ n.
+  {
+    const float l = cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
+    if (h == 0) stat[wave][n] = float2{l == 0.f ? -INFINITY : ms, l};  // (0: nothing seen; a NaN stays one)
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        f32x4 val;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) val[e] = oacc[db][4 * q4 + e];
+        const int c = 8 * db + 2 * q4 + h;
+        *(f32x4*)(my + n * (D * 4) + ((c ^ (n & (D / 4 - 1))) << 4)) = val;
+      }
+  }
+  __syncthreads();
+  constexpr int TPR = D / 8;  // threads of a row
+  const int orow = tid / TPR, c8 = tid % TPR;
+  if (orow > r_last - r0) return;
+  float top = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[w][orow].x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float2 st = stat[w][orow];
+    const unsigned char* src = smem + w * WREG + orow * (D * 4);
+    const f32x4 x0 = *(const f32x4*)(src + (((2 * c8) ^ (orow & (D / 4 - 1))) << 4));
+    const f32x4 x1 = *(const f32x4*)(src + (((2 * c8 + 1) ^ (orow & (D / 4 - 1))) << 4));
+    const float f = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - top);
+    l = __builtin_fmaf(st.y, f, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = __builtin_fmaf(x0[e], f, o[e]);
+      o[4 + e] = __builtin_fmaf(x1[e], f, o[4 + e]);
+    }
+  }
+  if (p.splits > 1) {
+    const int64_t prow = ((int64_t)(p.slot + p.split) * a.kv_heads + head) * BM + orow;
+    float* to = a.part_o + prow * D + c8 * 8;
+    *(f32x4*)to = f32x4{o[0], o[1], o[2], o[3]};
+    *(f32x4*)(to + 4) = f32x4{o[4], o[5], o[6], o[7]};
+    if (c8 == 0) a.part_s[prow] = float2{top, l};
+    return;
+  }
+  store_row<DT>(a, p.s, head, r0 + orow, c8, o, top, l);
+}
+
+// Row tiles whose keys went to several workgroups.  A thread has eight columns of a row and every PARTS-th of its shares; those of a row
+// meet in LDS.
+template <int DT, int D, int ROWS>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const AttendArgs a) {
+  constexpr int TPR = D / 8, GROUPS = 256 / TPR;
+  __shared__ float sums[256][10];
+  Place p;
+  const int unit = quotient(blockIdx.x, a.by_kv_heads);
+  const int head = blockIdx.x - unit * a.kv_heads;
+  if (!find_place<ROWS, true>(a, unit, p)) return;
+  const int r0 = p.tile * ROWS, count = min(ROWS, p.s.n * a.group - r0);
+  int at_once = 1;  // rows at once; the groups of threads left share a row's shares
+  while (at_once < count && at_once < GROUPS) at_once *= 2;
+  const int parts = GROUPS / at_once;
+  const int g = threadIdx.x / TPR, c8 = threadIdx.x % TPR;
+  const int sub = g / at_once;
+  for (int first = 0; first < count; first += at_once) {
+    const int r = first + g % at_once;
+    float top = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    if (r < count) {
+      auto fetch = [&](int s, float2& st, f32x4& x0, f32x4& x1) {
+        const int64_t prow = ((int64_t)(p.slot + s) * a.kv_heads + head) * ROWS + r;
+        st = a.part_s[prow];
+        const float* src = a.part_o + prow * D + c8 * 8;
+        x0 = *(const f32x4*)src;
+        x1 = *(const f32x4*)(src + 4);
+      };
+      auto add = [&](const float2& st, const f32x4& x0, const f32x4& x1) {
+        if (st.x == -INFINITY) return;  // a share that saw nothing
+        const float t = fmaxf(top, st.x), keep = __builtin_amdgcn_exp2f(top - t), w = __builtin_amdgcn_exp2f(st.x - t);
+        l = __builtin_fmaf(st.y, w, l * keep);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e] = __builtin_fmaf(x0[e], w, o[e] * keep);
+          o[4 + e] = __builtin_fmaf(x1[e], w, o[4 + e] * keep);
+        }
+        top = t;
+      };
+      for (int s = sub; s < p.splits; s += 4 * parts) {
+        float2 st[4];
+        f32x4 x0[4], x1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s + i * parts < p.splits) fetch(s + i * parts, st[i], x0[i], x1[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s + i * parts < p.splits) add(st[i], x0[i], x1[i]);
+      }
+    }
+    if (parts > 1) {
+      __syncthreads();
+      float* mine = sums[threadIdx.x];
+      mine[0] = top;
+      mine[1] = l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mine[2 + e] = o[e];
+      __syncthreads();
+      if (sub == 0) {
+        for (int i = 1; i < parts; ++i) {
+          const float* x = sums[threadIdx.x + i * at_once * TPR];
+          if (x[0] == -INFINITY) continue;
+          const float t = fmaxf(top, x[0]), keep = __builtin_amdgcn_exp2f(top - t), w = __builtin_amdgcn_exp2f(x[0] - t);
+          l = __builtin_fmaf(x[1], w, l * keep);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(x[2 + e], w, o[e] * keep);
+          top = t;
+        }
+      }
+    }
+    if (sub == 0 && r < count) store_row<DT>(a, p.s, head, r0 + r, c8, o, top, l);
+  }
+}
+
+hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream) {
+  if (places <= 0) return hipSuccess;
+  if (places > INT32_MAX) return hipErrorInvalidValue;
+  const unsigned grid = (unsigned)places;
+  if (dtype == 0 && dim == 64) paged_split_kernel<0, 64><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 64) paged_split_kernel<1, 64><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 0 && dim == 128) paged_split_kernel<0, 128><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 128) paged_split_kernel<1, 128><<<grid, 512, 0, stream>>>(a);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_merge(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream) {
+  if (places <= 0) return hipSuccess;
+  if (places > INT32_MAX) return hipErrorInvalidValue;
+  const unsigned grid = (unsigned)places;
+  if (dtype == 0 && dim == 64) paged_merge_kernel<0, 64, kFewRows><<<grid, 256, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 64) paged_merge_kernel<1, 64, kFewRows><<<grid, 256, 0, stream>>>(a);
+  else if (dtype == 0 && dim == 128) paged_merge_kernel<0, 128, kFewRows><<<grid, 256, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 128) paged_merge_kernel<1, 128, kFewRows><<<grid, 256, 0, stream>>>(a);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace ringattn
