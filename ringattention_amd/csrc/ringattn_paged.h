@@ -61,6 +61,10 @@ static __device__ __forceinline__ Seq seq_of(const Cache& c, int b) {
   return s;
 }
 
+static __device__ __forceinline__ Seq uniform(const Seq& s) {
+  return Seq{__builtin_amdgcn_readfirstlane(s.len), __builtin_amdgcn_readfirstlane(s.start), __builtin_amdgcn_readfirstlane(s.n)};
+}
+
 // The key tiles that rows of the new tokens [i0, i1] of a sequence see: `sink_tiles` first ones and those from `sink_tiles + skip` on, `count`
 // in all.  Tile u of them is tile u or u + skip of the sequence.
 struct Keys {
@@ -188,6 +192,45 @@ static __device__ __forceinline__ void store_row(const AttendArgs& a, const Seq&
   if (c8 == 0) a.lse[(int64_t)q_head * a.c.tokens + s.start + token] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
+// The pages of a wave's next 64 key tiles, a lane a tile: of its first 16 keys, of the 16 behind them; -1 where there is none.
+struct HeldPages {
+  int page0, page1;
+  // key: the first of this lane's tile; `there`: whether it has one
+  __device__ __forceinline__ void hold(const Cache& c, const int* table, int key, bool there) {
+    page0 = page1 = -1;
+    if (there) {
+      const int e0 = key >> c.page_shift, e1 = (key + 16) >> c.page_shift;
+      page0 = table[e0];
+      page1 = e1 == e0 ? page0 : e1 < c.table_pages ? table[e1] : -1;
+      if ((unsigned)page0 >= (unsigned)c.pages) page0 = -1;
+      if ((unsigned)page1 >= (unsigned)c.pages) page1 = -1;
+    }
+  }
+};
+// 16 keys x D to LDS, 1 KB a piece: offsets of this lane's 16 bytes of each piece from the first key's row.  A load's own offset moves
+// both ends, and the cache's rows may lie further apart than those in LDS: the difference is in the offsets.
+template <int D, class Swizzle> static __device__ __forceinline__ void half_tile_offsets(int (&goff)[D / 32], int token_stride, Swizzle swizzle) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const int r = 512 / D * j + lane / (D / 8);
+    goff[j] = r * token_stride - 1024 * j + (((lane % (D / 8)) ^ swizzle(r)) << 4);
+  }
+}
+template <int HALF> static __device__ __forceinline__ void load_half_tile(const char* base, unsigned dst, const int (&goff)[HALF]) {
+  if constexpr (HALF == 4)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+        "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+        "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base)
+        : "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(
+                     __builtin_amdgcn_readfirstlane(dst)),
+                 "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)
+                 : "m0");
+}
+
 hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
 hipError_t launch_paged_merge(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
 
@@ -224,6 +267,8 @@ struct EvictArgs {
   int* kept;       // [batch, kv_heads, budget]
   int* kept_lens;  // [batch]
   int kv_heads;
+  void* workspace;
+  size_t workspace_bytes;
 };
 hipError_t launch_paged_evict(const EvictArgs& a, int dim, hipStream_t stream);
 

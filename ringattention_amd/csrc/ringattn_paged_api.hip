@@ -287,6 +287,8 @@ int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* 
   a.last = keep_last;
   a.kept = kept;
   a.kept_lens = kept_lens;
+  a.workspace = plan->ws;
+  a.workspace_bytes = workspace_bytes(plan->p.dim);
   a.kv_heads = plan->kv_heads;
   RP_HIP(rp::launch_paged_evict(a, plan->p.dim, (hipStream_t)stream));
   return RINGATTN_OK;

@@ -53,69 +53,310 @@ hipError_t launch_paged_append(const AppendArgs& a, int dim, hipStream_t stream)
 }
 
 // ---- attention weight of the cached tokens ------------------------------------------
-constexpr int kWeightWaves = 8, kWeightKeys = kWeightWaves * kKeyTile;
+// Sequences of up to so many rows of a KV head have few: the waves share out the keys.
+constexpr int kWeightFewRows = 128;
+// Many: the waves share out the rows, for 64 keys, so that a tile of Q is fetched once for them.
+constexpr int kWeightWaves = 8, kManyKeys = 2 * kKeyTile;
 
-template <int DT, int D>
-__global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const WeightsArgs a) {
-  using E = Elem<DT>;
-  constexpr int KS = D / 16;
-  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, head = blockIdx.y;
-  const Seq s = seq_of(a.c, b);
-  if (s.n == 0) return;
-  const int rows = s.n * a.group, before = s.len - s.n;
-  constexpr float kLog2e = 1.4426950408889634f;
-  for (int key0 = (blockIdx.x * kWeightWaves + wave) * kKeyTile; key0 < s.len; key0 += gridDim.x * kWeightKeys) {
-    const int key = key0 + n, entry = key >> a.c.page_shift;
-    int page = entry < a.c.table_pages && key < s.len ? a.c.table[b * a.c.table_stride + entry] : -1;
-    if ((unsigned)page >= (unsigned)a.c.pages) page = -1;
-    s16x8 kfr[KS];
-    {
-      const char* src = a.c.k + page_row(a.c, max(page, 0), head, key) + h * 16;
+// w[e] of lane (n, h): 16 sums over the 32 lanes of a half at once, each halving of the lanes halving the sums that a lane
+// goes on with; lane n ends up with sum n >> 1.  38 instructions for the five steps of 16 separate sums.
+static __device__ __forceinline__ float sum_lanes(float (&w)[16]) {
+  const int lane = threadIdx.x & 63;
+  auto moved = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  using ror8 = std::integral_constant<int, 0x128>;         // within 16 lanes: lane ^ 8
+  using half_mirror = std::integral_constant<int, 0x141>;  // within 8: lane ^ 7
+  using quad_xor2 = std::integral_constant<int, 0x4e>;
+  using quad_xor1 = std::integral_constant<int, 0xb1>;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kfr[ks] = *(const s16x8*)(src + ks * 32);
+  for (int e = 0; e < 8; ++e) {  // odd rows of 16 lanes go on with w[e + 8]
+    // (inline asm: of the builtin's two results the compiler adds one to itself here)
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(w[e]), "+v"(w[e + 8]));
+    w[e] += w[e + 8];
+  }
+  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = (b3 ? w[e + 4] : w[e]) + moved(b3 ? w[e] : w[e + 4], ror8{});
+#pragma unroll
+  for (int e = 0; e < 2; ++e) w[e] = (b2 ? w[e + 2] : w[e]) + moved(b2 ? w[e] : w[e + 2], half_mirror{});
+  const float x = (b1 ? w[1] : w[0]) + moved(b1 ? w[0] : w[1], quad_xor2{});
+  return x + moved(x, quad_xor1{});
+}
+
+
+// What both kernels know of their sequence and KV head.
+template <int DT, int D> struct WeightRows {
+  const WeightsArgs& a;
+  const Seq s;
+  const int head, rows, before;
+  const int* const table;
+  const int lane, n, h;
+  __device__ __forceinline__ WeightRows(const WeightsArgs& args, const Seq& seq, int b, int head_)
+      : a(args), s(seq), head(head_), rows(seq.n * args.group), before(seq.len - seq.n), table(args.c.table + b * args.c.table_stride),
+        lane(threadIdx.x & 63), n(lane & 31), h(lane >> 5) {}
+
+  __device__ __forceinline__ void row_of(int r, int& token, int& q_head) const {
+    r = min(r, rows - 1);
+    token = quotient(r, a.by_group);
+    q_head = head * a.group + r - token * a.group;
+  }
+  __device__ __forceinline__ const char* q_row(int r) const {
+    int token, q_head;
+    row_of(r, token, q_head);
+    return a.q + (s.start + token) * a.q_ts + q_head * a.q_hs;
+  }
+  // log2(e) LSE of a row; +inf, against which every weight is 0, for a row that is not there or saw nothing
+  __device__ __forceinline__ float lse_of(int r) const {
+    int token, q_head;
+    row_of(r, token, q_head);
+    const float x = a.lse[(int64_t)q_head * a.c.tokens + s.start + token] * 1.4426950408889634f;
+    return r >= rows || x == -INFINITY ? INFINITY : x;
+  }
+  // the new tokens [i0, i1) that see any of the keys [key0, key0 + keys)
+  __device__ __forceinline__ void tokens_of(int key0, int keys, int& i0, int& i1) const {
+    i0 = a.causal ? max(0, key0 - before) : 0;
+    i1 = a.window > 0 && key0 >= a.sinks ? min(s.n, key0 + keys - 1 + a.window - before) : s.n;
+  }
+  // whether some of the rows [r0, r0 + 32) are not there or do not see some of the keys
+  __device__ __forceinline__ bool masked(int r0, int key0, int keys) const {
+    const int first = quotient(r0, a.by_group), last = quotient(min(r0 + 31, rows - 1), a.by_group);
+    return r0 + 32 > rows || key0 + keys > (a.causal ? min(s.len, before + first + 1) : s.len) ||
+           (a.window > 0 && key0 <= before + last - a.window && key0 + keys > a.sinks);
+  }
+  __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse, bool masked, int key0, int r) const {
+    if (!masked) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
+      return;
     }
-    // the new tokens that see any of these keys
-    int i0 = 0, i1 = s.n;
-    if (a.causal) i0 = max(0, key0 - before);
-    if (a.window > 0 && key0 >= a.sinks) i1 = min(s.n, key0 + kKeyTile - 1 + a.window - before);
+    const int token = quotient(min(r, rows - 1), a.by_group);
+    int lim = a.causal ? min(s.len, before + token + 1) : s.len;
+    const int low = a.window > 0 ? before + token - a.window : -1;
+    if (lse == INFINITY) lim = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int k = key0 + 8 * (e >> 2) + (e & 3) + 4 * h;
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
+      w[e] += k >= lim || (k <= low && k >= a.sinks) ? 0.f : x;
+    }
+  }
+  // Every key has one owner, which adds to its score once: no order to go by, and nothing to wait for.
+  __device__ __forceinline__ void add_score(int page, int key, float x) const {
+    if (page >= 0 && key < s.len)
+      unsafeAtomicAdd(a.scores + (((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1)), x);
+  }
+};
+
+// Few rows: a wave has 32 keys at a time, all rows.  Bound by the read of K: tiles come HBM -> LDS one ahead, and every compute unit has eight
+// waves of them.
+constexpr int kFewWaves = 4;
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(const WeightsArgs a) {
+  using E = Elem<DT>;
+  constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, HALF = D / 32;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kFewWaves * 2 * TILE];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x, b = blockIdx.z;
+  const Seq s = uniform(seq_of(a.c, b));
+  const WeightRows<DT, D> x(a, s, b, head);
+  if (x.rows == 0 || s.len == 0 || x.rows > kWeightFewRows) return;
+  const int n = x.n, h = x.h;
+  const Keys keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks);  // that any row sees
+  const int tiles = keys.count, step = gridDim.y * kFewWaves;
+  auto first_key = [&](int u) { return (u < keys.sink_tiles ? u : u + keys.skip) * kKeyTile; };
+  int u = blockIdx.y * kFewWaves + wave;
+  if (u >= tiles) return;
+  // the first 32 rows stay in registers
+  s16x8 qf[KS];
+  {
+    const char* q = x.q_row(n) + h * 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(q + ks * 32);
+  }
+  const float lse_first = x.lse_of(n);
+  unsigned char* my = smem + wave * 2 * TILE;
+  const unsigned my_lds = lds_offset(smem) + wave * 2 * TILE;
+  int koff[KS], goff[HALF];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  half_tile_offsets<D>(goff, a.c.token_stride, [](int r) { return k_swizzle<D>(r); });
+  HeldPages held;
+  int held_from = u;
+  auto hold = [&](int first) {
+    held_from = first;
+    held.hold(a.c, x.table, first_key(first + step * x.lane), first + step * x.lane < tiles);
+  };
+  hold(u);
+  int at = 0, p0, p1, next0 = 0, next1 = 0;  // place of tile u among the held ones; its pages
+  auto issue = [&](int key, int slot, int page0, int page1) {
+    load_half_tile(a.c.k + page_row(a.c, max(page0, 0), head, key), my_lds + slot * TILE, goff);
+    load_half_tile(a.c.k + page_row(a.c, max(page1, 0), head, key + 16), my_lds + slot * TILE + TILE / 2, goff);
+  };
+  p0 = __builtin_amdgcn_readlane(held.page0, 0);
+  p1 = __builtin_amdgcn_readlane(held.page1, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  issue(first_key(u), 0, p0, p1);
+  for (int slot = 0; u < tiles; u += step, slot ^= 1, p0 = next0, p1 = next1) {
+    const int key0 = first_key(u);
+    if (u + step < tiles) {
+      if (++at == 64) {
+        hold(u + step);
+        at = 0;
+      }
+      next0 = __builtin_amdgcn_readlane(held.page0, at);
+      next1 = __builtin_amdgcn_readlane(held.page1, at);
+      issue(first_key(u + step), slot ^ 1, next0, next1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * HALF) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    s16x8 kfr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kfr[ks] = *(const s16x8*)(my + slot * TILE + koff[ks]);
     float w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = 0.f;
-    for (int r0 = i0 * a.group; r0 < i1 * a.group; r0 += 32) {
-      const int r = min(r0 + n, rows - 1), token = quotient(r, a.by_group), q_head = head * a.group + r - token * a.group;
-      const char* qrow = a.q + (s.start + token) * a.q_ts + q_head * a.q_hs + h * 16;
-      float lse = a.lse[(int64_t)q_head * a.c.tokens + s.start + token] * kLog2e;
-      if (r0 + n >= rows || lse == -INFINITY) lse = INFINITY;  // no row, or one that saw nothing: weight 0
+    {
       f32x16 sacc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(qrow + ks * 32), sacc);
-      const int lim = a.causal ? min(s.len, before + token + 1) : s.len, low = a.window > 0 ? before + token - a.window : -1;
+      for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
+      x.weigh(w, sacc, lse_first, true, key0, n);
+    }
+#pragma unroll 1
+    for (int r0 = 32; r0 < x.rows; r0 += 32) {
+      const char* q = x.q_row(r0 + n) + h * 16;
+      const float lse = x.lse_of(r0 + n);
+      f32x16 sacc;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int k = key0 + 8 * (e >> 2) + (e & 3) + 4 * h;
-        const bool hidden = k >= lim || (k <= low && k >= a.sinks) || lse == INFINITY;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
-        w[e] += hidden ? 0.f : x;
+      for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(q + ks * 32), sacc);
+      x.weigh(w, sacc, lse, true, key0, r0 + n);
+    }
+    const float sum = sum_lanes(w);
+    const int e = n >> 1;
+    if ((n & 1) == 0) x.add_score(e < 8 ? p0 : p1, key0 + 8 * (e >> 2) + (e & 3) + 4 * h, sum);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// Many rows: a wave has 64 keys and every eighth tile of 32 rows, whose Q it brings to LDS one ahead; it needs no other wave until the sums
+// meet.  Bound by the exponentials: 32 of 16 cycles each to 16 MFMAs of 32.
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const WeightsArgs a) {
+  using E = Elem<DT>;
+  constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, CPR = D / 8, PIECES = TILE / 1024;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kWeightWaves * 2 * TILE];  // two tiles of Q of every wave
+  __shared__ float part[kWeightWaves][kManyKeys];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int head = blockIdx.x, block = blockIdx.y, in_all = gridDim.y;
+  // the blockIdx.z-th sequence of many rows: there are fewer of them than sequences
+  int b = -1;
+  Seq s{};
+  for (int b0 = 0, before = 0; b0 < a.c.batch && b < 0; b0 += 64) {
+    Seq mine{};
+    if (b0 + lane < a.c.batch) mine = seq_of(a.c, b0 + lane);
+    const uint64_t many = __builtin_amdgcn_ballot_w64(mine.n * a.group > kWeightFewRows);
+    const int wanted = (int)blockIdx.z - before, count = __builtin_popcountll(many);
+    if (wanted < count) {
+      const bool it = (many >> lane & 1) && __builtin_popcountll(many & (((uint64_t)1 << lane) - 1)) == wanted;
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(it));
+      s = Seq{__builtin_amdgcn_readlane(mine.len, l), __builtin_amdgcn_readlane(mine.start, l), __builtin_amdgcn_readlane(mine.n, l)};
+      b = b0 + l;
+    }
+    before += count;
+  }
+  if (b < 0) return;
+  const WeightRows<DT, D> x(a, s, b, head);
+  const int n = x.n, h = x.h;
+  auto page_of = [&](int key) {  // -1: not there, or behind the end
+    const int page = key < s.len ? x.table[key >> a.c.page_shift] : -1;
+    return (unsigned)page < (unsigned)a.c.pages ? page : -1;
+  };
+  unsigned char* my = smem + wave * 2 * TILE;
+  const unsigned my_lds = lds_offset(smem) + wave * 2 * TILE;
+  int qoff[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qoff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  auto fetch_q = [&](int r0, int slot) {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int r = 1024 / ROWB * j + lane / CPR;
+      const char* src = x.q_row(r0 + r) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                       __builtin_amdgcn_readfirstlane(my_lds + slot * TILE + 1024 * j)),
+                   "v"(src)
+                   : "m0");
+    }
+  };
+  const int blocks = (s.len + kManyKeys - 1) / kManyKeys;
+  // laps over the blocks go to and fro: under the mask the first blocks are seen by the most rows
+  for (int lap = 0; lap * in_all < blocks; ++lap) {
+    const int at = lap * in_all + (lap & 1 ? in_all - 1 - block : block);
+    if (at >= blocks) continue;
+    const int key0 = at * kManyKeys;
+    int i0, i1;
+    x.tokens_of(key0, kManyKeys, i0, i1);
+    const int r_begin = i0 * a.group, r_end = i1 * a.group;
+    s16x8 kfr[2][KS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = key0 + 32 * t + n;
+      const char* src = a.c.k + page_row(a.c, max(page_of(key), 0), head, key) + h * 16;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kfr[t][ks] = *(const s16x8*)(src + ks * 32);
+    }
+    float w[2][16];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[t][e] = 0.f;
+    int r0 = r_begin + 32 * wave, slot = 0;
+    float lse_next = 0.f;
+    if (r0 < r_end) {
+      fetch_q(r0, 0);
+      lse_next = x.lse_of(r0 + n);
+    }
+    for (; r0 < r_end; r0 += 32 * kWeightWaves, slot ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const float lse = lse_next;
+      s16x8 qfr[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qfr[ks] = *(const s16x8*)(my + slot * TILE + qoff[ks]);
+      const int next = r0 + 32 * kWeightWaves;
+      if (next < r_end) {
+        fetch_q(next, slot ^ 1);
+        lse_next = x.lse_of(next + n);
       }
+      const bool masked = x.masked(r0, key0, kManyKeys);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16 sacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[t][ks], qfr[ks], sacc);
+        x.weigh(w[t], sacc, lse, masked, key0 + 32 * t, r0 + n);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) w[e] += __shfl_xor(w[e], d);
-    // lane (n, h) of n < 16 has the sum of accumulator n of half h
-    float mine = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mine = n == e ? w[e] : mine;
-    const int k = key0 + 8 * (n >> 2) + (n & 3) + 4 * h;
-    const int at = __shfl(page, (k - key0) & 31);
-    if (n < 16 && at >= 0 && k < s.len) {
-      float* to = a.scores + (((int64_t)at * a.kv_heads + head) << a.c.page_shift) + (k & ((1 << a.c.page_shift) - 1));
-      *to += mine;
+    for (int t = 0; t < 2; ++t) {
+      const float sum = sum_lanes(w[t]);
+      const int e = n >> 1;
+      if ((n & 1) == 0) part[wave][32 * t + 8 * (e >> 2) + (e & 3) + 4 * h] = sum;
     }
+    __syncthreads();
+    if (threadIdx.x < kManyKeys) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWeightWaves; ++i) sum += part[i][threadIdx.x];
+      x.add_score(page_of(key0 + threadIdx.x), key0 + threadIdx.x, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -123,15 +364,26 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
   const int64_t keys = (int64_t)a.c.table_pages << a.c.page_shift;
   const int64_t pairs = (int64_t)a.c.batch * a.kv_heads;
   if (pairs <= 0 || keys <= 0) return hipSuccess;
-  int64_t blocks = (keys + kWeightKeys - 1) / kWeightKeys;
-  const int64_t enough = (4096 + pairs - 1) / pairs;
-  if (blocks > enough) blocks = enough;
-  if (a.kv_heads > 65535 || a.c.batch > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, (unsigned)a.kv_heads, (unsigned)a.c.batch);
-  if (dtype == 0 && dim == 64) paged_weights_kernel<0, 64><<<grid, 64 * kWeightWaves, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 64) paged_weights_kernel<1, 64><<<grid, 64 * kWeightWaves, 0, stream>>>(a);
-  else if (dtype == 0 && dim == 128) paged_weights_kernel<0, 128><<<grid, 64 * kWeightWaves, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 128) paged_weights_kernel<1, 128><<<grid, 64 * kWeightWaves, 0, stream>>>(a);
+  if (a.c.batch > 65535) return hipErrorInvalidValue;
+  // A launch for the sequences of few rows and one for those of many, where there may be any.  As many workgroups as the longest
+  // sequence could use, where that does not make them more than enough: they go on to further keys.
+  const int64_t rows = (int64_t)a.c.tokens * a.group;
+  auto grid = [&](int keys_each, int64_t sequences, int64_t enough) {
+    const int64_t blocks = (keys + keys_each - 1) / keys_each, each = (enough + sequences * a.kv_heads - 1) / (sequences * a.kv_heads);
+    return dim3((unsigned)a.kv_heads, (unsigned)(blocks < each ? blocks : each), (unsigned)sequences);
+  };
+  const int64_t with_many = rows / (kWeightFewRows + 1) < a.c.batch ? rows / (kWeightFewRows + 1) : a.c.batch;
+#define RA_LAUNCH_WEIGHTS(DT_, D_)                                                                                                      \
+  do {                                                                                                                                 \
+    if (a.c.batch > 1 || with_many == 0)                                                                                               \
+      paged_weights_few_kernel<DT_, D_><<<grid(kFewWaves * kKeyTile, a.c.batch, 2048), 64 * kFewWaves, 0, stream>>>(a);                 \
+    if (with_many > 0) paged_weights_kernel<DT_, D_><<<grid(kManyKeys, with_many, 512), 64 * kWeightWaves, 0, stream>>>(a);             \
+  } while (0)
+  if (dtype == 0 && dim == 64) RA_LAUNCH_WEIGHTS(0, 64);
+  else if (dtype == 1 && dim == 64) RA_LAUNCH_WEIGHTS(1, 64);
+  else if (dtype == 0 && dim == 128) RA_LAUNCH_WEIGHTS(0, 128);
+  else if (dtype == 1 && dim == 128) RA_LAUNCH_WEIGHTS(1, 128);
+#undef RA_LAUNCH_WEIGHTS
   else return hipErrorInvalidValue;
   return hipGetLastError();
 }
@@ -144,102 +396,238 @@ static __device__ __forceinline__ unsigned rank_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024, kDigit = 11;
+constexpr int kSelectThreads = 1024, kDigit = 11, kBins = 1 << kDigit, kPasses = 3;
+constexpr int kHeld = 8;  // ranks that a thread keeps in registers from pass to pass; those beyond are read again
+// Bits of digit `pass` of a rank, from the highest on, and where they begin.
+static __device__ __forceinline__ constexpr int digit_bits(int pass) { return pass < 2 ? kDigit : 32 - 2 * kDigit; }
+static __device__ __forceinline__ constexpr int digit_shift(int pass) { return pass == 0 ? 32 - kDigit : pass == 1 ? 32 - 2 * kDigit : 0; }
 
-__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a) {
-  __shared__ unsigned counts[1 << kDigit];
-  __shared__ int wave_total[kSelectThreads / 64];
-  __shared__ unsigned found_digit, found_above;
-  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int len = clamped(a.c.lens[b], 0, a.c.table_pages << a.c.page_shift);
-  int* kept = a.kept + ((int64_t)b * a.kv_heads + head) * a.budget;
-  const int stay = min(len, a.budget);
-  if (head == 0 && tid == 0) a.kept_lens[b] = stay;
-  for (int j = stay + tid; j < a.budget; j += kSelectThreads) kept[j] = -1;
-  if (len <= a.budget) {
-    for (int j = tid; j < len; j += kSelectThreads) kept[j] = j;
-    return;
-  }
-  const int* table = a.c.table + b * a.c.table_stride;
+// What is known of the rank of the last token that stays: its digits so far, and how many of those that share them stay.
+struct Found {
+  unsigned prefix, wanted;
+};
+
+// A slice of a sequence's KV head: its tokens whose scores decide, and their ranks.
+struct Slice {
+  int begin, end;
+  unsigned held[kHeld];
+};
+template <class Fn> static __device__ __forceinline__ void each_rank(const EvictArgs& a, const int* table, int head, Slice& s, bool first, Fn fn) {
+  const int mask = (1 << a.c.page_shift) - 1;
   auto rank_at = [&](int key) {
     const int page = table[key >> a.c.page_shift];
     if ((unsigned)page >= (unsigned)a.c.pages) return rank_of(-INFINITY);
-    return rank_of(a.scores[(((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))]);
+    return rank_of(a.scores[(((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & mask)]);
   };
-  const int from = a.first, to = len - a.last;  // the tokens whose scores decide
-  unsigned wanted = a.budget - a.first - a.last;  // of them, so many stay
-  // the rank of the last one that stays, digit by digit: `prefix` so far, `wanted` of those that share it stay
-  unsigned prefix = 0, known = 0;
-  for (int shift = 32; wanted > 0 && shift > 0;) {
-    const int bits = min(kDigit, shift);
-    shift -= bits;
-    for (int i = tid; i < 1 << kDigit; i += kSelectThreads) counts[i] = 0;
-    __syncthreads();
-    for (int key = from + tid; key < to; key += kSelectThreads) {
-      const unsigned r = rank_at(key);
-      if ((r & known) == prefix) atomicAdd(&counts[r >> shift & ((1u << bits) - 1)], 1u);
+  if (first) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int key = s.begin + i * kSelectThreads + (int)threadIdx.x;
+      s.held[i] = key < s.end ? rank_at(key) : 0;
     }
-    __syncthreads();
-    // the digit at which the count from the top reaches `wanted`: a thread has two of them, the highest first
-    const int hi = (1 << kDigit) - 1 - 2 * tid, c0 = (int)counts[hi], c1 = (int)counts[hi - 1];
-    const int both = c0 + c1, upto = wave_scan(both, lane);
-    if (lane == 63) wave_total[wave] = upto;
-    __syncthreads();
-    int above = upto - both;
-    for (int w = 0; w < wave; ++w) above += wave_total[w];
-    const int want = (int)wanted;
-    if (above < want && want <= above + c0) {
-      found_digit = hi;
-      found_above = above;
-    } else if (above + c0 < want && want <= above + both) {
-      found_digit = hi - 1;
-      found_above = above + c0;
-    }
-    __syncthreads();
-    prefix |= found_digit << shift;
-    known |= ((1u << bits) - 1) << shift;
-    wanted -= found_above;
-    __syncthreads();
   }
-  // in order: what ranks above stays, and the first `wanted` of those that rank the same.  A wave has 64 tokens at a time, one wave's
-  // after the other's.
-  const bool any = a.budget > a.first + a.last;
-  int placed = 0, equal_before = 0;
-  for (int key0 = 0; key0 < len; key0 += kSelectThreads) {
-    const int key = key0 + tid;
-    bool more = false, same = false;
-    if (key < len) {
-      if (key < from || key >= to) more = true;
-      else if (any) {
-        const unsigned r = rank_at(key);
-        more = r > prefix;
-        same = r == prefix;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    if (s.begin + i * kSelectThreads >= s.end) break;
+    const int key = s.begin + i * kSelectThreads + (int)threadIdx.x;
+    fn(key, s.held[i], key < s.end);
+  }
+  for (int key0 = s.begin + kHeld * kSelectThreads; key0 < s.end; key0 += kSelectThreads) {
+    const int key = key0 + (int)threadIdx.x;
+    fn(key, key < s.end ? rank_at(key) : 0, key < s.end);
+  }
+}
+
+// How many of a slice's ranks that begin with `prefix` have each value of the digit behind it.
+static __device__ __forceinline__ void count_digits(const EvictArgs& a, const int* table, int head, Slice& s, bool first, int pass, unsigned prefix,
+                                                    unsigned* counts) {
+  const int lane = threadIdx.x & 63, shift = digit_shift(pass), bits = digit_bits(pass);
+  const unsigned known = pass == 0 ? 0 : ~0u << (shift + bits);
+  for (int i = threadIdx.x; i < kBins; i += kSelectThreads) counts[i] = 0;
+  __syncthreads();
+  each_rank(a, table, head, s, first, [&](int, unsigned r, bool there) {
+    const bool counted = there && (r & known) == prefix;
+    const unsigned digit = r >> shift & ((1u << bits) - 1);
+    // scores that drew nothing all have one rank: the lanes that share the first one's digit are one addition
+    const uint64_t any = __builtin_amdgcn_ballot_w64(counted);
+    if (any == 0) return;
+    const int one = __builtin_ctzll(any);
+    const unsigned lead = __builtin_amdgcn_readlane(digit, one);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(counted && digit == lead);
+    if (lane == one) atomicAdd(&counts[lead], (unsigned)__builtin_popcountll(same));
+    else if (counted && digit != lead) atomicAdd(&counts[digit], 1u);
+  });
+  __syncthreads();
+}
+
+// The digit at which the counts, added up from the highest value on, reach f.wanted; a thread has the counts of two values, `c0` of the
+// higher one.  `shared`: room for a number of every wave and two more.
+static __device__ __forceinline__ void find_digit(unsigned c0, unsigned c1, int pass, Found& f, unsigned* shared) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = kBins - 1 - 2 * (int)threadIdx.x;
+  const int both = (int)(c0 + c1), upto = wave_scan(both, lane);
+  if (lane == 63) shared[wave] = upto;
+  __syncthreads();
+  int above = upto - both;
+  for (int w = 0; w < wave; ++w) above += shared[w];
+  const int want = (int)f.wanted;
+  unsigned* found = shared + kSelectThreads / 64;
+  if (above < want && want <= above + (int)c0) {
+    found[0] = hi;
+    found[1] = above;
+  } else if (above + (int)c0 < want && want <= above + both) {
+    found[0] = hi - 1;
+    found[1] = above + c0;
+  }
+  __syncthreads();
+  f.prefix |= found[0] << digit_shift(pass);
+  f.wanted -= found[1];
+  __syncthreads();
+}
+
+// Places of the tokens [begin, end) that stay, in order, from kept[placed] on: those outside [from, to), those that rank above
+// f.prefix, and of those that rank the same the first ones while fewer than f.wanted came before.
+static __device__ __forceinline__ void place_tokens(const EvictArgs& a, const int* table, int head, Slice& s, bool first, int* kept, int placed,
+                                                    int equal_before, const Found& f, unsigned* shared) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  each_rank(a, table, head, s, first, [&](int key, unsigned r, bool there) {
+    const bool more = there && f.wanted > 0 && r > f.prefix, same = there && f.wanted > 0 && r == f.prefix;
+    const uint64_t sames = __builtin_amdgcn_ballot_w64(same), mores = __builtin_amdgcn_ballot_w64(more);
+    if (lane == 0) shared[wave] = (unsigned)__builtin_popcountll(sames) << 16 | (unsigned)__builtin_popcountll(mores);
+    __syncthreads();
+    int eq = equal_before, ab = 0, eq_all = 0, ab_all = 0;
+    for (int w = 0; w < kSelectThreads / 64; ++w) {
+      const unsigned x = shared[w];
+      if (w < wave) {
+        eq += x >> 16;
+        ab += x & 0xffff;
+      }
+      eq_all += x >> 16;
+      ab_all += x & 0xffff;
+    }
+    __syncthreads();
+    const int wanted = (int)f.wanted;
+    eq += __builtin_popcountll(sames & below);  // those that rank the same in front of this one
+    ab += __builtin_popcountll(mores & below);
+    const int at = placed + ab + min(eq, wanted) - min(equal_before, wanted);
+    if ((more || (same && eq < wanted)) && at < a.budget) kept[at] = key;
+    placed += ab_all + min(equal_before + eq_all, wanted) - min(equal_before, wanted);
+    equal_before += eq_all;
+  });
+}
+
+// What every workgroup of a selection begins with.  The slices of [from, to) have as many tokens each.
+struct Selection {
+  int len, from, to;
+  int* kept;
+  const int* table;
+  Slice s;
+  unsigned wanted;
+};
+static __device__ __forceinline__ Selection selection_of(const EvictArgs& a, int head, int b, int slice, int slices) {
+  Selection x;
+  x.len = __builtin_amdgcn_readfirstlane(clamped(a.c.lens[b], 0, a.c.table_pages << a.c.page_shift));
+  x.kept = a.kept + ((int64_t)b * a.kv_heads + head) * a.budget;
+  x.table = a.c.table + b * a.c.table_stride;
+  x.from = a.first;
+  x.to = x.len - a.last;
+  const int count = x.to - x.from, each = ((count + slices - 1) / slices + 63) & ~63;
+  x.s.begin = min(x.to, x.from + slice * each);
+  x.s.end = min(x.to, x.s.begin + each);
+  x.wanted = a.budget - a.first - a.last;
+  return x;
+}
+// The first and the last tokens, or all of a sequence that is short enough; the end of the list.  True if there is more to select.
+static __device__ __forceinline__ bool place_ends(const EvictArgs& a, const Selection& x, int head, int b) {
+  const int tid = threadIdx.x, stay = min(x.len, a.budget);
+  if (head == 0 && tid == 0) a.kept_lens[b] = stay;
+  for (int j = stay + tid; j < a.budget; j += kSelectThreads) x.kept[j] = -1;
+  if (x.len <= a.budget) {
+    for (int j = tid; j < x.len; j += kSelectThreads) x.kept[j] = j;
+    return false;
+  }
+  for (int j = tid; j < a.first; j += kSelectThreads) x.kept[j] = j;
+  for (int j = tid; j < a.last; j += kSelectThreads) x.kept[a.budget - a.last + j] = x.len - a.last + j;
+  return x.wanted > 0;
+}
+
+// One workgroup for a sequence's KV head: all passes, the ranks of up to 8 K tokens in registers.
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a) {
+  __shared__ unsigned counts[kBins];
+  __shared__ unsigned shared[kSelectThreads / 64 + 2];
+  const int head = blockIdx.x, b = blockIdx.y, hi = kBins - 1 - 2 * (int)threadIdx.x;
+  Selection x = selection_of(a, head, b, 0, 1);
+  if (!place_ends(a, x, head, b)) return;
+  Found f{0, x.wanted};
+  for (int pass = 0; pass < kPasses; ++pass) {
+    count_digits(a, x.table, head, x.s, pass == 0, pass, f.prefix, counts);
+    find_digit(counts[hi], counts[hi - 1], pass, f, shared);
+  }
+  place_tokens(a, x.table, head, x.s, false, x.kept, a.first, 0, f, shared);
+}
+
+// The same by several workgroups, where there are few sequences and heads and they are long: a launch for each pass, in which
+// every workgroup adds up the counts that the launch before has left of all slices.
+//   counts [pairs][slices][kPasses][kBins], above [pairs][slices][kPasses] (tokens of the slice that rank above by a pass's digit), found [pairs][kPasses]
+template <int PASS>  // kPasses: the places
+__global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(const EvictArgs a, unsigned* all_counts, unsigned* all_above, Found* all_found) {
+  __shared__ unsigned counts[kBins];
+  __shared__ unsigned shared[kSelectThreads / 64 + 2];
+  const int slice = blockIdx.x, slices = gridDim.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, hi = kBins - 1 - 2 * tid;
+  const int lane = tid & 63, wave = tid >> 6;
+  const int64_t pair = (int64_t)b * a.kv_heads + head;
+  Selection x = selection_of(a, head, b, slice, slices);
+  if (PASS == 0 && slice == 0) place_ends(a, x, head, b);
+  if (x.len <= a.budget || x.wanted == 0) return;
+  unsigned* pair_counts = all_counts + pair * slices * (kPasses * kBins);
+  unsigned* pair_above = all_above + pair * slices * kPasses;
+  auto counts_of = [&](int s, int pass) { return (const uint2*)(pair_counts + (s * kPasses + pass) * kBins + hi - 1); };  // .y: the higher value
+  auto sum_of = [&](unsigned v) {  // over the workgroup
+    const unsigned w = wave_sum(v);
+    if (lane == 0) shared[wave] = w;
+    __syncthreads();
+    unsigned t = 0;
+    for (int i = 0; i < kSelectThreads / 64; ++i) t += shared[i];
+    __syncthreads();
+    return t;
+  };
+  Found f{0, x.wanted};
+  if constexpr (PASS > 1) f = all_found[pair * kPasses + PASS - 2];
+  unsigned digit = 0;
+  if constexpr (PASS > 0) {
+    unsigned c0 = 0, c1 = 0;
+    for (int s = 0; s < slices; ++s) {
+      const uint2 c = *counts_of(s, PASS - 1);
+      c0 += c.y;
+      c1 += c.x;
+    }
+    find_digit(c0, c1, PASS - 1, f, shared);
+    digit = f.prefix >> digit_shift(PASS - 1) & ((1u << digit_bits(PASS - 1)) - 1);
+  }
+  auto above_digit = [&](int s) {  // this thread's part of how many of slice s rank above by the digit just found
+    const uint2 c = *counts_of(s, PASS - 1);
+    return (hi > (int)digit ? c.y : 0) + (hi - 1 > (int)digit ? c.x : 0);
+  };
+  if constexpr (PASS < kPasses) {
+    if constexpr (PASS > 0) {
+      const unsigned above = sum_of(above_digit(slice));
+      if (tid == 0) {
+        pair_above[slice * kPasses + PASS - 1] = above;
+        if (slice == 0) all_found[pair * kPasses + PASS - 1] = f;
       }
     }
-    const uint64_t sames = __builtin_amdgcn_ballot_w64(same);
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    if (lane == 0) wave_total[wave] = __builtin_popcountll(sames);
-    __syncthreads();
-    int eq = equal_before, eq_all = 0;
-    for (int w = 0; w < kSelectThreads / 64; ++w) {
-      if (w < wave) eq += wave_total[w];
-      eq_all += wave_total[w];
-    }
-    equal_before += eq_all;
-    const bool stays = more || (same && eq + __builtin_popcountll(sames & below) < (int)wanted);
-    const uint64_t staying = __builtin_amdgcn_ballot_w64(stays);
-    __syncthreads();
-    if (lane == 0) wave_total[wave] = __builtin_popcountll(staying);
-    __syncthreads();
-    int at = placed, all = 0;
-    for (int w = 0; w < kSelectThreads / 64; ++w) {
-      if (w < wave) at += wave_total[w];
-      all += wave_total[w];
-    }
-    placed += all;
-    at += __builtin_popcountll(staying & below);
-    if (stays && at < a.budget) kept[at] = key;
-    __syncthreads();
+    count_digits(a, x.table, head, x.s, true, PASS, f.prefix, counts);
+    unsigned* to = pair_counts + (slice * kPasses + PASS) * kBins;
+    for (int i = tid; i < kBins; i += kSelectThreads) to[i] = counts[i];
+  } else {
+    // of the slices in front: tokens that rank above, and those that rank the same
+    unsigned above = 0, equal = 0;
+    for (int s = 0; s < slice; ++s) above += above_digit(s);
+    for (int i = tid; i < slice * kPasses; i += kSelectThreads) above += i % kPasses < kPasses - 1 ? pair_above[i] : 0;
+    for (int s = tid; s < slice; s += kSelectThreads) equal += pair_counts[(s * kPasses + kPasses - 1) * kBins + digit];
+    above = sum_of(above);
+    equal = sum_of(equal);
+    place_tokens(a, x.table, head, x.s, true, x.kept, a.first + (int)above + min((int)equal, (int)f.wanted), (int)equal, f, shared);
   }
 }
 
@@ -269,7 +657,25 @@ __global__ __launch_bounds__(256) void paged_move_kernel(const EvictArgs a, int 
 hipError_t launch_paged_evict(const EvictArgs& a, int dim, hipStream_t stream) {
   if (a.c.batch <= 0 || a.kv_heads <= 0) return hipSuccess;
   if (a.kv_heads > 65535 || a.c.batch > 65535) return hipErrorInvalidValue;
-  paged_select_kernel<<<dim3((unsigned)a.kv_heads, (unsigned)a.c.batch), kSelectThreads, 0, stream>>>(a);
+  // Slices of 4 K tokens, for as long as that many workgroups find a compute unit and their counts room in the workspace.
+  const int64_t pairs_ = (int64_t)a.c.batch * a.kv_heads, keys = (int64_t)a.c.table_pages << a.c.page_shift;
+  const int64_t slice_bytes = kPasses * (kBins + 1) * sizeof(unsigned), pair_bytes = kPasses * sizeof(Found);
+  int64_t slices = (keys + 4095) / 4096;
+  slices = slices < 512 / pairs_ ? slices : 512 / pairs_;
+  const int64_t room = (((int64_t)a.workspace_bytes - 8) / pairs_ - pair_bytes) / slice_bytes;
+  slices = slices < room ? slices : room;
+  if (keys <= kHeld * kSelectThreads || slices < 2) {
+    paged_select_kernel<<<dim3((unsigned)a.kv_heads, (unsigned)a.c.batch), kSelectThreads, 0, stream>>>(a);
+  } else {
+    unsigned* counts = (unsigned*)a.workspace;
+    unsigned* above = counts + pairs_ * slices * kPasses * kBins;
+    Found* found = (Found*)(above + ((pairs_ * slices * kPasses + 1) & ~(int64_t)1));
+    const dim3 grid((unsigned)slices, (unsigned)a.kv_heads, (unsigned)a.c.batch);
+    paged_select_slices_kernel<0><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
+    paged_select_slices_kernel<1><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
+    paged_select_slices_kernel<2><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
+    paged_select_slices_kernel<3><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int rows = 256 / (dim / 8);

@@ -72,47 +72,19 @@ __global__ __launch_bounds__(512, 2) void paged_split_kernel(const AttendArgs a)
       voff[db] = TILE + row8 * ROWB + ((c ^ v_swizzle<D>(row8)) << 4) + ((s & 1) << 3);
     }
   }
-  // Offsets of this lane's 16 bytes of the pieces of 16 keys; a load's own offset moves both ends, and the cache's rows may lie further
-  // apart than those in LDS: the difference is in the offsets.
   int goff_k[HALF], goff_v[HALF];
-#pragma unroll
-  for (int j = 0; j < HALF; ++j) {
-    const int r = 1024 / ROWB * j + lane / CPR;
-    goff_k[j] = r * a.c.token_stride - 1024 * j + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
-    goff_v[j] = r * a.c.token_stride - 1024 * j + (((lane % CPR) ^ v_swizzle<D>(r)) << 4);
-  }
-  auto load_half = [&](const char* base, unsigned dst, const int (&goff)[HALF]) {
-    if constexpr (HALF == 4)
-      asm volatile(
-          "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-          "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(
-              __builtin_amdgcn_readfirstlane(dst)),
-          "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base)
-          : "m0");
-    else
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(
-                       __builtin_amdgcn_readfirstlane(dst)),
-                   "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)
-                   : "m0");
-  };
+  half_tile_offsets<D>(goff_k, a.c.token_stride, [](int r) { return k_swizzle<D>(r); });
+  half_tile_offsets<D>(goff_v, a.c.token_stride, [](int r) { return v_swizzle<D>(r); });
 
-  // ---- the tiles of this wave: u_begin + wave, + 8, ...; a lane holds the pages of one of the next 64 of them (16 keys and the 16 behind
-  // them), -1 where there is none
+  // ---- the tiles of this wave: u_begin + wave, + 8, ...
   const int* table = a.c.table + (int64_t)p.b * a.c.table_stride;
   auto real_tile = [&](int u) { return u < keys.sink_tiles ? u : u + keys.skip; };
-  int page0, page1, first_held = 0;
+  HeldPages held;
+  int first_held = 0;
   auto hold_pages = [&](int u) {
     first_held = u;
     const int mine = u + WAVES * lane;
-    page0 = page1 = -1;
-    if (mine < u_end) {
-      const int key = real_tile(mine) * BN;
-      const int e0 = key >> a.c.page_shift, e1 = (key + 16) >> a.c.page_shift;
-      page0 = table[e0];
-      page1 = e1 == e0 ? page0 : e1 < a.c.table_pages ? table[e1] : -1;
-      if ((unsigned)page0 >= (unsigned)a.c.pages) page0 = -1;
-      if ((unsigned)page1 >= (unsigned)a.c.pages) page1 = -1;
-    }
+    held.hold(a.c, table, real_tile(mine) * BN, mine < u_end);
   };
   struct Tile {
     int key;             // its first key
@@ -124,15 +96,15 @@ __global__ __launch_bounds__(512, 2) void paged_split_kernel(const AttendArgs a)
     Tile x;
     x.key = real_tile(u) * BN;
     const int l = (u - first_held) / WAVES;
-    const int e0 = __builtin_amdgcn_readlane(page0, l), e1 = __builtin_amdgcn_readlane(page1, l);
+    const int e0 = __builtin_amdgcn_readlane(held.page0, l), e1 = __builtin_amdgcn_readlane(held.page1, l);
     x.gone = (e0 < 0 ? 1 : 0) | (e1 < 0 ? 2 : 0);
     x.at0 = page_row(a.c, max(e0, 0), head, x.key);
     x.at1 = page_row(a.c, max(e1, 0), head, x.key + 16);
     return x;
   };
   auto issue = [&](const char* pool, const Tile& x, unsigned dst, const int (&goff)[HALF]) {
-    load_half(pool + x.at0, dst, goff);
-    load_half(pool + x.at1, dst + TILE / 2, goff);
+    load_half_tile(pool + x.at0, dst, goff);
+    load_half_tile(pool + x.at1, dst + TILE / 2, goff);
   };
   auto issue_k = [&](const Tile& x) { issue(a.c.k, x, my_lds, goff_k); };
   auto issue_v = [&](const Tile& x) { issue(a.c.v, x, my_lds + TILE, goff_v); };

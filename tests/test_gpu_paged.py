@@ -252,6 +252,23 @@ def test_weights(lens, news, window, sinks, causal):
         assert torch.equal(again, 1 + scores)
 
 
+@pytest.mark.parametrize("dtype,dim,heads,hkv,page", [("bf16", 128, 8, 2, 16), ("fp16", 64, 3, 3, 64)])
+@pytest.mark.parametrize("lens,news,window,sinks,causal", [((1100,), (1100,), 0, 0, True), ((1100, 90, 700), (300, 1, 700), 0, 0, True), ((900, 513), (800, 513), 130, 70, True),
+                                                           ((1500, 40), (257, 200), 0, 0, False), ((333, 1290), (333, 129), 1, 0, True)])
+def test_weights_of_long_chunks(dtype, dim, heads, hkv, page, lens, news, window, sinks, causal):
+    c = Case(dtype, dim, heads, hkv, page, lens, news, window=window, sinks=sinks, causal=causal, seed=33)
+    c.table[0, 2] = -1
+    plan = plan_for(c)
+    gpu = on_gpu(c)
+    _, lse = plan.forward(c.q.cuda(), *gpu)
+    scores = torch.zeros(c.pages, hkv, page, device="cuda")
+    plan.weights(c.q.cuda(), lse, gpu[0], *gpu[2:], scores)
+    clean = Case(dtype, dim, heads, hkv, page, lens, news, window=window, sinks=sinks, causal=causal, seed=33, spare=0.0)
+    clean.table[0, 2] = -1
+    w, off = ref.weights(clean, lse.cpu())
+    near(scores, w, off, "scores")
+
+
 def test_weights_of_missing_pages_and_rows_that_saw_nothing():
     c = Case("bf16", 64, 4, 2, 16, (100, 40), (5, 60), seed=21)   # 20 rows of the second see nothing
     c.table[0, 2] = -1
@@ -314,6 +331,41 @@ def test_evict(kind, lens, budget, first, last):
                 if there[j]:
                     k[to, h, row], v[to, h, row], s[to, h, row] = k[at[j], h, j % page], v[at[j], h, j % page], s[at[j], h, j % page]
     assert torch.equal(gk.cpu(), k) and torch.equal(gv.cpu(), v) and torch.equal(gs.cpu().view(torch.int32), s.view(torch.int32))
+
+
+@pytest.mark.parametrize("kind", ["exp", "ties", "zeros", "odd", "tiny"])
+@pytest.mark.parametrize("lens,budget,first,last,heads", [((21000, 30001), 5000, 4, 100, 1), ((9000, 70), 60, 3, 7, 4), ((40000,), 39999, 0, 0, 2),
+                                                          ((33333, 9, 8200), 8192, 0, 8190, 2), ((12345,), 10, 5, 5, 1)])
+def test_evict_of_long_sequences(kind, lens, budget, first, last, heads):
+    """Selections that several workgroups share."""
+    page = 64
+    c = Case("bf16", 64, heads, heads, page, (0,) * len(lens), (0,) * len(lens), spare=0.0)
+    need = [-(-n // page) for n in lens]
+    order = torch.randperm(sum(need), generator=torch.Generator().manual_seed(31)).int()
+    c.lens, c.pages = list(lens), sum(need)
+    c.table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        c.table[b, :n] = order[sum(need[:b]):sum(need[:b]) + n]
+    c.table[0, 17] = c.pages + 10 ** 6
+    kept_pages = -(-budget // page)
+    pages = c.pages + len(lens) * kept_pages
+    kept_table = (torch.arange(len(lens) * kept_pages, dtype=torch.int32) + c.pages).reshape(len(lens), -1)
+    k = torch.randn(pages, heads, page, 64, device="cuda").bfloat16()
+    v, scores = torch.randn_like(k), fill_scores(c, kind, 32)
+    s = torch.cat([scores, torch.zeros(pages - c.pages, heads, page)]).cuda()
+    k2, v2, s2 = k.clone(), v.clone(), s.clone()
+    kept, kept_lens = plan_for(c).evict(k, v, s, c.table.cuda(), c.kv_lens().cuda(), kept_table.cuda(), budget, first, last)
+    for b, n in enumerate(lens):
+        at = torch.tensor([-1 if c.row(b, j) is None else c.row(b, j) for j in range(n)], dtype=torch.long)
+        for h in range(heads):
+            places = ref.kept(scores[at.clamp(min=0), h, torch.arange(n) % page], at >= 0, budget, first, last)
+            assert kept[b, h].tolist() == places + [-1] * (budget - len(places)), (b, h)
+            i, j = torch.arange(len(places)), torch.tensor(places)
+            i, j = i[at[j] >= 0], j[at[j] >= 0]
+            to, row = kept_table[b].long()[i // page], i % page
+            for x in (k2, v2, s2):
+                x[to, h, row] = x[at[j], h, j % page]
+    assert torch.equal(k, k2) and torch.equal(v, v2) and torch.equal(s.view(torch.int32), s2.view(torch.int32))
 
 
 @pytest.mark.parametrize("page", [16, 64])
