@@ -14,6 +14,7 @@ namespace paged {
 
 constexpr int kKeyTile = 32;      // keys of a tile
 constexpr int kFewRows = 32;      // query rows of a workgroup of paged_split_kernel
+constexpr int kManyRows = 256;    // ... of paged_walk_kernel
 constexpr int kMaxBatch = 4096;   // sequences of a call
 
 struct Cache {
@@ -161,6 +162,7 @@ template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_plac
       const int first = slots_before + of(slots_upto) - of(slots);
       p.tile = MERGE ? r : r / p.splits;
       p.split = MERGE ? 0 : r - p.tile * p.splits;
+      p.tile = of(tiles) - 1 - p.tile;  // the rows that see most first
       p.slot = first + p.tile * p.splits;
       return true;
     }
@@ -190,6 +192,66 @@ static __device__ __forceinline__ void store_row(const AttendArgs& a, const Seq&
     Store8<DT>::st(to + c8 * 16, o);
   }
   if (c8 == 0) a.lse[(int64_t)q_head * a.c.tokens + s.start + token] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// The same for a 32-row block of a wave's accumulators (O^T: lane (n, h) has four columns of every eight of row n), as store_block
+// stores it: rows [row0, r_last] of a sequence's KV head, 64 contiguous bytes of 16 rows at a time.
+template <int DT, int D>
+static __device__ __forceinline__ void store_rows(const AttendArgs& a, const Seq& s, int head, int row0, int r_last, const f32x16 (&acc)[D / 32],
+                                                  float l, float ms) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+  auto at = [&](int r, char* base, int64_t ts, int64_t hs) {
+    const int token = quotient(r, a.by_group);
+    return base + (s.start + token) * ts + (head * a.group + r - token * a.group) * hs;
+  };
+  if (a.out_fp32) {
+    if (row0 + n <= r_last) {
+      char* to = at(row0 + n, a.out, a.o_ts, a.o_hs) + 16 * h;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *(f32x4*)(to + 128 * db + 32 * q4) = f32x4{acc[db][4 * q4] * inv, acc[db][4 * q4 + 1] * inv, acc[db][4 * q4 + 2] * inv, acc[db][4 * q4 + 3] * inv};
+    }
+  } else {
+    const int r = row0 + (lane & 15), c = 2 * ((lane >> 4) & 1) + (lane >> 5);  // row (and row + 16), 16-byte piece of the 64
+    char* p0 = at(min(r, r_last), a.out, a.o_ts, a.o_hs) + 16 * c;
+    char* p1 = at(min(r + 16, r_last), a.out, a.o_ts, a.o_hs) + 16 * c;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      u32x4 x, y;  // columns [0, 8) + 8 h, and 16 further on
+      auto pack = [&](int e) {
+        typedef typename Elem<DT>::type T;
+        typedef T T2 __attribute__((ext_vector_type(2)));
+        const T2 v = {(T)(acc[db][e] * inv), (T)(acc[db][e + 1] * inv)};
+        return __builtin_bit_cast(unsigned, v);
+      };
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4& t = k == 0 ? x : y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto z = __builtin_amdgcn_permlane32_swap(pack(8 * k + 2 * i), pack(8 * k + 4 + 2 * i), false, false);
+          t[i] = z[0];
+          t[2 + i] = z[1];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const auto z = __builtin_amdgcn_permlane16_swap(x[e], y[e], false, false);
+        x[e] = z[0];
+        y[e] = z[1];
+      }
+      if (r <= r_last) *(u32x4*)(p0 + 64 * db) = x;
+      if (r + 16 <= r_last) *(u32x4*)(p1 + 64 * db) = y;
+    }
+  }
+  if (h == 0 && row0 + n <= r_last) {
+    const int token = quotient(row0 + n, a.by_group), q_head = head * a.group + row0 + n - token * a.group;
+    a.lse[(int64_t)q_head * a.c.tokens + s.start + token] = l == 0.f ? -INFINITY : (ms + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  }
 }
 
 // The pages of a wave's next 64 key tiles, a lane a tile: of its first 16 keys, of the 16 behind them; -1 where there is none.
@@ -232,7 +294,9 @@ template <int HALF> static __device__ __forceinline__ void load_half_tile(const 
 }
 
 hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
-hipError_t launch_paged_merge(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
+hipError_t launch_paged_walk(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
+// `rows`: of a row tile, kFewRows or kManyRows
+hipError_t launch_paged_merge(const AttendArgs& a, int rows, int dtype, int dim, int64_t places, hipStream_t stream);
 
 struct AppendArgs {
   Cache c;

@@ -31,10 +31,14 @@ inline bool plan_ok(const ringattn_paged_plan* pl) {
 }
 inline bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// Sequences of up to so many rows of a KV head go to paged_split_kernel, 32 rows a workgroup; those of more to paged_walk_kernel, 256.
+constexpr int kSplitRows = 128;
 // Workgroups that the key tiles of a launch are shared out to, and the fewest tiles of one.
-constexpr int kSplitWorkgroups = 1024, kSplitLeast = 8;
-// Row tiles whose keys are shared out leave no more than 2 kSplitWorkgroups sums: k > 1 shares where at least k / 2 are due (splits_of).
-constexpr int64_t kSplitSlots = 2 * kSplitWorkgroups + 16;
+constexpr int kSplitWorkgroups = 1024, kSplitLeast = 8, kWalkWorkgroups = 256, kWalkLeast = 8;
+// Row tiles whose keys are shared out leave no more than two sums for each of those: k > 1 shares where at least k / 2 are due (splits_of).
+constexpr int64_t kSplitSlots = 2 * kSplitWorkgroups + 16, kWalkSlots = 2 * kWalkWorkgroups + 16;
+// Rows of sums: of the two kernels of a call, one after the other.
+constexpr int64_t kSlotRows = kSplitSlots * rp::kFewRows > kWalkSlots * rp::kManyRows ? kSplitSlots * rp::kFewRows : kWalkSlots * rp::kManyRows;
 
 int validate(const ringattn_paged_params* p) {
   if (!p) return RINGATTN_ERR_NULL;
@@ -52,8 +56,8 @@ int validate(const ringattn_paged_params* p) {
   return RINGATTN_OK;
 }
 
-size_t split_o_bytes(int dim) { return (size_t)kSplitSlots * rp::kFewRows * dim * sizeof(float); }
-size_t workspace_bytes(int dim) { return split_o_bytes(dim) + (size_t)kSplitSlots * rp::kFewRows * sizeof(float2); }
+size_t part_o_bytes(int dim) { return (size_t)kSlotRows * dim * sizeof(float); }
+size_t workspace_bytes(int dim) { return part_o_bytes(dim) + (size_t)kSlotRows * sizeof(float2); }
 
 // The sequences of a call.
 int check_cache(const ringattn_paged_plan* pl, const ringattn_paged_cache* c, bool needs_v, bool needs_starts) {
@@ -211,7 +215,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.out = (char*)out;
   a.lse = lse;
   a.part_o = (float*)plan->ws;
-  a.part_s = (float2*)((char*)plan->ws + split_o_bytes(plan->p.dim));
+  a.part_s = (float2*)((char*)plan->ws + part_o_bytes(plan->p.dim));
   a.q_ts = q_token_stride * 2;
   a.q_hs = q_head_stride * 2;
   a.o_ts = out_token_stride * (fp32 ? 4 : 2);
@@ -225,16 +229,29 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
   a.out_fp32 = fp32;
-  a.rows_above = 0;
-  a.rows_upto = INT32_MAX;
-  a.workgroups = kSplitWorkgroups;
-  a.least_tiles = kSplitLeast;
-  // row tiles of any lengths: every sequence with new tokens begins one, and 32 rows more another
-  const int64_t sequences = cache->batch < tokens ? cache->batch : tokens;
-  const int64_t tiles = (int64_t)tokens * group / rp::kFewRows + sequences, shared = kSplitWorkgroups / kv + 1;
-  RP_HIP(rp::launch_paged_split(a, plan->p.dtype, plan->p.dim, (tiles + shared) * kv, stream));
-  // two shares and more of a row tile: there are no more such tiles than shares are due
-  RP_HIP(rp::launch_paged_merge(a, plan->p.dtype, plan->p.dim, (tiles < shared ? tiles : shared) * kv, stream));
+  // Row tiles of any lengths: every sequence with rows begins one, and as many rows more as a tile has another; two shares and more of a
+  // row tile: there are no more such tiles than shares are due.
+  const int64_t rows = (int64_t)tokens * group, sequences = cache->batch < tokens ? cache->batch : tokens;
+  if (sequences > 1 || rows <= kSplitRows) {
+    a.rows_above = 0;
+    a.rows_upto = kSplitRows;
+    a.workgroups = kSplitWorkgroups;
+    a.least_tiles = kSplitLeast;
+    const int64_t most = sequences * (kSplitRows / rp::kFewRows), shared = kSplitWorkgroups / kv + 1;
+    const int64_t tiles = rows / rp::kFewRows + sequences < most ? rows / rp::kFewRows + sequences : most;
+    RP_HIP(rp::launch_paged_split(a, plan->p.dtype, plan->p.dim, (tiles + shared) * kv, stream));
+    RP_HIP(rp::launch_paged_merge(a, rp::kFewRows, plan->p.dtype, plan->p.dim, (tiles < shared ? tiles : shared) * kv, stream));
+  }
+  if (rows > kSplitRows) {
+    a.rows_above = kSplitRows;
+    a.rows_upto = INT32_MAX;
+    a.workgroups = kWalkWorkgroups;
+    a.least_tiles = kWalkLeast;
+    const int64_t with_many = rows / (kSplitRows + 1) < sequences ? rows / (kSplitRows + 1) : sequences;
+    const int64_t tiles = rows / rp::kManyRows + with_many, shared = kWalkWorkgroups / kv + 1;
+    RP_HIP(rp::launch_paged_walk(a, plan->p.dtype, plan->p.dim, (tiles + shared) * kv, stream));
+    RP_HIP(rp::launch_paged_merge(a, rp::kManyRows, plan->p.dtype, plan->p.dim, (tiles < shared ? tiles : shared) * kv, stream));
+  }
   return RINGATTN_OK;
 }
 

@@ -138,7 +138,7 @@ template <int DT, int D> struct WeightRows {
     for (int e = 0; e < 16; ++e) {
       const int k = key0 + 8 * (e >> 2) + (e & 3) + 4 * h;
       const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
-      w[e] += k >= lim || (k <= low && k >= a.sinks) ? 0.f : x;
+      w[e] += bool((k >= lim) | ((k <= low) & (k >= a.sinks))) ? 0.f : x;  // (no branches)
     }
   }
   // Every key has one owner, which adds to its score once: no order to go by, and nothing to wait for.
@@ -596,6 +596,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   unsigned digit = 0;
   if constexpr (PASS > 0) {
     unsigned c0 = 0, c1 = 0;
+#pragma unroll 8
     for (int s = 0; s < slices; ++s) {
       const uint2 c = *counts_of(s, PASS - 1);
       c0 += c.y;
@@ -622,6 +623,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   } else {
     // of the slices in front: tokens that rank above, and those that rank the same
     unsigned above = 0, equal = 0;
+#pragma unroll 8
     for (int s = 0; s < slice; ++s) above += above_digit(s);
     for (int i = tid; i < slice * kPasses; i += kSelectThreads) above += i % kPasses < kPasses - 1 ? pair_above[i] : 0;
     for (int s = tid; s < slice; s += kSelectThreads) equal += pair_counts[(s * kPasses + kPasses - 1) * kBins + digit];

@@ -150,7 +150,7 @@ __global__ __launch_bounds__(512, 2) void paged_split_kernel(const AttendArgs a)
   };
   auto hidden = [&](const Tile& x, int e, int hh) {  // of accumulator e of a lane of half hh: is its key hidden from this lane's row?
     const int key = x.key + 8 * (e >> 2) + (e & 3) + 4 * hh;
-    return key >= lim || (key <= low && key >= a.sinks) || (x.gone >> (e >> 3) & 1);
+    return bool((key >= lim) | ((key <= low) & (key >= a.sinks)) | (x.gone >> (e >> 3) & 1));  // (no branches)
   };
 
   int u = u_begin + wave;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(512, 2) void paged_split_kernel(const AttendArgs a)
     if (masked) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (hidden(cur, e, h)) sacc[e] = -INFINITY;
+        sacc[e] = hidden(cur, e, h) ? -INFINITY : sacc[e];
     }
     // exponentials against the reference as it stands; the row maximum is only looked at when a sum of four of them is above
     // 2^14 (or not a number)
@@ -327,8 +327,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const AttendArgs a) {
   Place p;
   const int unit = quotient(blockIdx.x, a.by_kv_heads);
   const int head = blockIdx.x - unit * a.kv_heads;
-  if (!find_place<ROWS, true>(a, unit, p)) return;
-  const int r0 = p.tile * ROWS, count = min(ROWS, p.s.n * a.group - r0);
+  constexpr int BLOCKS = ROWS / 32;  // a workgroup has 32 rows of a row tile
+  const int block = unit % BLOCKS * 32;
+  if (!find_place<ROWS, true>(a, unit / BLOCKS, p)) return;
+  const int r0 = p.tile * ROWS + block, count = min(32, p.s.n * a.group - r0);
   int at_once = 1;  // rows at once; the groups of threads left share a row's shares
   while (at_once < count && at_once < GROUPS) at_once *= 2;
   const int parts = GROUPS / at_once;
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const AttendArgs a) {
     for (int e = 0; e < 8; ++e) o[e] = 0.f;
     if (r < count) {
       auto fetch = [&](int s, float2& st, f32x4& x0, f32x4& x1) {
-        const int64_t prow = ((int64_t)(p.slot + s) * a.kv_heads + head) * ROWS + r;
+        const int64_t prow = ((int64_t)(p.slot + s) * a.kv_heads + head) * ROWS + block + r;
         st = a.part_s[prow];
         const float* src = a.part_o + prow * D + c8 * 8;
         x0 = *(const f32x4*)src;
@@ -405,14 +407,21 @@ hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t p
   return hipGetLastError();
 }
 
-hipError_t launch_paged_merge(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream) {
+hipError_t launch_paged_merge(const AttendArgs& a, int rows, int dtype, int dim, int64_t places, hipStream_t stream) {
   if (places <= 0) return hipSuccess;
+  places *= rows / 32;
   if (places > INT32_MAX) return hipErrorInvalidValue;
   const unsigned grid = (unsigned)places;
-  if (dtype == 0 && dim == 64) paged_merge_kernel<0, 64, kFewRows><<<grid, 256, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 64) paged_merge_kernel<1, 64, kFewRows><<<grid, 256, 0, stream>>>(a);
-  else if (dtype == 0 && dim == 128) paged_merge_kernel<0, 128, kFewRows><<<grid, 256, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 128) paged_merge_kernel<1, 128, kFewRows><<<grid, 256, 0, stream>>>(a);
+#define RA_LAUNCH_MERGE(DT_, D_)                                                                       \
+  do {                                                                                                \
+    if (rows == kFewRows) paged_merge_kernel<DT_, D_, kFewRows><<<grid, 256, 0, stream>>>(a);          \
+    else paged_merge_kernel<DT_, D_, kManyRows><<<grid, 256, 0, stream>>>(a);                          \
+  } while (0)
+  if (dtype == 0 && dim == 64) RA_LAUNCH_MERGE(0, 64);
+  else if (dtype == 1 && dim == 64) RA_LAUNCH_MERGE(1, 64);
+  else if (dtype == 0 && dim == 128) RA_LAUNCH_MERGE(0, 128);
+  else if (dtype == 1 && dim == 128) RA_LAUNCH_MERGE(1, 128);
+#undef RA_LAUNCH_MERGE
   else return hipErrorInvalidValue;
   return hipGetLastError();
 }

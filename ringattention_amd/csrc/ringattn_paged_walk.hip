@@ -1,0 +1,402 @@
+// gfx950 (CDNA4) kernel: attention of many new tokens over a paged cache.
+//
+//   paged_walk_kernel : 256 query rows (tokens x heads of a group) of one KV head of a sequence and a share of the key tiles that they
+//       see; eight waves of 32 rows, S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMAs, K and V HBM -> LDS in 32-key tiles through two
+//       rings of four, one barrier per two tiles.  As in ring_walk_kernel the two waves of a SIMD take turns: while one has its
+//       products the other has its softmax.
+//
+// What the pages add: a wave's 1 KB of a tile lies in one page, whose number a lane looked up for it 64 tiles at a time, and a tile's place is
+// a product more; all rows of a page are memory of the pool, so the last tile of a sequence is read whole and masked.
+#include "ringattn_paged.h"
+
+namespace ringattn {
+namespace paged {
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void paged_walk_kernel(const AttendArgs a) {
+  using E = Elem<DT>;
+  constexpr int WAVES = 8, BM = kManyRows, BN = kKeyTile, NBUF = 4;
+  constexpr int CPR = D / 8, ROWB = D * 2, TILE = BN * ROWB, KS = D / 16, DB = D / 32;
+  constexpr int PIECES = TILE / 1024;  // 1 KB wave-loads per tile: 8 at d = 128, 4 at d = 64
+  constexpr float kLazyLog2 = 8.f;
+  static_assert(BM == 32 * WAVES, "one 32-row block per wave");
+  static_assert(PIECES == WAVES || 2 * PIECES == WAVES, "a tile is loaded by all waves, or K and V by half of them each");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * NBUF * TILE];
+
+  const unsigned smem_base = lds_offset(smem);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+
+  Place p;
+  const int unit = quotient(blockIdx.x, a.by_kv_heads);
+  const int head = blockIdx.x - unit * a.kv_heads;
+  if (!find_place<BM, false>(a, unit, p)) return;
+  const int rows = p.s.n * a.group;
+  const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
+  const Keys keys = keys_of(p.s, quotient(r0, a.by_group), quotient(r_last, a.by_group), a.causal, a.window, a.sinks);
+  const int u_begin = (int)((int64_t)p.split * keys.count / p.splits);
+  const int n_tiles = (int)((int64_t)(p.split + 1) * keys.count / p.splits) - u_begin;  // of this share: tile t is tile u_begin + t
+
+  // this lane's row; rows beyond the range read the last valid one
+  const int row = min(r0 + 32 * wave + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
+  const int before = p.s.len - p.s.n;
+  // What the masks and other seldom taken paths are worked out from: the compiler would keep all of it in registers through every tile.
+  auto fresh = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto first_key = [&](int t) { return (u_begin + t < keys.sink_tiles ? u_begin + t : u_begin + t + keys.skip) * BN; };
+  auto tile_of = [&](int real) { return (real < keys.sink_tiles ? real : max(keys.sink_tiles, real - keys.skip)) - u_begin; };
+  // tiles of this wave that may need a mask: from t_up on, and below t_low
+  int t_up, t_low = 0;
+  {
+    const int i0 = quotient(min(r0 + 32 * wave, r_last), a.by_group), i1 = quotient(min(r0 + 32 * wave + 31, r_last), a.by_group);
+    t_up = __builtin_amdgcn_readfirstlane(tile_of(max(0, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
+    if (a.window > 0 && before + i1 - a.window >= 0) t_low = __builtin_amdgcn_readfirstlane(tile_of((before + i1 - a.window) / BN + 1));
+  }
+
+  s16x8 qf[KS];
+  {
+    const char* qrow = a.q + (p.s.start + token) * a.q_ts + q_head * a.q_hs + h * 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(qrow + ks * 32);
+  }
+  // the 1 KB piece of a tile this wave loads: all waves a piece of K and of V each (d = 128), or waves 0-3 the K tile and waves 4-7 the V
+  // tile (d = 64)
+  const int piece = PIECES == WAVES ? wave : wave & (PIECES - 1);
+  const int piece_row = piece * (1024 / ROWB);
+  int goff_k, goff_v;
+  {
+    const int r = lane / CPR, c = lane % CPR;
+    goff_k = r * a.c.token_stride + ((c ^ k_swizzle<D>(piece_row + r)) << 4);
+    goff_v = r * a.c.token_stride + ((c ^ v_swizzle<D>(piece_row + r)) << 4);
+  }
+  int koff[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  int voff[DB];
+  {
+    const int s = lane & 15, g1 = (lane >> 4) & 1;
+    const int row8 = 4 * h + (s >> 2);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int c = 2 * (2 * db + g1) + ((s & 3) >> 1);
+      voff[db] = row8 * ROWB + ((c ^ v_swizzle<D>(row8)) << 4) + ((s & 1) << 3);
+    }
+  }
+
+  // ---- pages: of the 64 tiles that the loads are at and the 64 before them (K runs ahead of V, and the loads of the masks)
+  const int* table = a.c.table + (int64_t)p.b * a.c.table_stride;
+  int held = -1, page_now = -1, page_prev = -1;               // which 64 tiles; the pages of this wave's piece of them
+  uint64_t gone0 = 0, gone1 = 0, gone0_prev = 0, gone1_prev = 0;  // tiles whose first, second 16 keys have no page
+  auto hold = [&](int block) {
+    HeldPages x;
+    const int mine = 64 * block + fresh(lane);
+    const bool there = mine < n_tiles;
+    x.hold(a.c, table, first_key(mine), there);
+    page_prev = page_now;
+    gone0_prev = gone0;
+    gone1_prev = gone1;
+    page_now = max(0, piece_row < 16 ? x.page0 : x.page1);  // page 0 is read in the place of one that is not there, and hidden
+    gone0 = __builtin_amdgcn_ballot_w64(there && x.page0 < 0);
+    gone1 = __builtin_amdgcn_ballot_w64(there && x.page1 < 0);
+    held = block;
+  };
+  auto hold_for = [&](int t) {  // before the loads of the tiles up to t, at most 63 past those that are held
+    if (min(t, n_tiles - 1) >> 6 > held) hold(held + 1);
+  };
+  auto piece_at = [&](int t) -> int64_t {  // from the start of the pool
+    t = min(t, n_tiles - 1);  // loads past the last tile read it again
+    const int page = __builtin_amdgcn_readlane(t >> 6 == held ? page_now : page_prev, t & 63);
+    return page_row(a.c, page, head, first_key(t) + piece_row);
+  };
+  auto scalar = [](const char* x) {  // (it is, but the compiler holds it in vector registers where scalar ones run out)
+    const uint64_t u = (uint64_t)x;
+    return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)u) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32);
+  };
+  auto issue_k = [&](int t) {
+    if (PIECES < WAVES && wave >= PIECES) return;
+    load_lds_16_settled(scalar(a.c.k + piece_at(t)), goff_k, __builtin_amdgcn_readfirstlane(smem_base + (t & (NBUF - 1)) * TILE + piece * 1024));
+  };
+  auto issue_v = [&](int t) {
+    if (PIECES < WAVES && wave < PIECES) return;
+    load_lds_16_settled(scalar(a.c.v + piece_at(t)), goff_v, __builtin_amdgcn_readfirstlane(smem_base + (NBUF + (t & (NBUF - 1))) * TILE + piece * 1024));
+  };
+  auto gone_of = [&](int t) {
+    const uint64_t g0 = t >> 6 == held ? gone0 : gone0_prev, g1 = t >> 6 == held ? gone1 : gone1_prev;
+    return (int)(g0 >> (t & 63) & 1) | (int)(g1 >> (t & 63) & 1) << 1;
+  };
+  auto any_gone = [&]() { return ((gone0 | gone1) | (gone0_prev | gone1_prev)) != 0; };
+  auto may_be_masked = [&](int t) { return t >= t_up || t < t_low || any_gone(); };
+  // which keys this lane's row sees: those below `lim` that are above `low`, or sinks
+  struct Sight {
+    int lim, low;
+  };
+  auto sight = [&]() {
+    const int t = fresh(token);
+    return Sight{a.causal ? min(p.s.len, before + t + 1) : p.s.len, a.window > 0 ? before + t - a.window : -1};
+  };
+  auto hidden = [&](const Sight& x, int key0, int gone, int e, int hh) {  // is the key of accumulator e of a lane of half hh hidden?
+    const int key = key0 + 8 * (e >> 2) + (e & 3) + 4 * hh;
+    return bool((key >= x.lim) | ((key <= x.low) & (key >= a.sinks)) | (gone >> (e >> 3) & 1));  // (no branches)
+  };
+
+  float m = -INFINITY;  // reference max (raw score units)
+  float ms = 0.f;       // m * k2, 0 while m is -inf
+  float ls[2] = {0.f, 0.f};
+  f32x16 oacc[DB], sacc;  // sacc: scores of the tile in flight, written by an MFMA phase, consumed by the next softmax phase
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+  s16x8 pf[2];  // its probabilities in B-operand layout
+
+  auto qk = [&](int kslot) {
+    const unsigned char* ks_lds = smem + kslot * TILE;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sacc = E::mma(*(const s16x8*)(ks_lds + koff[ks]), qf[ks], sacc);
+  };
+  auto mask_tile = [&](int t) {
+    if (!may_be_masked(t)) return;
+    const int key0 = first_key(t), gone = gone_of(t), half = fresh(lane) >> 5;
+    const Sight x = sight();
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      sacc[e] = hidden(x, key0, gone, e, half) ? -INFINITY : sacc[e];
+  };
+  // The reference moves when some row's tile maximum is far above it (or it is unset): until then exponentials may exceed 1, by 2^kLazyLog2.
+  auto move_reference = [&]() {
+    float m0 = m, m1 = m;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      m0 = fmaxf(fmaxf(m0, sacc[e]), sacc[e + 1]);
+      m1 = fmaxf(fmaxf(m1, sacc[e + 2]), sacc[e + 3]);
+    }
+    const float cand = cross_half_max(fmaxf(m0, m1));
+    if (__builtin_amdgcn_ballot_w64((cand - m) * a.scale_log2 > kLazyLog2) != 0) {
+      const float cs = (cand == -INFINITY) ? 0.f : cand * a.scale_log2;
+      const float alpha = __builtin_amdgcn_exp2f(m * a.scale_log2 - cs);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ls[i] *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
+      m = cand;
+      ms = cs;
+    }
+  };
+  // P = exp2(S k2 - m k2); the sums from the unrounded values, the operands of the next product rounded to the storage type: no more than
+  // the output's own rounding
+  auto softmax_phase = [&]() {
+    move_reference();
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      typename E::vec8 pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], a.scale_log2, -ms));
+        ls[e & 1] += x;
+        pv[e] = (typename E::type)x;
+      }
+      pf[t2] = __builtin_bit_cast(s16x8, pv);
+    }
+  };
+  // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where a masked tile's V holds such a value, the product is
+  // taken key by key, over the visible ones.
+  auto odd_values = [&](int t, int vslot) {
+    if (!may_be_masked(t)) return false;
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    constexpr unsigned kExp = DT == 0 ? 0x7c007c00u : 0x7f807f80u, kOne = DT == 0 ? 0x04000400u : 0x00800080u;
+    unsigned top = 0;
+#pragma unroll 1
+    for (int i = 0; i < PIECES; ++i) {
+      const u32x4 x = *(const u32x4*)(smem + (NBUF + vslot) * TILE + 1024 * i + 16 * fresh(lane));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top |= (x[e] & kExp) + kOne;  // an exponent of ones carries into the sign's place
+    }
+    return __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) != 0;
+  };
+  auto pv_by_key = [&](int t, int vslot) {
+    const int key0 = first_key(t), gone = gone_of(t);
+    const Sight sees = sight();
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {
+      float mine = 0.f;
+#pragma unroll
+      for (int f = 0; f < 16; ++f) {
+        const float x = (float)__builtin_bit_cast(typename E::vec8, pf[f >> 3])[f & 7];
+        mine = e == f ? x : mine;
+      }
+      float of_lower = mine, of_upper = mine;
+      swap_halves(of_lower, of_upper);
+#pragma unroll 1
+      for (int hh = 0; hh < 2; ++hh) {
+        if (hidden(sees, key0, gone, e, hh)) continue;
+        const float w = hh ? of_upper : of_lower;
+        const int half = fresh(lane) >> 5;
+        const int key = 8 * (e >> 2) + (e & 3) + 4 * hh;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const typename E::vec4 x =
+                *(const typename E::vec4*)(smem + (NBUF + vslot) * TILE + key * ROWB + (((4 * db + q4) ^ v_swizzle<D>(key)) << 4) + 8 * half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[db][4 * q4 + i] = __builtin_fmaf(w, (float)x[i], oacc[db][4 * q4 + i]);
+          }
+      }
+    }
+  };
+  auto phase_fence = [&]() { __builtin_amdgcn_sched_barrier(0); };  // keeps the compiler from mixing the phases
+  // The MFMA phase of a tile: O += P(t) V(t), then S(t+1) = K(t+1) Q^T, eight fragment reads ahead of the MFMAs that consume them.
+  auto mfma_phase = [&](int vslot, int kslot) __attribute__((always_inline)) {
+    phase_fence();
+    const unsigned char* vs_lds = smem + (NBUF + vslot) * TILE;
+    const unsigned char* ks_lds = smem + kslot * TILE;
+    s16x8 vfr[2 * DB], kfr[KS];
+    s16x4 half_frag{};
+    auto read = [&](int i) {  // halves of the V^T fragments in the order of their MFMAs; then the K fragments
+      if (i < 4 * DB) {
+        const int f = i / 2;
+        const unsigned char* src = vs_lds + 16 * (f / DB) * ROWB + 8 * (i & 1) * ROWB + voff[f % DB];
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src));
+        if (i & 1) vfr[f] = __builtin_shufflevector(half_frag, x, 0, 1, 2, 3, 4, 5, 6, 7);
+        else half_frag = x;
+      } else if (i < 4 * DB + KS) {
+        kfr[i - 4 * DB] = *(const s16x8*)(ks_lds + koff[i - 4 * DB]);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) read(i);
+    phase_fence();
+#pragma unroll
+    for (int f = 0; f < 2 * DB; ++f) {
+      oacc[f % DB] = E::mma(vfr[f], pf[f / DB], oacc[f % DB]);
+      phase_fence();
+      read(8 + 2 * f);
+      read(9 + 2 * f);
+      phase_fence();
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
+  };
+  auto ring_barrier = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+
+  // The walk, for one half of the workgroup.  At the start of block t the waves of the first half hold P(t), those of the second half the
+  // raw scores S(t).  Block t: the even ones start with the barrier of the pair (t, t+1) -- K(t+1), K(t+2), V(t), V(t+1), issued during
+  // the previous pair, have landed, and every wave is past block t-1, so the ring slots of K(t-1), K(t), V(t-2), V(t-1) are free
+  // for K(t+3), K(t+4), V(t+2), V(t+3), which are issued during this pair -- then
+  //     first half :  O += P(t) V(t), S(t+1) = K(t+1) Q^T  |  softmax of S(t+1)
+  //     second half:  softmax of S(t)                      |  O += P(t) V(t), S(t+1) = K(t+1) Q^T
+  // Groups of four tiles that need no mask have their ring slots at compile time; the others, and the last few, go tile by tile.
+  auto walk = [&](auto second_c) __attribute__((always_inline)) {
+    constexpr bool SECOND = decltype(second_c)::value;
+    auto issue_loads = [&](int t, bool even) __attribute__((always_inline)) {
+      if (even) {
+        issue_k(t + 3);
+        issue_k(t + 4);
+      } else {
+        issue_v(t + 1);
+        issue_v(t + 2);
+      }
+    };
+    auto plain_block = [&](auto slot_c, int t) __attribute__((always_inline)) {
+      constexpr int SLOT = decltype(slot_c)::value;  // t mod 4
+      if ((SLOT & 1) == 0) ring_barrier();
+      if (SECOND) issue_loads(t, (SLOT & 1) == 0);
+      phase_fence();
+      if (!SECOND) mfma_phase(SLOT, (SLOT + 1) & 3);
+      else softmax_phase();
+      phase_fence();
+      if (!SECOND) issue_loads(t, (SLOT & 1) == 0);
+      phase_fence();
+      if (!SECOND) softmax_phase();
+      else mfma_phase(SLOT, (SLOT + 1) & 3);
+      phase_fence();
+    };
+    auto masked_block = [&](int t) __attribute__((always_inline)) {
+      hold_for(t + 4);
+      if ((t & 1) == 0) ring_barrier();
+      if (SECOND) {
+        issue_loads(t, (t & 1) == 0);
+        softmax_phase();
+      }
+      phase_fence();
+      if (odd_values(t, t & 3)) {
+        pv_by_key(t, t & 3);
+        qk((t + 1) & 3);
+      } else {
+        mfma_phase(t & 3, (t + 1) & 3);
+      }
+      phase_fence();
+      mask_tile(t + 1);
+      if (!SECOND) {
+        issue_loads(t, (t & 1) == 0);
+        if (t + 1 < n_tiles) softmax_phase();  // (the scores past the last tile are of nothing)
+      }
+      phase_fence();
+    };
+    mask_tile(0);
+    if (!SECOND) softmax_phase();
+    for (int t = 0; t < n_tiles;) {
+      // block t has the products of tile t and the scores of tile t + 1
+      if (t + 4 < min(n_tiles, t_up) && t >= t_low && !any_gone()) {
+        hold_for(t + 6);
+        plain_block(std::integral_constant<int, 0>{}, t);
+        plain_block(std::integral_constant<int, 1>{}, t + 1);
+        plain_block(std::integral_constant<int, 2>{}, t + 2);
+        plain_block(std::integral_constant<int, 3>{}, t + 3);
+        t += 4;
+      } else {
+        const int end = min(t + 4, n_tiles);
+#pragma unroll 1
+        for (; t < end; ++t) masked_block(t);
+      }
+    }
+  };
+  if (n_tiles > 0) {
+    hold(0);
+    issue_k(0);
+    issue_k(1);
+    issue_k(2);
+    issue_v(0);
+    issue_v(1);
+    __builtin_amdgcn_s_waitcnt(0);  // retire the Q loads with a wait the compiler can see (and the tiles)
+    ring_barrier();
+    qk(0);
+    if (wave < WAVES / 2) walk(std::false_type{});
+    else walk(std::true_type{});
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // re-reads of the last tile
+  }
+
+  const float l = cross_half_sum(ls[0] + ls[1]);
+  if (p.splits > 1) {
+    const int64_t prow = ((int64_t)(p.slot + p.split) * a.kv_heads + head) * BM + 32 * wave;
+    store_block<2, D>(oacc, 1.f, (char*)(a.part_o + prow * D), D * 4, r_last + 1 - r0 - 32 * wave);
+    if (h == 0 && r0 + 32 * wave + n <= r_last) a.part_s[prow + n] = float2{l == 0.f ? -INFINITY : ms, l};
+    return;
+  }
+  store_rows<DT, D>(a, p.s, head, r0 + 32 * wave, r_last, oacc, l, ms);
+}
+
+hipError_t launch_paged_walk(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream) {
+  if (places <= 0) return hipSuccess;
+  if (places > INT32_MAX) return hipErrorInvalidValue;
+  const unsigned grid = (unsigned)places;
+  if (dtype == 0 && dim == 64) paged_walk_kernel<0, 64><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 64) paged_walk_kernel<1, 64><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 0 && dim == 128) paged_walk_kernel<0, 128><<<grid, 512, 0, stream>>>(a);
+  else if (dtype == 1 && dim == 128) paged_walk_kernel<1, 128><<<grid, 512, 0, stream>>>(a);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace ringattn

@@ -20,9 +20,9 @@ def params(dim=64, heads=8, kv_heads=2, dtype=0, scale=0.0, page_size=16, max_ba
 @pytest.fixture()
 def memory():
     """(aligned address, bytes) of host memory that stands in for a workspace and tensors: nothing of it is touched."""
-    x = np.zeros(80 << 20, dtype=np.uint8)
+    x = np.zeros(160 << 20, dtype=np.uint8)
     base = x.ctypes.data + (-x.ctypes.data % 16)
-    yield base, (80 << 20) - 16
+    yield base, (160 << 20) - 16
     del x
 
 
