@@ -14,7 +14,7 @@ TORCH_LIB_PATH = os.path.join(PKG_DIR, "libringattn_torch.so")
 CALLS_PATH = os.path.join(PKG_DIR, "ringattn_calls.so")
 
 SOURCES = ["ringattn_kernels.hip", "ringattn_walk.hip", "ringattn_steps.hip", "ringattn_thin.hip", "ringattn_dealt.hip", "ringattn_walk64.hip", "ringattn_pair.hip", "ringattn_split.hip", "ringattn_split_steps.hip", "ringattn_split_columns.hip", "ringattn_api.hip",
-           "ringattn_paged_split.hip", "ringattn_paged_walk.hip", "ringattn_paged_cache.hip", "ringattn_paged_api.hip", "ringattn_datagen.cpp"]
+           "ringattn_paged_attend.hip", "ringattn_paged_cache.hip", "ringattn_paged_api.hip", "ringattn_datagen.cpp"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_*_f32 out of scalar float code.
 HIPCC_FLAGS = [
@@ -59,6 +59,8 @@ def library_sources():
     return [os.path.join(CSRC, s) for s in SOURCES] + [os.path.join(CSRC, "ringattn_kernels.h"), os.path.join(CSRC, "ringattn_jobs.h"), os.path.join(CSRC, "ringattn_news.h"), os.path.join(CSRC, "ringattn_device.h"),
                                                        os.path.join(CSRC, "ringattn_walk_rows.h"),
                                                        os.path.join(CSRC, "ringattn_paged.h"),
+                                                       os.path.join(CSRC, "ringattn_paged_few.h"),
+                                                       os.path.join(CSRC, "ringattn_paged_many.h"),
                                                        os.path.join(CSRC, "ringattn_split_rows.h"),
                                                        os.path.join(CSRC, "ringattn_walk64_loop.inc"),
                                                        os.path.join(CSRC, "ringattn_walk64_loop_d64.inc"),

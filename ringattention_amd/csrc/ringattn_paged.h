@@ -13,8 +13,12 @@ namespace ringattn {
 namespace paged {
 
 constexpr int kKeyTile = 32;      // keys of a tile
-constexpr int kFewRows = 32;      // query rows of a workgroup of paged_split_kernel
-constexpr int kManyRows = 256;    // ... of paged_walk_kernel
+constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence's KV head has few of them (ringattn_paged_few.h)
+constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
+constexpr int kFewRowsMost = 128; // few: up to so many (ringattn_paged_fwd says when more)
+constexpr int kFewWorkgroups = 256, kFewLeast = 16;                     // see few_rows
+constexpr int kManyWorkgroups = 256, kManyLeast = 8;  // see find_place
+constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kMaxBatch = 4096;   // sequences of a call
 
 struct Cache {
@@ -31,22 +35,29 @@ struct Cache {
   int batch, tokens;    // sequences; new tokens at most (rows of q)
 };
 
+// What row tiles whose keys went to several workgroups leave to be put together.
+struct Parts {
+  float* o;       // sums of a part's rows
+  float2* stat;   // their references (log2 units) and the sums of their weights
+  int* arrived;   // few rows: how many parts of a row tile are there; 0 between launches
+};
+
 struct AttendArgs {
   Cache c;
   const char* q;
   char* out;
   float* lse;             // [heads, tokens]
-  float* part_o;          // [slots, rows of a tile, D]
-  float2* part_s;         // [slots, rows of a tile]: reference (log2 units), sum
   int64_t q_ts, q_hs, o_ts, o_hs;  // bytes between tokens, between heads
   int kv_heads, group;
   Divisor by_group, by_kv_heads;
   float scale_log2;
   int causal, window, sinks;
   int out_fp32;
-  int rows_above, rows_upto;  // a launch has the sequences with rows_above < rows <= rows_upto
-  float workgroups;           // the key tiles of a launch are shared out to about so many workgroups
-  int least_tiles;            // ... of so many key tiles at least
+  int few_most;           // rows of a sequence's KV head up to which it has few
+  int many_cut;           // whether key tiles are shared out where there are many rows
+  int few_shift;          // few rows: key tiles are dealt out 2^few_shift at a time, so that 2^30 suffice
+  int few_workgroups;     // the launch's first workgroups have the sequences of few rows, the others those of many
+  Parts few, many;
 };
 
 struct Seq {
@@ -86,58 +97,61 @@ static __device__ __forceinline__ Keys keys_of(const Seq& s, int i0, int i1, int
   return k;
 }
 
-// What a sequence brings to a launch: row tiles, and the most key tiles that one of them sees.
-template <int ROWS> static __device__ __forceinline__ void load_of(const AttendArgs& a, const Seq& s, int& tiles, int& keys) {
+// What a sequence brings to a launch: row tiles of few or of many rows, and the most key tiles that one of them sees.
+template <bool MANY> static __device__ __forceinline__ void load_of(const AttendArgs& a, const Seq& s, int& tiles, int& keys) {
+  constexpr int ROWS = MANY ? kManyRows : kFewRows;
   const int rows = s.n * a.group;
-  tiles = rows > a.rows_above && rows <= a.rows_upto ? (rows + ROWS - 1) / ROWS : 0;
+  tiles = (rows > a.few_most) == MANY ? (rows + ROWS - 1) / ROWS : 0;
   keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks).count;
   if (a.window > 0) {  // a row tile sees no more than its own window, wherever that begins, and the first tokens
     const int most = (a.window + ROWS - 1 + kKeyTile - 1) / kKeyTile + 1 + (a.sinks + kKeyTile - 1) / kKeyTile;
     keys = min(keys, most);
   }
+  keys = max(keys, 1);  // rows that see nothing are written too
 }
 
-// The shares that a launch cuts the key tiles of a row tile into: so many that the whole launch makes about a.workgroups
-// workgroups, each of a.least_tiles tiles at least.
-static __device__ __forceinline__ int splits_of(const AttendArgs& a, int keys, float share) {
-  return max(1, (int)ceilf(keys / fmaxf(share, (float)a.least_tiles)));
+// Inclusive sums over the lanes of a wave: within rows of 16 lanes, then from row to row.
+static __device__ __forceinline__ int wave_scan(int x) {
+  auto plus = [&](auto ctrl, auto rows) { x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, true); };
+  using all = std::integral_constant<int, 0xf>;
+  plus(std::integral_constant<int, 0x111>{}, all{});  // row_shr:1
+  plus(std::integral_constant<int, 0x112>{}, all{});
+  plus(std::integral_constant<int, 0x114>{}, all{});
+  plus(std::integral_constant<int, 0x118>{}, all{});
+  plus(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // lane 15 of rows 0 and 2 to rows 1 and 3
+  plus(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to rows 2 and 3
+  return x;
 }
-
-template <class T> static __device__ __forceinline__ T wave_sum(T x) {
+static __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+static __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
   return x;
 }
-static __device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
 
+// Many rows: the key tiles of a row tile are cut into even shares, so many that the whole launch makes about kManyWorkgroups workgroups,
+// each of kManyLeast tiles at least.
 struct Place {
   Seq s;
   int b;
   int tile, split, splits;  // row tile, which share of its key tiles of how many
-  int slot;                 // where the partial of the row tile's first share lies (splits > 1)
+  int slot;                 // where the part of the row tile's first share lies (splits > 1)
 };
-// The place-th unit of work of a KV head.  MERGE: units are row tiles whose keys were shared out; else the shares themselves.  Every
-// wave works it out for itself, a lane a sequence, so that there is no barrier.  False beyond the last.
-template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
+// The place-th share of a KV head; MERGE: the place-th row tile that was cut.  Every wave works it out for itself, a lane a sequence, so that
+// there is no barrier.  False beyond the last.
+template <bool MERGE> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
   const int lane = threadIdx.x & 63;
   float total = 0.f;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
     float work = 0.f;
     if (b0 + lane < a.c.batch) {
       int tiles, keys;
-      load_of<ROWS>(a, seq_of(a.c, b0 + lane), tiles, keys);
+      load_of<true>(a, seq_of(a.c, b0 + lane), tiles, keys);
       work = (float)tiles * (float)keys;
     }
     total += wave_sum(work);
   }
-  const float share = total * a.kv_heads / a.workgroups;
+  const float share = fmaxf(total * a.kv_heads / kManyWorkgroups, (float)kManyLeast);
   int before = 0, slots_before = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
     Seq s{0, 0, 0};
@@ -145,12 +159,11 @@ template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_plac
     if (b0 + lane < a.c.batch) {
       int keys;
       s = seq_of(a.c, b0 + lane);
-      load_of<ROWS>(a, s, tiles, keys);
-      splits = splits_of(a, keys, share);
+      load_of<true>(a, s, tiles, keys);
+      splits = a.many_cut ? max(1, (int)ceilf(keys / share)) : 1;
     }
-    const int slots = splits > 1 ? tiles * splits : 0;
-    const int units = MERGE ? (splits > 1 ? tiles : 0) : tiles * splits;
-    const int upto = wave_scan(units, lane), slots_upto = wave_scan(slots, lane);
+    const int shares = tiles * splits, slots = splits > 1 ? shares : 0, units = !MERGE ? shares : splits > 1 ? tiles : 0;
+    const int upto = wave_scan(units), slots_upto = wave_scan(slots);
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(before + upto > place);
     if (beyond) {
       const int l = __builtin_ctzll(beyond);
@@ -162,8 +175,8 @@ template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_plac
       const int first = slots_before + of(slots_upto) - of(slots);
       p.tile = MERGE ? r : r / p.splits;
       p.split = MERGE ? 0 : r - p.tile * p.splits;
-      p.tile = of(tiles) - 1 - p.tile;  // the rows that see most first
       p.slot = first + p.tile * p.splits;
+      p.tile = of(tiles) - 1 - p.tile;  // the rows that see most first
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -171,6 +184,26 @@ template <int ROWS, bool MERGE> static __device__ __forceinline__ bool find_plac
   }
   return false;
 }
+
+// Parts go from workgroup to workgroup, which may sit on different XCDs with an L2 each: they are written through to and read from what all
+// XCDs share (relaxed atomics of agent scope, eight bytes each).  With plain accesses and fences instead, every fence writes back
+// an L2: one token over 128 K, 16 heads 202 us with 256 workgroups, 248 with 1024.
+static __device__ __forceinline__ void put8(void* to, uint64_t x) {
+  __hip_atomic_store((uint64_t*)to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+static __device__ __forceinline__ uint64_t get8(const void* from) {
+  return __hip_atomic_load((const uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+static __device__ __forceinline__ void put_part(float* to, const f32x4& x) {
+  put8(to, __builtin_bit_cast(uint64_t, float2{x[0], x[1]}));
+  put8(to + 2, __builtin_bit_cast(uint64_t, float2{x[2], x[3]}));
+}
+static __device__ __forceinline__ f32x4 get_part4(const float* from) {
+  const float2 x = __builtin_bit_cast(float2, get8(from)), y = __builtin_bit_cast(float2, get8(from + 2));
+  return f32x4{x.x, x.y, y.x, y.y};
+}
+static __device__ __forceinline__ void put_stat(float2* to, const float2& x) { put8(to, __builtin_bit_cast(uint64_t, x)); }
+static __device__ __forceinline__ float2 get_stat(const float2* from) { return __builtin_bit_cast(float2, get8(from)); }
 
 // Byte offset of row `key` of a page's KV head from the start of the pool.
 static __device__ __forceinline__ int64_t page_row(const Cache& c, int page, int head, int key) {
@@ -195,9 +228,9 @@ static __device__ __forceinline__ void store_row(const AttendArgs& a, const Seq&
 }
 
 // The same for a 32-row block of a wave's accumulators (O^T: lane (n, h) has four columns of every eight of row n), as store_block
-// stores it: rows [row0, r_last] of a sequence's KV head, 64 contiguous bytes of 16 rows at a time.
-template <int DT, int D>
-static __device__ __forceinline__ void store_rows(const AttendArgs& a, const Seq& s, int head, int row0, int r_last, const f32x16 (&acc)[D / 32],
+// stores it: rows [row0, r_last] of a sequence's KV head, 64 contiguous bytes of 16 rows at a time; NB 32-column blocks from db0 on.
+template <int DT, int NB>
+static __device__ __forceinline__ void store_rows(const AttendArgs& a, const Seq& s, int head, int row0, int r_last, const f32x16 (&acc)[NB], int db0,
                                                   float l, float ms) {
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
@@ -208,19 +241,19 @@ static __device__ __forceinline__ void store_rows(const AttendArgs& a, const Seq
   };
   if (a.out_fp32) {
     if (row0 + n <= r_last) {
-      char* to = at(row0 + n, a.out, a.o_ts, a.o_hs) + 16 * h;
+      char* to = at(row0 + n, a.out, a.o_ts, a.o_hs) + 128 * db0 + 16 * h;
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
           *(f32x4*)(to + 128 * db + 32 * q4) = f32x4{acc[db][4 * q4] * inv, acc[db][4 * q4 + 1] * inv, acc[db][4 * q4 + 2] * inv, acc[db][4 * q4 + 3] * inv};
     }
   } else {
     const int r = row0 + (lane & 15), c = 2 * ((lane >> 4) & 1) + (lane >> 5);  // row (and row + 16), 16-byte piece of the 64
-    char* p0 = at(min(r, r_last), a.out, a.o_ts, a.o_hs) + 16 * c;
-    char* p1 = at(min(r + 16, r_last), a.out, a.o_ts, a.o_hs) + 16 * c;
+    char* p0 = at(min(r, r_last), a.out, a.o_ts, a.o_hs) + 64 * db0 + 16 * c;
+    char* p1 = at(min(r + 16, r_last), a.out, a.o_ts, a.o_hs) + 64 * db0 + 16 * c;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
+    for (int db = 0; db < NB; ++db) {
       u32x4 x, y;  // columns [0, 8) + 8 h, and 16 further on
       auto pack = [&](int e) {
         typedef typename Elem<DT>::type T;
@@ -248,7 +281,7 @@ static __device__ __forceinline__ void store_rows(const AttendArgs& a, const Seq
       if (r + 16 <= r_last) *(u32x4*)(p1 + 64 * db) = y;
     }
   }
-  if (h == 0 && row0 + n <= r_last) {
+  if (db0 == 0 && h == 0 && row0 + n <= r_last) {
     const int token = quotient(row0 + n, a.by_group), q_head = head * a.group + row0 + n - token * a.group;
     a.lse[(int64_t)q_head * a.c.tokens + s.start + token] = l == 0.f ? -INFINITY : (ms + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
   }
@@ -279,24 +312,25 @@ template <int D, class Swizzle> static __device__ __forceinline__ void half_tile
     goff[j] = r * token_stride - 1024 * j + (((lane % (D / 8)) ^ swizzle(r)) << 4);
   }
 }
+// Non-temporal: these rows are read once, and what all compute units have on the way at a time is as large as L2 (us with and without: 48
+// sequences of some 4 K tokens, 16/4 heads 74.8, 84.4; one of 128 K, 16 heads 190.6, 198.9).
 template <int HALF> static __device__ __forceinline__ void load_half_tile(const char* base, unsigned dst, const int (&goff)[HALF]) {
   if constexpr (HALF == 4)
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-        "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\t"
+        "global_load_lds_dwordx4 %3, %5 offset:2048 nt\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072 nt" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
         "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base)
         : "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt" ::"s"(
                      __builtin_amdgcn_readfirstlane(dst)),
                  "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)
                  : "m0");
 }
 
-hipError_t launch_paged_split(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
-hipError_t launch_paged_walk(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream);
-// `rows`: of a row tile, kFewRows or kManyRows
-hipError_t launch_paged_merge(const AttendArgs& a, int rows, int dtype, int dim, int64_t places, hipStream_t stream);
+// A launch of a.few_workgroups workgroups and `many_places` more for each KV head; a.many_cut: and one that puts together the row tiles
+// whose keys were shared out, of which there are up to `cut_tiles`.
+hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream);
 
 struct AppendArgs {
   Cache c;

@@ -31,14 +31,7 @@ inline bool plan_ok(const ringattn_paged_plan* pl) {
 }
 inline bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-// Sequences of up to so many rows of a KV head go to paged_split_kernel, 32 rows a workgroup; those of more to paged_walk_kernel, 256.
-constexpr int kSplitRows = 128;
-// Workgroups that the key tiles of a launch are shared out to, and the fewest tiles of one.
-constexpr int kSplitWorkgroups = 1024, kSplitLeast = 8, kWalkWorkgroups = 256, kWalkLeast = 8;
-// Row tiles whose keys are shared out leave no more than two sums for each of those: k > 1 shares where at least k / 2 are due (splits_of).
-constexpr int64_t kSplitSlots = 2 * kSplitWorkgroups + 16, kWalkSlots = 2 * kWalkWorkgroups + 16;
-// Rows of sums: of the two kernels of a call, one after the other.
-constexpr int64_t kSlotRows = kSplitSlots * rp::kFewRows > kWalkSlots * rp::kManyRows ? kSplitSlots * rp::kFewRows : kWalkSlots * rp::kManyRows;
+constexpr int kTokensEach = 4;
 
 int validate(const ringattn_paged_params* p) {
   if (!p) return RINGATTN_ERR_NULL;
@@ -56,8 +49,14 @@ int validate(const ringattn_paged_params* p) {
   return RINGATTN_OK;
 }
 
-size_t part_o_bytes(int dim) { return (size_t)kSlotRows * dim * sizeof(float); }
-size_t workspace_bytes(int dim) { return part_o_bytes(dim) + (size_t)kSlotRows * sizeof(float2); }
+// The workspace: counters, which are 0 between calls; then the parts of row tiles that several workgroups share.  A call that selects tokens
+// to keep has its counts where the parts lie.
+constexpr size_t kCounterBytes = (rp::kFewWorkgroups * sizeof(int) + 255) & ~(size_t)255;
+size_t few_stat_bytes() { return (size_t)rp::kFewSlots * rp::kFewRows * sizeof(float2); }
+size_t many_stat_bytes() { return (size_t)rp::kManySlots * rp::kManyRows * sizeof(float2); }
+size_t few_o_bytes(int dim) { return (size_t)rp::kFewSlots * rp::kFewRows * dim * sizeof(float); }
+size_t many_o_bytes(int dim) { return (size_t)rp::kManySlots * rp::kManyRows * dim * sizeof(float); }
+size_t workspace_bytes(int dim) { return kCounterBytes + few_stat_bytes() + many_stat_bytes() + few_o_bytes(dim) + many_o_bytes(dim); }
 
 // The sequences of a call.
 int check_cache(const ringattn_paged_plan* pl, const ringattn_paged_cache* c, bool needs_v, bool needs_starts) {
@@ -142,7 +141,17 @@ int ringattn_paged_plan_create(const ringattn_paged_params* params, void* worksp
   pl->page_shift = __builtin_ctz((unsigned)params->page_size);
   pl->ws = workspace;
   if (!workspace) {
-    const hipError_t e = hipMalloc(&pl->ws, need);
+    hipError_t e = hipMalloc(&pl->ws, need);
+    if (e == hipSuccess) {
+      hipStream_t own = nullptr;  // (a stream of its own: nothing else is waited for)
+      e = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
+      if (e == hipSuccess) {
+        e = hipMemsetAsync(pl->ws, 0, kCounterBytes, own);
+        if (e == hipSuccess) e = hipStreamSynchronize(own);
+        (void)hipStreamDestroy(own);
+      }
+      if (e != hipSuccess) (void)hipFree(pl->ws);
+    }
     if (e != hipSuccess) {
       delete pl;
       const int rc = ringattn::hip_failed(e);
@@ -214,8 +223,12 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.q = (const char*)q;
   a.out = (char*)out;
   a.lse = lse;
-  a.part_o = (float*)plan->ws;
-  a.part_s = (float2*)((char*)plan->ws + part_o_bytes(plan->p.dim));
+  char* ws = (char*)plan->ws;
+  a.few.arrived = (int*)ws;
+  a.few.stat = (float2*)(ws += kCounterBytes);
+  a.many.stat = (float2*)(ws += few_stat_bytes());
+  a.few.o = (float*)(ws += many_stat_bytes());
+  a.many.o = (float*)(ws += few_o_bytes(plan->p.dim));
   a.q_ts = q_token_stride * 2;
   a.q_hs = q_head_stride * 2;
   a.o_ts = out_token_stride * (fp32 ? 4 : 2);
@@ -229,29 +242,20 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
   a.out_fp32 = fp32;
-  // Row tiles of any lengths: every sequence with rows begins one, and as many rows more as a tile has another; two shares and more of a
-  // row tile: there are no more such tiles than shares are due.
   const int64_t rows = (int64_t)tokens * group, sequences = cache->batch < tokens ? cache->batch : tokens;
-  if (sequences > 1 || rows <= kSplitRows) {
-    a.rows_above = 0;
-    a.rows_upto = kSplitRows;
-    a.workgroups = kSplitWorkgroups;
-    a.least_tiles = kSplitLeast;
-    const int64_t most = sequences * (kSplitRows / rp::kFewRows), shared = kSplitWorkgroups / kv + 1;
-    const int64_t tiles = rows / rp::kFewRows + sequences < most ? rows / rp::kFewRows + sequences : most;
-    RP_HIP(rp::launch_paged_split(a, plan->p.dtype, plan->p.dim, (tiles + shared) * kv, stream));
-    RP_HIP(rp::launch_paged_merge(a, rp::kFewRows, plan->p.dtype, plan->p.dim, (tiles < shared ? tiles : shared) * kv, stream));
-  }
-  if (rows > kSplitRows) {
-    a.rows_above = kSplitRows;
-    a.rows_upto = INT32_MAX;
-    a.workgroups = kWalkWorkgroups;
-    a.least_tiles = kWalkLeast;
-    const int64_t with_many = rows / (kSplitRows + 1) < sequences ? rows / (kSplitRows + 1) : sequences;
-    const int64_t tiles = rows / rp::kManyRows + with_many, shared = kWalkWorkgroups / kv + 1;
-    RP_HIP(rp::launch_paged_walk(a, plan->p.dtype, plan->p.dim, (tiles + shared) * kv, stream));
-    RP_HIP(rp::launch_paged_merge(a, rp::kManyRows, plan->p.dtype, plan->p.dim, (tiles < shared ? tiles : shared) * kv, stream));
-  }
+  // Which sequences have few rows: where a call is made of single tokens, or of some at a time, all of them, so that no workgroup
+  // has to find out that there are no others, and nothing is launched for those.
+  a.few_most = sequences > 1 && tokens < kTokensEach * sequences ? INT32_MAX : rp::kFewRowsMost;
+  a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
+  // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
+  const int64_t few_tiles = rows / rp::kFewRows + sequences, see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile;
+  while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
+  // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute
+  // units their keys are not shared out; else there is a share each, and no more besides than are due.
+  const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < sequences ? might : sequences;
+  const int64_t tiles = with_many > 0 ? rows / rp::kManyRows + with_many : 0, due = rp::kManyWorkgroups / kv + 1;
+  a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < rp::kManyWorkgroups;
+  RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, tiles + (a.many_cut ? due : 0), tiles < due ? tiles : due, stream));
   return RINGATTN_OK;
 }
 
@@ -304,8 +308,8 @@ int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* 
   a.last = keep_last;
   a.kept = kept;
   a.kept_lens = kept_lens;
-  a.workspace = plan->ws;
-  a.workspace_bytes = workspace_bytes(plan->p.dim);
+  a.workspace = (char*)plan->ws + kCounterBytes;
+  a.workspace_bytes = workspace_bytes(plan->p.dim) - kCounterBytes;
   a.kv_heads = plan->kv_heads;
   RP_HIP(rp::launch_paged_evict(a, plan->p.dim, (hipStream_t)stream));
   return RINGATTN_OK;

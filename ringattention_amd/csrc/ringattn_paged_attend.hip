@@ -1,0 +1,40 @@
+// gfx950 (CDNA4) kernel: attention of new tokens over a paged cache (ringattn_paged_few.h and ringattn_paged_many.h hold the programs).
+//
+//   paged_attend_kernel : one launch for a whole batch.  Its first workgroups have the sequences of few query rows, a run of key tiles
+//       each; the others those of many, 256 rows each.  A batch may have both -- a chunk of one prompt beside the next tokens of other
+//       sequences --, and which sequences have how many rows only the device knows.
+#include "ringattn_paged_few.h"
+#include "ringattn_paged_many.h"
+
+namespace ringattn {
+namespace paged {
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void paged_attend_kernel(const AttendArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kFewLds<D> > kManyLds<D> ? kFewLds<D> : kManyLds<D>];
+  if ((int)blockIdx.x < a.few_workgroups) few_rows<DT, D>(a, smem, blockIdx.x);
+  else many_rows<DT, D>(a, smem, blockIdx.x - a.few_workgroups);
+}
+
+template <int DT, int D> __global__ __launch_bounds__(2 * D) void paged_merge_kernel(const AttendArgs a) { merge_many<DT, D>(a, blockIdx.x); }
+
+hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream) {
+  const int64_t blocks = a.few_workgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) : 0;
+  if (blocks <= 0) return hipSuccess;
+  if (blocks > INT32_MAX || merges > INT32_MAX) return hipErrorInvalidValue;
+#define RA_LAUNCH_ATTEND(DT_, D_)                                                                             \
+  do {                                                                                                       \
+    paged_attend_kernel<DT_, D_><<<(unsigned)blocks, 512, 0, stream>>>(a);                                    \
+    if (merges > 0) paged_merge_kernel<DT_, D_><<<(unsigned)merges, 2 * D_, 0, stream>>>(a);                  \
+  } while (0)
+  if (dtype == 0 && dim == 64) RA_LAUNCH_ATTEND(0, 64);
+  else if (dtype == 1 && dim == 64) RA_LAUNCH_ATTEND(1, 64);
+  else if (dtype == 0 && dim == 128) RA_LAUNCH_ATTEND(0, 128);
+  else if (dtype == 1 && dim == 128) RA_LAUNCH_ATTEND(1, 128);
+#undef RA_LAUNCH_ATTEND
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace ringattn

@@ -464,7 +464,7 @@ static __device__ __forceinline__ void count_digits(const EvictArgs& a, const in
 // higher one.  `shared`: room for a number of every wave and two more.
 static __device__ __forceinline__ void find_digit(unsigned c0, unsigned c1, int pass, Found& f, unsigned* shared) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = kBins - 1 - 2 * (int)threadIdx.x;
-  const int both = (int)(c0 + c1), upto = wave_scan(both, lane);
+  const int both = (int)(c0 + c1), upto = wave_scan(both);
   if (lane == 63) shared[wave] = upto;
   __syncthreads();
   int above = upto - both;
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   unsigned* pair_above = all_above + pair * slices * kPasses;
   auto counts_of = [&](int s, int pass) { return (const uint2*)(pair_counts + (s * kPasses + pass) * kBins + hi - 1); };  // .y: the higher value
   auto sum_of = [&](unsigned v) {  // over the workgroup
-    const unsigned w = wave_sum(v);
+    const unsigned w = (unsigned)wave_sum((int)v);
     if (lane == 0) shared[wave] = w;
     __syncthreads();
     unsigned t = 0;

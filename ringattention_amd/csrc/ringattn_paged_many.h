@@ -1,19 +1,20 @@
-// gfx950 (CDNA4) kernel: attention of many new tokens over a paged cache.
+// gfx950 (CDNA4): attention of many new tokens over a paged cache, the workgroup's program (ringattn_paged_attend.hip wraps it).
 //
-//   paged_walk_kernel : 256 query rows (tokens x heads of a group) of one KV head of a sequence and a share of the key tiles that they
-//       see; eight waves of 32 rows, S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMAs, K and V HBM -> LDS in 32-key tiles through two
-//       rings of four, one barrier per two tiles.  As in ring_walk_kernel the two waves of a SIMD take turns: while one has its
-//       products the other has its softmax.
+// 256 query rows (tokens x heads of a group) of one KV head of a sequence and a share of the key tiles that they see; eight waves of 32
+// rows, S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMAs, K and V HBM -> LDS in 32-key tiles through two rings of four, one barrier per
+// two tiles.  As in ring_walk_kernel the two waves of a SIMD take turns: while one has its products the other has its softmax.
 //
-// What the pages add: a wave's 1 KB of a tile lies in one page, whose number a lane looked up for it 64 tiles at a time, and a tile's place is
-// a product more; all rows of a page are memory of the pool, so the last tile of a sequence is read whole and masked.
+// What the pages add: a wave's 1 KB of a tile lies in one page, whose number a lane looked up for it 64 tiles at a time, and a tile's
+// place is a product more; all rows of a page are memory of the pool, so the last tile of a sequence is read whole and masked.
+#pragma once
 #include "ringattn_paged.h"
 
 namespace ringattn {
 namespace paged {
 
-template <int DT, int D>
-__global__ __launch_bounds__(512, 2) void paged_walk_kernel(const AttendArgs a) {
+template <int D> constexpr int kManyLds = 8 * kKeyTile * D * 2;
+
+template <int DT, int D> static __device__ __forceinline__ void many_rows(const AttendArgs& a, unsigned char* smem, int block) {
   using E = Elem<DT>;
   constexpr int WAVES = 8, BM = kManyRows, BN = kKeyTile, NBUF = 4;
   constexpr int CPR = D / 8, ROWB = D * 2, TILE = BN * ROWB, KS = D / 16, DB = D / 32;
@@ -21,7 +22,6 @@ __global__ __launch_bounds__(512, 2) void paged_walk_kernel(const AttendArgs a) 
   constexpr float kLazyLog2 = 8.f;
   static_assert(BM == 32 * WAVES, "one 32-row block per wave");
   static_assert(PIECES == WAVES || 2 * PIECES == WAVES, "a tile is loaded by all waves, or K and V by half of them each");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * NBUF * TILE];
 
   const unsigned smem_base = lds_offset(smem);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -29,9 +29,9 @@ __global__ __launch_bounds__(512, 2) void paged_walk_kernel(const AttendArgs a) 
   const int n = lane & 31, h = lane >> 5;
 
   Place p;
-  const int unit = quotient(blockIdx.x, a.by_kv_heads);
-  const int head = blockIdx.x - unit * a.kv_heads;
-  if (!find_place<BM, false>(a, unit, p)) return;
+  const int unit = quotient(block, a.by_kv_heads);
+  const int head = block - unit * a.kv_heads;
+  if (!find_place<false>(a, unit, p)) return;
   const int rows = p.s.n * a.group;
   const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
   const Keys keys = keys_of(p.s, quotient(r0, a.by_group), quotient(r_last, a.by_group), a.causal, a.window, a.sinks);
@@ -377,25 +377,47 @@ __global__ __launch_bounds__(512, 2) void paged_walk_kernel(const AttendArgs a) 
   }
 
   const float l = cross_half_sum(ls[0] + ls[1]);
-  if (p.splits > 1) {
-    const int64_t prow = ((int64_t)(p.slot + p.split) * a.kv_heads + head) * BM + 32 * wave;
-    store_block<2, D>(oacc, 1.f, (char*)(a.part_o + prow * D), D * 4, r_last + 1 - r0 - 32 * wave);
-    if (h == 0 && r0 + 32 * wave + n <= r_last) a.part_s[prow + n] = float2{l == 0.f ? -INFINITY : ms, l};
+  if (p.splits > 1) {  // as the registers lie: a wave's accumulators as 1 KB a store
+    const int64_t slot = (int64_t)(p.slot + p.split) * a.kv_heads + head;
+    float* to = a.many.o + (slot * WAVES + wave) * (32 * D) + lane * 4;
+#pragma unroll
+    for (int i = 0; i < DB * 4; ++i)
+      *(f32x4*)(to + 256 * i) = f32x4{oacc[i / 4][i % 4 * 4], oacc[i / 4][i % 4 * 4 + 1], oacc[i / 4][i % 4 * 4 + 2], oacc[i / 4][i % 4 * 4 + 3]};
+    if (h == 0) a.many.stat[slot * BM + 32 * wave + n] = float2{l == 0.f ? -INFINITY : ms, l};
     return;
   }
-  store_rows<DT, D>(a, p.s, head, r0 + 32 * wave, r_last, oacc, l, ms);
+  store_rows<DT, DB>(a, p.s, head, r0 + 32 * wave, r_last, oacc, 0, l, ms);
 }
 
-hipError_t launch_paged_walk(const AttendArgs& a, int dtype, int dim, int64_t places, hipStream_t stream) {
-  if (places <= 0) return hipSuccess;
-  if (places > INT32_MAX) return hipErrorInvalidValue;
-  const unsigned grid = (unsigned)places;
-  if (dtype == 0 && dim == 64) paged_walk_kernel<0, 64><<<grid, 512, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 64) paged_walk_kernel<1, 64><<<grid, 512, 0, stream>>>(a);
-  else if (dtype == 0 && dim == 128) paged_walk_kernel<0, 128><<<grid, 512, 0, stream>>>(a);
-  else if (dtype == 1 && dim == 128) paged_walk_kernel<1, 128><<<grid, 512, 0, stream>>>(a);
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+// The shares of a row tile added up in their order: a workgroup has the 32 rows of a wave of them, its waves 32 columns each.
+template <int DT, int D> static __device__ __forceinline__ void merge_many(const AttendArgs& a, int block) {
+  constexpr int BLOCKS = kManyRows / 32;
+  const int lane = threadIdx.x & 63, n = lane & 31, db = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Place p;
+  const int unit = quotient(block, a.by_kv_heads), head = block - unit * a.kv_heads, rows_of = unit % BLOCKS;
+  if (!find_place<true>(a, unit / BLOCKS, p)) return;
+  const int r0 = p.tile * kManyRows, r_last = min(r0 + kManyRows, p.s.n * a.group) - 1;
+  if (r0 + 32 * rows_of > r_last) return;
+  const int64_t slot = (int64_t)p.slot * a.kv_heads + head;  // of share 0; those of the others are kv_heads apart
+  float top = -INFINITY, l = 0.f;
+  f32x16 acc[1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t at = slot + (int64_t)s * a.kv_heads;
+    const float2 st = a.many.stat[at * kManyRows + 32 * rows_of + n];
+    const float* from = a.many.o + (at * BLOCKS + rows_of) * (32 * D) + db * 1024 + lane * 4;
+    f32x4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *(const f32x4*)(from + 256 * i);
+    const float t = fmaxf(top, st.x), keep = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t), w = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - t);
+    l = __builtin_fmaf(st.y, w, l * keep);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][e] = __builtin_fmaf(x[e / 4][e % 4], w, acc[0][e] * keep);
+    top = t;
+  }
+  store_rows<DT, 1>(a, p.s, head, r0 + 32 * rows_of, r_last, acc, db, l, top);
 }
 
 }  // namespace paged
