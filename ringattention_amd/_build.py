@@ -140,7 +140,7 @@ def build_torch_shim(verbose=False):
 
 
 def calls_sources():
-    return [os.path.join(CSRC, "ringattn_calls.cpp")]
+    return [os.path.join(CSRC, "ringattn_calls.cpp"), os.path.join(REPO_DIR, "include", "ringattn.h")]
 
 
 def build_calls():
@@ -157,7 +157,7 @@ def build_calls():
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    for inc in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]:
+    for inc in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], os.path.join(REPO_DIR, "include")]:
         cmd += ["-isystem", inc]
     cmd += [os.path.join(CSRC, "ringattn_calls.cpp"), "-o", tmp, "-L", torch_lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
             f"-Wl,-rpath,{torch_lib}"]

@@ -118,7 +118,8 @@ def load():
         fn.restype = restype
         fn.argtypes = argtypes
     # where the entry points lie that ringattn_calls calls
-    lib.addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ("ringattn_fwd", "ringattn_rank_step_fwd")}
+    lib.addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "ringattn_fwd", "ringattn_rank_step_fwd", "ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict")}
     _lib = lib
     return lib
 

@@ -72,8 +72,20 @@ class PagedAttention:
         ws_ptr, ws_bytes = (None, 0) if workspace is None else (ctypes.c_void_p(int(workspace[0])), int(workspace[1]))
         check(self.lib.ringattn_paged_plan_create(ctypes.byref(self.params), ws_ptr, ws_bytes, ctypes.byref(self.handle)),
               "ringattn_paged_plan_create")
+        # Checks and launch of a call with tensors of the caller's in native code (csrc/ringattn_calls.cpp), made when first asked for; it
+        # gives None where something is unusual, and the call then goes the general way.
+        calls = _lib.load_calls()
+        self._call_type = calls.Paged if calls and self.device is not None else None
+        self._native = {}
+
+    def _made(self, kind):
+        entry = self.lib.addresses[("ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict")[kind]]
+        self._native[kind] = call = self._call_type(entry, self.handle.value, kind, self.heads, self.kv_heads, self.dim, self.page_size,
+                                                    self.max_batch, self.max_tokens, self.device, self.torch_dtype, self.out_dtype)
+        return call
 
     def close(self):
+        self._call_type, self._native = None, {}
         if self.handle:
             check(self.lib.ringattn_paged_plan_destroy(self.handle), "ringattn_paged_plan_destroy")
             self.handle = ctypes.c_void_p()
@@ -150,6 +162,10 @@ class PagedAttention:
 
     def append(self, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores=None, stream=None):
         """Rows k, v [tokens, kv_heads, dim] of the new tokens into the cache, as the last of each sequence's kv_lens tokens; their scores to 0."""
+        if self._call_type:
+            rc = (self._native.get(0) or self._made(0))(k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores, stream)
+            if rc is not None:
+                return check(rc, "ringattn_paged_append")
         shape = self._tokens(k, "k", self.kv_heads)
         cache = self._cache(k_cache, v_cache, page_table, kv_lens, q_starts)
         _check_rows((k, "k", self.torch_dtype, shape), (v, "v", self.torch_dtype, shape))
@@ -165,6 +181,11 @@ class PagedAttention:
 
     def forward(self, q, k_cache, v_cache, page_table, kv_lens, q_starts, out=None, lse=None, stream=None):
         """Attention of the new tokens q [tokens, heads, dim] over the cache (their own rows are in it).  Returns (out, lse)."""
+        if out is not None and lse is not None and self._call_type:
+            rc = (self._native.get(1) or self._made(1))(q, k_cache, v_cache, page_table, kv_lens, q_starts, out, lse, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_fwd")
+                return out, lse
         shape = self._tokens(q, "q", self.heads)
         cache = self._cache(k_cache, v_cache, page_table, kv_lens, q_starts)
         _check_rows((q, "q", self.torch_dtype, shape))
@@ -186,6 +207,11 @@ class PagedAttention:
     def weights(self, q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream=None):
         """Adds to scores what forward(q, ...) that returned `lse` gave to every cached token: the sum of its attention weights over the
         new tokens and the query heads of each KV head.  Returns scores."""
+        if self._call_type:
+            rc = (self._native.get(2) or self._made(2))(q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_weights")
+                return scores
         shape = self._tokens(q, "q", self.heads)
         cache = self._cache(k_cache, None, page_table, kv_lens, q_starts)
         _check_rows((q, "q", self.torch_dtype, shape))
@@ -203,6 +229,12 @@ class PagedAttention:
         scores, for each KV head its own -- with their scores to the pages of kept_table, which are in none of page_table.
         Returns (kept, kept_lens): the places the tokens had [batch, kv_heads, budget], -1 behind the last, and the lengths that go with
         kept_table."""
+        if kept is not None and kept_lens is not None and self._call_type:
+            rc = (self._native.get(3) or self._made(3))(k_cache, v_cache, scores, page_table, kv_lens, kept_table, budget, keep_first, keep_last,
+                                                        kept, kept_lens, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_evict")
+                return kept, kept_lens
         batch, budget = page_table.shape[0], int(budget)
         if kept_table.dim() != 2 or kept_table.shape[0] != batch or kept_table.shape[1] * self.page_size < budget:
             raise ValueError(f"kept_table must be [{batch}, pages for {budget} tokens]")

@@ -503,6 +503,42 @@ def test_calls_on_another_stream_and_plans_side_by_side():
             assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
 
 
+def test_the_general_way_of_a_call_does_the_same():
+    """Calls are checked and made by ringattn_calls where everything is as expected; without it the same launches are made."""
+    c = Case("bf16", 64, 4, 2, 16, (61, 333, 0), (1, 140, 0), seed=34, spare=0.0)
+    g = torch.Generator().manual_seed(35)
+    new_k, new_v = (torch.randn(c.tokens, 2, 64, generator=g).bfloat16().cuda() for _ in range(2))
+    kept_table = torch.arange(c.pages - 2, c.pages, dtype=torch.int32).repeat(3, 1).cuda()[:, :2].contiguous()
+    results = []
+    for native in (True, False):
+        plan = plan_for(c)
+        if not native:
+            plan._call_type = None
+        k, v, table, lens, starts = on_gpu(c)
+        q = c.q.cuda()
+        scores = torch.zeros(c.pages, 2, 16, device="cuda")
+        plan.append(new_k, new_v, k, v, table, lens, starts, scores)
+        out, lse = torch.zeros_like(q), torch.zeros(4, c.tokens, device="cuda")
+        plan.forward(q, k, v, table, lens, starts, out, lse)
+        plan.weights(q, lse, k, table, lens, starts, scores)
+        kept, kept_lens = torch.zeros(3, 2, 20, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+        plan.evict(k[:, :, :], v, scores, table, lens, kept_table, 20, 2, 3, kept, kept_lens)
+        results.append((k[:-2], v[:-2], out, lse, scores[:-2], kept, kept_lens))
+        assert bool(plan._native) == native
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+    for bad in (q[:, :3], q.float(), q.cpu(), q.transpose(1, 2)):   # refused as the general way refuses them
+        with pytest.raises(ValueError):
+            plan_for(c).forward(bad, k, v, table, lens, starts, out, lse)
+    with pytest.raises(ValueError):
+        plan_for(c).weights(q, lse, k, table, lens, starts, scores.double())
+    plan = plan_for(c)
+    plan.append(new_k, new_v, k, v, table, lens, starts)
+    plan.close()
+    with pytest.raises(Exception, match="plan"):
+        plan.append(new_k, new_v, k, v, table, lens, starts)
+
+
 def test_nothing_to_do():
     plan = paged.PagedAttention(4, 64, kv_heads=2, dtype="fp16", page_size=16, max_batch=2, max_tokens=4)
     k = torch.zeros(3, 2, 16, 64, dtype=torch.float16, device="cuda")

@@ -160,6 +160,21 @@ def test_tensors_that_do_not_fit(memory):
     plan.close()
 
 
+def test_native_calls_leave_what_is_unusual_to_the_general_way():
+    calls = _lib.load_calls()
+    half = torch.float16
+    for bad in ((0, 1, 0, 8, 2, 64, 16, 4, 64, 0, half, half), (1, 1, 4, 8, 2, 64, 16, 4, 64, 0, half, half), (1, 1, 0, 8, 2, 64, 16, 4, 64, 0, 1, half), (1, 1)):
+        with pytest.raises((ValueError, TypeError)):
+            calls.Paged(*bad)
+    for kind, n in enumerate((9, 9, 8, 12)):
+        call = calls.Paged(1, 1, kind, 8, 2, 64, 16, 4, 64, 0, half, half)
+        for wrong in (n - 1, n + 1):
+            with pytest.raises(TypeError):
+                call(*(None,) * wrong)
+        assert call(*(None,) * n) is None
+        assert call(*(torch.zeros(1, 2, 16, 64, dtype=half),) * (n - 1), None) is None
+
+
 def test_the_reference_is_plain_attention():
     """paged_reference.attend on one sequence in order against a dense softmax; the weights sum to one a row."""
     c = ref.Case("bf16", 64, 4, 2, 16, (40, 3), (40, 5), seed=1)
