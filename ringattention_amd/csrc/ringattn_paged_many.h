@@ -72,9 +72,13 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     goff_k = r * a.c.token_stride + ((c ^ k_swizzle<D>(piece_row + r)) << 4);
     goff_v = r * a.c.token_stride + ((c ^ v_swizzle<D>(piece_row + r)) << 4);
   }
-  int koff[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) koff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  // a K fragment's offset: that of the first one with the number of its slice in bits that are free (one register, not eight)
+  const int koff0 = n * ROWB + ((h ^ k_swizzle<D>(n)) << 4);
+  auto koff = [&](int ks) {
+    int x = koff0;
+    if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(x) : "n"(32 * ks), "v"(koff0));
+    return x;
+  };
   int voff[DB];
   {
     const int s = lane & 15, g1 = (lane >> 4) & 1;
@@ -157,7 +161,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
 #pragma unroll
     for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) sacc = E::mma(*(const s16x8*)(ks_lds + koff[ks]), qf[ks], sacc);
+    for (int ks = 0; ks < KS; ++ks) sacc = E::mma(*(const s16x8*)(ks_lds + koff(ks)), qf[ks], sacc);
   };
   auto mask_tile = [&](int t) {
     if (!may_be_masked(t)) return;
@@ -265,7 +269,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
         if (i & 1) vfr[f] = __builtin_shufflevector(half_frag, x, 0, 1, 2, 3, 4, 5, 6, 7);
         else half_frag = x;
       } else if (i < 4 * DB + KS) {
-        kfr[i - 4 * DB] = *(const s16x8*)(ks_lds + koff[i - 4 * DB]);
+        kfr[i - 4 * DB] = *(const s16x8*)(ks_lds + koff(i - 4 * DB));
       }
     };
 #pragma unroll
@@ -295,7 +299,8 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   // for K(t+3), K(t+4), V(t+2), V(t+3), which are issued during this pair -- then
   //     first half :  O += P(t) V(t), S(t+1) = K(t+1) Q^T  |  softmax of S(t+1)
   //     second half:  softmax of S(t)                      |  O += P(t) V(t), S(t+1) = K(t+1) Q^T
-  // Groups of four tiles that need no mask have their ring slots at compile time; the others, and the last few, go tile by tile.
+  // Groups of four tiles that need no mask have their ring slots at compile time; the others, and the last few, go tile by tile, and so
+  // does everything behind a page that is not there.
   auto walk = [&](auto second_c) __attribute__((always_inline)) {
     constexpr bool SECOND = decltype(second_c)::value;
     auto issue_loads = [&](int t, bool even) __attribute__((always_inline)) {
@@ -345,21 +350,22 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     };
     mask_tile(0);
     if (!SECOND) softmax_phase();
-    for (int t = 0; t < n_tiles;) {
-      // block t has the products of tile t and the scores of tile t + 1
-      if (t + 4 < min(n_tiles, t_up) && t >= t_low && !any_gone()) {
-        hold_for(t + 6);
-        plain_block(std::integral_constant<int, 0>{}, t);
-        plain_block(std::integral_constant<int, 1>{}, t + 1);
-        plain_block(std::integral_constant<int, 2>{}, t + 2);
-        plain_block(std::integral_constant<int, 3>{}, t + 3);
-        t += 4;
-      } else {
-        const int end = min(t + 4, n_tiles);
+    // block t has the products of tile t and the scores of tile t + 1.  Three loops one after the other, not one with two ways through it:
+    // where two meet again the compiler has two sets of accumulators (64 moves a group, and registers in scratch)
+    int t = 0;
+    const int masked_first = min((max(t_low, 0) + 3) & ~3, n_tiles);
 #pragma unroll 1
-        for (; t < end; ++t) masked_block(t);
-      }
+    for (; t < masked_first; ++t) masked_block(t);
+#pragma unroll 1
+    for (; t + 4 < min(n_tiles, t_up) && !any_gone(); t += 4) {
+      hold_for(t + 6);
+      plain_block(std::integral_constant<int, 0>{}, t);
+      plain_block(std::integral_constant<int, 1>{}, t + 1);
+      plain_block(std::integral_constant<int, 2>{}, t + 2);
+      plain_block(std::integral_constant<int, 3>{}, t + 3);
     }
+#pragma unroll 1
+    for (; t < n_tiles; ++t) masked_block(t);
   };
   if (n_tiles > 0) {
     hold(0);
