@@ -124,9 +124,17 @@ static __device__ __forceinline__ int wave_scan(int x) {
 }
 static __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 static __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+  auto plus = [&](auto ctrl, auto rows) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, true));
+  };
+  using all = std::integral_constant<int, 0xf>;
+  plus(std::integral_constant<int, 0x111>{}, all{});
+  plus(std::integral_constant<int, 0x112>{}, all{});
+  plus(std::integral_constant<int, 0x114>{}, all{});
+  plus(std::integral_constant<int, 0x118>{}, all{});
+  plus(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  plus(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // Many rows: the key tiles of a row tile are cut into even shares, so many that the whole launch makes about kManyWorkgroups workgroups,
@@ -142,7 +150,7 @@ struct Place {
 template <bool MERGE> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
   const int lane = threadIdx.x & 63;
   float total = 0.f;
-  for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
+  for (int b0 = 0; a.many_cut && b0 < a.c.batch; b0 += 64) {
     float work = 0.f;
     if (b0 + lane < a.c.batch) {
       int tiles, keys;

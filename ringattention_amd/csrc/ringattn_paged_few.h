@@ -338,7 +338,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       bool odd = false;
       if (masked) {
         unsigned top = 0;
-#pragma unroll 1
+#pragma unroll 4
         for (int i = 0; i < TILE / 1024; ++i) {
           typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
           const u32x4 x = *(const u32x4*)(my + TILE + 1024 * i + 16 * lane);

@@ -12,7 +12,7 @@
 namespace ringattn {
 namespace paged {
 
-template <int D> constexpr int kManyLds = 8 * kKeyTile * D * 2;
+template <int D> constexpr int kManyLds = 8 * kKeyTile * D * 2 + 16;
 
 template <int DT, int D> static __device__ __forceinline__ void many_rows(const AttendArgs& a, unsigned char* smem, int block) {
   using E = Elem<DT>;
@@ -48,13 +48,19 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   };
   auto first_key = [&](int t) { return (u_begin + t < keys.sink_tiles ? u_begin + t : u_begin + t + keys.skip) * BN; };
   auto tile_of = [&](int real) { return (real < keys.sink_tiles ? real : max(keys.sink_tiles, real - keys.skip)) - u_begin; };
-  // tiles of this wave that may need a mask: from t_up on, and below t_low
-  int t_up, t_low = 0;
-  {
-    const int i0 = quotient(min(r0 + 32 * wave, r_last), a.by_group), i1 = quotient(min(r0 + 32 * wave + 31, r_last), a.by_group);
-    t_up = __builtin_amdgcn_readfirstlane(tile_of(max(0, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
-    if (a.window > 0 && before + i1 - a.window >= 0) t_low = __builtin_amdgcn_readfirstlane(tile_of((before + i1 - a.window) / BN + 1));
-  }
+  // tiles that may need a mask: from `up` on, and below `low`; of this wave's rows, and of all rows of the workgroup
+  struct Clear {
+    int up, low;
+  };
+  auto clear_of = [&](int first, int last) {
+    const int i0 = quotient(min(first, r_last), a.by_group), i1 = quotient(min(last, r_last), a.by_group);
+    Clear x;
+    x.up = __builtin_amdgcn_readfirstlane(tile_of(max(0, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
+    x.low = a.window > 0 && before + i1 - a.window >= 0 ? __builtin_amdgcn_readfirstlane(tile_of((before + i1 - a.window) / BN + 1)) : 0;
+    return x;
+  };
+  const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31), every = clear_of(r0, r_last);
+  const int t_up = mine.up, t_low = mine.low;
 
   s16x8 qf[KS];
   {
@@ -167,6 +173,12 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     if (!may_be_masked(t)) return;
     const int key0 = first_key(t), gone = gone_of(t), half = fresh(lane) >> 5;
     const Sight x = sight();
+    if (gone == 0 && key0 >= a.sinks) {  // the keys between `low` and `lim`, as one comparison each
+      const unsigned from = key0 + 4 * half - x.low - 1, count = max(0, x.lim - x.low - 1);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sacc[e] = from + (8 * (e >> 2) + (e & 3)) < count ? sacc[e] : -INFINITY;
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       sacc[e] = hidden(x, key0, gone, e, half) ? -INFINITY : sacc[e];
@@ -207,21 +219,21 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
       pf[t2] = __builtin_bit_cast(s16x8, pv);
     }
   };
-  // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where a masked tile's V holds such a value, the product is
-  // taken key by key, over the visible ones.
-  auto odd_values = [&](int t, int vslot) {
-    if (!may_be_masked(t)) return false;
+  // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where the V of a tile that some row has masked holds such
+  // a value, the products of masked tiles are taken key by key from there on, over the visible ones.  A wave looks at what it loaded
+  // itself, when it has arrived and in front of the barrier behind which the others use it.
+  int* odd_seen = (int*)(smem + 2 * NBUF * TILE);
+  auto look_at_v = [&](int t) {
+    if ((PIECES < WAVES && wave < PIECES) || t >= n_tiles || !(t >= every.up || t < every.low || any_gone())) return;
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     constexpr unsigned kExp = DT == 0 ? 0x7c007c00u : 0x7f807f80u, kOne = DT == 0 ? 0x04000400u : 0x00800080u;
+    const u32x4 x = *(const u32x4*)(smem + (NBUF + (t & (NBUF - 1))) * TILE + piece * 1024 + 16 * fresh(lane));
     unsigned top = 0;
-#pragma unroll 1
-    for (int i = 0; i < PIECES; ++i) {
-      const u32x4 x = *(const u32x4*)(smem + (NBUF + vslot) * TILE + 1024 * i + 16 * fresh(lane));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top |= (x[e] & kExp) + kOne;  // an exponent of ones carries into the sign's place
-    }
-    return __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) != 0;
+    for (int e = 0; e < 4; ++e) top |= (x[e] & kExp) + kOne;  // an exponent of ones carries into the sign's place
+    if (top & 0x80008000u) *odd_seen = 1;
   };
+  auto odd_values = [&](int t) { return may_be_masked(t) && __builtin_amdgcn_readfirstlane(*(volatile int*)odd_seen) != 0; };
   auto pv_by_key = [&](int t, int vslot) {
     const int key0 = first_key(t), gone = gone_of(t);
     const Sight sees = sight();
@@ -292,6 +304,13 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
+  // The same in front of tile t, whose V and the next one's it lets in: where masked blocks may follow in some wave.
+  auto looking_barrier = [&](int t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    look_at_v(t);
+    look_at_v(t + 1);
+    __syncthreads();
+  };
 
   // The walk, for one half of the workgroup.  At the start of block t the waves of the first half hold P(t), those of the second half the
   // raw scores S(t).  Block t: the even ones start with the barrier of the pair (t, t+1) -- K(t+1), K(t+2), V(t), V(t+1), issued during
@@ -328,13 +347,13 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     };
     auto masked_block = [&](int t) __attribute__((always_inline)) {
       hold_for(t + 4);
-      if ((t & 1) == 0) ring_barrier();
+      if ((t & 1) == 0) looking_barrier(t);
       if (SECOND) {
         issue_loads(t, (t & 1) == 0);
         softmax_phase();
       }
       phase_fence();
-      if (odd_values(t, t & 3)) {
+      if (odd_values(t)) {
         pv_by_key(t, t & 3);
         qk((t + 1) & 3);
       } else {
@@ -353,12 +372,14 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     // block t has the products of tile t and the scores of tile t + 1.  Three loops one after the other, not one with two ways through it:
     // where two meet again the compiler has two sets of accumulators (64 moves a group, and registers in scratch)
     int t = 0;
-    const int masked_first = min((max(t_low, 0) + 3) & ~3, n_tiles);
+    // (by the rows of the workgroup: what a wave does not mask itself it may have to look at for another)
+    const int masked_first = min((max(every.low, 0) + 3) & ~3, n_tiles);
 #pragma unroll 1
     for (; t < masked_first; ++t) masked_block(t);
 #pragma unroll 1
-    for (; t + 4 < min(n_tiles, t_up) && !any_gone(); t += 4) {
+    for (; t + 4 < min(n_tiles, every.up); t += 4) {
       hold_for(t + 6);
+      if (any_gone()) break;
       plain_block(std::integral_constant<int, 0>{}, t);
       plain_block(std::integral_constant<int, 1>{}, t + 1);
       plain_block(std::integral_constant<int, 2>{}, t + 2);
@@ -367,6 +388,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
 #pragma unroll 1
     for (; t < n_tiles; ++t) masked_block(t);
   };
+  if (tid == 0) *odd_seen = 0;
   if (n_tiles > 0) {
     hold(0);
     issue_k(0);

@@ -120,6 +120,35 @@ def test_pages_that_are_not_there():
     assert torch.equal(out, out2) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("lost", [2048, 2047, 2079, 4096, 31, 4000])
+@pytest.mark.parametrize("new", [1, 140])
+def test_a_page_that_is_not_there_far_into_a_sequence(lost, new):
+    """Around the places where the pages of the next 64 key tiles are looked up."""
+    c = Case("bf16", 64, 2, 1, 16, (4500,), (new,), seed=36)
+    c.table[0, lost // 16] = -1
+    check_forward(c)
+    c = Case("fp16", 128, 2, 1, 16, (4500,), (new,), seed=37)
+    c.table[0, lost // 16] = 2 ** 30
+    plan, _, lse = check_forward(c)
+    k, _, table, lens, starts = on_gpu(c)
+    scores = torch.zeros(c.pages, 1, 16, device="cuda")
+    plan.weights(c.q.cuda(), lse, k, table, lens, starts, scores)
+    clean = Case("fp16", 128, 2, 1, 16, (4500,), (new,), seed=37, spare=0.0)
+    clean.table[0, lost // 16] = -1
+    w, off = ref.weights(clean, lse.cpu())
+    near(scores, w, off, "scores")
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [4400, 4431, 4499])
+def test_odd_values_in_a_long_chunk(value, at):
+    """V of a new token that earlier ones of the chunk do not see, in every place of a tile's pair."""
+    for dtype, dim in (("bf16", 128), ("fp16", 64)):
+        c = Case(dtype, dim, 4, 2, 16, (4500,), (400,), seed=38)
+        c.v[c.row(0, at), :, at % 16, 3] = value
+        check_forward(c)
+
+
 def test_lengths_that_are_not_true_stay_within_the_tensors():
     """Lengths beyond the table, negative ones, starts beyond the tokens or descending: nothing is read or written outside."""
     c = Case("bf16", 64, 4, 2, 16, (60, 90, 40), (3, 40, 2), seed=14)
