@@ -360,6 +360,8 @@ struct WeightsArgs {
   Divisor by_group;
   float scale_log2;
   int causal, window, sinks;
+  int few_most;  // as in AttendArgs
+  int q_even;    // 32 rows are whole tokens, and lie within 2 GiB
 };
 hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream);
 

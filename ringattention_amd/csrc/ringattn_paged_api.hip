@@ -31,7 +31,9 @@ inline bool plan_ok(const ringattn_paged_plan* pl) {
 }
 inline bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-constexpr int kTokensEach = 4;
+// Rows of a KV head up to which a sequence has few: where a call is made of single tokens, or of some at a time, all of them, so that no
+// workgroup has to find out that there are no others, and nothing is launched for those.
+int few_most(int tokens, int batch) { return batch > 1 && tokens < (int64_t)4 * batch ? INT32_MAX : rp::kFewRowsMost; }
 
 int validate(const ringattn_paged_params* p) {
   if (!p) return RINGATTN_ERR_NULL;
@@ -243,9 +245,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.sinks = plan->p.sinks;
   a.out_fp32 = fp32;
   const int64_t rows = (int64_t)tokens * group, sequences = cache->batch < tokens ? cache->batch : tokens;
-  // Which sequences have few rows: where a call is made of single tokens, or of some at a time, all of them, so that no workgroup
-  // has to find out that there are no others, and nothing is launched for those.
-  a.few_most = sequences > 1 && tokens < kTokensEach * sequences ? INT32_MAX : rp::kFewRowsMost;
+  a.few_most = few_most(tokens, cache->batch);
   a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
   const int64_t few_tiles = rows / rp::kFewRows + sequences, see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile;
@@ -282,6 +282,8 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   a.causal = plan->p.causal != 0;
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
+  a.few_most = few_most(tokens, cache->batch);
+  a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < INT32_MAX;
   RP_HIP(rp::launch_paged_weights(a, plan->p.dtype, plan->p.dim, (hipStream_t)stream));
   return RINGATTN_OK;
 }

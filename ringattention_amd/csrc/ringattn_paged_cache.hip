@@ -53,8 +53,7 @@ hipError_t launch_paged_append(const AppendArgs& a, int dim, hipStream_t stream)
 }
 
 // ---- attention weight of the cached tokens ------------------------------------------
-// Sequences of up to so many rows of a KV head have few: the waves share out the keys.
-constexpr int kWeightFewRows = 128;
+// Where a sequence's KV head has few rows (a.few_most) the waves share out the keys.
 // Many: the waves share out the rows, for 64 keys, so that a tile of Q is fetched once for them.
 constexpr int kWeightWaves = 8, kManyKeys = 2 * kKeyTile;
 
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
   const int head = blockIdx.x, b = blockIdx.z;
   const Seq s = uniform(seq_of(a.c, b));
   const WeightRows<DT, D> x(a, s, b, head);
-  if (x.rows == 0 || s.len == 0 || x.rows > kWeightFewRows) return;
+  if (x.rows == 0 || s.len == 0 || x.rows > a.few_most) return;
   const int n = x.n, h = x.h;
   const Keys keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks);  // that any row sees
   const int tiles = keys.count, step = gridDim.y * kFewWaves;
@@ -259,7 +258,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const 
   for (int b0 = 0, before = 0; b0 < a.c.batch && b < 0; b0 += 64) {
     Seq mine{};
     if (b0 + lane < a.c.batch) mine = seq_of(a.c, b0 + lane);
-    const uint64_t many = __builtin_amdgcn_ballot_w64(mine.n * a.group > kWeightFewRows);
+    const uint64_t many = __builtin_amdgcn_ballot_w64(mine.n * a.group > a.few_most);
     const int wanted = (int)blockIdx.z - before, count = __builtin_popcountll(many);
     if (wanted < count) {
       const bool it = (many >> lane & 1) && __builtin_popcountll(many & (((uint64_t)1 << lane) - 1)) == wanted;
@@ -278,19 +277,50 @@ __global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const 
   };
   unsigned char* my = smem + wave * 2 * TILE;
   const unsigned my_lds = lds_offset(smem) + wave * 2 * TILE;
-  int qoff[KS];
+  const int qoff0 = n * ROWB + ((h ^ k_swizzle<D>(n)) << 4);
+  auto qoff = [&](int ks) {  // the number of the slice in bits that are free: one register, not eight
+    int o = qoff0;
+    if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(32 * ks), "v"(qoff0));
+    return o;
+  };
+  // A tile of Q, 1 KB a piece.  Where 32 rows are whole tokens (a.q_even) a piece's rows lie at fixed offsets from the tile's first, and so
+  // do the rows of their LSEs; elsewhere, and where the last rows are not there, every row's place is worked out.  (Worked out for
+  // every tile it cost as much as the exponentials: a prompt of 8 K tokens, 16/4 heads 250 us.)
+  int at_piece[PIECES], lse_at = 0;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qoff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
+  for (int j = 0; j < PIECES; ++j) at_piece[j] = 0;
+  if (a.q_even) {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int r = 1024 / ROWB * j + lane / CPR, token = quotient(r, a.by_group);
+      at_piece[j] = (int)(token * a.q_ts + (r - token * a.group) * a.q_hs) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
+    }
+    const int token = quotient(n, a.by_group);
+    lse_at = (n - token * a.group) * a.c.tokens + token;
+  }
   auto fetch_q = [&](int r0, int slot) {
+    const unsigned to = my_lds + slot * TILE;
+    if (a.q_even && r0 + 32 <= x.rows) {
+      const char* first = a.q + (s.start + quotient(r0, a.by_group)) * a.q_ts + (int64_t)head * a.group * a.q_hs;
 #pragma unroll
+      for (int j = 0; j < PIECES; ++j) load_lds_16_settled(first, at_piece[j], __builtin_amdgcn_readfirstlane(to + 1024 * j));
+      return;
+    }
+#pragma unroll 1
     for (int j = 0; j < PIECES; ++j) {
       const int r = 1024 / ROWB * j + lane / CPR;
       const char* src = x.q_row(r0 + r) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
-                       __builtin_amdgcn_readfirstlane(my_lds + slot * TILE + 1024 * j)),
-                   "v"(src)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to + 1024 * j)), "v"(src)
                    : "m0");
     }
+  };
+  auto fetch_lse = [&](int r0) {
+    if (a.q_even && r0 + 32 <= x.rows) {
+      const float* first = a.lse + (int64_t)head * a.group * a.c.tokens + s.start + quotient(r0, a.by_group);
+      const float z = first[lse_at] * 1.4426950408889634f;
+      return z == -INFINITY ? INFINITY : z;
+    }
+    return x.lse_of(r0 + n);
   };
   const int blocks = (s.len + kManyKeys - 1) / kManyKeys;
   // laps over the blocks go to and fro: under the mask the first blocks are seen by the most rows
@@ -318,18 +348,18 @@ __global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const 
     float lse_next = 0.f;
     if (r0 < r_end) {
       fetch_q(r0, 0);
-      lse_next = x.lse_of(r0 + n);
+      lse_next = fetch_lse(r0);
     }
     for (; r0 < r_end; r0 += 32 * kWeightWaves, slot ^= 1) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const float lse = lse_next;
       s16x8 qfr[KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qfr[ks] = *(const s16x8*)(my + slot * TILE + qoff[ks]);
+      for (int ks = 0; ks < KS; ++ks) qfr[ks] = *(const s16x8*)(my + slot * TILE + qoff(ks));
       const int next = r0 + 32 * kWeightWaves;
       if (next < r_end) {
         fetch_q(next, slot ^ 1);
-        lse_next = x.lse_of(next + n);
+        lse_next = fetch_lse(next);
       }
       const bool masked = x.masked(r0, key0, kManyKeys);
 #pragma unroll
@@ -372,7 +402,7 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
     const int64_t blocks = (keys + keys_each - 1) / keys_each, each = (enough + sequences * a.kv_heads - 1) / (sequences * a.kv_heads);
     return dim3((unsigned)a.kv_heads, (unsigned)(blocks < each ? blocks : each), (unsigned)sequences);
   };
-  const int64_t with_many = rows / (kWeightFewRows + 1) < a.c.batch ? rows / (kWeightFewRows + 1) : a.c.batch;
+  const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < a.c.batch ? might : a.c.batch;
 #define RA_LAUNCH_WEIGHTS(DT_, D_)                                                                                                      \
   do {                                                                                                                                 \
     if (a.c.batch > 1 || with_many == 0)                                                                                               \
