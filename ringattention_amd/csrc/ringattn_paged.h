@@ -19,6 +19,8 @@ constexpr int kFewRowsMost = 128; // few: up to so many (ringattn_paged_fwd says
 constexpr int kFewWorkgroups = 256, kFewLeast = 16;                     // see few_rows
 constexpr int kManyWorkgroups = 256, kManyLeast = 8;  // see find_place
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
+constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel
+constexpr int kWeightUnits = 512;   // parts of rows that there can be, where it shares them out
 constexpr int kMaxBatch = 4096;   // sequences of a call
 
 struct Cache {
@@ -326,8 +328,8 @@ template <int HALF> static __device__ __forceinline__ void load_half_tile(const 
   if constexpr (HALF == 4)
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\t"
-        "global_load_lds_dwordx4 %3, %5 offset:2048 nt\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072 nt" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
-        "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base)
+        "global_load_lds_dwordx4 %3, %5 offset:2048 nt\n\tglobal_load_lds_dwordx4 %4, %5 offset:%6 nt" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+        "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base), "n"(3 << 10)
         : "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt" ::"s"(
@@ -362,6 +364,8 @@ struct WeightsArgs {
   int causal, window, sinks;
   int few_most;  // as in AttendArgs
   int q_even;    // 32 rows are whole tokens, and lie within 2 GiB
+  float* parts;  // many rows: sums of the parts of a block of keys, kManyKeys each
+  int* arrived;  // ... and how many of them are there; 0 between launches
 };
 hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream);
 

@@ -53,7 +53,8 @@ int validate(const ringattn_paged_params* p) {
 
 // The workspace: counters, which are 0 between calls; then the parts of row tiles that several workgroups share.  A call that selects tokens
 // to keep has its counts where the parts lie.
-constexpr size_t kCounterBytes = (rp::kFewWorkgroups * sizeof(int) + 255) & ~(size_t)255;
+constexpr size_t kCounterBytes = rp::kWeightUnits * sizeof(int);
+static_assert(rp::kWeightUnits >= rp::kFewWorkgroups);
 size_t few_stat_bytes() { return (size_t)rp::kFewSlots * rp::kFewRows * sizeof(float2); }
 size_t many_stat_bytes() { return (size_t)rp::kManySlots * rp::kManyRows * sizeof(float2); }
 size_t few_o_bytes(int dim) { return (size_t)rp::kFewSlots * rp::kFewRows * dim * sizeof(float); }
@@ -283,7 +284,9 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
   a.few_most = few_most(tokens, cache->batch);
-  a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < INT32_MAX;
+  a.arrived = (int*)plan->ws;
+  a.parts = (float*)((char*)plan->ws + kCounterBytes);
+  a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < 1 << 29;
   RP_HIP(rp::launch_paged_weights(a, plan->p.dtype, plan->p.dim, (hipStream_t)stream));
   return RINGATTN_OK;
 }

@@ -54,8 +54,8 @@ hipError_t launch_paged_append(const AppendArgs& a, int dim, hipStream_t stream)
 
 // ---- attention weight of the cached tokens ------------------------------------------
 // Where a sequence's KV head has few rows (a.few_most) the waves share out the keys.
-// Many: the waves share out the rows, for 64 keys, so that a tile of Q is fetched once for them.
-constexpr int kWeightWaves = 8, kManyKeys = 2 * kKeyTile;
+// Many: the waves share out the rows, for 128 keys, so that a tile of Q is fetched once for them.
+constexpr int kWeightWaves = 8, kWeightPairs = kWeightWaves / 2, kWeightParts = 16, kWeightLaps = 2;
 
 // w[e] of lane (n, h): 16 sums over the 32 lanes of a half at once, each halving of the lanes halving the sums that a lane
 // goes on with; lane n ends up with sum n >> 1.  38 instructions for the five steps of 16 separate sums.
@@ -105,11 +105,14 @@ template <int DT, int D> struct WeightRows {
     row_of(r, token, q_head);
     return a.q + (s.start + token) * a.q_ts + q_head * a.q_hs;
   }
-  // log2(e) LSE of a row; +inf, against which every weight is 0, for a row that is not there or saw nothing
-  __device__ __forceinline__ float lse_of(int r) const {
+  __device__ __forceinline__ const float* lse_place(int r) const {
     int token, q_head;
     row_of(r, token, q_head);
-    const float x = a.lse[(int64_t)q_head * a.c.tokens + s.start + token] * 1.4426950408889634f;
+    return a.lse + (int64_t)q_head * a.c.tokens + s.start + token;
+  }
+  // log2(e) LSE of a row; +inf, against which every weight is 0, for a row that is not there or saw nothing
+  __device__ __forceinline__ float lse_of(int r) const {
+    const float x = *lse_place(r) * 1.4426950408889634f;
     return r >= rows || x == -INFINITY ? INFINITY : x;
   }
   // the new tokens [i0, i1) that see any of the keys [key0, key0 + keys)
@@ -117,28 +120,22 @@ template <int DT, int D> struct WeightRows {
     i0 = a.causal ? max(0, key0 - before) : 0;
     i1 = a.window > 0 && key0 >= a.sinks ? min(s.n, key0 + keys - 1 + a.window - before) : s.n;
   }
-  // whether some of the rows [r0, r0 + 32) are not there or do not see some of the keys
-  __device__ __forceinline__ bool masked(int r0, int key0, int keys) const {
-    const int first = quotient(r0, a.by_group), last = quotient(min(r0 + 31, rows - 1), a.by_group);
-    return r0 + 32 > rows || key0 + keys > (a.causal ? min(s.len, before + first + 1) : s.len) ||
-           (a.window > 0 && key0 <= before + last - a.window && key0 + keys > a.sinks);
-  }
-  __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse, bool masked, int key0, int r) const {
-    if (!masked) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
-      return;
-    }
+  // scores that weigh nothing: of row r, of the 16 keys that a lane has from key0 on
+  __device__ __forceinline__ void hide(f32x16& sacc, int key0, int r) const {
     const int token = quotient(min(r, rows - 1), a.by_group);
-    int lim = a.causal ? min(s.len, before + token + 1) : s.len;
+    const int lim = r >= rows ? 0 : a.causal ? min(s.len, before + token + 1) : s.len;
     const int low = a.window > 0 ? before + token - a.window : -1;
-    if (lse == INFINITY) lim = 0;
+    int first = key0 + 4 * h, sinks = a.sinks;
+    asm volatile("" : "+v"(first), "+v"(sinks));  // (nothing of these comparisons is kept from tile to tile: it took 100 registers)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int k = key0 + 8 * (e >> 2) + (e & 3) + 4 * h;
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
-      w[e] += bool((k >= lim) | ((k <= low) & (k >= a.sinks))) ? 0.f : x;  // (no branches)
+      const int k = first + 8 * (e >> 2) + (e & 3);
+      sacc[e] = bool((k >= lim) | ((k <= low) & (k >= sinks))) ? -INFINITY : sacc[e];  // (no branches)
     }
+  }
+  __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse) const {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
   }
   // Every key has one owner, which adds to its score once: no order to go by, and nothing to wait for.
   __device__ __forceinline__ void add_score(int page, int key, float x) const {
@@ -222,7 +219,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
-      x.weigh(w, sacc, lse_first, true, key0, n);
+      x.hide(sacc, key0, n);
+      x.weigh(w, sacc, lse_first);
     }
 #pragma unroll 1
     for (int r0 = 32; r0 < x.rows; r0 += 32) {
@@ -233,7 +231,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(q + ks * 32), sacc);
-      x.weigh(w, sacc, lse, true, key0, r0 + n);
+      x.hide(sacc, key0, r0 + n);
+      x.weigh(w, sacc, lse);
     }
     const float sum = sum_lanes(w);
     const int e = n >> 1;
@@ -242,15 +241,23 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
   }
 }
 
-// Many rows: a wave has 64 keys and every eighth tile of 32 rows, whose Q it brings to LDS one ahead; it needs no other wave until the sums
-// meet.  Bound by the exponentials: 32 of 16 cycles each to 16 MFMAs of 32.
+// Many rows: a workgroup has 128 keys and some of the rows that see them, kWeightPairs tiles of 32 rows at a time; two waves share a
+// tile, 64 keys each.  Q and LSE come to LDS two steps ahead, and while a wave's products of one tile are on the matrix cores it has the
+// exponentials of the tile before: 16 MFMAs of 32 cycles to 32 x (fma 4, exp 8, add 4) cycles of vector arithmetic, which the two share a SIMD's
+// issue for.  A prompt of 8 K tokens, 16/4 heads of 128, causal: 160 us, 860 TFLOP/s (250 with every tile's places worked out, 202 with
+// a Q tile for each wave and nothing on the way while it has the exponentials, 180 with no equal shares of the triangle).  Bound by power as much as
+// by the order of things: with queries and keys of 0 the same launch takes 140 us.  Workgroups of four waves, two to a compute unit, take
+// 162: of two waves of a SIMD that wait for nothing together the older one gets most of its issue, and when it is done the younger is alone.
 template <int DT, int D>
-__global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const WeightsArgs a) {
+__global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(const WeightsArgs a) {
   using E = Elem<DT>;
-  constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, CPR = D / 8, PIECES = TILE / 1024;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kWeightWaves * 2 * TILE];  // two tiles of Q of every wave
-  __shared__ float part[kWeightWaves][kManyKeys];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, CPR = D / 8, PIECES = TILE / 2048;  // (pieces of 1 KB that a wave brings of its tile)
+  constexpr int STEP = 32 * kWeightPairs;
+  constexpr int LSES = kWeightPairs * TILE, SLOT = LSES + kWeightWaves * 256;  // of a step: tiles; LSEs, a lane's own
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * SLOT];
+  __shared__ float part[kWeightPairs][kManyKeys];
+  __shared__ int last;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, pair = wave >> 1, half = wave & 1;
   const int head = blockIdx.x, block = blockIdx.y, in_all = gridDim.y;
   // the blockIdx.z-th sequence of many rows: there are fewer of them than sequences
   int b = -1;
@@ -270,122 +277,202 @@ __global__ __launch_bounds__(64 * kWeightWaves) void paged_weights_kernel(const 
   }
   if (b < 0) return;
   const WeightRows<DT, D> x(a, s, b, head);
-  const int n = x.n, h = x.h;
+  const int n = x.n, h = x.h, before = x.before;
   auto page_of = [&](int key) {  // -1: not there, or behind the end
     const int page = key < s.len ? x.table[key >> a.c.page_shift] : -1;
     return (unsigned)page < (unsigned)a.c.pages ? page : -1;
   };
-  unsigned char* my = smem + wave * 2 * TILE;
-  const unsigned my_lds = lds_offset(smem) + wave * 2 * TILE;
-  const int qoff0 = n * ROWB + ((h ^ k_swizzle<D>(n)) << 4);
-  auto qoff = [&](int ks) {  // the number of the slice in bits that are free: one register, not eight
-    int o = qoff0;
-    if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(32 * ks), "v"(qoff0));
-    return o;
-  };
-  // A tile of Q, 1 KB a piece.  Where 32 rows are whole tokens (a.q_even) a piece's rows lie at fixed offsets from the tile's first, and so
-  // do the rows of their LSEs; elsewhere, and where the last rows are not there, every row's place is worked out.  (Worked out for
-  // every tile it cost as much as the exponentials: a prompt of 8 K tokens, 16/4 heads 250 us.)
+  const unsigned q_lds = lds_offset(smem) + pair * TILE + half * (PIECES * 1024), lse_lds = lds_offset(smem) + LSES + wave * 256;
+  const int qoff = pair * TILE + n * ROWB + ((h ^ k_swizzle<D>(n)) << 4);
+  // A tile of Q, 1 KB a piece, half of them by each of the two waves.  Where 32 rows are whole tokens (a.q_even) a piece's rows lie at
+  // fixed offsets from the tile's first, and so do the rows of their LSEs; elsewhere, and where the last rows are not there, every row's
+  // place is worked out.  (Worked out for every tile it cost as much as the exponentials: a prompt of 8 K tokens, 16/4 heads 250 us.)
   int at_piece[PIECES], lse_at = 0;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j) at_piece[j] = 0;
   if (a.q_even) {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-      const int r = 1024 / ROWB * j + lane / CPR, token = quotient(r, a.by_group);
+      const int r = 1024 / ROWB * (half * PIECES + j) + lane / CPR, token = quotient(r, a.by_group);
       at_piece[j] = (int)(token * a.q_ts + (r - token * a.group) * a.q_hs) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
     }
     const int token = quotient(n, a.by_group);
-    lse_at = (n - token * a.group) * a.c.tokens + token;
+    lse_at = ((n - token * a.group) * a.c.tokens + token) * 4;
   }
-  auto fetch_q = [&](int r0, int slot) {
-    const unsigned to = my_lds + slot * TILE;
-    if (a.q_even && r0 + 32 <= x.rows) {
-      const char* first = a.q + (s.start + quotient(r0, a.by_group)) * a.q_ts + (int64_t)head * a.group * a.q_hs;
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) load_lds_16_settled(first, at_piece[j], __builtin_amdgcn_readfirstlane(to + 1024 * j));
-      return;
-    }
-#pragma unroll 1
-    for (int j = 0; j < PIECES; ++j) {
-      const int r = 1024 / ROWB * j + lane / CPR;
-      const char* src = x.q_row(r0 + r) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to + 1024 * j)), "v"(src)
-                   : "m0");
-    }
-  };
-  auto fetch_lse = [&](int r0) {
-    if (a.q_even && r0 + 32 <= x.rows) {
-      const float* first = a.lse + (int64_t)head * a.group * a.c.tokens + s.start + quotient(r0, a.by_group);
-      const float z = first[lse_at] * 1.4426950408889634f;
-      return z == -INFINITY ? INFINITY : z;
-    }
-    return x.lse_of(r0 + n);
-  };
+  const int64_t q_step = (int64_t)quotient(STEP, a.by_group) * a.q_ts;
+  const int lse_step = quotient(STEP, a.by_group);
+  // Blocks of keys; where there are workgroups enough, each block's rows are cut into as many parts, whose sums the last one to be done adds up,
+  // in their order.  Under the mask the first blocks are seen by the most rows, and laps over the blocks go to and fro.
   const int blocks = (s.len + kManyKeys - 1) / kManyKeys;
-  // laps over the blocks go to and fro: under the mask the first blocks are seen by the most rows
-  for (int lap = 0; lap * in_all < blocks; ++lap) {
-    const int at = lap * in_all + (lap & 1 ? in_all - 1 - block : block);
-    if (at >= blocks) continue;
-    const int key0 = at * kManyKeys;
+  const bool room = (int)(gridDim.x * gridDim.z) * in_all <= kWeightUnits / kWeightLaps;  // for all parts' sums
+  const int parts = room ? clamped(min(kWeightLaps * in_all / max(blocks, 1), x.rows / (4 * STEP)), 1, kWeightParts) : 1;
+  for (int lap = 0; lap * in_all < blocks * parts; ++lap) {
+    const int unit = lap * in_all + (lap & 1 ? in_all - 1 - block : block);
+    if (unit >= blocks * parts) continue;
+    const int at = unit / parts, my_part = unit - at * parts;
+    const int key0 = at * kManyKeys, my_key0 = key0 + 64 * half;
     int i0, i1;
     x.tokens_of(key0, kManyKeys, i0, i1);
-    const int r_begin = i0 * a.group, r_end = i1 * a.group;
+    const int r_begin = i0 * a.group, steps = max(0, (i1 - i0) * a.group + STEP - 1) / STEP;
+    int t = my_part * steps / parts;
+    const int t_end = (my_part + 1) * steps / parts;
+    // steps whose rows are all there and lie evenly, and the first of them
+    const int even_end = a.q_even ? (x.rows - r_begin) / STEP : 0;
+    const int first_token = s.start + quotient(r_begin + t * STEP + 32 * pair, a.by_group);
+    const char* q_next = a.q + first_token * a.q_ts + (int64_t)head * a.group * a.q_hs;
+    const float* lse_next = a.lse + (int64_t)head * a.group * a.c.tokens + first_token;
+    auto fetch = [&](int step, int to) {  // PIECES + 1 loads; steps come in their order
+      if (step < even_end) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) load_lds_16_settled(q_next, at_piece[j], q_lds + to + 1024 * j);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lse_lds + to), "v"(lse_at), "s"(lse_next) : "m0");
+        q_next += q_step;
+        lse_next += lse_step;
+        return;
+      }
+      const int r0 = r_begin + step * STEP + 32 * pair;
+#pragma unroll 1
+      for (int j = 0; j < PIECES; ++j) {
+        const int r = 1024 / ROWB * (half * PIECES + j) + lane / CPR;
+        const char* src = x.q_row(r0 + r) + (((lane % CPR) ^ k_swizzle<D>(r)) << 4);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(q_lds + to + 1024 * j), "v"(src) : "m0");
+      }
+      const float* lse = x.lse_place(r0 + n);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" ::"s"(lse_lds + to), "v"(lse) : "m0");
+    };
+    // the steps all of whose rows see all of the keys
+    int seen_from = 0, seen_to = (x.rows - r_begin) / STEP;
+    if (a.causal) seen_from = (max(0, key0 + kManyKeys - 1 - before - i0) * a.group + STEP - 1) / STEP;
+    if (key0 + kManyKeys > s.len) seen_to = 0;
+    if (a.window > 0 && key0 + kManyKeys > a.sinks) seen_to = min(seen_to, clamped(key0 + a.window - before - i0, 0, s.n) * a.group / STEP);
+    const unsigned seen = max(0, seen_to - seen_from);
     s16x8 kfr[2][KS];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = key0 + 32 * t + n;
+    for (int c = 0; c < 2; ++c) {
+      const int key = my_key0 + 32 * c + n;
       const char* src = a.c.k + page_row(a.c, max(page_of(key), 0), head, key) + h * 16;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kfr[t][ks] = *(const s16x8*)(src + ks * 32);
+      for (int ks = 0; ks < KS; ++ks) kfr[c][ks] = *(const s16x8*)(src + ks * 32);
     }
     float w[2][16];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) w[t][e] = 0.f;
-    int r0 = r_begin + 32 * wave, slot = 0;
-    float lse_next = 0.f;
-    if (r0 < r_end) {
-      fetch_q(r0, 0);
-      lse_next = fetch_lse(r0);
-    }
-    for (; r0 < r_end; r0 += 32 * kWeightWaves, slot ^= 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const float lse = lse_next;
-      s16x8 qfr[KS];
+      for (int e = 0; e < 16; ++e) w[c][e] = 0.f;
+    int here = 0, next = SLOT, free = 2 * SLOT;
+    // Tile t's products.  Every wave's own loads of it have come before the barrier, so behind it all have; and behind it all have read the
+    // tile before, whose slot takes the one two steps ahead.
+    s16x8 qfr[KS];
+    auto receive = [&](float& z) {
+      if (t + 1 < t_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PIECES + 1) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const int from = here + qoff;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qfr[ks] = *(const s16x8*)(my + slot * TILE + qoff(ks));
-      const int next = r0 + 32 * kWeightWaves;
-      if (next < r_end) {
-        fetch_q(next, slot ^ 1);
-        lse_next = fetch_lse(next);
+      for (int ks = 0; ks < KS; ++ks) {  // (the number of the slice in bits that are free: one register, not eight)
+        int o = from;
+        if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(32 * ks), "v"(from));
+        qfr[ks] = *(const s16x8*)(smem + o);
       }
-      const bool masked = x.masked(r0, key0, kManyKeys);
+      const float raw = *(const float*)(smem + here + LSES + threadIdx.x * 4) * 1.4426950408889634f;
+      z = raw == -INFINITY ? INFINITY : raw;
+      if (t + 2 < t_end) fetch(t + 2, free);
+      const int last = free;
+      free = here;
+      here = next;
+      next = last;
+    };
+    auto multiply = [&](f32x16 (&sacc)[2]) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x16 sacc;
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+        for (int e = 0; e < 16; ++e) sacc[c][e] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[t][ks], qfr[ks], sacc);
-        x.weigh(w[t], sacc, lse, masked, key0 + 32 * t, r0 + n);
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) sacc[c] = E::mma(kfr[c][ks], qfr[ks], sacc[c]);
+    };
+    auto hide = [&](f32x16 (&sacc)[2], int step) {
+      if ((unsigned)(step - seen_from) >= seen) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) x.hide(sacc[c], my_key0 + 32 * c, r_begin + step * STEP + 32 * pair + n);
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    auto weigh = [&](const f32x16 (&sacc)[2], float z) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          w[c][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c][e], a.scale_log2, -z));
+          asm volatile("" : "+v"(w[c][e]));  // (here, not where the sums are used next)
+        }
+    };
+    auto both = [&](f32x16 (&next)[2], float& z_next, f32x16 (&sacc)[2], float z) {
+      receive(z_next);
+      hide(sacc, t - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(next);
+      weigh(sacc, z);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 32 / KS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (t < t_end) {
+      fetch(t, here);
+      if (t + 1 < t_end) fetch(t + 1, next);
+      f32x16 odd[2], even[2];
+      float z_odd, z_even;
+      receive(z_even);
+      multiply(even);
+      for (++t; t + 1 < t_end; t += 2) {
+        both(odd, z_odd, even, z_even);
+        ++t;
+        both(even, z_even, odd, z_odd);
+        --t;
+      }
+      if (t < t_end) {
+        both(odd, z_odd, even, z_even);
+        hide(odd, t);
+        weigh(odd, z_odd);
+      } else {
+        hide(even, t - 1);
+        weigh(even, z_even);
+      }
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float sum = sum_lanes(w[t]);
+    for (int c = 0; c < 2; ++c) {
+      const float sum = sum_lanes(w[c]);
       const int e = n >> 1;
-      if ((n & 1) == 0) part[wave][32 * t + 8 * (e >> 2) + (e & 3) + 4 * h] = sum;
+      if ((n & 1) == 0) part[pair][64 * half + 32 * c + 8 * (e >> 2) + (e & 3) + 4 * h] = sum;
     }
     __syncthreads();
+    float sum = 0.f;
     if (threadIdx.x < kManyKeys) {
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kWeightWaves; ++i) sum += part[i][threadIdx.x];
-      x.add_score(page_of(key0 + threadIdx.x), key0 + threadIdx.x, sum);
+      for (int i = 0; i < kWeightPairs; ++i) sum += part[i][threadIdx.x];
     }
+    if (parts > 1) {  // (of no more units than kWeightLaps laps)
+      const int first = (blockIdx.z * gridDim.x + head) * kWeightLaps * in_all + at * parts;
+      if (threadIdx.x < kManyKeys)
+        __hip_atomic_store(a.parts + (int64_t)(first + my_part) * kManyKeys + threadIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(a.arrived + first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        if (last) __hip_atomic_store(a.arrived + first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+      }
+      __syncthreads();
+      if (!last) continue;
+      if (threadIdx.x < kManyKeys) {
+        sum = 0.f;
+        for (int i = 0; i < parts; ++i)
+          sum += __hip_atomic_load(a.parts + (int64_t)(first + i) * kManyKeys + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    if (threadIdx.x < kManyKeys) x.add_score(page_of(key0 + threadIdx.x), key0 + threadIdx.x, sum);
     __syncthreads();
   }
 }
@@ -399,15 +486,17 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
   // sequence could use, where that does not make them more than enough: they go on to further keys.
   const int64_t rows = (int64_t)a.c.tokens * a.group;
   auto grid = [&](int keys_each, int64_t sequences, int64_t enough) {
-    const int64_t blocks = (keys + keys_each - 1) / keys_each, each = (enough + sequences * a.kv_heads - 1) / (sequences * a.kv_heads);
-    return dim3((unsigned)a.kv_heads, (unsigned)(blocks < each ? blocks : each), (unsigned)sequences);
+    const int64_t blocks = (keys + keys_each - 1) / keys_each, each = enough / (sequences * a.kv_heads);
+    return dim3((unsigned)a.kv_heads, (unsigned)(blocks < each ? blocks : each > 1 ? each : 1), (unsigned)sequences);
   };
   const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < a.c.batch ? might : a.c.batch;
 #define RA_LAUNCH_WEIGHTS(DT_, D_)                                                                                                      \
   do {                                                                                                                                 \
     if (a.c.batch > 1 || with_many == 0)                                                                                               \
       paged_weights_few_kernel<DT_, D_><<<grid(kFewWaves * kKeyTile, a.c.batch, 2048), 64 * kFewWaves, 0, stream>>>(a);                 \
-    if (with_many > 0) paged_weights_kernel<DT_, D_><<<grid(kManyKeys, with_many, 512), 64 * kWeightWaves, 0, stream>>>(a);             \
+    if (with_many > 0)                                                                                                                 \
+      paged_weights_kernel<DT_, D_>                                                                                                    \
+          <<<grid(kManyKeys / kWeightParts, with_many, kWeightUnits / kWeightLaps), 64 * kWeightWaves, 0, stream>>>(a);                 \
   } while (0)
   if (dtype == 0 && dim == 64) RA_LAUNCH_WEIGHTS(0, 64);
   else if (dtype == 1 && dim == 64) RA_LAUNCH_WEIGHTS(1, 64);

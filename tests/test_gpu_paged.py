@@ -298,6 +298,29 @@ def test_weights_of_long_chunks(dtype, dim, heads, hkv, page, lens, news, window
     near(scores, w, off, "scores")
 
 
+@pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
+                                                                  ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
+def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
+    # few blocks of keys: their rows go to several workgroups, twice the same bits and with attention on the same workspace in between;
+    # many short prompts: more sequences and heads than that is done for
+    c = Case(dtype, dim, heads, hkv, 64, lens, news, causal=causal, seed=41)
+    plan = plan_for(c)
+    gpu = on_gpu(c)
+    q = c.q.cuda()
+    _, lse = plan.forward(q, *gpu)
+    runs = []
+    for _ in range(3):
+        scores = torch.zeros(c.pages, hkv, c.page, device="cuda")
+        plan.weights(q, lse, gpu[0], *gpu[2:], scores)
+        out, lse_again = plan.forward(q, *gpu)
+        runs.append(scores)
+        assert torch.equal(lse_again, lse)
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    clean = Case(dtype, dim, heads, hkv, 64, lens, news, causal=causal, seed=41, spare=0.0)
+    w, off = ref.weights(clean, lse.cpu())
+    near(runs[0], w, off, "scores")
+
+
 def test_weights_of_missing_pages_and_rows_that_saw_nothing():
     c = Case("bf16", 64, 4, 2, 16, (100, 40), (5, 60), seed=21)   # 20 rows of the second see nothing
     c.table[0, 2] = -1
