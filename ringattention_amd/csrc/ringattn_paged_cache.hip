@@ -531,29 +531,30 @@ struct Slice {
   int begin, end;
   unsigned held[kHeld];
 };
-template <class Fn> static __device__ __forceinline__ void each_rank(const EvictArgs& a, const int* table, int head, Slice& s, bool first, Fn fn) {
+// Ranks of up to kHeld tokens of a thread, from key0 on.  All pages first, then all scores, with nothing in between that a lane might skip.
+static __device__ __forceinline__ void load_ranks(const EvictArgs& a, const int* table, int head, int key0, int end, unsigned (&r)[kHeld]) {
   const int mask = (1 << a.c.page_shift) - 1;
-  auto rank_at = [&](int key) {
-    const int page = table[key >> a.c.page_shift];
-    if ((unsigned)page >= (unsigned)a.c.pages) return rank_of(-INFINITY);
-    return rank_of(a.scores[(((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & mask)]);
-  };
-  if (first) {
+  auto key_at = [&](int i) { return max(min(key0 + i * kSelectThreads + (int)threadIdx.x, end - 1), 0); };
+  int page[kHeld];
+  float x[kHeld];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int key = s.begin + i * kSelectThreads + (int)threadIdx.x;
-      s.held[i] = key < s.end ? rank_at(key) : 0;
-    }
-  }
+  for (int i = 0; i < kHeld; ++i) page[i] = table[key_at(i) >> a.c.page_shift];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    if (s.begin + i * kSelectThreads >= s.end) break;
-    const int key = s.begin + i * kSelectThreads + (int)threadIdx.x;
-    fn(key, s.held[i], key < s.end);
+    const int there = (unsigned)page[i] < (unsigned)a.c.pages ? page[i] : 0;
+    x[i] = a.scores[(((int64_t)there * a.kv_heads + head) << a.c.page_shift) + (key_at(i) & mask)];
   }
-  for (int key0 = s.begin + kHeld * kSelectThreads; key0 < s.end; key0 += kSelectThreads) {
-    const int key = key0 + (int)threadIdx.x;
-    fn(key, key < s.end ? rank_at(key) : 0, key < s.end);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) r[i] = rank_of((unsigned)page[i] < (unsigned)a.c.pages ? x[i] : -INFINITY);
+}
+// fn(first key, ranks) for every kHeld x kSelectThreads tokens of a slice
+template <class Fn> static __device__ __forceinline__ void each_ranks(const EvictArgs& a, const int* table, int head, Slice& s, bool first, Fn fn) {
+  if (first) load_ranks(a, table, head, s.begin, s.end, s.held);
+  fn(s.begin, s.held);
+  for (int key0 = s.begin + kHeld * kSelectThreads; key0 < s.end; key0 += kHeld * kSelectThreads) {
+    unsigned r[kHeld];
+    load_ranks(a, table, head, key0, s.end, r);
+    fn(key0, r);
   }
 }
 
@@ -564,17 +565,21 @@ static __device__ __forceinline__ void count_digits(const EvictArgs& a, const in
   const unsigned known = pass == 0 ? 0 : ~0u << (shift + bits);
   for (int i = threadIdx.x; i < kBins; i += kSelectThreads) counts[i] = 0;
   __syncthreads();
-  each_rank(a, table, head, s, first, [&](int, unsigned r, bool there) {
-    const bool counted = there && (r & known) == prefix;
-    const unsigned digit = r >> shift & ((1u << bits) - 1);
-    // scores that drew nothing all have one rank: the lanes that share the first one's digit are one addition
-    const uint64_t any = __builtin_amdgcn_ballot_w64(counted);
-    if (any == 0) return;
-    const int one = __builtin_ctzll(any);
-    const unsigned lead = __builtin_amdgcn_readlane(digit, one);
-    const uint64_t same = __builtin_amdgcn_ballot_w64(counted && digit == lead);
-    if (lane == one) atomicAdd(&counts[lead], (unsigned)__builtin_popcountll(same));
-    else if (counted && digit != lead) atomicAdd(&counts[digit], 1u);
+  each_ranks(a, table, head, s, first, [&](int key0, const unsigned (&ranks)[kHeld]) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const unsigned r = ranks[i];
+      const bool counted = key0 + i * kSelectThreads + (int)threadIdx.x < s.end && (r & known) == prefix;
+      const unsigned digit = r >> shift & ((1u << bits) - 1);
+      // scores that drew nothing all have one rank: the lanes that share the first one's digit are one addition
+      const uint64_t any = __builtin_amdgcn_ballot_w64(counted);
+      if (any == 0) continue;
+      const int one = __builtin_ctzll(any);
+      const unsigned lead = __builtin_amdgcn_readlane(digit, one);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(counted && digit == lead);
+      if (lane == one) atomicAdd(&counts[lead], (unsigned)__builtin_popcountll(same));
+      else if (counted && digit != lead) atomicAdd(&counts[digit], 1u);
+    }
   });
   __syncthreads();
 }
@@ -586,8 +591,7 @@ static __device__ __forceinline__ void find_digit(unsigned c0, unsigned c1, int 
   const int both = (int)(c0 + c1), upto = wave_scan(both);
   if (lane == 63) shared[wave] = upto;
   __syncthreads();
-  int above = upto - both;
-  for (int w = 0; w < wave; ++w) above += shared[w];
+  const int above = upto - both + wave_sum(lane < wave ? (int)shared[lane] : 0);  // (of the waves in front)
   const int want = (int)f.wanted;
   unsigned* found = shared + kSelectThreads / 64;
   if (above < want && want <= above + (int)c0) {
@@ -606,32 +610,36 @@ static __device__ __forceinline__ void find_digit(unsigned c0, unsigned c1, int 
 // Places of the tokens [begin, end) that stay, in order, from kept[placed] on: those outside [from, to), those that rank above
 // f.prefix, and of those that rank the same the first ones while fewer than f.wanted came before.
 static __device__ __forceinline__ void place_tokens(const EvictArgs& a, const int* table, int head, Slice& s, bool first, int* kept, int placed,
-                                                    int equal_before, const Found& f, unsigned* shared) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                                                    int equal_before, const Found& f, unsigned* counts) {
+  static_assert(kHeld * (kSelectThreads / 64) == 128, "two of them a lane");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wanted = (int)f.wanted;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  each_rank(a, table, head, s, first, [&](int key, unsigned r, bool there) {
-    const bool more = there && f.wanted > 0 && r > f.prefix, same = there && f.wanted > 0 && r == f.prefix;
-    const uint64_t sames = __builtin_amdgcn_ballot_w64(same), mores = __builtin_amdgcn_ballot_w64(more);
-    if (lane == 0) shared[wave] = (unsigned)__builtin_popcountll(sames) << 16 | (unsigned)__builtin_popcountll(mores);
-    __syncthreads();
-    int eq = equal_before, ab = 0, eq_all = 0, ab_all = 0;
-    for (int w = 0; w < kSelectThreads / 64; ++w) {
-      const unsigned x = shared[w];
-      if (w < wave) {
-        eq += x >> 16;
-        ab += x & 0xffff;
-      }
-      eq_all += x >> 16;
-      ab_all += x & 0xffff;
+  each_ranks(a, table, head, s, first, [&](int key0, const unsigned (&r)[kHeld]) {
+    // how many of 64 tokens rank above (low 16 bits) and the same (high), 64 after 64, and of all in front of them
+    uint64_t mores[kHeld], sames[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const bool there = key0 + i * kSelectThreads + (int)threadIdx.x < s.end && wanted > 0;
+      mores[i] = __builtin_amdgcn_ballot_w64(there && r[i] > f.prefix);
+      sames[i] = __builtin_amdgcn_ballot_w64(there && r[i] == f.prefix);
+      if (lane == 0) counts[i * (kSelectThreads / 64) + wave] = (unsigned)__builtin_popcountll(sames[i]) << 16 | (unsigned)__builtin_popcountll(mores[i]);
     }
     __syncthreads();
-    const int wanted = (int)f.wanted;
-    eq += __builtin_popcountll(sames & below);  // those that rank the same in front of this one
-    ab += __builtin_popcountll(mores & below);
-    const int at = placed + ab + min(eq, wanted) - min(equal_before, wanted);
-    if ((more || (same && eq < wanted)) && at < a.budget) kept[at] = key;
-    placed += ab_all + min(equal_before + eq_all, wanted) - min(equal_before, wanted);
-    equal_before += eq_all;
+    const int x0 = (int)counts[lane], x1 = (int)counts[64 + lane], s0 = wave_scan(x0), s1 = wave_scan(x1);
+    __syncthreads();
+    const unsigned first64 = __builtin_amdgcn_readlane(s0, 63), all = first64 + __builtin_amdgcn_readlane(s1, 63);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int at64 = i * (kSelectThreads / 64) + wave;
+      const unsigned front = at64 < 64 ? __builtin_amdgcn_readlane(s0 - x0, at64) : first64 + __builtin_amdgcn_readlane(s1 - x1, at64 - 64);
+      const int eq = equal_before + (int)(front >> 16) + __builtin_popcountll(sames[i] & below);  // those that rank the same in front of this one
+      const int ab = (int)(front & 0xffff) + __builtin_popcountll(mores[i] & below);
+      const int at = placed + ab + min(eq, wanted) - min(equal_before, wanted);
+      const bool stays = (mores[i] >> lane & 1) || ((sames[i] >> lane & 1) && eq < wanted);
+      if (stays && at < a.budget) kept[at] = key0 + i * kSelectThreads + (int)threadIdx.x;
+    }
+    placed += (int)(all & 0xffff) + min(equal_before + (int)(all >> 16), wanted) - min(equal_before, wanted);
+    equal_before += all >> 16;
   });
 }
 
@@ -682,12 +690,13 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
     count_digits(a, x.table, head, x.s, pass == 0, pass, f.prefix, counts);
     find_digit(counts[hi], counts[hi - 1], pass, f, shared);
   }
-  place_tokens(a, x.table, head, x.s, false, x.kept, a.first, 0, f, shared);
+  place_tokens(a, x.table, head, x.s, false, x.kept, a.first, 0, f, counts);
 }
 
 // The same by several workgroups, where there are few sequences and heads and they are long: a launch for each pass, in which
 // every workgroup adds up the counts that the launch before has left of all slices.
-//   counts [pairs][slices][kPasses][kBins], above [pairs][slices][kPasses] (tokens of the slice that rank above by a pass's digit), found [pairs][kPasses]
+//   counts [pairs][slices][kPasses][kBins], above [pairs][slices][kPasses] (tokens of the slices in front that rank above by a pass's digit),
+//   found [pairs][kPasses]
 template <int PASS>  // kPasses: the places
 __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(const EvictArgs a, unsigned* all_counts, unsigned* all_above, Found* all_found) {
   __shared__ unsigned counts[kBins];
@@ -712,25 +721,24 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   };
   Found f{0, x.wanted};
   if constexpr (PASS > 1) f = all_found[pair * kPasses + PASS - 2];
-  unsigned digit = 0;
+  unsigned above = 0, equal = 0;  // in the slices in front: by the digit just found, tokens that rank above, those that rank the same
   if constexpr (PASS > 0) {
-    unsigned c0 = 0, c1 = 0;
-#pragma unroll 8
+    unsigned c0 = 0, c1 = 0, front0 = 0, front1 = 0;
+#pragma unroll 16
     for (int s = 0; s < slices; ++s) {
       const uint2 c = *counts_of(s, PASS - 1);
+      front0 += s < slice ? c.y : 0;
+      front1 += s < slice ? c.x : 0;
       c0 += c.y;
       c1 += c.x;
     }
     find_digit(c0, c1, PASS - 1, f, shared);
-    digit = f.prefix >> digit_shift(PASS - 1) & ((1u << digit_bits(PASS - 1)) - 1);
+    const int digit = (int)(f.prefix >> digit_shift(PASS - 1) & ((1u << digit_bits(PASS - 1)) - 1));
+    above = sum_of((hi > digit ? front0 : 0) + (hi - 1 > digit ? front1 : 0));
+    equal = (hi == digit ? front0 : 0) + (hi - 1 == digit ? front1 : 0);
   }
-  auto above_digit = [&](int s) {  // this thread's part of how many of slice s rank above by the digit just found
-    const uint2 c = *counts_of(s, PASS - 1);
-    return (hi > (int)digit ? c.y : 0) + (hi - 1 > (int)digit ? c.x : 0);
-  };
   if constexpr (PASS < kPasses) {
     if constexpr (PASS > 0) {
-      const unsigned above = sum_of(above_digit(slice));
       if (tid == 0) {
         pair_above[slice * kPasses + PASS - 1] = above;
         if (slice == 0) all_found[pair * kPasses + PASS - 1] = f;
@@ -740,15 +748,9 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
     unsigned* to = pair_counts + (slice * kPasses + PASS) * kBins;
     for (int i = tid; i < kBins; i += kSelectThreads) to[i] = counts[i];
   } else {
-    // of the slices in front: tokens that rank above, and those that rank the same
-    unsigned above = 0, equal = 0;
-#pragma unroll 8
-    for (int s = 0; s < slice; ++s) above += above_digit(s);
-    for (int i = tid; i < slice * kPasses; i += kSelectThreads) above += i % kPasses < kPasses - 1 ? pair_above[i] : 0;
-    for (int s = tid; s < slice; s += kSelectThreads) equal += pair_counts[(s * kPasses + kPasses - 1) * kBins + digit];
-    above = sum_of(above);
+    for (int pass = 0; pass < kPasses - 1; ++pass) above += pair_above[slice * kPasses + pass];
     equal = sum_of(equal);
-    place_tokens(a, x.table, head, x.s, true, x.kept, a.first + (int)above + min((int)equal, (int)f.wanted), (int)equal, f, shared);
+    place_tokens(a, x.table, head, x.s, true, x.kept, a.first + (int)above + min((int)equal, (int)f.wanted), (int)equal, f, counts);
   }
 }
 
