@@ -16,7 +16,7 @@ constexpr int kKeyTile = 32;      // keys of a tile
 constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence's KV head has few of them (ringattn_paged_few.h)
 constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
 constexpr int kFewRowsMost = 128; // few: up to so many (ringattn_paged_fwd says when more)
-constexpr int kFewWorkgroups = 256, kFewLeast = 16;                     // see few_rows
+constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewMerge = 16;     // see few_rows
 constexpr int kManyWorkgroups = 256, kManyLeast = 8;  // see find_place
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel
@@ -41,7 +41,7 @@ struct Cache {
 struct Parts {
   float* o;       // sums of a part's rows
   float2* stat;   // their references (log2 units) and the sums of their weights
-  int* arrived;   // few rows: how many parts of a row tile are there; 0 between launches
+  int* arrived;   // few rows: how many parts of a row tile are there, [2 kFewWorkgroups]; 0 between launches
 };
 
 struct AttendArgs {

@@ -54,7 +54,7 @@ int validate(const ringattn_paged_params* p) {
 // The workspace: counters, which are 0 between calls; then the parts of row tiles that several workgroups share.  A call that selects tokens
 // to keep has its counts where the parts lie.
 constexpr size_t kCounterBytes = rp::kWeightUnits * sizeof(int);
-static_assert(rp::kWeightUnits >= rp::kFewWorkgroups);
+static_assert(rp::kWeightUnits >= 2 * rp::kFewWorkgroups);
 size_t few_stat_bytes() { return (size_t)rp::kFewSlots * rp::kFewRows * sizeof(float2); }
 size_t many_stat_bytes() { return (size_t)rp::kManySlots * rp::kManyRows * sizeof(float2); }
 size_t few_o_bytes(int dim) { return (size_t)rp::kFewSlots * rp::kFewRows * dim * sizeof(float); }

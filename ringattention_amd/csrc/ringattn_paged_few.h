@@ -55,10 +55,21 @@ struct Piece {
   }
 };
 
+// A part's row, eight columns of it.
+template <int D> static __device__ __forceinline__ void put_row(const AttendArgs& a, int slot, int r, int c8, const float (&o)[8], float top, float l) {
+  const int64_t prow = (int64_t)slot * kFewRows + r;
+  float* to = a.few.o + prow * D + c8 * 8;
+  put_part(to, f32x4{o[0], o[1], o[2], o[3]});
+  put_part(to + 4, f32x4{o[4], o[5], o[6], o[7]});
+  if (c8 == 0) put_stat(a.few.stat + prow, float2{top, l});
+}
+
 // The parts of a row tile, `count` rows of it, put together by all threads of the workgroup: a thread has eight columns of a row and
-// every so-many-th of its parts, and those of a row meet in LDS.  slot(i): where part i lies.
+// every so-many-th of its parts, and those of a row meet in LDS.  slot(i): where part i lies; to: where their sum goes as one part, or -1: these
+// are all of the row tile's.
 template <int DT, int D, class Slot>
-static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Seq& s, int head, int r0, int count, int parts, Slot slot, float (*sums)[10]) {
+static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Seq& s, int head, int r0, int count, int parts, Slot slot, int to,
+                                                   float (*sums)[10]) {
   constexpr int TPR = D / 8, GROUPS = 512 / TPR;
   int at_once = 1;  // rows at once; the groups of threads left share a row's parts
   while (at_once < count) at_once *= 2;
@@ -114,7 +125,12 @@ static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Se
       }
     }
   }
-  if (sub == 0 && r < count) store_row<DT>(a, s, head, r0 + r, c8, o, top, l);
+  if (sub != 0 || r >= count) return;
+  if (to < 0) {
+    store_row<DT>(a, s, head, r0 + r, c8, o, top, l);
+  } else {  // (into a slot that this thread alone, or one of its row's, has read)
+    put_row<D>(a, to, r, c8, o, top, l);
+  }
 }
 
 template <int D> constexpr int kFewWaveLds = 2 * kKeyTile * D * 2;  // a K and a V tile; at the end the wave's acc-O
@@ -442,11 +458,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       if (whole) {
         store_row<DT>(a, p.s, head, r0 + orow, c8, o, top, l);
       } else {
-        const int64_t prow = (int64_t)slot * BM + orow;
-        float* to = a.few.o + prow * D + c8 * 8;
-        put_part(to, f32x4{o[0], o[1], o[2], o[3]});
-        put_part(to + 4, f32x4{o[4], o[5], o[6], o[7]});
-        if (c8 == 0) put_stat(a.few.stat + prow, float2{top, l});
+        put_row<D>(a, slot, orow, c8, o, top, l);
       }
     }
     if (!whole) {
@@ -458,22 +470,44 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   if (__builtin_amdgcn_readfirstlane(left[0].parts + left[1].parts) == 0) return;
   // Every wave waits for its own stores to be where all XCDs see them, the barrier for every wave, and only then the parts are counted; the
   // loads of one that finds itself the last are issued behind the barrier that follows its count.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a barrier alone does not wait for stores)
-  __syncthreads();
+  auto settle = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a barrier alone does not wait for stores)
+    __syncthreads();
+  };
+  auto of = [&](int y) { return __builtin_amdgcn_readfirstlane(y); };
+  auto count = [&](int* arrived, int parts) {  // whether this is the last of them
+    const bool last = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    if (last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    return last;
+  };
+  settle();
+  // Of more than kFewMerge parts, as many at a time become one first, by the last workgroup of theirs, and those the row tile: one that fetches
+  // them all has long waits one after the other.  (One token, 128 K cached, one KV head, 16 heads: 93 us by one, 38 by 8, 16 or 32 at a
+  // time; 32 heads 160 and 49.  16 KV heads have 16 parts each and do not come here.)
   if (tid < 2 && left[tid].parts > 0) {
-    int* arrived = a.few.arrived + left[tid].first_run;
-    const int before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    left[tid].last = before == left[tid].parts - 1;
-    if (left[tid].last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    const int parts = left[tid].parts, first = left[tid].first_run, at = (w - first) & ~(kFewMerge - 1), some = min(kFewMerge, parts - at);
+    // (one alone is not counted: its counter is that of the first ones of the row tile that begins in this run)
+    if (parts <= kFewMerge) left[tid].last = count(a.few.arrived + first, parts);
+    else left[tid].last = some == 1 || count(a.few.arrived + kFewWorkgroups + first + at, some);
   }
   __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    auto of = [&](int y) { return __builtin_amdgcn_readfirstlane(y); };
-    const int parts = of(left[i].parts), first_run = of(left[i].first_run);
+    const int parts = of(left[i].parts), first = of(left[i].first_run);
     if (parts == 0 || of(left[i].last) == 0) continue;
-    merge_parts<DT, D>(a, uniform(left[i].s), of(left[i].head), of(left[i].r0), of(left[i].count), parts,
-                       [&](int k) { return 2 * (first_run + k) + (k == 0 ? 1 : 0); }, (float (*)[10])smem);
+    const Seq s = uniform(left[i].s);
+    const int head = of(left[i].head), r0 = of(left[i].r0), rows = of(left[i].count), at = (w - first) & ~(kFewMerge - 1);
+    auto slot = [&](int k) { return 2 * (first + k) + (k == 0 ? 1 : 0); };
+    if (parts > kFewMerge) {
+      merge_parts<DT, D>(a, s, head, r0, rows, min(kFewMerge, parts - at), [&](int k) { return slot(at + k); }, slot(at), (float (*)[10])smem);
+      settle();
+      if (tid == 0) left[i].last = count(a.few.arrived + first, (parts + kFewMerge - 1) / kFewMerge);
+      __syncthreads();
+      if (of(left[i].last) == 0) continue;
+    }
+    const bool two = parts > kFewMerge;
+    merge_parts<DT, D>(a, s, head, r0, rows, two ? (parts + kFewMerge - 1) / kFewMerge : parts, [&](int k) { return slot(two ? k * kFewMerge : k); }, -1,
+                       (float (*)[10])smem);
     __syncthreads();
   }
 }

@@ -298,6 +298,19 @@ def test_weights_of_long_chunks(dtype, dim, heads, hkv, page, lens, news, window
     near(scores, w, off, "scores")
 
 
+@pytest.mark.parametrize("dtype,dim,heads,lens", [("bf16", 128, 8, (8600, 9000, 300)), ("fp16", 64, 4, (8704,)), ("bf16", 64, 32, (16900, 40))])
+def test_parts_by_the_dozen(dtype, dim, heads, lens):
+    # one KV head: the keys of a row go to more workgroups than one puts together, the last of which is alone or begins the next sequence's
+    c = Case(dtype, dim, heads, 1, 64, lens, (1,) * len(lens), seed=42)
+    check_forward(c)
+    plan = plan_for(c)
+    gpu = on_gpu(c)
+    out, lse = plan.forward(c.q.cuda(), *gpu)
+    for _ in range(3):
+        again, lse_again = plan.forward(c.q.cuda(), *gpu)
+        assert torch.equal(out, again) and torch.equal(lse, lse_again)
+
+
 @pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
                                                                   ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
 def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
