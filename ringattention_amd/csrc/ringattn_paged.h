@@ -17,7 +17,7 @@ constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence'
 constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
 constexpr int kFewRowsMost = 128; // few: up to so many (ringattn_paged_fwd says when more)
 constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewMerge = 16;     // see few_rows
-constexpr int kManyWorkgroups = 256, kManyLeast = 8;  // see find_place
+constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel
 constexpr int kWeightUnits = 512;   // parts of rows that there can be, where it shares them out

@@ -16,16 +16,16 @@ __global__ __launch_bounds__(512, 2) void paged_attend_kernel(const AttendArgs a
   else many_rows<DT, D>(a, smem, blockIdx.x - a.few_workgroups);
 }
 
-template <int DT, int D> __global__ __launch_bounds__(2 * D) void paged_merge_kernel(const AttendArgs a) { merge_many<DT, D>(a, blockIdx.x); }
+template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void paged_merge_kernel(const AttendArgs a) { merge_many<DT, D>(a, blockIdx.x); }
 
 hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream) {
-  const int64_t blocks = a.few_workgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) : 0;
+  const int64_t blocks = a.few_workgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) * (dim / 32) : 0;
   if (blocks <= 0) return hipSuccess;
   if (blocks > INT32_MAX || merges > INT32_MAX) return hipErrorInvalidValue;
 #define RA_LAUNCH_ATTEND(DT_, D_)                                                                             \
   do {                                                                                                       \
     paged_attend_kernel<DT_, D_><<<(unsigned)blocks, 512, 0, stream>>>(a);                                    \
-    if (merges > 0) paged_merge_kernel<DT_, D_><<<(unsigned)merges, 2 * D_, 0, stream>>>(a);                  \
+    if (merges > 0) paged_merge_kernel<DT_, D_><<<(unsigned)merges, 64 * kMergeSharers, 0, stream>>>(a);                  \
   } while (0)
   if (dtype == 0 && dim == 64) RA_LAUNCH_ATTEND(0, 64);
   else if (dtype == 1 && dim == 64) RA_LAUNCH_ATTEND(1, 64);

@@ -417,13 +417,17 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   store_rows<DT, DB>(a, p.s, head, r0 + 32 * wave, r_last, oacc, 0, l, ms);
 }
 
-// The shares of a row tile added up in their order: a workgroup has the 32 rows of a wave of them, its waves 32 columns each.
+// The shares of a row tile added up in an order of their own: a workgroup has 32 columns of the 32 rows of a wave, its waves every so-many-th
+// share.  (A chunk of 16 tokens, 128 K cached, 16 heads on one, 256 shares: 97 us with one wave for all shares and the four column blocks in a
+// workgroup, 69, 52 and 51 with two, four and eight waves and a workgroup for each; four sequences of 4 K, 64 tokens each, 8 shares:
+// 41, 40, 40 and 47.)
 template <int DT, int D> static __device__ __forceinline__ void merge_many(const AttendArgs& a, int block) {
-  constexpr int BLOCKS = kManyRows / 32;
-  const int lane = threadIdx.x & 63, n = lane & 31, db = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int BLOCKS = kManyRows / 32, DB = D / 32;
+  __shared__ float sums[kMergeSharers - 1][18][64];
+  const int lane = threadIdx.x & 63, n = lane & 31, sharer = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Place p;
-  const int unit = quotient(block, a.by_kv_heads), head = block - unit * a.kv_heads, rows_of = unit % BLOCKS;
-  if (!find_place<true>(a, unit / BLOCKS, p)) return;
+  const int unit = quotient(block, a.by_kv_heads), head = block - unit * a.kv_heads, rows_of = unit / DB % BLOCKS, db = unit % DB;
+  if (!find_place<true>(a, unit / (DB * BLOCKS), p)) return;
   const int r0 = p.tile * kManyRows, r_last = min(r0 + kManyRows, p.s.n * a.group) - 1;
   if (r0 + 32 * rows_of > r_last) return;
   const int64_t slot = (int64_t)p.slot * a.kv_heads + head;  // of share 0; those of the others are kv_heads apart
@@ -431,19 +435,36 @@ template <int DT, int D> static __device__ __forceinline__ void merge_many(const
   f32x16 acc[1];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
+  auto add = [&](const float2& st, auto of) {
+    const float t = fmaxf(top, st.x), keep = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t), w = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - t);
+    l = __builtin_fmaf(st.y, w, l * keep);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][e] = __builtin_fmaf(of(e), w, acc[0][e] * keep);
+    top = t;
+  };
 #pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
+  for (int s = sharer; s < p.splits; s += kMergeSharers) {
     const int64_t at = slot + (int64_t)s * a.kv_heads;
     const float2 st = a.many.stat[at * kManyRows + 32 * rows_of + n];
     const float* from = a.many.o + (at * BLOCKS + rows_of) * (32 * D) + db * 1024 + lane * 4;
     f32x4 x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = *(const f32x4*)(from + 256 * i);
-    const float t = fmaxf(top, st.x), keep = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t), w = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - t);
-    l = __builtin_fmaf(st.y, w, l * keep);
+    add(st, [&](int e) { return x[e / 4][e % 4]; });
+  }
+  if (sharer > 0) {
+    float (*mine)[64] = sums[sharer - 1];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[0][e] = __builtin_fmaf(x[e / 4][e % 4], w, acc[0][e] * keep);
-    top = t;
+    for (int e = 0; e < 16; ++e) mine[e][lane] = acc[0][e];
+    mine[16][lane] = top;
+    mine[17][lane] = l;
+  }
+  __syncthreads();
+  if (sharer > 0) return;
+#pragma unroll
+  for (int i = 0; i < kMergeSharers - 1; ++i) {
+    const float (*x)[64] = sums[i];
+    add(float2{x[16][lane], x[17][lane]}, [&](int e) { return x[e][lane]; });
   }
   store_rows<DT, 1>(a, p.s, head, r0 + 32 * rows_of, r_last, acc, db, l, top);
 }

@@ -311,6 +311,17 @@ def test_parts_by_the_dozen(dtype, dim, heads, lens):
         assert torch.equal(out, again) and torch.equal(lse, lse_again)
 
 
+@pytest.mark.parametrize("dtype,dim,heads,lens,news", [("bf16", 128, 16, (20000,), (16,)), ("fp16", 64, 8, (9000, 5000), (40, 17))])
+def test_shares_by_the_dozen(dtype, dim, heads, lens, news):
+    c = Case(dtype, dim, heads, 1, 64, lens, news, seed=43)   # many rows, and their keys in dozens of shares
+    check_forward(c)
+    plan = plan_for(c)
+    gpu = on_gpu(c)
+    out, lse = plan.forward(c.q.cuda(), *gpu)
+    again, lse_again = plan.forward(c.q.cuda(), *gpu)
+    assert torch.equal(out, again) and torch.equal(lse, lse_again)
+
+
 @pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
                                                                   ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
 def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
