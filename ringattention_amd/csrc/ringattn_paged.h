@@ -15,7 +15,10 @@ namespace paged {
 constexpr int kKeyTile = 32;      // keys of a tile
 constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence's KV head has few of them (ringattn_paged_few.h)
 constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
-constexpr int kFewRowsMost = 128; // few: up to so many (ringattn_paged_fwd says when more)
+// Up to so many rows of a sequence's KV head are few.  Attention, us as few and as many, 32 heads on 8: one sequence of 32 K, 9 tokens 55 and 51,
+// 17 tokens 97 and 51, 32 tokens 71 and 52; 16 sequences of 4 K, 16 tokens (64 rows) 79 and 87, 17 tokens 155 and 83.  Weights, the
+// latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48 tokens 63 and 67.
+constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
 constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewMerge = 16;     // see few_rows
 constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be

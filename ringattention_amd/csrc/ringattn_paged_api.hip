@@ -33,7 +33,7 @@ inline bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (byt
 
 // Rows of a KV head up to which a sequence has few: where a call is made of single tokens, or of some at a time, all of them, so that no
 // workgroup has to find out that there are no others, and nothing is launched for those.
-int few_most(int tokens, int batch) { return batch > 1 && tokens < (int64_t)4 * batch ? INT32_MAX : rp::kFewRowsMost; }
+int few_most(int tokens, int batch, int most) { return batch > 1 && tokens < (int64_t)4 * batch ? INT32_MAX : most; }
 
 int validate(const ringattn_paged_params* p) {
   if (!p) return RINGATTN_ERR_NULL;
@@ -246,7 +246,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.sinks = plan->p.sinks;
   a.out_fp32 = fp32;
   const int64_t rows = (int64_t)tokens * group, sequences = cache->batch < tokens ? cache->batch : tokens;
-  a.few_most = few_most(tokens, cache->batch);
+  a.few_most = few_most(tokens, cache->batch, rp::kFewRowsMost);
   a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
   const int64_t few_tiles = rows / rp::kFewRows + sequences, see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile;
@@ -283,7 +283,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   a.causal = plan->p.causal != 0;
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
-  a.few_most = few_most(tokens, cache->batch);
+  a.few_most = few_most(tokens, cache->batch, rp::kWeightFewRowsMost);
   a.arrived = (int*)plan->ws;
   a.parts = (float*)((char*)plan->ws + kCounterBytes);
   a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < 1 << 29;
