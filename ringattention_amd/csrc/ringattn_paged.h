@@ -23,7 +23,7 @@ constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewMerge = 16;     // see f
 constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel
-constexpr int kWeightUnits = 512;   // parts of rows that there can be, where it shares them out
+constexpr int kWeightUnits = 2048;   // parts of rows that there can be, where it shares them out
 constexpr int kMaxBatch = 4096;   // sequences of a call
 
 struct Cache {

@@ -249,7 +249,8 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.few_most = few_most(tokens, cache->batch, rp::kFewRowsMost);
   a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
-  const int64_t few_tiles = rows / rp::kFewRows + sequences, see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile;
+  const int64_t few_tiles = rows / rp::kFewRows + sequences;
+  const int64_t see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile + rp::kFewLeast;
   while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
   // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute
   // units their keys are not shared out; else there is a share each, and no more besides than are due.

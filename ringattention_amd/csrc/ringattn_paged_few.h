@@ -20,7 +20,8 @@ struct Lanes {
   Seq s;
   int tiles, keys;  // row tiles, and units of each (an upper bound of what its rows see, the same for all of a sequence)
   int upto;         // units of all sequences up to this one
-  __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before) {
+  // round: to multiples of kFewLeast
+  __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round) {
     const int lane = threadIdx.x & 63;
     s = Seq{0, 0, 0};
     tiles = 0;
@@ -28,6 +29,8 @@ struct Lanes {
     if (b0 + lane < a.c.batch) {
       s = seq_of(a.c, b0 + lane);
       load_of<false>(a, s, tiles, keys);
+      keys = max(keys, kFewLeast);
+      if (round) keys = (keys + kFewLeast - 1) / kFewLeast * kFewLeast;
       keys = ((keys - 1) >> a.few_shift) + 1;
     }
     upto = before + wave_scan(tiles * keys * a.kv_heads);
@@ -160,9 +163,18 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   // The runs: `each` units of all of them.  Every wave works out for itself where its run lies, without a barrier; up to 64 sequences stay
   // in its registers.
   Lanes lanes;
+  // A row tile costs its beginning and end, some 5 us, whatever it sees: it counts as kFewLeast key tiles at least, and where runs of so
+  // many suffice for all, every row tile begins a run.  (Counted as what they see: 113 sequences of one token, 4 heads 79 us against 23;
+  // prompts of some 40 tokens, 39 of them, 2 KV heads 95 against 19.)
+  const int least = max(1, kFewLeast >> a.few_shift);
   int total = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total);
-  const int each = max((total + kFewWorkgroups - 1) / kFewWorkgroups, max(1, kFewLeast >> a.few_shift));
+  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true);
+  const bool round = total <= kFewWorkgroups * least;
+  if (!round) {
+    total = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false);
+  }
+  const int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
   const int end = min((int64_t)total, (int64_t)(w + 1) * each);
   // The parts that this run leaves: of a row tile that began before it, and of one that goes on behind it.  They are counted when the
   // run is through, and not each on its own, which would keep the workgroup waiting for its stores (some 8 us a part).
@@ -176,7 +188,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       p.find(a, lanes, 0, pos);
     } else {
       for (int b0 = 0, before = 0; b0 < a.c.batch; b0 += 64) {
-        before = lanes.add(a, b0, before);
+        before = lanes.add(a, b0, before, round);
         if (p.find(a, lanes, b0, pos)) break;
       }
     }
