@@ -20,6 +20,7 @@ struct Lanes {
   Seq s;
   int tiles, keys;  // row tiles, and units of each (an upper bound of what its rows see, the same for all of a sequence)
   int upto;         // units of all sequences up to this one
+  int most = 0, fewest = INT32_MAX;  // key tiles that a row tile of any sequence sees
   // round: to multiples of kFewLeast
   __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round) {
     const int lane = threadIdx.x & 63;
@@ -29,6 +30,10 @@ struct Lanes {
     if (b0 + lane < a.c.batch) {
       s = seq_of(a.c, b0 + lane);
       load_of<false>(a, s, tiles, keys);
+      if (tiles > 0) {
+        most = max(most, keys);
+        fewest = min(fewest, keys);
+      }
       keys = max(keys, kFewLeast);
       if (round) keys = (keys + kFewLeast - 1) / kFewLeast * kFewLeast;
       keys = ((keys - 1) >> a.few_shift) + 1;
@@ -142,7 +147,7 @@ struct Left {
   Seq s;
   int head, r0, count, first_run, parts, last;
 };
-template <int D> constexpr int kFewLds = 8 * kFewWaveLds<D> + 8 * kFewRows * (int)sizeof(float2) + 2 * (int)sizeof(Left);
+template <int D> constexpr int kFewLds = 8 * kFewWaveLds<D> + 8 * kFewRows * (int)sizeof(float2) + 2 * (int)sizeof(Left) + 16 * (int)sizeof(int);
 
 template <int DT, int D> static __device__ __forceinline__ void few_rows(const AttendArgs& a, unsigned char* smem, int w) {
   using E = Elem<DT>;
@@ -169,12 +174,15 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   const int least = max(1, kFewLeast >> a.few_shift);
   int total = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true);
-  const bool round = total <= kFewWorkgroups * least;
+  const bool round = total <= kFewWorkgroups * least, all_small = __builtin_amdgcn_ballot_w64(lanes.most > kFewLeast) == 0;
+  const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewLeast) != 0;
   if (!round) {
     total = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false);
   }
-  const int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
+  const int small = ((kFewLeast - 1) >> a.few_shift) + 1;  // units of a row tile that sees no more than kFewLeast
+  int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
+  if (all_small) each = (each + small - 1) / small * small;
   const int end = min((int64_t)total, (int64_t)(w + 1) * each);
   // The parts that this run leaves: of a row tile that began before it, and of one that goes on behind it.  They are counted when the
   // run is through, and not each on its own, which would keep the workgroup waiting for its stores (some 8 us a part).
@@ -182,22 +190,62 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   Left* left = (Left*)(smem + WAVES * WREG + WAVES * BM * sizeof(float2));
   if (tid < 2) left[tid].parts = 0;
 
-  for (int pos = w * each; pos < end;) {
-    Piece p;
-    if (a.c.batch <= 64) {
-      p.find(a, lanes, 0, pos);
-    } else {
-      for (int b0 = 0, before = 0; b0 < a.c.batch; b0 += 64) {
-        before = lanes.add(a, b0, before, round);
-        if (p.find(a, lanes, b0, pos)) break;
+  int (*counts)[WAVES] = (int (*)[WAVES])((unsigned char*)left + 2 * sizeof(Left));
+  for (int pos = w * each, turn = 0; pos < end; turn ^= 1) {
+    auto find = [&](Piece& p, int at) {
+      if (a.c.batch <= 64) {
+        p.find(a, lanes, 0, at);
+      } else {
+        for (int b0 = 0, before = 0; b0 < a.c.batch; b0 += 64) {
+          before = lanes.add(a, b0, before, round);
+          if (p.find(a, lanes, b0, at)) break;
+        }
       }
+    };
+    auto keys_at = [&](const Piece& p) {
+      const int first = p.tile * BM, last = min(first + BM, p.s.n * a.group) - 1;
+      return keys_of(p.s, quotient(first, a.by_group), quotient(last, a.by_group), a.causal, a.window, a.sinks);
+    };
+    // Where some of the next eight row tiles see little, each is a wave's own: they begin and end beside each other, and do not meet.  Against eight
+    // waves a row tile one after the other, that is `most` tiles in a wave instead of `in_row` beginnings and ends.  (Us alone and not: 94
+    // sequences of some six tokens, 8 KV heads 10 and 30; 81 of some 1 K and a window of 48, 32 heads, some with 40 new tokens 63 and
+    // 130; 110 of some 90 tokens, 4 heads 21 and 28.)
+    Piece p;
+    const int mine = pos + wave * small;  // (where this wave's begins if those before it are as small)
+    bool alone = false;
+    int in_row = 0;
+    if (some_small) {
+      int count = -1;
+      if (mine + small <= end) {
+        find(p, mine);
+        if (p.from == 0 && p.keys == small) count = keys_at(p).count;
+      }
+      counts[turn][wave] = count;
+      __syncthreads();
+      int most = 0;
+      bool on = true;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const int c = __builtin_amdgcn_readfirstlane(counts[turn][i]);
+        on = on && c >= 0;
+        if (on) {
+          ++in_row;
+          most = max(most, c);
+        }
+      }
+      alone = most <= 4 * (in_row - 1);
     }
-    const int upto = min(p.keys, p.from + (end - pos)), unit_begin = pos - p.from;
-    pos += upto - p.from;
+    if (!alone) find(p, pos);
+    else if (wave >= in_row) {
+      pos += in_row * small;
+      continue;
+    }
+    const int begin = alone ? mine : pos, upto = min(p.keys, p.from + (end - begin)), unit_begin = begin - p.from;
+    pos += alone ? in_row * small : upto - p.from;
     const int rows = p.s.n * a.group, head = p.head;
     const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
     const int i0 = quotient(r0, a.by_group), i1 = quotient(r_last, a.by_group);
-    const Keys keys = keys_of(p.s, i0, i1, a.causal, a.window, a.sinks);
+    const Keys keys = keys_at(p);
     auto tile_at_unit = [&](int u) { return p.keys == keys.count || u == 0 ? u : u == p.keys ? keys.count : (int)((int64_t)u * keys.count / p.keys); };
     const int u_begin = tile_at_unit(p.from), u_end = tile_at_unit(upto);
 
@@ -218,32 +266,38 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
 
     unsigned char* my = smem + wave * WREG;
     const unsigned my_lds = lds_offset(smem) + wave * WREG;
-    int koff[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) koff[ks] = n * ROWB + (((2 * ks + h) ^ k_swizzle<D>(n)) << 4);
-    int voff[DB];
+    const int koff0 = n * ROWB + ((h ^ k_swizzle<D>(n)) << 4);
+    auto koff = [&](int ks) {  // the number of the slice in bits that are free: one register, not eight (which would be kept elsewhere)
+      int o = koff0;
+      if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(32 * ks), "v"(koff0));
+      return o;
+    };
+    int voff0;
     {
       const int s = lane & 15, g1 = (lane >> 4) & 1;
-      const int row8 = 4 * h + (s >> 2);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const int c = 2 * (2 * db + g1) + ((s & 3) >> 1);
-        voff[db] = TILE + row8 * ROWB + ((c ^ v_swizzle<D>(row8)) << 4) + ((s & 1) << 3);
-      }
+      const int row8 = 4 * h + (s >> 2), c = 2 * g1 + ((s & 3) >> 1);
+      voff0 = TILE + row8 * ROWB + ((c ^ v_swizzle<D>(row8)) << 4) + ((s & 1) << 3);
     }
+    auto voff = [&](int db) {
+      int o = voff0;
+      if (db > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(64 * db), "v"(voff0));
+      return o;
+    };
     int goff_k[HALF], goff_v[HALF];
     half_tile_offsets<D>(goff_k, a.c.token_stride, [](int r) { return k_swizzle<D>(r); });
     half_tile_offsets<D>(goff_v, a.c.token_stride, [](int r) { return v_swizzle<D>(r); });
 
-    // ---- the tiles of this wave: u_begin + wave, + 8, ...
+    // ---- the tiles of this wave: u_begin + wave, + 8, ..., or all
+    const int stride_log = alone ? 0 : 3;
+    static_assert(WAVES == 8, "");
     const int* table = a.c.table + (int64_t)p.b * a.c.table_stride;
     auto real_tile = [&](int u) { return u < keys.sink_tiles ? u : u + keys.skip; };
     HeldPages held;
     int first_held = 0;
     auto hold_pages = [&](int u) {
       first_held = u;
-      const int mine = u + WAVES * lane;
-      held.hold(a.c, table, real_tile(mine) * BN, mine < u_end);
+      const int lanes_tile = u + (lane << stride_log);
+      held.hold(a.c, table, real_tile(lanes_tile) * BN, lanes_tile < u_end);
     };
     struct Tile {
       int key;             // its first key
@@ -251,10 +305,10 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       int64_t at0, at1;
     };
     auto tile_at = [&](int u) {
-      if (u - first_held >= 64 * WAVES) hold_pages(u);
+      if ((u - first_held) >> stride_log >= 64) hold_pages(u);
       Tile x;
       x.key = real_tile(u) * BN;
-      const int l = (u - first_held) / WAVES;
+      const int l = (u - first_held) >> stride_log;
       const int e0 = __builtin_amdgcn_readlane(held.page0, l), e1 = __builtin_amdgcn_readlane(held.page1, l);
       x.gone = (e0 < 0 ? 1 : 0) | (e1 < 0 ? 2 : 0);
       x.at0 = page_row(a.c, max(e0, 0), head, x.key);
@@ -312,7 +366,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       return bool((key >= lim) | ((key <= low) & (key >= a.sinks)) | (x.gone >> (e >> 3) & 1));  // (no branches)
     };
 
-    int u = u_begin + wave;
+    int u = u_begin + (alone ? 0 : wave);
     bool more = u < u_end;
     Tile cur{}, nxt{};
     if (more) {
@@ -323,14 +377,14 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
     }
     __builtin_amdgcn_s_waitcnt(0);  // retire the Q loads with a wait the compiler can see (and the first tiles)
     for (int pass = 1; more; pass = 0) {  // pass: 1 while there is no reference to take exponentials against
-      u += WAVES;
+      u += 1 << stride_log;
       more = u < u_end;
       if (more) nxt = tile_at(u);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");  // K is in, V may still be on its way
       {
         s16x8 kfr[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kfr[ks] = *(const s16x8*)(my + koff[ks]);
+        for (int ks = 0; ks < KS; ++ks) kfr[ks] = *(const s16x8*)(my + koff(ks));
         // the fragments are in registers: the K buffer takes the next tile
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
@@ -407,7 +461,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
         s16x8 vfr[2 * DB];
         auto read_v = [&](int f) {
           if (f >= 2 * DB) return;
-          const unsigned char* vrow = my + 16 * (f / DB) * ROWB + voff[f % DB];
+          const unsigned char* vrow = my + 16 * (f / DB) * ROWB + voff(f % DB);
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vrow));
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vrow + 8 * ROWB));
           vfr[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -427,6 +481,10 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       cur = nxt;
     }
 
+    if (alone) {
+      store_rows<DT, DB>(a, p.s, head, r0, r_last, oacc, 0, cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3])), ms);
+      continue;
+    }
     // This wave's state where the workgroup can read it: acc-O as fp32 over its own tiles, 16-byte chunk c of row n at chunk c ^ n.
     {
       const float l = cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));

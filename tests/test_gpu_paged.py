@@ -322,6 +322,24 @@ def test_shares_by_the_dozen(dtype, dim, heads, lens, news):
     assert torch.equal(out, again) and torch.equal(lse, lse_again)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (5, 0), (40, 3)])
+@pytest.mark.parametrize("dtype,dim,heads,hkv,batch,longest", [("bf16", 128, 16, 8, 60, 130), ("fp16", 64, 12, 12, 150, 40), ("bf16", 64, 32, 16, 50, 500)])
+def test_small_sequences_by_the_hundred(dtype, dim, heads, hkv, batch, longest, window, sinks):
+    # more row tiles than workgroups: those that see little are a wave's own, eight in a row or fewer, those that see more are not; sequences
+    # without anything new or without anything cached in between, pages that are not there, odd values in hidden places
+    lens = [(7 * i * i + 3 * i) % longest if i % 9 else longest * (i % 18 == 0) for i in range(batch)]
+    news = [0 if i % 11 == 3 else 1 + (i % 5 == 0) * (i % 7) for i in range(batch)]
+    for odd in (0.0, math.nan):
+        c = Case(dtype, dim, heads, hkv, 16, lens, news, window=window, sinks=sinks, seed=44, spare=odd)
+        if c.table.shape[1] > 2:
+            c.table[batch // 2, 1] = -1
+        _, out, lse = check_forward(c)
+        plan = plan_for(c)
+        again, lse_again = plan.forward(c.q.cuda(), *on_gpu(c))
+        rows = int(c.starts[-1])
+        assert torch.equal(out[:rows], again[:rows]) and torch.equal(lse[:, :rows], lse_again[:, :rows])
+
+
 @pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
                                                                   ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
 def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
