@@ -19,7 +19,7 @@ constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_m
 // 17 tokens 97 and 51, 32 tokens 71 and 52; 16 sequences of 4 K, 16 tokens (64 rows) 79 and 87, 17 tokens 155 and 83.  Weights, the
 // latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48 tokens 63 and 67.
 constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
-constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewMerge = 16;     // see few_rows
+constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewSmall = 32, kFewMerge = 16;     // see few_rows
 constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel

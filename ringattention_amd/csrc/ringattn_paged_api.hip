@@ -250,13 +250,17 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
   const int64_t few_tiles = rows / rp::kFewRows + sequences;
-  const int64_t see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile + rp::kFewLeast;
+  const int64_t see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile + rp::kFewSmall;
   while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
-  // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute
-  // units their keys are not shared out; else there is a share each, and no more besides than are due.
+  // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute units
+  // their keys are not shared out, unless some sequence may be much longer than others; else there is a share each, and no more besides than
+  // are due.  (Us with and without shares, 32 heads on 8 of 128: a chunk of 512 over 8 K, 64 row tiles, 91 and 193; 509 tokens over 2.3 K,
+  // 16 heads on 4, 34 and 65; prompts of 1 K, 32 heads, 128 row tiles, 50 and 44; eight chunks of 512, one over 32 K, seven over 1 K, 512
+  // row tiles, 347 and 742; 16 of them, one over 16 K, 1024 row tiles, 410 and 397.)
   const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < sequences ? might : sequences;
   const int64_t tiles = with_many > 0 ? rows / rp::kManyRows + with_many : 0, due = rp::kManyWorkgroups / kv + 1;
-  a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < rp::kManyWorkgroups;
+  const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see, most = see < in_window ? see : in_window;
+  a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < (most >= 512 ? 4 * rp::kManyWorkgroups : rp::kManyWorkgroups);
   RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, tiles + (a.many_cut ? due : 0), tiles < due ? tiles : due, stream));
   return RINGATTN_OK;
 }

@@ -16,16 +16,20 @@ __global__ __launch_bounds__(512, 2) void paged_attend_kernel(const AttendArgs a
   else many_rows<DT, D>(a, smem, blockIdx.x - a.few_workgroups);
 }
 
-template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void paged_merge_kernel(const AttendArgs a) { merge_many<DT, D>(a, blockIdx.x); }
+// As many workgroups as are at work at a time: how many row tiles were cut only the device knows.
+template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void paged_merge_kernel(const AttendArgs a) {
+  __shared__ float sums[2][kMergeSharers - 1][18][64];  // in turn, so that one barrier each suffices
+  for (int64_t block = blockIdx.x, turn = 0; block < INT32_MAX && merge_many<DT, D>(a, (int)block, sums[turn]); block += gridDim.x, turn ^= 1) {}
+}
 
 hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream) {
   const int64_t blocks = a.few_workgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) * (dim / 32) : 0;
   if (blocks <= 0) return hipSuccess;
-  if (blocks > INT32_MAX || merges > INT32_MAX) return hipErrorInvalidValue;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
 #define RA_LAUNCH_ATTEND(DT_, D_)                                                                             \
   do {                                                                                                       \
     paged_attend_kernel<DT_, D_><<<(unsigned)blocks, 512, 0, stream>>>(a);                                    \
-    if (merges > 0) paged_merge_kernel<DT_, D_><<<(unsigned)merges, 64 * kMergeSharers, 0, stream>>>(a);                  \
+    if (merges > 0) paged_merge_kernel<DT_, D_><<<(unsigned)(merges < 1024 ? merges : 1024), 64 * kMergeSharers, 0, stream>>>(a);                  \
   } while (0)
   if (dtype == 0 && dim == 64) RA_LAUNCH_ATTEND(0, 64);
   else if (dtype == 1 && dim == 64) RA_LAUNCH_ATTEND(1, 64);

@@ -21,7 +21,7 @@ struct Lanes {
   int tiles, keys;  // row tiles, and units of each (an upper bound of what its rows see, the same for all of a sequence)
   int upto;         // units of all sequences up to this one
   int most = 0, fewest = INT32_MAX;  // key tiles that a row tile of any sequence sees
-  // round: to multiples of kFewLeast
+  // round: to multiples of kFewLeast; else kFewSmall at least
   __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round) {
     const int lane = threadIdx.x & 63;
     s = Seq{0, 0, 0};
@@ -34,8 +34,7 @@ struct Lanes {
         most = max(most, keys);
         fewest = min(fewest, keys);
       }
-      keys = max(keys, kFewLeast);
-      if (round) keys = (keys + kFewLeast - 1) / kFewLeast * kFewLeast;
+      keys = round ? (keys + kFewLeast - 1) / kFewLeast * kFewLeast : max(keys, kFewSmall);
       keys = ((keys - 1) >> a.few_shift) + 1;
     }
     upto = before + wave_scan(tiles * keys * a.kv_heads);
@@ -168,21 +167,22 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   // The runs: `each` units of all of them.  Every wave works out for itself where its run lies, without a barrier; up to 64 sequences stay
   // in its registers.
   Lanes lanes;
-  // A row tile costs its beginning and end, some 5 us, whatever it sees: it counts as kFewLeast key tiles at least, and where runs of so
-  // many suffice for all, every row tile begins a run.  (Counted as what they see: 113 sequences of one token, 4 heads 79 us against 23;
-  // prompts of some 40 tokens, 39 of them, 2 KV heads 95 against 19.)
-  const int least = max(1, kFewLeast >> a.few_shift);
+  // Where runs of kFewLeast key tiles suffice for all, every row tile begins a run.  Elsewhere a row tile, whatever it sees, costs its
+  // beginning and end, some 5 us, and the parts' way through memory where a run ends inside it: it counts as kFewSmall key tiles at
+  // least, and where none sees more, runs are of whole row tiles.  (Us with neither, and with 16 and 32 for kFewSmall: 113 sequences of one
+  // token, 4 heads 79, 23, 10; 40 of 700, 8 KV heads -, 35, 30; 48 of some 3 K, 4 KV heads 75, 73, 70.  With 32 for kFewLeast one of 4 K, 8 KV
+  // heads takes 15 instead of 14, and one of 16 K has half as many workgroups.)
+  const int least = max(1, kFewLeast >> a.few_shift), small = max(1, kFewSmall >> a.few_shift);  // units
   int total = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true);
-  const bool round = total <= kFewWorkgroups * least, all_small = __builtin_amdgcn_ballot_w64(lanes.most > kFewLeast) == 0;
-  const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewLeast) != 0;
+  const bool round = total <= kFewWorkgroups * least, all_small = __builtin_amdgcn_ballot_w64(lanes.most > kFewSmall) == 0;
+  const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewSmall) != 0;
   if (!round) {
     total = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false);
   }
-  const int small = ((kFewLeast - 1) >> a.few_shift) + 1;  // units of a row tile that sees no more than kFewLeast
   int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
-  if (all_small) each = (each + small - 1) / small * small;
+  if (!round && all_small) each = (each + small - 1) / small * small;
   const int end = min((int64_t)total, (int64_t)(w + 1) * each);
   // The parts that this run leaves: of a row tile that began before it, and of one that goes on behind it.  They are counted when the
   // run is through, and not each on its own, which would keep the workgroup waiting for its stores (some 8 us a part).

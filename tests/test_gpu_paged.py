@@ -340,6 +340,21 @@ def test_small_sequences_by_the_hundred(dtype, dim, heads, hkv, batch, longest, 
         assert torch.equal(out[:rows], again[:rows]) and torch.equal(lse[:, :rows], lse_again[:, :rows])
 
 
+@pytest.mark.parametrize("lens,news", [((5000, 70, 0, 2100), (1, 1, 0, 1)), ((40,) * 12, (1,) * 12), ((3000, 9, 1500), (40, 9, 130))])
+def test_tables_with_room_for_very_long_sequences(lens, news):
+    # 2^30 tokens a sequence: the key tiles that there might be are dealt out several at a time, the few that there are all the same
+    c = Case("fp16", 64, 32, 32, 1024, lens, news, seed=45)
+    wide = torch.full((len(lens), 1 << 20), -1, dtype=torch.int32)
+    wide[:, :c.table.shape[1]] = c.table
+    plan = plan_for(c)
+    k, v, table, kv_lens, starts = on_gpu(c)
+    out, lse = plan.forward(c.q.cuda(), k, v, wide.cuda(), kv_lens, starts)
+    o, z, tol, tol_z = ref.attend(c)
+    rows = int(c.starts[-1])
+    near(out[:rows], o[:rows], tol[:rows], "out")
+    near(lse[:, :rows], z[:, :rows], tol_z[:, :rows], "lse")
+
+
 @pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
                                                                   ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
 def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
