@@ -365,7 +365,8 @@ int ringattn_paged_append(ringattn_paged_plan* plan, const ringattn_paged_cache*
  * is its token p = L - n + i and sees token j iff 0 <= j <= p (causal; else j < L), and, with a window, j > p - window or
  * j < sinks.  A query that sees nothing gets O = 0 and LSE = -inf.
  *   q   : [tokens, heads, dim] by strides (elements, multiples of 8)
- *   out : the same shape, by strides of its own; fp32 with RINGATTN_FLAG_PAGED_PARTIALS (strides multiples of 4)
+ *   out : the same shape, by strides of its own (token by token or head by head, with or without room between); fp32 with
+ *         RINGATTN_FLAG_PAGED_PARTIALS (strides multiples of 4)
  *   lse : [heads, tokens] fp32, natural log
  */
 int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,

@@ -54,7 +54,7 @@ int validate(const ringattn_paged_params* p) {
 // The workspace: counters, which are 0 between calls; then the parts of row tiles that several workgroups share.  A call that selects tokens
 // to keep has its counts where the parts lie.
 constexpr size_t kCounterBytes = rp::kWeightUnits * sizeof(int);
-static_assert(rp::kWeightUnits >= 2 * rp::kFewWorkgroups);
+static_assert(rp::kWeightUnits >= 2 * rp::kFewWorkgroups && rp::kWeightUnits * rp::kManyKeys <= rp::kFewSlots * rp::kFewRows * 64);
 size_t few_stat_bytes() { return (size_t)rp::kFewSlots * rp::kFewRows * sizeof(float2); }
 size_t many_stat_bytes() { return (size_t)rp::kManySlots * rp::kManyRows * sizeof(float2); }
 size_t few_o_bytes(int dim) { return (size_t)rp::kFewSlots * rp::kFewRows * dim * sizeof(float); }
@@ -83,7 +83,10 @@ int check_rows(const ringattn_paged_plan* pl, int tokens, int heads, int64_t ts,
   const int64_t most = (int64_t)1 << 36;
   if (ts < 0 || hs < 0 || ts > most || hs > most) return RINGATTN_ERR_SHAPE;
   if ((ts | hs) & (unit - 1)) return RINGATTN_ERR_ALIGN;
-  if (written && ((tokens > 1 && ts < pl->p.dim) || (heads > 1 && hs < pl->p.dim))) return RINGATTN_ERR_SHAPE;
+  const int64_t dim = pl->p.dim, heads_span = heads > 1 ? (heads - 1) * hs + dim : dim;
+  const double tokens_span = (double)(tokens - 1) * (double)ts + dim;  // (may pass 64 bits)
+  if (written && ((tokens > 1 && ts < dim) || (heads > 1 && hs < dim) || (tokens > 1 && heads > 1 && ts < heads_span && (double)hs < tokens_span)))
+    return RINGATTN_ERR_SHAPE;
   return RINGATTN_OK;
 }
 #define RP_CHECK(expr)                            \

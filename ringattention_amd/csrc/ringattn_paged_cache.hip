@@ -118,7 +118,8 @@ template <int DT, int D> struct WeightRows {
   // the new tokens [i0, i1) that see any of the keys [key0, key0 + keys)
   __device__ __forceinline__ void tokens_of(int key0, int keys, int& i0, int& i1) const {
     i0 = a.causal ? max(0, key0 - before) : 0;
-    i1 = a.window > 0 && key0 >= a.sinks ? min(s.n, key0 + keys - 1 + a.window - before) : s.n;
+    i1 = s.n;
+    if (a.window > 0 && key0 >= a.sinks) i1 = max(i0, (int)min((int64_t)s.n, (int64_t)key0 + keys - 1 + a.window - before));
   }
   // scores that weigh nothing: of row r, of the 16 keys that a lane has from key0 on
   __device__ __forceinline__ void hide(f32x16& sacc, int key0, int r) const {
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
     int seen_from = 0, seen_to = (x.rows - r_begin) / STEP;
     if (a.causal) seen_from = (max(0, key0 + kManyKeys - 1 - before - i0) * a.group + STEP - 1) / STEP;
     if (key0 + kManyKeys > s.len) seen_to = 0;
-    if (a.window > 0 && key0 + kManyKeys > a.sinks) seen_to = min(seen_to, clamped(key0 + a.window - before - i0, 0, s.n) * a.group / STEP);
+    if (a.window > 0 && key0 + kManyKeys > a.sinks) seen_to = min(seen_to, (int)max((int64_t)0, min((int64_t)s.n, (int64_t)key0 + a.window - before - i0)) * a.group / STEP);
     const unsigned seen = max(0, seen_to - seen_from);
     s16x8 kfr[2][KS];
 #pragma unroll

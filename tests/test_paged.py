@@ -121,6 +121,28 @@ def test_calls(ralib, memory):
     assert fwd(cache()) == E_PLAN
 
 
+def test_rows_of_out_do_not_lie_on_each_other(ralib, memory):
+    """Token by token or head by head, with or without room; a stride that has two rows in one place is refused before anything is launched."""
+    base, size = memory
+    h = ctypes.c_void_p()
+    assert ralib.ringattn_paged_plan_create(ctypes.byref(params()), ctypes.c_void_p(base), size, ctypes.byref(h)) == OK
+    x = base
+    c = dict(k=x, v=x, page_stride=2 * 16 * 64, head_stride=16 * 64, token_stride=64, pages=8, table_pages=4, table_stride=4, page_table=x, kv_lens=x,
+             q_starts=x)
+
+    def fwd(ot, oh, tokens=5, batch=0):   # (without sequences: checked, and nothing to do)
+        cache = ctypes.byref(RingattnPagedCache(batch=batch, **c))
+        return ralib.ringattn_paged_fwd(h, cache, x, tokens, 512, 64, x, ot, oh, x, None)
+
+    for ot, oh in ((512, 64), (64, 320), (1024, 64), (512 + 8, 64), (64, 328), (72, 360), (1024, 128), (2 ** 36, 64), (64, 2 ** 36)):
+        assert fwd(ot, oh) == OK, (ot, oh)
+    for ot, oh in ((64, 64), (504, 64), (64, 312), (128, 64), (64, 128), (448, 64), (512, 72)):
+        for batch in (0, 2):
+            assert fwd(ot, oh, batch=batch) == E_SHAPE, (ot, oh)
+    assert fwd(0, 64, tokens=1) == OK and fwd(64, 64, tokens=1) == OK
+    assert ralib.ringattn_paged_plan_destroy(h) == OK
+
+
 def test_tensors_that_do_not_fit(memory):
     plan = paged.PagedAttention(8, 64, kv_heads=2, page_size=16, max_batch=4, max_tokens=64, workspace=memory)
     assert plan.workspace_bytes() > 0
