@@ -392,6 +392,63 @@ def test_weights_of_missing_pages_and_rows_that_saw_nothing():
     near(scores, w + 0.5, off + 2.0 ** -24, "scores")
 
 
+def all_of(c, plan, gpu):
+    out, lse = plan.forward(c.q.cuda(), *gpu)
+    scores = torch.zeros(c.pages, c.kv_heads, c.page, device="cuda")
+    plan.weights(c.q.cuda(), lse, gpu[0], *gpu[2:], scores)
+    return out, lse, scores
+
+
+@pytest.mark.parametrize("lens,news", [((700, 33), (1, 1)), ((900, 40), (500, 40))])
+def test_a_window_that_reaches_past_everything(lens, news):
+    plain = Case("bf16", 64, 4, 2, 16, lens, news, seed=46)
+    gpu = on_gpu(plain)
+    want = all_of(plain, plan_for(plain), gpu)
+    for window, sinks in ((2 ** 30, 0), (2 ** 30, 2 ** 30), (900, 3), (5, 2 ** 30)):   # (the last: sinks that are everything)
+        c = Case("bf16", 64, 4, 2, 16, lens, news, window=window, sinks=sinks, seed=46)
+        got = all_of(c, plan_for(c), gpu)
+        for x, y in zip(got, want):
+            near(x, y.double().cpu(), 2.0 ** -7 * y.double().cpu().abs() + 2.0 ** -20, (window, sinks))
+
+
+@pytest.mark.parametrize("heads,hkv", [(40, 1), (33, 1), (14, 2), (130, 1)])
+@pytest.mark.parametrize("lens,news", [((300, 70), (1, 5)), ((200, 7), (90, 7))])
+def test_groups_of_any_size(heads, hkv, lens, news):
+    c = Case("fp16", 64, heads, hkv, 32, lens, news, seed=47)
+    check_forward(c)
+    clean = Case("fp16", 64, heads, hkv, 32, lens, news, seed=47, spare=0.0)
+    _, lse, scores = all_of(c, plan_for(c), on_gpu(c))
+    w, off = ref.weights(clean, lse.cpu())
+    near(scores, w, off, "scores")
+
+
+def test_as_many_sequences_as_a_call_may_have():
+    lens = [1 + (37 * i) % 50 for i in range(4096)]
+    news = [(i % 3 != 0) + (i % 512 == 5) * 20 for i in range(4096)]
+    news = [min(n, l) for n, l in zip(news, lens)]
+    c = Case("bf16", 64, 4, 2, 16, lens, news, seed=48)
+    check_forward(c)
+    clean = Case("bf16", 64, 4, 2, 16, lens, news, seed=48, spare=0.0)
+    plan, gpu = plan_for(c), on_gpu(c)
+    _, lse, scores = all_of(c, plan, gpu)
+    w, off = ref.weights(clean, lse.cpu())
+    near(scores, w, off, "scores")
+    # and their eviction to 16 tokens each: those that drew most, in their order
+    kept_table = torch.arange(4096, dtype=torch.int32).view(-1, 1) + c.pages
+    k = torch.cat([gpu[0], torch.zeros(4096, 2, 16, 64, dtype=gpu[0].dtype, device="cuda")])
+    v = torch.cat([gpu[1], torch.zeros(4096, 2, 16, 64, dtype=gpu[1].dtype, device="cuda")])
+    scores = torch.cat([scores, torch.zeros(4096, 2, 16, device="cuda")])
+    kept, kept_lens = plan.evict(k, v, scores, gpu[2], gpu[3], kept_table.cuda(), 16)
+    assert kept_lens.tolist() == [min(n, 16) for n in lens]
+    flat = scores.cpu()
+    for b in range(0, 4096, 37):
+        pages = c.table[b]
+        for g in range(2):
+            mine = torch.tensor([flat[pages[j // 16], g, j % 16].item() for j in range(lens[b])])
+            best = sorted(sorted(range(lens[b]), key=lambda j: (-mine[j].item(), j))[:16])
+            assert [x for x in kept[b, g].tolist() if x >= 0] == best, (b, g)
+
+
 def fill_scores(c, kind, seed):
     g = torch.Generator().manual_seed(seed)
     x = torch.randn(c.pages, c.kv_heads, c.page, generator=g)
