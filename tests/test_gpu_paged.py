@@ -607,6 +607,50 @@ def test_a_serving_loop():
                     held_k[b][h], held_v[b][h], drawn[b][h] = held_k[b][h][stay], held_v[b][h][stay], drawn[b][h][stay]
 
 
+def test_captured_calls_of_long_and_short_sequences():
+    """One graph, replayed with lengths that go every way: parts in two steps, row tiles of a wave's own, shares of many rows, rows of a block of
+    keys in parts -- and nothing at all; another plan's eager calls on the same workspace in between."""
+    heads, hkv, page, d, B, T, cap = 8, 1, 64, 64, 300, 800, 9000
+    g = torch.Generator().manual_seed(49)
+    pages = cap // page + 1
+    k, v = (torch.randn(2 * pages, hkv, page, d, generator=g).half().cuda() for _ in range(2))
+    table = torch.randint(0, 2 * pages, (B, pages), generator=g, dtype=torch.int32).cuda()   # (read only: shared as it falls)
+    q = torch.randn(T, heads, d, generator=g).half().cuda()
+    lens, starts = torch.zeros(B, dtype=torch.int32, device="cuda"), torch.zeros(B + 1, dtype=torch.int32, device="cuda")
+    room = torch.zeros(paged.PagedAttention(heads, d, kv_heads=hkv, max_batch=B, max_tokens=T).workspace_bytes(), dtype=torch.uint8, device="cuda")
+    made = dict(kv_heads=hkv, max_batch=B, max_tokens=T, workspace=(room.data_ptr(), room.numel()))
+    plan, other = paged.PagedAttention(heads, d, **made), paged.PagedAttention(heads, d, **made)
+    apart = paged.PagedAttention(heads, d, kv_heads=hkv, max_batch=B, max_tokens=T)
+    out, lse = torch.zeros_like(q), torch.zeros(heads, T, device="cuda")
+    own = torch.arange(2 * pages, dtype=torch.int32, device="cuda").view(2, pages)    # for the weights: no page twice
+    scores = torch.zeros(2 * pages, hkv, page, device="cuda")
+
+    def step(plan, out, lse, scores):
+        plan.forward(q, k, v, table, lens, starts, out=out, lse=lse)
+        plan.weights(q, lse, k, own, lens[:2], starts[:3], scores)
+
+    step(plan, out, lse, scores)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(plan, out, lse, scores)
+    for L, n in (([9000, 1], [1, 1]), ([5, 7], [1, 1]), ([9000, 8700], [300, 200]), ([1 + i % 60 for i in range(B)], [1] * B), ([], []), ([900, 8000], [600, 1]),
+                 ([9000, 1], [1, 1])):
+        L, n = L + [0] * (B - len(L)), n + [0] * (B - len(n))
+        lens.copy_(torch.tensor(L, dtype=torch.int32))
+        starts.copy_(torch.tensor([sum(n[:i]) for i in range(B + 1)], dtype=torch.int32))
+        want = [torch.zeros_like(x) for x in (out, lse, scores)]
+        step(apart, *want)
+        for x in (out, lse, scores):
+            x.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip((out, lse, scores), want)), L[:3]
+        got = [torch.zeros_like(x) for x in want]
+        step(other, *got)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), L[:3]
+
+
 def test_captured_calls_follow_the_lengths_on_the_device():
     """append, forward, weights and evict in one graph, replayed with other lengths, tokens and tables, with eager work in between."""
     heads, hkv, d, page, B = 8, 2, 128, 16, 4
