@@ -198,25 +198,17 @@ template <bool MERGE> static __device__ __forceinline__ bool find_place(const At
   return false;
 }
 
-// Parts go from workgroup to workgroup, which may sit on different XCDs with an L2 each: they are written through to and read from what all
-// XCDs share (relaxed atomics of agent scope, eight bytes each).  With plain accesses and fences instead, every fence writes back
-// an L2: one token over 128 K, 16 heads 202 us with 256 workgroups, 248 with 1024.
-static __device__ __forceinline__ void put8(void* to, uint64_t x) {
-  __hip_atomic_store((uint64_t*)to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-static __device__ __forceinline__ uint64_t get8(const void* from) {
-  return __hip_atomic_load((const uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
+// Parts go from workgroup to workgroup, which may sit on different XCDs with an L2 each: they are written through to what all XCDs share.
+// Who reads them makes its XCD's caches forget what they hold first (merge_parts), and then reads as usual.  With a release fence on the
+// writers' side each writes back an L2: one token over 128 K, 16 heads 202 us with 256 workgroups, 248 with 1024.  With reads past the
+// caches, eight bytes a lane, a row tile of 8 parts of 32 rows took 15 us to put together, 10 with a wave's beside each other, 4 so.
 static __device__ __forceinline__ void put_part(float* to, const f32x4& x) {
-  put8(to, __builtin_bit_cast(uint64_t, float2{x[0], x[1]}));
-  put8(to + 2, __builtin_bit_cast(uint64_t, float2{x[2], x[3]}));
+  // (the registers of a store of 16 bytes may not be written in the next cycle, which the compiler minds for stores of its own)
+  asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(to), "v"(x) : "memory");
 }
-static __device__ __forceinline__ f32x4 get_part4(const float* from) {
-  const float2 x = __builtin_bit_cast(float2, get8(from)), y = __builtin_bit_cast(float2, get8(from + 2));
-  return f32x4{x.x, x.y, y.x, y.y};
+static __device__ __forceinline__ void put_stat(float2* to, const float2& x) {
+  __hip_atomic_store((uint64_t*)to, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-static __device__ __forceinline__ void put_stat(float2* to, const float2& x) { put8(to, __builtin_bit_cast(uint64_t, x)); }
-static __device__ __forceinline__ float2 get_stat(const float2* from) { return __builtin_bit_cast(float2, get8(from)); }
 
 // Byte offset of row `key` of a page's KV head from the start of the pool.
 static __device__ __forceinline__ int64_t page_row(const Cache& c, int page, int head, int key) {
@@ -327,18 +319,24 @@ template <int D, class Swizzle> static __device__ __forceinline__ void half_tile
 }
 // Non-temporal: these rows are read once, and what all compute units have on the way at a time is as large as L2 (us with and without: 48
 // sequences of some 4 K tokens, 16/4 heads 74.8, 84.4; one of 128 K, 16 heads 190.6, 198.9).
-template <int HALF> static __device__ __forceinline__ void load_half_tile(const char* base, unsigned dst, const int (&goff)[HALF]) {
-  if constexpr (HALF == 4)
-    asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\t"
-        "global_load_lds_dwordx4 %3, %5 offset:2048 nt\n\tglobal_load_lds_dwordx4 %4, %5 offset:%6 nt" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
-        "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base), "n"(3 << 10)
-        : "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt" ::"s"(
-                     __builtin_amdgcn_readfirstlane(dst)),
-                 "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)
-                 : "m0");
+template <bool ONCE, int HALF> static __device__ __forceinline__ void load_half_tile(const char* base, unsigned dst, const int (&goff)[HALF]) {
+#define RA_LOAD(hint)                                                                                                                             \
+  do {                                                                                                                                            \
+    if constexpr (HALF == 4)                                                                                                                      \
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5" hint "\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024" hint      \
+                   "\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048" hint "\n\tglobal_load_lds_dwordx4 %4, %5 offset:%6" hint ::"s"(              \
+                       __builtin_amdgcn_readfirstlane(dst)),                                                                                      \
+                   "v"(goff[0]), "v"(goff[1]), "v"(goff[2 % HALF]), "v"(goff[3 % HALF]), "s"(base), "n"(3 << 10)                                  \
+                   : "m0");                                                                                                                       \
+    else                                                                                                                                          \
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3" hint "\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" hint ::"s"( \
+                       __builtin_amdgcn_readfirstlane(dst)),                                                                                      \
+                   "v"(goff[0]), "v"(goff[1 % HALF]), "s"(base)                                                                                   \
+                   : "m0");                                                                                                                       \
+  } while (0)
+  if constexpr (ONCE) RA_LOAD(" nt");
+  else RA_LOAD("");
+#undef RA_LOAD
 }
 
 // A launch of a.few_workgroups workgroups and `many_places` more for each KV head; a.many_cut: and one that puts together the row tiles

@@ -187,8 +187,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
   hold(u);
   int at = 0, p0, p1, next0 = 0, next1 = 0;  // place of tile u among the held ones; its pages
   auto issue = [&](int key, int slot, int page0, int page1) {
-    load_half_tile(a.c.k + page_row(a.c, max(page0, 0), head, key), my_lds + slot * TILE, goff);
-    load_half_tile(a.c.k + page_row(a.c, max(page1, 0), head, key + 16), my_lds + slot * TILE + TILE / 2, goff);
+    load_half_tile<true>(a.c.k + page_row(a.c, max(page0, 0), head, key), my_lds + slot * TILE, goff);
+    load_half_tile<true>(a.c.k + page_row(a.c, max(page1, 0), head, key + 16), my_lds + slot * TILE + TILE / 2, goff);
   };
   p0 = __builtin_amdgcn_readlane(held.page0, 0);
   p1 = __builtin_amdgcn_readlane(held.page1, 0);

@@ -56,18 +56,18 @@ struct Piece {
     keys = of(x.keys);
     const int at = pos - (of(x.upto) - of(x.tiles) * keys * a.kv_heads), unit = at / keys;
     from = at - unit * keys;
-    tile = quotient(unit, a.by_kv_heads);
-    head = unit - tile * a.kv_heads;
+    head = unit / of(x.tiles);
+    tile = unit - head * of(x.tiles);
     return true;
   }
 };
 
-// A part's row, eight columns of it.
+// A part's row, eight columns of it: 16 bytes of every thread beside each other, twice.
 template <int D> static __device__ __forceinline__ void put_row(const AttendArgs& a, int slot, int r, int c8, const float (&o)[8], float top, float l) {
   const int64_t prow = (int64_t)slot * kFewRows + r;
-  float* to = a.few.o + prow * D + c8 * 8;
+  float* to = a.few.o + prow * D + c8 * 4;
   put_part(to, f32x4{o[0], o[1], o[2], o[3]});
-  put_part(to + 4, f32x4{o[4], o[5], o[6], o[7]});
+  put_part(to + D / 2, f32x4{o[4], o[5], o[6], o[7]});
   if (c8 == 0) put_stat(a.few.stat + prow, float2{top, l});
 }
 
@@ -86,31 +86,33 @@ static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Se
   float top = -INFINITY, l = 0.f, o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  auto add = [&](float ref, float sum, const f32x4& x0, const f32x4& x1) {  // (a reference of -inf: nothing seen)
+    const float t = fmaxf(top, ref), z = t == -INFINITY ? 0.f : t, keep = __builtin_amdgcn_exp2f(top - z), w = __builtin_amdgcn_exp2f(ref - z);
+    l = ref == -INFINITY ? l : __builtin_fmaf(sum, w, l * keep);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = ref == -INFINITY ? o[e] : __builtin_fmaf(x0[e], w, o[e] * keep);
+      o[4 + e] = ref == -INFINITY ? o[4 + e] : __builtin_fmaf(x1[e], w, o[4 + e] * keep);
+    }
+    top = t;
+  };
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   if (r < count) {
-    constexpr int kBatch = 8;  // parts on their way together
+    constexpr int kBatch = 4;  // parts on their way together
+#pragma unroll 1
     for (int i = sub; i < parts; i += kBatch * sharers) {
       float2 st[kBatch];
       f32x4 x0[kBatch], x1[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int64_t prow = (int64_t)slot(min(i + j * sharers, parts - 1)) * kFewRows + r;
-        st[j] = get_stat(a.few.stat + prow);
-        const float* src = a.few.o + prow * D + c8 * 8;
-        x0[j] = get_part4(src);
-        x1[j] = get_part4(src + 4);
+        st[j] = a.few.stat[prow];
+        const float* src = a.few.o + prow * D + c8 * 4;
+        x0[j] = *(const f32x4*)src;
+        x1[j] = *(const f32x4*)(src + D / 2);
       }
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (i + j * sharers >= parts || st[j].x == -INFINITY) continue;  // (-inf: a part that saw nothing)
-        const float t = fmaxf(top, st[j].x), keep = __builtin_amdgcn_exp2f(top - t), w = __builtin_amdgcn_exp2f(st[j].x - t);
-        l = __builtin_fmaf(st[j].y, w, l * keep);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[e] = __builtin_fmaf(x0[j][e], w, o[e] * keep);
-          o[4 + e] = __builtin_fmaf(x1[j][e], w, o[4 + e] * keep);
-        }
-        top = t;
-      }
+      for (int j = 0; j < kBatch; ++j) add(i + j * sharers < parts ? st[j].x : -INFINITY, st[j].y, x0[j], x1[j]);
     }
   }
   if (sharers > 1) {
@@ -121,14 +123,10 @@ static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Se
     for (int e = 0; e < 8; ++e) mine[2 + e] = o[e];
     __syncthreads();
     if (sub == 0) {
+#pragma unroll 1
       for (int i = 1; i < sharers; ++i) {
         const float* x = sums[threadIdx.x + i * at_once * TPR];
-        if (x[0] == -INFINITY) continue;
-        const float t = fmaxf(top, x[0]), keep = __builtin_amdgcn_exp2f(top - t), w = __builtin_amdgcn_exp2f(x[0] - t);
-        l = __builtin_fmaf(x[1], w, l * keep);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(x[2 + e], w, o[e] * keep);
-        top = t;
+        add(x[0], x[1], f32x4{x[2], x[3], x[4], x[5]}, f32x4{x[6], x[7], x[8], x[9]});
       }
     }
   }
@@ -148,7 +146,7 @@ struct Left {
 };
 template <int D> constexpr int kFewLds = 8 * kFewWaveLds<D> + 8 * kFewRows * (int)sizeof(float2) + 2 * (int)sizeof(Left) + 16 * (int)sizeof(int);
 
-template <int DT, int D> static __device__ __forceinline__ void few_rows(const AttendArgs& a, unsigned char* smem, int w) {
+template <int DT, int D> static __device__ __forceinline__ void few_rows(const AttendArgs& a, unsigned char* smem, int block) {
   using E = Elem<DT>;
   constexpr int WAVES = 8, BM = kFewRows, BN = kKeyTile;
   constexpr int ROWB = D * 2, TILE = BN * ROWB;
@@ -183,10 +181,12 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   }
   int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
   if (!round && all_small) each = (each + small - 1) / small * small;
+  // Runs beside each other on one XCD, an eighth of them each: row tiles of a sequence's KV head, which read the same keys, find them in its L2.
+  const int runs = total > 0 ? (total - 1) / each + 1 : 0, of_xcd = (runs + 7) / 8, w = (block & 7) * of_xcd + (block >> 3);
+  if (block >> 3 >= of_xcd || w >= runs) return;
   const int end = min((int64_t)total, (int64_t)(w + 1) * each);
   // The parts that this run leaves: of a row tile that began before it, and of one that goes on behind it.  They are counted when the
   // run is through, and not each on its own, which would keep the workgroup waiting for its stores (some 8 us a part).
-  if (w * (int64_t)each >= total) return;
   Left* left = (Left*)(smem + WAVES * WREG + WAVES * BM * sizeof(float2));
   if (tid < 2) left[tid].parts = 0;
 
@@ -316,8 +316,13 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
       return x;
     };
     auto issue = [&](const char* pool, const Tile& x, unsigned dst, const int (&goff)[HALF]) {
-      load_half_tile(pool + x.at0, dst, goff);
-      load_half_tile(pool + x.at1, dst + TILE / 2, goff);
+      if (rows <= BM) {
+        load_half_tile<true>(pool + x.at0, dst, goff);
+        load_half_tile<true>(pool + x.at1, dst + TILE / 2, goff);
+      } else {  // other row tiles read them too
+        load_half_tile<false>(pool + x.at0, dst, goff);
+        load_half_tile<false>(pool + x.at1, dst + TILE / 2, goff);
+      }
     };
     auto issue_k = [&](const Tile& x) { issue(a.c.k, x, my_lds, goff_k); };
     auto issue_v = [&](const Tile& x) { issue(a.c.v, x, my_lds + TILE, goff_v); };
@@ -568,16 +573,21 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
     const Seq s = uniform(left[i].s);
     const int head = of(left[i].head), r0 = of(left[i].r0), rows = of(left[i].count), at = (w - first) & ~(kFewMerge - 1);
     auto slot = [&](int k) { return 2 * (first + k) + (k == 0 ? 1 : 0); };
-    if (parts > kFewMerge) {
-      merge_parts<DT, D>(a, s, head, r0, rows, min(kFewMerge, parts - at), [&](int k) { return slot(at + k); }, slot(at), (float (*)[10])smem);
-      settle();
-      if (tid == 0) left[i].last = count(a.few.arrived + first, (parts + kFewMerge - 1) / kFewMerge);
-      __syncthreads();
-      if (of(left[i].last) == 0) continue;
+    // (one piece of code for both steps: it is fetched as it is first run, and that takes longer than what it does)
+#pragma unroll 1
+    for (int step = parts > kFewMerge ? kFewMerge : 1; step > 0;) {
+      const bool whole = step == 1 && parts <= kFewMerge, group = step == kFewMerge;
+      const int from = group ? at : 0, by = whole || group ? 1 : kFewMerge;
+      const int n_parts = group ? min(kFewMerge, parts - at) : whole ? parts : (parts + kFewMerge - 1) / kFewMerge;
+      merge_parts<DT, D>(a, s, head, r0, rows, n_parts, [&](int k) { return slot(from + k * by); }, group ? slot(at) : -1, (float (*)[10])smem);
+      step = 0;
+      if (group) {
+        settle();
+        if (tid == 0) left[i].last = count(a.few.arrived + first, (parts + kFewMerge - 1) / kFewMerge);
+        __syncthreads();
+        step = of(left[i].last);
+      }
     }
-    const bool two = parts > kFewMerge;
-    merge_parts<DT, D>(a, s, head, r0, rows, two ? (parts + kFewMerge - 1) / kFewMerge : parts, [&](int k) { return slot(two ? k * kFewMerge : k); }, -1,
-                       (float (*)[10])smem);
     __syncthreads();
   }
 }
