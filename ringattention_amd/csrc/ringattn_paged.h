@@ -198,13 +198,16 @@ template <bool MERGE> static __device__ __forceinline__ bool find_place(const At
   return false;
 }
 
-// Parts go from workgroup to workgroup, which may sit on different XCDs with an L2 each: they are written through to what all XCDs share.
-// Who reads them makes its XCD's caches forget what they hold first (merge_parts), and then reads as usual.  With a release fence on the
-// writers' side each writes back an L2: one token over 128 K, 16 heads 202 us with 256 workgroups, 248 with 1024.  With reads past the
-// caches, eight bytes a lane, a row tile of 8 parts of 32 rows took 15 us to put together, 10 with a wave's beside each other, 4 so.
+// Parts go from workgroup to workgroup, which may sit on different XCDs with an L2 each: they are written through to and read from what all
+// XCDs share.  With a release fence on the writers' side each writes back an L2: one token over 128 K, 16 heads 202 us with 256 workgroups,
+// 248 with 1024; with an acquire fence on the readers' side each empties one: 48 single tokens over some 3 K 72 us instead of 70.
+// Read eight bytes a lane, a row tile of 8 parts of 32 rows took 15 us to put together, 10 with a wave's bytes beside each other, 4 with 16 a lane.
 static __device__ __forceinline__ void put_part(float* to, const f32x4& x) {
   // (the registers of a store of 16 bytes may not be written in the next cycle, which the compiler minds for stores of its own)
   asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(to), "v"(x) : "memory");
+}
+static __device__ __forceinline__ float2 get_stat(const float2* from) {
+  return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 static __device__ __forceinline__ void put_stat(float2* to, const float2& x) {
   __hip_atomic_store((uint64_t*)to, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -56,7 +56,7 @@ struct Piece {
     keys = of(x.keys);
     const int at = pos - (of(x.upto) - of(x.tiles) * keys * a.kv_heads), unit = at / keys;
     from = at - unit * keys;
-    head = unit / of(x.tiles);
+    head = of(x.tiles) == 1 ? unit : unit / of(x.tiles);
     tile = unit - head * of(x.tiles);
     return true;
   }
@@ -96,7 +96,9 @@ static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Se
     }
     top = t;
   };
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  // reads past the caches (bit 4 of the cache policy), 16 bytes a lane: as a buffer, whose loads the compiler waits for itself
+  const auto buffer = __builtin_amdgcn_make_buffer_rsrc(a.few.o, 0, kFewSlots * kFewRows * D * 4, 0x00027000);
+  auto fetch = [&](int at) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, at, 0, 16)); };
   if (r < count) {
     constexpr int kBatch = 4;  // parts on their way together
 #pragma unroll 1
@@ -105,11 +107,10 @@ static __device__ __forceinline__ void merge_parts(const AttendArgs& a, const Se
       f32x4 x0[kBatch], x1[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int64_t prow = (int64_t)slot(min(i + j * sharers, parts - 1)) * kFewRows + r;
-        st[j] = a.few.stat[prow];
-        const float* src = a.few.o + prow * D + c8 * 4;
-        x0[j] = *(const f32x4*)src;
-        x1[j] = *(const f32x4*)(src + D / 2);
+        const int prow = slot(min(i + j * sharers, parts - 1)) * kFewRows + r, at = prow * (D * 4) + c8 * 16;
+        st[j] = get_stat(a.few.stat + prow);
+        x0[j] = fetch(at);
+        x1[j] = fetch(at + D * 2);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) add(i + j * sharers < parts ? st[j].x : -INFINITY, st[j].y, x0[j], x1[j]);
@@ -182,7 +183,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
   if (!round && all_small) each = (each + small - 1) / small * small;
   // Runs beside each other on one XCD, an eighth of them each: row tiles of a sequence's KV head, which read the same keys, find them in its L2.
-  const int runs = total > 0 ? (total - 1) / each + 1 : 0, of_xcd = (runs + 7) / 8, w = (block & 7) * of_xcd + (block >> 3);
+  const int runs = round ? total >> __builtin_ctz(least) : (total - 1) / each + 1, of_xcd = (runs + 7) / 8, w = (block & 7) * of_xcd + (block >> 3);
   if (block >> 3 >= of_xcd || w >= runs) return;
   const int end = min((int64_t)total, (int64_t)(w + 1) * each);
   // The parts that this run leaves: of a row tile that began before it, and of one that goes on behind it.  They are counted when the
