@@ -19,6 +19,10 @@ constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_m
 // 17 tokens 97 and 51, 32 tokens 71 and 52; 16 sequences of 4 K, 16 tokens (64 rows) 79 and 87, 17 tokens 155 and 83.  Weights, the
 // latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48 tokens 63 and 67.
 constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
+// Of attention where there is little to do for all (ringattn_paged_fwd): us as many and as few, 32 heads on 8: four chunks of 64 over 1 K, 256 rows, 32
+// key tiles a workgroup 26 and 17; one over 8 K, 64 tiles 32 and 27; of 128, 512 rows, 128 tiles 40 and 40; 16 chunks of 24 over 4 K, 96 rows,
+// 187 tiles 109 and 127; four of 256 over 1 K, 1024 rows, 128 tiles 45 and 56.  8 heads, two chunks of 512 over 2 K, 64 tiles 34 and 23.
+constexpr int kFewRowsMore = 512, kFewMore = 96;
 constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewSmall = 32, kFewMerge = 16;     // see few_rows
 constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be

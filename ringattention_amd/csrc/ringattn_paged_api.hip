@@ -249,11 +249,14 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   a.sinks = plan->p.sinks;
   a.out_fp32 = fp32;
   const int64_t rows = (int64_t)tokens * group, sequences = cache->batch < tokens ? cache->batch : tokens;
-  a.few_most = few_most(tokens, cache->batch, rp::kFewRowsMost);
-  a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
-  // of few rows, every sequence has one row tile and one for 32 rows more; what they see at most, in so large units that 2^30 suffice
+  // What sequences see at most, in key tiles, and their row tiles if all have few rows; in units so large that 2^30 suffice for both.
   const int64_t few_tiles = rows / rp::kFewRows + sequences;
   const int64_t see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile + rp::kFewSmall;
+  const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see, most = see < in_window ? see : in_window;
+  // More rows are few where that cannot make more work than kFewMore key tiles a workgroup, whose parts are fewer and smaller.
+  const bool little = few_tiles * kv * most <= (int64_t)rp::kFewMore * rp::kFewWorkgroups;
+  a.few_most = few_most(tokens, cache->batch, little ? rp::kFewRowsMore : rp::kFewRowsMost);
+  a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
   // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute units
   // their keys are not shared out, unless some sequence may be much longer than others; else there is a share each, and no more besides than
@@ -262,7 +265,6 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   // row tiles, 347 and 742; 16 of them, one over 16 K, 1024 row tiles, 410 and 397.)
   const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < sequences ? might : sequences;
   const int64_t tiles = with_many > 0 ? rows / rp::kManyRows + with_many : 0, due = rp::kManyWorkgroups / kv + 1;
-  const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see, most = see < in_window ? see : in_window;
   a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < (most >= 512 ? 4 * rp::kManyWorkgroups : rp::kManyWorkgroups);
   RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, tiles + (a.many_cut ? due : 0), tiles < due ? tiles : due, stream));
   return RINGATTN_OK;
