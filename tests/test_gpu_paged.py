@@ -355,6 +355,32 @@ def test_tables_with_room_for_very_long_sequences(lens, news):
     near(lse[:, :rows], z[:, :rows], tol_z[:, :rows], "lse")
 
 
+def with_room(c, tokens=1 << 21):
+    """The same sequences in tables that might hold much longer ones: which kernel has what goes by what a call may hold."""
+    more = torch.full((len(c.lens), tokens // c.page - c.table.shape[1]), -1, dtype=torch.int32)
+    c.table = torch.cat([c.table, more], 1)
+    return c
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 0), (130, 35)])
+@pytest.mark.parametrize("lens,news", RAGGED + [((333, 90), (130, 66)), ((2200,), (70,)), ((515, 2, 700), (300, 1, 64))])
+def test_forward_in_tables_with_room(lens, news, window, sinks):
+    for dtype, dim, heads, hkv, page in (("bf16", 128, 8, 2, 16), ("fp16", 64, 4, 1, 64)):
+        check_forward(with_room(Case(dtype, dim, heads, hkv, page, lens, news, window=window, sinks=sinks, seed=50)))
+
+
+@pytest.mark.parametrize("lost", [2048, 2047, 31, 4000])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_missing_pages_and_odd_values_in_tables_with_room(lost, value):
+    c = with_room(Case("bf16", 128, 4, 2, 16, (4200,), (140,), seed=51))
+    c.table[0, lost // 16] = -1
+    c.v[int(c.table[0, 4195 // 16]), :, 4195 % 16:] = value   # hidden from all but the last rows
+    check_forward(c)
+    c = with_room(Case("fp16", 64, 8, 2, 32, (900, 300), (100, 90), window=100, sinks=3, seed=52))
+    c.v[int(c.table[0, 20]), :, 5:] = value                   # behind the windows of most rows
+    check_forward(c)
+
+
 @pytest.mark.parametrize("dtype,dim,heads,hkv,lens,news,causal", [("bf16", 128, 8, 2, (2000,), (2000,), True), ("fp16", 64, 8, 1, (2100, 700), (2000, 600), False),
                                                                   ("fp16", 64, 256, 32, (128,) * 10, (128,) * 10, True)])
 def test_weights_of_rows_shared_out(dtype, dim, heads, hkv, lens, news, causal):
