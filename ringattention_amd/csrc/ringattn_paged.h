@@ -15,9 +15,10 @@ namespace paged {
 constexpr int kKeyTile = 32;      // keys of a tile
 constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence's KV head has few of them (ringattn_paged_few.h)
 constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
-// Up to so many rows of a sequence's KV head are few.  Attention, us as few and as many, 32 heads on 8: one sequence of 32 K, 9 tokens 55 and 51,
-// 17 tokens 97 and 51, 32 tokens 71 and 52; 16 sequences of 4 K, 16 tokens (64 rows) 79 and 87, 17 tokens 155 and 83.  Weights, the
-// latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48 tokens 63 and 67.
+// Up to so many rows of a sequence's KV head are few.  Attention, us as few and as many, 32 heads on 8: one sequence of 32 K, 16 tokens (64 rows) 34
+// and 51, 24 tokens 78 and 51, 32 tokens 41 and 51, over 32800 58 and 50; 16 sequences of 4 K, 16 tokens 53 and 87, 24 tokens 129 and 105, 32
+// tokens 97 and 104.  Weights, the latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48
+// tokens 63 and 67.
 constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
 // Of attention where there is little to do for all (ringattn_paged_fwd): us as many and as few, 32 heads on 8: four chunks of 64 over 1 K, 256 rows, 32
 // key tiles a workgroup 26 and 17; one over 8 K, 64 tiles 32 and 27; of 128, 512 rows, 128 tiles 40 and 40; 16 chunks of 24 over 4 K, 96 rows,
@@ -147,7 +148,7 @@ static __device__ __forceinline__ float wave_sum(float x) {
 }
 
 // Many rows: the key tiles of a row tile are cut into even shares, so many that the whole launch makes about kManyWorkgroups workgroups,
-// each of kManyLeast tiles at least.
+// each of kManyLeast tiles at least.  (A chunk of 512 over 2 K, 8 heads, us with 8, 12, 16 and 32 tiles: 28, 31, 35, 45.)
 struct Place {
   Seq s;
   int b;
