@@ -20,6 +20,9 @@ constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_m
 // tokens 97 and 104.  Weights, the latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48
 // tokens 63 and 67.
 constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
+// Of one sequence alone, whose row tiles make even runs: 24 tokens (96 rows) over 32 K 39 as few and 52 as many, over 100 K 121 and 163; 32 tokens 43 and
+// 55, 137 and 148; 40 tokens 53 and 54, 157 and 146.
+constexpr int kFewRowsAlone = 128;
 // Of attention where there is little to do for all (ringattn_paged_fwd): us as many and as few, 32 heads on 8: four chunks of 64 over 1 K, 256 rows, 32
 // key tiles a workgroup 26 and 17; one over 8 K, 64 tiles 32 and 27; of 128, 512 rows, 128 tiles 40 and 40; 16 chunks of 24 over 4 K, 96 rows,
 // 187 tiles 109 and 127; four of 256 over 1 K, 1024 rows, 128 tiles 45 and 56.  8 heads, two chunks of 512 over 2 K, 64 tiles 34 and 23.

@@ -255,7 +255,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see, most = see < in_window ? see : in_window;
   // More rows are few where that cannot make more work than kFewMore key tiles a workgroup, whose parts are fewer and smaller.
   const bool little = few_tiles * kv * most <= (int64_t)rp::kFewMore * rp::kFewWorkgroups;
-  a.few_most = few_most(tokens, cache->batch, little ? rp::kFewRowsMore : rp::kFewRowsMost);
+  a.few_most = few_most(tokens, cache->batch, little ? rp::kFewRowsMore : cache->batch == 1 ? rp::kFewRowsAlone : rp::kFewRowsMost);
   a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
   // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute units

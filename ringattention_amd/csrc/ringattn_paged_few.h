@@ -21,8 +21,8 @@ struct Lanes {
   int tiles, keys;  // row tiles, and units of each (an upper bound of what its rows see, the same for all of a sequence)
   int upto;         // units of all sequences up to this one
   int most = 0, fewest = INT32_MAX;  // key tiles that a row tile of any sequence sees
-  // round: to multiples of kFewLeast; else kFewSmall at least
-  __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round) {
+  // round: to multiples of kFewLeast; else kFewSmall at least, or `fixed` of them
+  __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round, int fixed) {
     const int lane = threadIdx.x & 63;
     s = Seq{0, 0, 0};
     tiles = 0;
@@ -35,7 +35,7 @@ struct Lanes {
         fewest = min(fewest, keys);
       }
       keys = round ? (keys + kFewLeast - 1) / kFewLeast * kFewLeast : max(keys, kFewSmall);
-      keys = ((keys - 1) >> a.few_shift) + 1;
+      keys = fixed > 0 ? fixed : ((keys - 1) >> a.few_shift) + 1;
     }
     upto = before + wave_scan(tiles * keys * a.kv_heads);
     return __builtin_amdgcn_readlane(upto, 63);
@@ -173,15 +173,33 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   // heads takes 15 instead of 14, and one of 16 K has half as many workgroups.)
   const int least = max(1, kFewLeast >> a.few_shift), small = max(1, kFewSmall >> a.few_shift);  // units
   int total = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true);
+  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true, 0);
   const bool round = total <= kFewWorkgroups * least, all_small = __builtin_amdgcn_ballot_w64(lanes.most > kFewSmall) == 0;
   const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewSmall) != 0;
   if (!round) {
     total = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false);
+    for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false, 0);
   }
   int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
   if (!round && all_small) each = (each + small - 1) / small * small;
+  // Row tiles that all see as much -- one sequence, or several as long as each other -- are cut into as many runs each, where that takes no less
+  // than 7/8 of the workgroups, so that no run ends inside one.  (Us with and without, 32 heads on 8: 16 tokens over 32800 34 and 54, over 10000 21 and 34; 16 single
+  // tokens over 4 K, 4 KV heads 30 and 35; one over 50 K, 16 heads 77 and 84.)
+  int fixed = 0;
+  if (!round && !all_small) {
+    const uint64_t have = __builtin_amdgcn_ballot_w64(lanes.most > 0);
+    const int same = __builtin_amdgcn_readlane(lanes.most, __builtin_ctzll(have));
+    if (__builtin_amdgcn_ballot_w64(lanes.most > 0 && (lanes.most != same || lanes.fewest != same)) == 0) {
+      const int units = ((same - 1) >> a.few_shift) + 1, row_tiles = total / units, runs_each = kFewWorkgroups / max(row_tiles, 1);
+      if (row_tiles * runs_each >= kFewWorkgroups * 7 / 8) {
+        each = (units + runs_each - 1) / runs_each;
+        fixed = each * runs_each;
+        total = row_tiles * fixed;
+        lanes.upto = lanes.upto / units * fixed;
+        lanes.keys = fixed;
+      }
+    }
+  }
   // Runs beside each other on one XCD, an eighth of them each: row tiles of a sequence's KV head, which read the same keys, find them in its L2.
   const int runs = round ? total >> __builtin_ctz(least) : (total - 1) / each + 1, of_xcd = (runs + 7) / 8, w = (block & 7) * of_xcd + (block >> 3);
   if (block >> 3 >= of_xcd || w >= runs) return;
@@ -198,7 +216,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
         p.find(a, lanes, 0, at);
       } else {
         for (int b0 = 0, before = 0; b0 < a.c.batch; b0 += 64) {
-          before = lanes.add(a, b0, before, round);
+          before = lanes.add(a, b0, before, round, fixed);
           if (p.find(a, lanes, b0, at)) break;
         }
       }
