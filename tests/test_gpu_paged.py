@@ -355,6 +355,22 @@ def test_tables_with_room_for_very_long_sequences(lens, news):
     near(lse[:, :rows], z[:, :rows], tol_z[:, :rows], "lse")
 
 
+@pytest.mark.parametrize("dtype,dim,heads,hkv,lens,new,window", [("fp16", 64, 8, 1, (2000,) * 80, 1, 0), ("bf16", 128, 16, 8, (10000,), 24, 0), ("bf16", 64, 8, 8, (6000,) * 2, 3, 0),
+                                                                   ("fp16", 128, 32, 4, (5003,) * 5, 1, 0), ("fp16", 64, 16, 16, (4096,), 33, 2100)])
+def test_sequences_as_long_as_each_other(dtype, dim, heads, hkv, lens, new, window):
+    # their row tiles are cut into as many runs each, with a row tile counting as more than it sees where that does not go up
+    c = Case(dtype, dim, heads, hkv, 64, lens, (new,) * len(lens), window=window, seed=53)
+    c.table[0, 3] = -1
+    check_forward(c)
+    plan, gpu = plan_for(c), on_gpu(c)
+    out, lse = plan.forward(c.q.cuda(), *gpu)
+    again, lse_again = plan.forward(c.q.cuda(), *gpu)
+    assert torch.equal(out, again) and torch.equal(lse, lse_again)
+    # one of them shorter than the others
+    c.lens[-1] -= 1500
+    check_forward(c)
+
+
 def with_room(c, tokens=1 << 21):
     """The same sequences in tables that might hold much longer ones: which kernel has what goes by what a call may hold."""
     more = torch.full((len(c.lens), tokens // c.page - c.table.shape[1]), -1, dtype=torch.int32)
