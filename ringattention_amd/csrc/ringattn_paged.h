@@ -69,7 +69,7 @@ struct AttendArgs {
   int few_most;           // rows of a sequence's KV head up to which it has few
   int many_cut;           // whether key tiles are shared out where there are many rows
   int few_shift;          // few rows: key tiles are dealt out 2^few_shift at a time, so that 2^30 suffice
-  int few_workgroups;     // the launch's first workgroups have the sequences of few rows, the others those of many
+  int few_begin;          // workgroups [few_begin, few_begin + kFewWorkgroups) have the sequences of few rows, the others those of many
   Parts few, many;
 };
 
@@ -350,7 +350,7 @@ template <bool ONCE, int HALF> static __device__ __forceinline__ void load_half_
 #undef RA_LOAD
 }
 
-// A launch of a.few_workgroups workgroups and `many_places` more for each KV head; a.many_cut: and one that puts together the row tiles
+// A launch of kFewWorkgroups workgroups and `many_places` more for each KV head; a.many_cut: and one that puts together the row tiles
 // whose keys were shared out, of which there are up to `cut_tiles`.
 hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream);
 

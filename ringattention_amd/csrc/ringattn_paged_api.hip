@@ -256,7 +256,6 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   // More rows are few where that cannot make more work than kFewMore key tiles a workgroup, whose parts are fewer and smaller.
   const bool little = few_tiles * kv * most <= (int64_t)rp::kFewMore * rp::kFewWorkgroups;
   a.few_most = few_most(tokens, cache->batch, little ? rp::kFewRowsMore : cache->batch == 1 ? rp::kFewRowsAlone : rp::kFewRowsMost);
-  a.few_workgroups = sequences > 1 || rows <= a.few_most ? rp::kFewWorkgroups : 0;
   while (few_tiles * kv * (((see - 1) >> a.few_shift) + 1) > (int64_t)1 << 30) ++a.few_shift;
   // Row tiles of any lengths: every sequence of many rows begins one, and 256 rows more another.  Where they alone fill the compute units
   // their keys are not shared out, unless some sequence may be much longer than others; else there is a share each, and no more besides than
@@ -266,7 +265,11 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   const int64_t might = rows / ((int64_t)a.few_most + 1), with_many = might < sequences ? might : sequences;
   const int64_t tiles = with_many > 0 ? rows / rp::kManyRows + with_many : 0, due = rp::kManyWorkgroups / kv + 1;
   a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < (most >= 512 ? 4 * rp::kManyWorkgroups : rp::kManyWorkgroups);
-  RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, tiles + (a.many_cut ? due : 0), tiles < due ? tiles : due, stream));
+  const int64_t places = tiles + (a.many_cut ? due : 0);
+  // Workgroups of few rows first; of a sequence alone, whose rows are many if q is full, last, where they cost a full one next to nothing (us
+  // with and without them: 4096 tokens over 32 K, 32 heads 1867 and 1867; with a window of 1024, 8 KV heads 94.9 and 94.2).
+  a.few_begin = sequences == 1 ? (int)(places * kv) : 0;
+  RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, places, tiles < due ? tiles : due, stream));
   return RINGATTN_OK;
 }
 

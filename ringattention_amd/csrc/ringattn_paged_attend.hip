@@ -1,8 +1,9 @@
 // gfx950 (CDNA4) kernel: attention of new tokens over a paged cache (ringattn_paged_few.h and ringattn_paged_many.h hold the programs).
 //
-//   paged_attend_kernel : one launch for a whole batch.  Its first workgroups have the sequences of few query rows, a run of key tiles
+//   paged_attend_kernel : one launch for a whole batch.  256 of its workgroups have the sequences of few query rows, a run of key tiles
 //       each; the others those of many, 256 rows each.  A batch may have both -- a chunk of one prompt beside the next tokens of other
-//       sequences --, and which sequences have how many rows only the device knows.
+//       sequences --, and which sequences have how many rows only the device knows: also of a sequence alone, whose new tokens may be
+//       fewer than the rows of q.
 #include "ringattn_paged_few.h"
 #include "ringattn_paged_many.h"
 
@@ -12,8 +13,9 @@ namespace paged {
 template <int DT, int D>
 __global__ __launch_bounds__(512, 2) void paged_attend_kernel(const AttendArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kFewLds<D> > kManyLds<D> ? kFewLds<D> : kManyLds<D>];
-  if ((int)blockIdx.x < a.few_workgroups) few_rows<DT, D>(a, smem, blockIdx.x);
-  else many_rows<DT, D>(a, smem, blockIdx.x - a.few_workgroups);
+  const int few = (int)blockIdx.x - a.few_begin;
+  if ((unsigned)few < (unsigned)kFewWorkgroups) few_rows<DT, D>(a, smem, few);
+  else many_rows<DT, D>(a, smem, few < 0 ? (int)blockIdx.x : few - kFewWorkgroups);
 }
 
 // As many workgroups as are at work at a time: how many row tiles were cut only the device knows.
@@ -23,8 +25,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void p
 }
 
 hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream) {
-  const int64_t blocks = a.few_workgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) * (dim / 32) : 0;
-  if (blocks <= 0) return hipSuccess;
+  const int64_t blocks = kFewWorkgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) * (dim / 32) : 0;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
 #define RA_LAUNCH_ATTEND(DT_, D_)                                                                             \
   do {                                                                                                       \

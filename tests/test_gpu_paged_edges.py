@@ -1,0 +1,63 @@
+"""Calls of the paged cache's operators that their documentation allows and that are easily forgotten: sequences much shorter than the
+call's tensors, rows that are not numbers, outputs over inputs, lengths and starts that are not true.  Against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as ref
+from paged_reference import Case
+from test_gpu_paged import near, on_gpu, plan_for
+
+pytestmark = pytest.mark.gpu
+
+PADDED = 600   # rows of q of a call of one sequence, however few of them are its new tokens
+
+
+def padded_case(dtype, dim, heads, hkv, new, room, window=0, sinks=0, seed=60, spare=float("nan")):
+    """One sequence of 700 tokens, `new` of them new, q of PADDED rows; `room`: a table for 128 K tokens."""
+    c = Case(dtype, dim, heads, hkv, 16, (700,), (new,), window=window, sinks=sinks, seed=seed, extra_rows=PADDED - new, spare=spare)
+    if room:
+        table = torch.full((1, 8192), -1, dtype=torch.int32)
+        table[:, :c.table.shape[1]] = c.table
+        c.table = table
+    return c
+
+
+def check_padded_forward(c, out, lse):
+    new = c.news[0]
+    o, z, tol, tol_z = ref.attend(c)
+    near(out[:new], o[:new], tol[:new], "out")
+    near(lse[:, :new], z[:, :new], tol_z[:, :new], "lse")
+    assert (out[new:] == 7).all() and (lse[:, new:] == 7).all()
+
+
+@pytest.mark.parametrize("new", [0, 1, 5, 31, 32, 33, 127, 128, 129, 300, 600])
+@pytest.mark.parametrize("dtype,dim,heads,hkv,room,window,sinks", [("bf16", 128, 8, 2, False, 0, 0), ("fp16", 64, 4, 1, True, 0, 0), ("bf16", 64, 4, 4, True, 40, 3)])
+def test_forward_of_one_sequence_of_fewer_tokens_than_rows(new, dtype, dim, heads, hkv, room, window, sinks):
+    c = padded_case(dtype, dim, heads, hkv, new, room, window, sinks)
+    out, lse = torch.full_like(c.q, 7.0).cuda(), torch.full((heads, PADDED), 7.0, device="cuda")
+    plan_for(c).forward(c.q.cuda(), *on_gpu(c), out, lse)
+    check_padded_forward(c, out, lse)
+
+
+def test_captured_forward_of_a_prompts_last_chunk_and_next_tokens():
+    """Captured for whole chunks of one prompt, replayed for its short last one, for single tokens, for nothing, and for a whole one again."""
+    full = padded_case("bf16", 128, 8, 2, PADDED, True)
+    plan, (k, v, table, lens, starts), q = plan_for(full), on_gpu(full), full.q.cuda()
+    out, lse = torch.zeros_like(q), torch.zeros(8, PADDED, device="cuda")
+    plan.forward(q, k, v, table, lens, starts, out, lse)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        plan.forward(q, k, v, table, lens, starts, out, lse)
+    for new in (20, 1, 0, 32, 33, PADDED, 1):
+        c = padded_case("bf16", 128, 8, 2, new, True)
+        q.copy_(c.q), k.copy_(c.k), v.copy_(c.v), table.copy_(c.table), starts.copy_(c.starts)
+        out.fill_(7), lse.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_padded_forward(c, out, lse)
+        again, lse_again = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
+        plan.forward(q, k, v, table, lens, starts, again, lse_again)
+        assert torch.equal(again, out) and torch.equal(lse_again, lse)
