@@ -296,7 +296,10 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   a.causal = plan->p.causal != 0;
   a.window = plan->p.window;
   a.sinks = plan->p.sinks;
-  a.few_most = few_most(tokens, cache->batch, rp::kWeightFewRowsMost);
+  // One sequence has one launch: of few rows if q has few; else of many, also where its new tokens turn out to be fewer than the rows of q, so
+  // that none count as few.  (Us over 32 K, 32 heads on 8, new tokens in q of as many rows and of 512: 1 22 and 68, 16 33 and 67, 48 68 and 75.
+  // A second launch in every call of one sequence would take some 4.)
+  a.few_most = cache->batch == 1 && (int64_t)tokens * a.group > rp::kWeightFewRowsMost ? 0 : few_most(tokens, cache->batch, rp::kWeightFewRowsMost);
   a.arrived = (int*)plan->ws;
   a.parts = (float*)((char*)plan->ws + kCounterBytes);
   a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < 1 << 29;

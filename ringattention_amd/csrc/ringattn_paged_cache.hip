@@ -483,10 +483,11 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
   const int64_t pairs = (int64_t)a.c.batch * a.kv_heads;
   if (pairs <= 0 || keys <= 0) return hipSuccess;
   if (a.c.batch > 65535) return hipErrorInvalidValue;
-  // A launch for the sequences of few rows and one for those of many, where there may be any.  As many workgroups as the longest
-  // sequence could use, where that does not make them more than enough: they go on to further keys.  (Of many rows, 256 for one sequence, all of
-  // which has equal shares; of several, any may have few rows and leave its workgroups idle: 85 sequences of some 1 K tokens, ten of which
-  // have 60 to 100 new ones, 16 heads on 2: 181 us with 256, 62 with 1024.)
+  // A launch for the sequences of few rows and one for those of many, where there may be any; one sequence has one of the two, whichever its
+  // rows turn out to be (ringattn_paged_weights).  As many workgroups as the longest sequence could use, where that does not make them more
+  // than enough: they go on to further keys.  (Of many rows, 256 for one sequence, all of which has equal shares; of several, any may have few
+  // rows and leave its workgroups idle: 85 sequences of some 1 K tokens, ten of which have 60 to 100 new ones, 16 heads on 2: 181 us with
+  // 256, 62 with 1024.)
   const int64_t rows = (int64_t)a.c.tokens * a.group;
   auto grid = [&](int keys_each, int64_t sequences, int64_t enough) {
     const int64_t blocks = (keys + keys_each - 1) / keys_each, each = enough / (sequences * a.kv_heads);

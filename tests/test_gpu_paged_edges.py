@@ -61,3 +61,39 @@ def test_captured_forward_of_a_prompts_last_chunk_and_next_tokens():
         again, lse_again = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
         plan.forward(q, k, v, table, lens, starts, again, lse_again)
         assert torch.equal(again, out) and torch.equal(lse_again, lse)
+
+
+@pytest.mark.parametrize("new", [0, 1, 5, 47, 48, 49, 191, 192, 193, 600])
+@pytest.mark.parametrize("dtype,dim,heads,hkv,room,window,sinks", [("bf16", 128, 8, 2, False, 0, 0), ("fp16", 64, 4, 1, True, 0, 0), ("bf16", 64, 4, 4, True, 40, 3)])
+def test_weights_of_one_sequence_of_fewer_tokens_than_rows(new, dtype, dim, heads, hkv, room, window, sinks):
+    c = padded_case(dtype, dim, heads, hkv, new, room, window, sinks, spare=0.0)
+    lse = torch.zeros(heads, PADDED)
+    lse[:, :new] = ref.attend(c)[1][:, :new]
+    k, _, table, lens, starts = on_gpu(c)
+    scores = torch.full((c.pages, hkv, 16), 0.5, device="cuda")
+    plan_for(c).weights(c.q.cuda(), lse.cuda(), k, table, lens, starts, scores)
+    w, off = ref.weights(c, lse)
+    near(scores, w + 0.5, off + 2.0 ** -24 * (w + 0.5), "scores")
+
+
+def test_captured_weights_of_a_prompts_last_chunk_and_next_tokens():
+    full = padded_case("bf16", 128, 8, 2, PADDED, True, spare=0.0)
+    plan, (k, _, table, lens, starts), q = plan_for(full), on_gpu(full), full.q.cuda()
+    lse, scores = torch.zeros(8, PADDED, device="cuda"), torch.zeros(full.pages, 2, 16, device="cuda")
+    plan.weights(q, lse, k, table, lens, starts, scores)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        plan.weights(q, lse, k, table, lens, starts, scores)
+    for new in (20, 1, 0, 48, 49, PADDED, 1):
+        c = padded_case("bf16", 128, 8, 2, new, True, spare=0.0)
+        z = torch.zeros(8, PADDED)
+        z[:, :new] = ref.attend(c)[1][:, :new]
+        starts.copy_(c.starts), lse.copy_(z), scores.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        w, off = ref.weights(c, z)
+        near(scores, w, off, "scores")
+        again = torch.zeros_like(scores)
+        plan.weights(q, lse, k, table, lens, starts, again)
+        assert torch.equal(again, scores)
