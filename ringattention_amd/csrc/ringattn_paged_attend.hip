@@ -20,7 +20,9 @@ __global__ __launch_bounds__(512, 2) void paged_attend_kernel(const AttendArgs a
 
 // As many workgroups as are at work at a time: how many row tiles were cut only the device knows.
 template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void paged_merge_kernel(const AttendArgs a) {
-  __shared__ float sums[2][kMergeSharers - 1][18][64];  // in turn, so that one barrier each suffices
+  // In turn, so that one barrier each suffices: what one call of merge_many reads behind its barrier, the call after the next writes in front
+  // of its own, and between the two lies that of the next.
+  __shared__ float sums[2][kMergeSharers - 1][18][64];
   for (int64_t block = blockIdx.x, turn = 0; block < INT32_MAX && merge_many<DT, D>(a, (int)block, sums[turn]); block += gridDim.x, turn ^= 1) {}
 }
 

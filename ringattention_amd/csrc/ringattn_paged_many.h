@@ -420,7 +420,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
 // The shares of a row tile added up in an order of their own: a workgroup has 32 columns of the 32 rows of a wave, its waves every so-many-th
 // share.  (A chunk of 16 tokens, 128 K cached, 16 heads on one, 256 shares: 97 us with one wave for all shares and the four column blocks in a
 // workgroup, 69, 52 and 51 with two, four and eight waves and a workgroup for each; four sequences of 4 K, 64 tokens each, 8 shares:
-// 41, 40, 40 and 47.)  False behind the last.
+// 41, 40, 40 and 47.)  One barrier a call, whatever there is to do.  False behind the last.
 template <int DT, int D> static __device__ __forceinline__ bool merge_many(const AttendArgs& a, int block, float (*sums)[18][64]) {
   constexpr int BLOCKS = kManyRows / 32, DB = D / 32;
   const int lane = threadIdx.x & 63, n = lane & 31, sharer = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -428,7 +428,10 @@ template <int DT, int D> static __device__ __forceinline__ bool merge_many(const
   const int unit = quotient(block, a.by_kv_heads), head = block - unit * a.kv_heads, rows_of = unit / DB % BLOCKS, db = unit % DB;
   if (!find_place<true>(a, unit / (DB * BLOCKS), p)) return false;
   const int r0 = p.tile * kManyRows, r_last = min(r0 + kManyRows, p.s.n * a.group) - 1;
-  if (r0 + 32 * rows_of > r_last) return true;
+  if (r0 + 32 * rows_of > r_last) {  // (rows of no token: the same for all waves)
+    __syncthreads();
+    return true;
+  }
   const int64_t slot = (int64_t)p.slot * a.kv_heads + head;  // of share 0; those of the others are kv_heads apart
   float top = -INFINITY, l = 0.f;
   f32x16 acc[1];

@@ -7,7 +7,7 @@ import torch
 
 import paged_reference as ref
 from paged_reference import Case
-from test_gpu_paged import near, on_gpu, plan_for
+from test_gpu_paged import check_forward, near, on_gpu, plan_for
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,14 @@ def test_captured_weights_of_a_prompts_last_chunk_and_next_tokens():
         again = torch.zeros_like(scores)
         plan.weights(q, lse, k, table, lens, starts, again)
         assert torch.equal(again, scores)
+
+
+@pytest.mark.parametrize("dim,lens,news", [(128, (1024, 1000), (460, 460)), (64, (1024, 1000), (512, 530))])
+def test_shares_of_row_tiles_of_which_some_have_few_rows(dim, lens, news):
+    """More pieces of row tiles to put together than workgroups do it, so that one has several in turn -- one with rows, one without, one with rows."""
+    c = Case("bf16", dim, 32, 8, 64, lens, news, seed=66)
+    plan, out, lse = check_forward(c)
+    q, gpu = c.q.cuda(), on_gpu(c)
+    for _ in range(20):
+        again, lse_again = plan.forward(q, *gpu)
+        assert torch.equal(again, out) and torch.equal(lse_again, lse)
