@@ -387,7 +387,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
  * their order, to the pages of kept_table ([batch, kept_pages] by rows of kept_stride ints, entries of the same pools; kept_pages *
  * page_size >= budget), which share no page with page_table.  A sequence of no more than `budget` tokens is copied whole.
  *   kept      : [batch, kv_heads, budget] the places (in page_table) of the kept tokens, -1 behind the last
- *   kept_lens : [batch] min(kv_lens, budget): the kv_lens that go with kept_table
+ *   kept_lens : [batch] min(kv_lens, budget): the kv_lens that go with kept_table (may be the array kv_lens itself)
  * To the calls above the kept tokens are the tokens of the sequence: causality and windows count them, not what lay between them.
  */
 int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, float* scores, const int* kept_table, int kept_pages,

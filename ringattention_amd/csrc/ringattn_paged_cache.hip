@@ -669,9 +669,8 @@ static __device__ __forceinline__ Selection selection_of(const EvictArgs& a, int
   return x;
 }
 // The first and the last tokens, or all of a sequence that is short enough; the end of the list.  True if there is more to select.
-static __device__ __forceinline__ bool place_ends(const EvictArgs& a, const Selection& x, int head, int b) {
+static __device__ __forceinline__ bool place_ends(const EvictArgs& a, const Selection& x) {
   const int tid = threadIdx.x, stay = min(x.len, a.budget);
-  if (head == 0 && tid == 0) a.kept_lens[b] = stay;
   for (int j = stay + tid; j < a.budget; j += kSelectThreads) x.kept[j] = -1;
   if (x.len <= a.budget) {
     for (int j = tid; j < x.len; j += kSelectThreads) x.kept[j] = j;
@@ -688,7 +687,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   __shared__ unsigned shared[kSelectThreads / 64 + 2];
   const int head = blockIdx.x, b = blockIdx.y, hi = kBins - 1 - 2 * (int)threadIdx.x;
   Selection x = selection_of(a, head, b, 0, 1);
-  if (!place_ends(a, x, head, b)) return;
+  if (!place_ends(a, x)) return;
   Found f{0, x.wanted};
   for (int pass = 0; pass < kPasses; ++pass) {
     count_digits(a, x.table, head, x.s, pass == 0, pass, f.prefix, counts);
@@ -709,7 +708,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   const int lane = tid & 63, wave = tid >> 6;
   const int64_t pair = (int64_t)b * a.kv_heads + head;
   Selection x = selection_of(a, head, b, slice, slices);
-  if (PASS == 0 && slice == 0) place_ends(a, x, head, b);
+  if (PASS == 0 && slice == 0) place_ends(a, x);
   if (x.len <= a.budget || x.wanted == 0) return;
   unsigned* pair_counts = all_counts + pair * slices * (kPasses * kBins);
   unsigned* pair_above = all_above + pair * slices * kPasses;
@@ -758,12 +757,14 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   }
 }
 
-// 16 bytes a thread of a kept token's K and V.
+// 16 bytes a thread of a kept token's K and V.  The lengths are written here, not where tokens are selected: kept_lens may be the call's own lens,
+// which every workgroup of a selection reads, and here one that has been written already says the same.
 __global__ __launch_bounds__(256) void paged_move_kernel(const EvictArgs a, int row16) {
   const int head = blockIdx.y, b = blockIdx.z;
   const int rows = 256 / row16, c16 = threadIdx.x % row16;
   const int* kept = a.kept + ((int64_t)b * a.kv_heads + head) * a.budget;
   const int len = clamped(a.c.lens[b], 0, a.c.table_pages << a.c.page_shift), stay = min(len, a.budget);
+  if (head == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.kept_lens[b] = stay;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int mask = (1 << a.c.page_shift) - 1;
   for (int j = blockIdx.x * rows + threadIdx.x / row16; j < stay; j += gridDim.x * rows) {

@@ -228,7 +228,7 @@ class PagedAttention:
         """Copies `budget` tokens of every sequence -- its first keep_first, its last keep_last, and between them those of the largest
         scores, for each KV head its own -- with their scores to the pages of kept_table, which are in none of page_table.
         Returns (kept, kept_lens): the places the tokens had [batch, kv_heads, budget], -1 behind the last, and the lengths that go with
-        kept_table."""
+        kept_table (may be the tensor kv_lens itself)."""
         if kept is not None and kept_lens is not None and self._call_type:
             rc = (self._native.get(3) or self._made(3))(k_cache, v_cache, scores, page_table, kv_lens, kept_table, budget, keep_first, keep_last,
                                                         kept, kept_lens, stream)

@@ -108,3 +108,29 @@ def test_shares_of_row_tiles_of_which_some_have_few_rows(dim, lens, news):
     for _ in range(20):
         again, lse_again = plan.forward(q, *gpu)
         assert torch.equal(again, out) and torch.equal(lse_again, lse)
+
+
+@pytest.mark.parametrize("lens,budget,hkv", [((300, 20, 700, 64), 64, 4), ((21000, 9), 5000, 3), ((40,) * 200, 30, 8)])
+def test_kept_lengths_in_place_of_the_lengths(lens, budget, hkv):
+    """kept_lens may be kv_lens itself: a loop that goes on with the kept tokens has its lengths at once."""
+    page = 16
+    B, need = len(lens), [-(-n // page) for n in lens]
+    pages = sum(need) + B * -(-budget // page)
+    g = torch.Generator().manual_seed(64)
+    table = torch.full((B, max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(sum(need[:b]), sum(need[:b]) + n)
+    kept_table = (torch.arange(pages - sum(need), dtype=torch.int32) + sum(need)).reshape(B, -1).cuda()
+    k = torch.randn(pages, hkv, page, 64, generator=g).half().cuda()
+    scores = torch.rand(pages, hkv, page, generator=g).cuda()
+    results = []
+    for same in (False, True):
+        plan = plan_for(Case("fp16", 64, hkv, hkv, page, lens, (0,) * B, seed=65))
+        kv_lens = torch.tensor(lens, dtype=torch.int32).cuda()
+        k2, v2, s2 = k.clone(), -k, scores.clone()
+        kept = torch.full((B, hkv, budget), -7, dtype=torch.int32, device="cuda")
+        kept_lens = kv_lens if same else torch.zeros_like(kv_lens)
+        plan.evict(k2, v2, s2, table.cuda(), kv_lens, kept_table, budget, 2, 5, kept, kept_lens)
+        results.append([x.cpu() for x in (k2, v2, s2, kept, kept_lens)])
+    assert results[0][4].tolist() == [min(n, budget) for n in lens]
+    assert all(torch.equal(x, y) for x, y in zip(*results))
