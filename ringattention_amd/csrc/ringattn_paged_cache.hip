@@ -21,22 +21,20 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a, i
   const int c16 = (int)(item % row16);
   const int64_t th = item / row16;
   const int head = (int)(th % a.kv_heads), t = (int)(th / a.kv_heads);
-  // the sequence that token t is of: the last one that begins at or before it
+  // the sequence that token t is of: the last one that begins at or before it; its lengths and starts are held to the same as everywhere
   int lo = 0, hi = a.c.batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (a.c.starts[mid] <= t) lo = mid;
     else hi = mid;
   }
-  const int start = a.c.starts[lo], end = a.c.starts[lo + 1];
-  if (t < start || t >= end) return;  // in front of the first, behind the last
-  const int64_t key = (int64_t)a.c.lens[lo] - end + t;
-  const int64_t entry = key >> a.c.page_shift;
-  if (key < 0 || entry >= a.c.table_pages) return;
-  const int page = a.c.table[lo * a.c.table_stride + entry];
+  const Seq s = seq_of(a.c, lo);
+  const int i = t - s.start, key = s.len - s.n + i;
+  if (i < 0 || i >= s.n || key < 0) return;  // in front of the first, behind the last; more new tokens than there are tokens
+  const int page = a.c.table[lo * a.c.table_stride + (key >> a.c.page_shift)];
   if ((unsigned)page >= (unsigned)a.c.pages) return;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  const int64_t from = t * a.ts + head * a.hs + c16 * 16, to = page_row(a.c, page, head, (int)key) + c16 * 16;
+  const int64_t from = t * a.ts + head * a.hs + c16 * 16, to = page_row(a.c, page, head, key) + c16 * 16;
   const u32x4 x = *(const u32x4*)(a.k + from), y = *(const u32x4*)(a.v + from);
   *(u32x4*)(a.c.k + to) = x;
   *(u32x4*)(a.c.v + to) = y;

@@ -134,3 +134,41 @@ def test_kept_lengths_in_place_of_the_lengths(lens, budget, hkv):
         results.append([x.cpu() for x in (k2, v2, s2, kept, kept_lens)])
     assert results[0][4].tolist() == [min(n, budget) for n in lens]
     assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_append_and_forward_take_the_same_places():
+    """Lengths beyond the table and starts beyond the tokens are held to them, the same way by every call: what append wrote is what forward of the same
+    call takes for the new tokens."""
+    heads = hkv = 2
+    B, cap, page, d, T = 4, 4, 16, 64, 30
+    g = torch.Generator().manual_seed(62)
+    for lens, starts in (([100, 64, 10 ** 9, 40], [0, 5, 9, 20, 30]), ([64, 30, 50, 60], [0, 5, 9, 20, 1000]), ([64, 30, 50, 2 ** 31 - 1], [-9, 5, 9, 20, 2 ** 31 - 1]),
+                         ([30, 30, 30, 30], [0, 0, 0, 0, 31]), ([0, -5, 3, 64], [0, 2, 4, 9, 30])):
+        c = Case("bf16", d, heads, hkv, page, (cap * page,) * B, (0,) * B, seed=63, spare=0.0, extra_rows=T)
+        c.table = c.table[:, :cap].contiguous()
+        c.q = torch.randn(T, heads, d, generator=g).bfloat16()
+        new_k, new_v = (torch.randn(T, hkv, d, generator=g).bfloat16() for _ in range(2))
+        k, v, table, _, _ = on_gpu(c)
+        scores = torch.ones(c.pages, hkv, page, device="cuda")
+        l, s = torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda()
+        plan = plan_for(c)
+        plan.append(new_k.cuda(), new_v.cuda(), k, v, table, l, s, scores)
+        out, lse = torch.zeros(T, heads, d).bfloat16().cuda(), torch.zeros(heads, T, device="cuda")
+        plan.forward(c.q.cuda(), k, v, table, l, s, out, lse)
+        # the same with what is held to, by the definition
+        c.lens = [min(max(n, 0), cap * page) for n in lens]
+        held = [min(max(x, 0), T) for x in starts]
+        c.starts, c.news = torch.tensor(held, dtype=torch.int32), [held[b + 1] - held[b] for b in range(B)]
+        want_scores = torch.ones(c.pages, hkv, page)
+        for b in range(B):
+            for i in range(c.news[b]):
+                j = c.lens[b] - c.news[b] + i
+                if j >= 0:
+                    p = c.row(b, j)
+                    c.k[p, :, j % page], c.v[p, :, j % page], want_scores[p, :, j % page] = new_k[held[b] + i], new_v[held[b] + i], 0
+        assert torch.equal(k.cpu(), c.k) and torch.equal(v.cpu(), c.v) and torch.equal(scores.cpu(), want_scores), (lens, starts)
+        o, z, tol, tol_z = ref.attend(c)
+        rows = torch.zeros(T, dtype=torch.bool)
+        rows[held[0]:held[-1]] = True
+        near(out[rows], o[rows], tol[rows], "out")
+        near(lse[:, rows], z[:, rows], tol_z[:, rows], "lse")
