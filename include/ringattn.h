@@ -342,7 +342,8 @@ typedef struct ringattn_paged_cache {
   const int* page_table;    /* [batch, table_pages] */
   const int* kv_lens;       /* [batch] tokens of the sequence in the cache, the new ones of this call among them, as its last */
   const int* q_starts;      /* [batch + 1] ascending: the new tokens of sequence b are rows [q_starts[b], q_starts[b + 1]) of q,
-                               k_new and v_new; rows behind the last sequence are left as they were (not read by ringattn_paged_evict) */
+                               k_new and v_new; rows behind the last sequence are left as they were (not read by ringattn_paged_evict).
+                               Of starts that do not ascend only this is certain: nothing outside the tensors is read or written */
   int batch;
 } ringattn_paged_cache;
 

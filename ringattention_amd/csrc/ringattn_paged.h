@@ -77,7 +77,8 @@ struct Seq {
   int len, start, n;
 };
 static __device__ __forceinline__ int clamped(int x, int lo, int hi) { return min(max(x, lo), hi); }
-// Lengths are data: whatever they hold, nothing outside the tensors is touched.
+// Lengths are data: whatever they hold, nothing outside the tensors is touched.  (A sequence's own are held to its table and to the call's tokens
+// here; few_rows looks at what starts that do not ascend make of them all together.)
 static __device__ __forceinline__ Seq seq_of(const Cache& c, int b) {
   Seq s;
   s.len = clamped(c.lens[b], 0, c.table_pages << c.page_shift);

@@ -21,6 +21,7 @@ struct Lanes {
   int tiles, keys;  // row tiles, and units of each (an upper bound of what its rows see, the same for all of a sequence)
   int upto;         // units of all sequences up to this one
   int most = 0, fewest = INT32_MAX;  // key tiles that a row tile of any sequence sees
+  float news = 0.f;                  // new tokens of this lane's sequences
   // round: to multiples of kFewLeast; else kFewSmall at least, or `fixed` of them
   __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round, int fixed) {
     const int lane = threadIdx.x & 63;
@@ -29,6 +30,7 @@ struct Lanes {
     keys = 1;
     if (b0 + lane < a.c.batch) {
       s = seq_of(a.c, b0 + lane);
+      news += (float)s.n;
       load_of<false>(a, s, tiles, keys);
       if (tiles > 0) {
         most = max(most, keys);
@@ -174,6 +176,9 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   const int least = max(1, kFewLeast >> a.few_shift), small = max(1, kFewSmall >> a.few_shift);  // units
   int total = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true, 0);
+  // Starts that go down and up again have sequences share the call's tokens, and a.few_shift lets 32 bits suffice for sequences that do not: with
+  // as many new tokens in all as the call has, 2^30.  Where they have more than a few shared ones, nothing is done for those of few rows.
+  if (wave_sum(lanes.news) > 1.75f * a.c.tokens) return;
   const bool round = total <= kFewWorkgroups * least, all_small = __builtin_amdgcn_ballot_w64(lanes.most > kFewSmall) == 0;
   const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewSmall) != 0;
   if (!round) {

@@ -7,6 +7,7 @@ import torch
 
 import paged_reference as ref
 from paged_reference import Case
+from ringattention_amd import paged
 from test_gpu_paged import check_forward, near, on_gpu, plan_for
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +173,39 @@ def test_append_and_forward_take_the_same_places():
         rows[held[0]:held[-1]] = True
         near(out[rows], o[rows], tol[rows], "out")
         near(lse[:, rows], z[:, rows], tol_z[:, rows], "lse")
+
+
+def guarded(shape, dtype, value, room=1 << 18):
+    """(a tensor filled with `value`, the memory it is a part of, where it lies): `room` elements of a value of their own on both sides."""
+    n = math.prod(shape)
+    whole = torch.full((n + 2 * room,), 77, dtype=dtype, device="cuda")
+    whole[room:room + n] = value
+    return whole[room:room + n].view(shape), whole, slice(room, room + n)
+
+
+def untouched_outside(whole, inside):
+    return bool((whole[:inside.start] == 77).all()) and bool((whole[inside.stop:] == 77).all())
+
+
+def test_starts_that_go_up_and_down_thousands_of_times():
+    """2048 sequences that all claim the call's 64 tokens, each over a million cached ones whose pages are not there: 5 x 2^30 key tiles in all, far
+    more than tokens that are nobody's twice can have."""
+    B, T, heads, page, cap = 4096, 64, 40, 1024, 1024
+    plan = paged.PagedAttention(heads, 64, dtype="fp16", page_size=page, max_batch=B, max_tokens=T)
+    table = torch.full((B, cap), -1, dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), cap * page, dtype=torch.int32, device="cuda")
+    starts = torch.zeros(B + 1, dtype=torch.int32, device="cuda")
+    starts[1::2] = T
+    q = torch.zeros(T, heads, 64, dtype=torch.float16, device="cuda")
+    k = torch.zeros(1, heads, page, 64, dtype=torch.float16, device="cuda")
+    out, out_all, out_at = guarded((T, heads, 64), torch.float16, 5)
+    lse, lse_all, lse_at = guarded((heads, T), torch.float32, 5)
+    plan.forward(q, k, k, table, lens, starts, out, lse)
+    torch.cuda.synchronize()
+    assert untouched_outside(out_all, out_at) and untouched_outside(lse_all, lse_at)
+    # and the plan's next call is as good as any
+    starts.fill_(T)
+    starts[0] = 0
+    plan.forward(q, k, k, table, lens, starts, out, lse)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    assert untouched_outside(out_all, out_at) and untouched_outside(lse_all, lse_at)
