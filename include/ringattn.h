@@ -376,7 +376,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
 /*
  * Attention weight that the cached tokens have drawn: scores[page, kv head, row] += sum over the new tokens and the query heads of
  * the KV head of exp(scale q k - lse), for what ringattn_paged_fwd with the same cache, q and plan sees; lse as it wrote it (rows
- * of -inf weigh nothing).  scores: [pages, kv_heads, page_size] fp32.  cache->v is not read and may be NULL.  A page that
+ * of -inf weigh nothing, a row of NaN makes NaN of what it sees and of nothing else).  scores: [pages, kv_heads, page_size] fp32.  cache->v is not read and may be NULL.  A page that
  * several sequences share gets the weights of all of them, added in no certain order; without such pages every run gives the same bits.
  */
 int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,

@@ -119,8 +119,11 @@ template <int DT, int D> struct WeightRows {
     i1 = s.n;
     if (a.window > 0 && key0 >= a.sinks) i1 = max(i0, (int)min((int64_t)s.n, (int64_t)key0 + keys - 1 + a.window - before));
   }
-  // scores that weigh nothing: of row r, of the 16 keys that a lane has from key0 on
-  __device__ __forceinline__ void hide(f32x16& sacc, int key0, int r) const {
+  // scores that weigh nothing: of row r, of the 16 keys that a lane has from key0 on.  z: its log2(e) LSE.  One that is no number makes no
+  // number of -inf either, so that there the scores of the keys that the row sees are none, and z is 0.
+  __device__ __forceinline__ void hide(f32x16& sacc, int key0, int r, float& z) const {
+    const float none = z == z ? 0.f : z;
+    z = z == z ? z : 0.f;
     const int token = quotient(min(r, rows - 1), a.by_group);
     const int lim = r >= rows ? 0 : a.causal ? min(s.len, before + token + 1) : s.len;
     const int low = a.window > 0 ? before + token - a.window : -1;
@@ -129,7 +132,7 @@ template <int DT, int D> struct WeightRows {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int k = first + 8 * (e >> 2) + (e & 3);
-      sacc[e] = bool((k >= lim) | ((k <= low) & (k >= sinks))) ? -INFINITY : sacc[e];  // (no branches)
+      sacc[e] = bool((k >= lim) | ((k <= low) & (k >= sinks))) ? -INFINITY : sacc[e] + none;  // (no branches)
     }
   }
   __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse) const {
@@ -218,20 +221,21 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
-      x.hide(sacc, key0, n);
-      x.weigh(w, sacc, lse_first);
+      float z = lse_first;
+      x.hide(sacc, key0, n, z);
+      x.weigh(w, sacc, z);
     }
 #pragma unroll 1
     for (int r0 = 32; r0 < x.rows; r0 += 32) {
       const char* q = x.q_row(r0 + n) + h * 16;
-      const float lse = x.lse_of(r0 + n);
+      float z = x.lse_of(r0 + n);
       f32x16 sacc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(q + ks * 32), sacc);
-      x.hide(sacc, key0, r0 + n);
-      x.weigh(w, sacc, lse);
+      x.hide(sacc, key0, r0 + n, z);
+      x.weigh(w, sacc, z);
     }
     const float sum = sum_lanes(w);
     const int e = n >> 1;
@@ -390,10 +394,14 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
 #pragma unroll
         for (int c = 0; c < 2; ++c) sacc[c] = E::mma(kfr[c][ks], qfr[ks], sacc[c]);
     };
-    auto hide = [&](f32x16 (&sacc)[2], int step) {
+    auto hide = [&](f32x16 (&sacc)[2], int step, float& z) {
       if ((unsigned)(step - seen_from) >= seen) {
+        const float from = z;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) x.hide(sacc[c], my_key0 + 32 * c, r_begin + step * STEP + 32 * pair + n);
+        for (int c = 0; c < 2; ++c) {
+          z = from;
+          x.hide(sacc[c], my_key0 + 32 * c, r_begin + step * STEP + 32 * pair + n, z);
+        }
       }
     };
     auto weigh = [&](const f32x16 (&sacc)[2], float z) {
@@ -407,7 +415,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
     };
     auto both = [&](f32x16 (&next)[2], float& z_next, f32x16 (&sacc)[2], float z) {
       receive(z_next);
-      hide(sacc, t - 1);
+      hide(sacc, t - 1, z);
       __builtin_amdgcn_sched_barrier(0);
       multiply(next);
       weigh(sacc, z);
@@ -434,10 +442,10 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
       }
       if (t < t_end) {
         both(odd, z_odd, even, z_even);
-        hide(odd, t);
+        hide(odd, t, z_odd);
         weigh(odd, z_odd);
       } else {
-        hide(even, t - 1);
+        hide(even, t - 1, z_even);
         weigh(even, z_even);
       }
     }

@@ -209,3 +209,32 @@ def test_starts_that_go_up_and_down_thousands_of_times():
     plan.forward(q, k, k, table, lens, starts, out, lse)
     assert (out == 0).all() and (lse == -math.inf).all()
     assert untouched_outside(out_all, out_at) and untouched_outside(lse_all, lse_at)
+
+
+@pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 40, 3), (True, 5, 0), (False, 0, 0)])
+@pytest.mark.parametrize("lens,news", [((100, 40), (5, 30)), ((700,), (300,)), ((900, 90), (400, 1)), ((90, 33, 300), (1, 1, 1))])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_weights_of_rows_whose_lse_is_no_number(lens, news, causal, window, sinks, value):
+    """Their weights are no numbers where they see a key (0 for -inf), and nothing where they do not: later tokens, tokens in front of the window."""
+    for dtype, dim, heads, hkv in (("bf16", 128, 4, 2), ("fp16", 64, 3, 3)):
+        c = Case(dtype, dim, heads, hkv, 16, lens, news, window=window, sinks=sinks, causal=causal, seed=61, spare=0.0)
+        lse = ref.attend(c)[1].float()
+        at = [int(c.starts[b]) + n // 2 for b, n in enumerate(news)]   # a token in the middle of each chunk, one head of it
+        for i, t in enumerate(at):
+            lse[i % heads, t] = value
+        k, _, table, lens_, starts = on_gpu(c)
+        scores = torch.zeros(c.pages, hkv, 16, device="cuda")
+        plan_for(c).weights(c.q.cuda(), lse.cuda(), k, table, lens_, starts, scores)
+        clean = lse.clone()
+        for i, t in enumerate(at):
+            clean[i % heads, t] = -math.inf
+        w, off = ref.weights(c, clean)   # of all other rows
+        if value == math.inf:            # exp(s - inf) = 0
+            near(scores, w, off, "scores")
+            continue
+        for i, t in enumerate(at) if value != value else ():
+            b, g = i, i % heads // (heads // hkv)
+            _, there = c.rows(c.k, b, g)
+            for j in c.seen(b, there)[t - int(c.starts[b])].nonzero().flatten().tolist():
+                w[c.row(b, j), g, j % 16] = math.nan
+        near(scores, w, off, "scores")
