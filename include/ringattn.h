@@ -316,11 +316,12 @@ typedef struct ringattn_paged_params {
                             sequence: see RINGATTN_FLAG_PAGED_PARTIALS) */
   int window;            /* 0: no limit.  w > 0 (causal only): a token sees the last w tokens up to itself ... */
   int sinks;             /* ... and, with a window, the first `sinks` tokens of the sequence (up to itself) */
-  int flags;             /* RINGATTN_FLAG_PAGED_PARTIALS */
+  int flags;             /* RINGATTN_FLAG_PAGED_PARTIALS, RINGATTN_FLAG_PAGED_KEEP_PRESENT */
 } ringattn_paged_params;
 
 #define RINGATTN_FLAG_PAGED_PARTIALS 1 /* O is written as fp32, a partial for ringattn_merge: a sequence whose cache is spread
                                           over several pools (or GPUs) is attended pool by pool and merged by the LSEs */
+#define RINGATTN_FLAG_PAGED_KEEP_PRESENT 4 /* ringattn_paged_evict keeps no token whose page is not there */
 
 typedef struct ringattn_paged_plan ringattn_paged_plan;
 
@@ -390,6 +391,10 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
  *   kept      : [batch, kv_heads, budget] the places (in page_table) of the kept tokens, -1 behind the last
  *   kept_lens : [batch] min(kv_lens, budget): the kv_lens that go with kept_table (may be the array kv_lens itself)
  * To the calls above the kept tokens are the tokens of the sequence: causality and windows count them, not what lay between them.
+ * A token whose page is not there can be among those that stay: one of the first or the last, of a sequence that is copied whole, or of one that
+ * has too few others.  It has no row to copy, so that its row of the kept pages stays as it was -- and what that holds would be seen by the calls
+ * that go on with kept_table.  A caller that has given pages away makes its plan with RINGATTN_FLAG_PAGED_KEEP_PRESENT: such tokens rank below every
+ * score and are then taken out of the list, and kept_lens is how many are left (the same for each KV head).
  */
 int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, float* scores, const int* kept_table, int kept_pages,
                          int64_t kept_stride, int budget, int keep_first, int keep_last, int* kept, int* kept_lens, void* stream);

@@ -389,6 +389,7 @@ struct EvictArgs {
   int64_t kept_stride;
   int kept_pages;
   int budget, first, last;
+  int present;     // tokens whose page is not there do not stay
   int* kept;       // [batch, kv_heads, budget]
   int* kept_lens;  // [batch]
   int kv_heads;

@@ -46,7 +46,7 @@ int validate(const ringattn_paged_params* p) {
   if (p->max_tokens < 1 || (int64_t)p->max_tokens * p->heads > (int64_t)1 << 30) return RINGATTN_ERR_SHAPE;
   if (p->window < 0 || p->sinks < 0 || p->window > 1 << 30 || p->sinks > 1 << 30) return RINGATTN_ERR_SHAPE;
   if ((p->window > 0 && !p->causal) || (p->sinks > 0 && p->window == 0)) return RINGATTN_ERR_SHAPE;
-  if (p->flags & ~RINGATTN_FLAG_PAGED_PARTIALS) return RINGATTN_ERR_SHAPE;
+  if (p->flags & ~(RINGATTN_FLAG_PAGED_PARTIALS | RINGATTN_FLAG_PAGED_KEEP_PRESENT)) return RINGATTN_ERR_SHAPE;
   if (!std::isfinite(p->softmax_scale)) return RINGATTN_ERR_SHAPE;
   return RINGATTN_OK;
 }
@@ -327,6 +327,7 @@ int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* 
   a.budget = budget;
   a.first = keep_first;
   a.last = keep_last;
+  a.present = (plan->p.flags & RINGATTN_FLAG_PAGED_KEEP_PRESENT) != 0;
   a.kept = kept;
   a.kept_lens = kept_lens;
   a.workspace = (char*)plan->ws + kCounterBytes;

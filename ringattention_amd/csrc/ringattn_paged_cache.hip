@@ -8,6 +8,7 @@
 //       same bits in every run.
 //   paged_select_kernel  : the places of a sequence's KV head that stay.  The budget-th largest score is found by its bits, from the
 //       highest on, in counts of how many scores share the bits so far.
+//   paged_present_kernel : takes those whose page is not there out of them, where they are not to stay.
 //   paged_move_kernel    : K, V and scores of the kept tokens to the pages of the table that is to hold them.
 #include "ringattn_paged.h"
 
@@ -518,7 +519,7 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
 }
 
 // ---- eviction ----------------------------------------------------------------------
-// Larger scores have larger ranks; a NaN and a token whose page is not there rank with -inf.
+// Larger scores have larger ranks; a NaN ranks with -inf, and so does a token whose page is not there, or below it where such are not to stay.
 static __device__ __forceinline__ unsigned rank_of(float x) {
   if (!(x == x)) x = -INFINITY;
   const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);  // (-0 as 0)
@@ -544,6 +545,7 @@ struct Slice {
 // Ranks of up to kHeld tokens of a thread, from key0 on.  All pages first, then all scores, with nothing in between that a lane might skip.
 static __device__ __forceinline__ void load_ranks(const EvictArgs& a, const int* table, int head, int key0, int end, unsigned (&r)[kHeld]) {
   const int mask = (1 << a.c.page_shift) - 1;
+  const unsigned gone = a.present ? 0 : rank_of(-INFINITY);
   auto key_at = [&](int i) { return max(min(key0 + i * kSelectThreads + (int)threadIdx.x, end - 1), 0); };
   int page[kHeld];
   float x[kHeld];
@@ -555,7 +557,7 @@ static __device__ __forceinline__ void load_ranks(const EvictArgs& a, const int*
     x[i] = a.scores[(((int64_t)there * a.kv_heads + head) << a.c.page_shift) + (key_at(i) & mask)];
   }
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) r[i] = rank_of((unsigned)page[i] < (unsigned)a.c.pages ? x[i] : -INFINITY);
+  for (int i = 0; i < kHeld; ++i) r[i] = (unsigned)page[i] < (unsigned)a.c.pages ? rank_of(x[i]) : gone;
 }
 // fn(first key, ranks) for every kHeld x kSelectThreads tokens of a slice
 template <class Fn> static __device__ __forceinline__ void each_ranks(const EvictArgs& a, const int* table, int head, Slice& s, bool first, Fn fn) {
@@ -763,14 +765,42 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
   }
 }
 
+// Where only tokens whose page is there are to stay: the others out of the list, which is as long for all KV heads, since they rank below everything.
+// A thread a place, 1024 at a time, and written no further than it has been read.  (Two dependent reads a turn, some 0.9 us: of the evictions in the
+// table the batch to 4 K tokens takes 4 us more, the long one to 32 K 29.)
+__global__ __launch_bounds__(kSelectThreads) void paged_present_kernel(const EvictArgs a) {
+  __shared__ int counts[2][kSelectThreads / 64];  // in turn, so that one barrier each suffices
+  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int* kept = a.kept + ((int64_t)b * a.kv_heads + head) * a.budget;
+  const int* table = a.c.table + b * a.c.table_stride;
+  int placed = 0;
+  for (int j0 = 0, turn = 0; j0 < a.budget; j0 += kSelectThreads, turn ^= 1) {
+    const int key = j0 + tid < a.budget ? kept[j0 + tid] : -1;
+    const bool there = key >= 0 && (unsigned)table[key >> a.c.page_shift] < (unsigned)a.c.pages;
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(there);
+    if (lane == 0) counts[turn][wave] = __builtin_popcountll(mine);
+    __syncthreads();
+    int front = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSelectThreads / 64; ++i) {
+      front += i < wave ? counts[turn][i] : 0;
+      all += counts[turn][i];
+    }
+    if (there) kept[placed + front + __builtin_popcountll(mine & (((uint64_t)1 << lane) - 1))] = key;
+    placed += all;
+  }
+  for (int j = placed + tid; j < a.budget; j += kSelectThreads) kept[j] = -1;
+  if (head == 0 && tid == 0) a.kept_lens[b] = placed;  // (which may be the call's own lens: nothing here goes by those)
+}
+
 // 16 bytes a thread of a kept token's K and V.  The lengths are written here, not where tokens are selected: kept_lens may be the call's own lens,
 // which every workgroup of a selection reads, and here one that has been written already says the same.
 __global__ __launch_bounds__(256) void paged_move_kernel(const EvictArgs a, int row16) {
   const int head = blockIdx.y, b = blockIdx.z;
   const int rows = 256 / row16, c16 = threadIdx.x % row16;
   const int* kept = a.kept + ((int64_t)b * a.kv_heads + head) * a.budget;
-  const int len = clamped(a.c.lens[b], 0, a.c.table_pages << a.c.page_shift), stay = min(len, a.budget);
-  if (head == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.kept_lens[b] = stay;
+  const int stay = a.present ? a.kept_lens[b] : min(clamped(a.c.lens[b], 0, a.c.table_pages << a.c.page_shift), a.budget);
+  if (!a.present && head == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.kept_lens[b] = stay;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int mask = (1 << a.c.page_shift) - 1;
   for (int j = blockIdx.x * rows + threadIdx.x / row16; j < stay; j += gridDim.x * rows) {
@@ -812,6 +842,7 @@ hipError_t launch_paged_evict(const EvictArgs& a, int dim, hipStream_t stream) {
     paged_select_slices_kernel<2><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
     paged_select_slices_kernel<3><<<grid, kSelectThreads, 0, stream>>>(a, counts, above, found);
   }
+  if (a.present) paged_present_kernel<<<dim3((unsigned)a.kv_heads, (unsigned)a.c.batch), kSelectThreads, 0, stream>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int rows = 256 / (dim / 8);

@@ -22,6 +22,7 @@ from ._lib import RingattnPagedCache, RingattnPagedParams, check
 from .api import DTYPE_CODE, TORCH_DTYPE, _check_tensors, _stream_ptr
 
 FLAG_PAGED_PARTIALS = 1
+FLAG_PAGED_KEEP_PRESENT = 4
 
 
 def _check_rows(*specs):
@@ -54,11 +55,12 @@ class PagedAttention:
 
     `window` > 0: a token sees the last `window` tokens up to itself and the first `sinks` of the sequence.  `causal=False`:
     it sees every cached token; `partials`: out is float32, a partial (O, LSE) for api.merge -- together, for a sequence whose cache is
-    spread over several pools or GPUs.  `workspace`: a (device address, bytes) pair the caller owns and keeps alive, instead of an
-    allocation by the plan.  One call at a time, and replays of captured calls in turn: they share the plan's workspace."""
+    spread over several pools or GPUs.  `keep_present`: evict() keeps no token whose page is not there.  `workspace`: a (device
+    address, bytes) pair the caller owns and keeps alive, instead of an allocation by the plan.  One call at a time, and replays of
+    captured calls in turn: they share the plan's workspace."""
 
     def __init__(self, heads, dim, kv_heads=0, dtype="fp16", page_size=64, max_batch=64, max_tokens=8192, causal=True, softmax_scale=0.0,
-                 window=0, sinks=0, partials=False, workspace=None):
+                 window=0, sinks=0, partials=False, workspace=None, keep_present=False):
         self.lib = _lib.load()
         self.heads, self.dim, self.kv_heads, self.page_size = int(heads), int(dim), int(kv_heads) or int(heads), int(page_size)
         self.max_batch, self.max_tokens = int(max_batch), int(max_tokens)
@@ -66,7 +68,8 @@ class PagedAttention:
         self.torch_dtype = TORCH_DTYPE[code]
         self.out_dtype = torch.float32 if partials else self.torch_dtype
         self.params = RingattnPagedParams(self.dim, self.heads, int(kv_heads), code, float(softmax_scale), self.page_size, self.max_batch,
-                                          self.max_tokens, int(bool(causal)), int(window), int(sinks), FLAG_PAGED_PARTIALS if partials else 0)
+                                          self.max_tokens, int(bool(causal)), int(window), int(sinks),
+                                          (FLAG_PAGED_PARTIALS if partials else 0) | (FLAG_PAGED_KEEP_PRESENT if keep_present else 0))
         self.handle = ctypes.c_void_p()
         self.device = torch.cuda.current_device() if workspace is None and torch.cuda.is_available() else None
         ws_ptr, ws_bytes = (None, 0) if workspace is None else (ctypes.c_void_p(int(workspace[0])), int(workspace[1]))
@@ -228,7 +231,11 @@ class PagedAttention:
         """Copies `budget` tokens of every sequence -- its first keep_first, its last keep_last, and between them those of the largest
         scores, for each KV head its own -- with their scores to the pages of kept_table, which are in none of page_table.
         Returns (kept, kept_lens): the places the tokens had [batch, kv_heads, budget], -1 behind the last, and the lengths that go with
-        kept_table (may be the tensor kv_lens itself)."""
+        kept_table (may be the tensor kv_lens itself).
+
+        A token that stays although its page is not there -- of a short sequence, or of the first or last -- is not copied: its row of the
+        kept pages holds what it held, and would be seen.  Where pages have been given away, make the plan with keep_present: kept_lens is
+        then what is left of min(kv_lens, budget) without such tokens."""
         if kept is not None and kept_lens is not None and self._call_type:
             rc = (self._native.get(3) or self._made(3))(k_cache, v_cache, scores, page_table, kv_lens, kept_table, budget, keep_first, keep_last,
                                                         kept, kept_lens, stream)

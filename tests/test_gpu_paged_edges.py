@@ -8,7 +8,7 @@ import torch
 import paged_reference as ref
 from paged_reference import Case
 from ringattention_amd import paged
-from test_gpu_paged import check_forward, near, on_gpu, plan_for
+from test_gpu_paged import check_forward, fill_scores, near, on_gpu, plan_for
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +238,94 @@ def test_weights_of_rows_whose_lse_is_no_number(lens, news, causal, window, sink
             for j in c.seen(b, there)[t - int(c.starts[b])].nonzero().flatten().tolist():
                 w[c.row(b, j), g, j % 16] = math.nan
         near(scores, w, off, "scores")
+
+
+def kept_present(scores, there, budget, first, last):
+    """Places that stay of one sequence's KV head where only tokens that are there do."""
+    L, there = len(scores), there.tolist()
+    if L <= budget:
+        return [j for j in range(L) if there[j]]
+    value = [-math.inf if math.isnan(x) else x for x in scores.tolist()]
+    middle = sorted((j for j in range(first, L - last) if there[j]), key=lambda j: (-value[j], j))[:budget - first - last]
+    return sorted([j for j in [*range(first), *range(L - last, L)] if there[j]] + middle)
+
+
+@pytest.mark.parametrize("kind", ["exp", "odd", "zeros"])
+@pytest.mark.parametrize("lens,budget,first,last,hkv", [((300, 20, 700, 64, 0), 64, 20, 33, 3), ((90, 17, 33), 40, 0, 0, 2), ((21000, 9, 9000), 5000, 4, 100, 2),
+                                                        ((2100,) * 40, 1500, 100, 100, 1)])
+def test_evict_keeps_only_tokens_that_are_there(kind, lens, budget, first, last, hkv):
+    """Every third page is not there: no token of it stays, the lengths say so, and what goes on with the kept ones sees no row that nobody wrote."""
+    page, d, B = 16, 64, len(lens)
+    c = Case("bf16", d, hkv, hkv, page, lens, (0,) * B, seed=67, spare=0.0)
+    c.table[:, ::3] = -1
+    if B > 2:
+        c.table[2, 5], c.table[1] = c.pages + 10 ** 6, -1     # of the second none is there at all
+    scores = fill_scores(c, kind, 68)
+    kept_pages = -(-budget // page)
+    pages = c.pages + B * kept_pages
+    kept_table = (torch.arange(B * kept_pages, dtype=torch.int32) + c.pages).reshape(B, -1)
+    k, v = (torch.cat([x, torch.full((pages - c.pages, hkv, page, d), math.nan).to(x.dtype)]) for x in (c.k, c.v))
+    s = torch.cat([scores, torch.full((pages - c.pages, hkv, page), 9.0)])
+    plan = plan_for(c, keep_present=True)
+    results = []
+    for same in (False, True):
+        gk, gv, gs, lens_ = k.cuda(), v.cuda(), s.cuda(), c.kv_lens().cuda()
+        kept = torch.full((B, hkv, budget), 10 ** 9, dtype=torch.int32, device="cuda")
+        kept_lens = lens_ if same else torch.zeros_like(lens_)
+        plan.evict(gk, gv, gs, c.table.cuda(), lens_, kept_table.cuda(), budget, first, last, kept, kept_lens)
+        results.append([x.cpu() for x in (gk.view(torch.int16), gv.view(torch.int16), gs.view(torch.int32), kept, kept_lens)])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    kept, kept_lens = results[0][3], results[0][4].tolist()
+    for b, n in enumerate(lens):
+        at = c.table[b].long()[torch.arange(n) // page]
+        there = (at >= 0) & (at < c.pages)
+        for h in range(hkv):
+            places = kept_present(scores[at.clamp(0, c.pages - 1), h, torch.arange(n) % page], there, budget, first, last)
+            assert kept[b, h].tolist() == places + [-1] * (budget - len(places)) and kept_lens[b] == len(places), (b, h)
+            i, j = torch.arange(len(places)), torch.tensor(places, dtype=torch.long)
+            to, row = kept_table[b].long()[i // page], i % page
+            for x in (k, v, s):
+                x[to, h, row] = x[at[j], h, j % page]
+    for x, y in zip((k.view(torch.int16), v.view(torch.int16), s.view(torch.int32)), results[0]):
+        assert torch.equal(x, y)
+    # a step over the kept tokens
+    after = Case("bf16", d, hkv, hkv, page, kept_lens, tuple(min(n, 1) for n in kept_lens), seed=69)
+    after.k, after.v, after.table, after.pages = k, v, kept_table, pages
+    check_forward(after)
+
+
+def test_captured_eviction_of_tokens_that_are_there():
+    page, hkv, B, cap, budget = 16, 2, 3, 80, 200
+    g = torch.Generator().manual_seed(70)
+    pages = B * cap + B * -(-budget // page)
+    base = [torch.randn(pages, hkv, page, 64, generator=g).half().cuda() for _ in range(2)] + [torch.rand(pages, hkv, page, generator=g).cuda()]
+    kept_table = (torch.arange(pages - B * cap, dtype=torch.int32) + B * cap).reshape(B, -1).cuda()
+    table, lens = torch.zeros(B, cap, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    plan = paged.PagedAttention(4, 64, kv_heads=hkv, page_size=page, max_batch=B, max_tokens=4, keep_present=True)
+    state = [x.clone() for x in base] + [torch.zeros(B, hkv, budget, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")]
+
+    def step():
+        k, v, s, kept, kept_lens = state
+        plan.evict(k, v, s, table, lens, kept_table, budget, 3, 20, kept, kept_lens)
+
+    def fresh():
+        for x, y in zip(state, base + [-2, -2]):
+            x.copy_(y) if isinstance(y, torch.Tensor) else x.fill_(y)
+
+    step()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for i, L in enumerate(([1000, 30, 0], [7, 1280, 250], [640, 200, 201])):
+        t = torch.randperm(B * cap, generator=g).reshape(B, cap).int()
+        t[torch.rand(B, cap, generator=g) < 0.1 * (i + 1)] = -1
+        table.copy_(t), lens.copy_(torch.tensor(L, dtype=torch.int32))
+        fresh()
+        step()
+        torch.cuda.synchronize()
+        eager = [x.clone() for x in state]
+        fresh()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(state, eager)), L
+        assert (state[4] <= torch.tensor(L, device="cuda")).all() and ((state[3] >= 0).sum(dim=2) == state[4][:, None]).all()
