@@ -64,6 +64,10 @@ class PagedAttention:
         self.lib = _lib.load()
         self.heads, self.dim, self.kv_heads, self.page_size = int(heads), int(dim), int(kv_heads) or int(heads), int(page_size)
         self.max_batch, self.max_tokens = int(max_batch), int(max_tokens)
+        for name, x in (("heads", heads), ("dim", dim), ("kv_heads", kv_heads), ("page_size", page_size), ("max_batch", max_batch),
+                        ("max_tokens", max_tokens), ("window", window), ("sinks", sinks)):
+            if not -2 ** 31 <= int(x) < 2 ** 31:   # (a field of the struct would take what is left of it)
+                raise ValueError(f"{name} must fit 32 bits")
         code = DTYPE_CODE[dtype]
         self.torch_dtype = TORCH_DTYPE[code]
         self.out_dtype = torch.float32 if partials else self.torch_dtype
