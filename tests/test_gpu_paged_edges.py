@@ -329,3 +329,66 @@ def test_captured_eviction_of_tokens_that_are_there():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(state, eager)), L
         assert (state[4] <= torch.tensor(L, device="cuda")).all() and ((state[3] >= 0).sum(dim=2) == state[4][:, None]).all()
+
+
+@pytest.mark.parametrize("lens,starts", [([10 ** 9, -5, 2 ** 31 - 1], [0, 3, 43, 45]), ([60, 90, 40], [0, 3, 400, 2 ** 31 - 1]), ([60, 90, 40], [-7, 30, 3, 45]),
+                                         ([-2 ** 31, 90, 2 ** 31 - 1], [-2 ** 31, 2 ** 31 - 1, -2 ** 31, 45]), ([60, 90, 40], [45, 45, 45, 45]), ([1, 0, 2], [0, 20, 20, 45])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (17, 3)])
+def test_lengths_that_are_not_true_write_nothing_else(lens, starts, window, sinks):
+    """Lengths and starts of any kind: rows that no sequence has, places that no token has and what lies around the tensors stay as they were, and
+    sequences whose lengths and starts, held to the table and the tokens, are ones of their own get what is theirs."""
+    heads, hkv, page, d, T, budget = 4, 2, 16, 64, 45, 20
+    c = Case("bf16", d, heads, hkv, page, (60, 90, 40), (3, 40, 2), window=window, sinks=sinks, seed=14, spare=0.0, extra_pages=8)
+    held = [min(max(x, 0), T) for x in starts]
+    c.starts = torch.tensor(held, dtype=torch.int32)
+    c.news = [max(0, held[b + 1] - held[b]) for b in range(3)]
+    room = c.table.shape[1] * page
+    c.lens = [min(max(n, 0), room) for n in lens]
+    plan = plan_for(c)
+    assert c.tokens == T
+    l, s = torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda()
+    table, q = c.table.cuda(), c.q.cuda()
+    of = [guarded(c.k.shape, torch.bfloat16, 0) for _ in range(2)] + [guarded((c.pages, hkv, page), torch.float32, 0.5)]
+    (k, v, scores), places = [x[0] for x in of], [x[1:] for x in of]
+    k.copy_(c.k), v.copy_(c.v)
+    out, *out_at = guarded((T, heads, d), torch.bfloat16, 5)
+    lse, *lse_at = guarded((heads, T), torch.float32, 5)
+    plan.forward(q, k, v, table, l, s, out, lse)
+    claims = torch.zeros(T, dtype=torch.int64)
+    for b in range(3):
+        claims[held[b]:held[b] + c.news[b]] += 1
+    o, z, tol, tol_z = ref.attend(c)
+    one = claims == 1
+    near(out[one], o[one], tol[one], "out")
+    near(lse[:, one], z[:, one], tol_z[:, one], "lse")
+    assert (out[claims == 0] == 5).all() and (lse[:, claims == 0] == 5).all()
+    # the weights, by an LSE of every row that is claimed once; rows of several sequences weigh nothing
+    z = torch.where(one, z.float(), -math.inf)
+    plan.weights(q, z.cuda(), k, table, l, s, scores)
+    w, off = ref.weights(c, z)
+    near(scores, w + 0.5, off + 2.0 ** -24 * (w + 0.5), "scores")
+    # new rows: where append may write
+    new = torch.full((T, hkv, d), 3.0, dtype=torch.bfloat16, device="cuda")
+    plan.append(new, new, k, v, table, l, s, scores)
+    want = c.k.clone()
+    for b in range(3 if int(claims.max()) < 2 else 0):
+        for j in range(max(0, c.lens[b] - c.news[b]), c.lens[b]):
+            if c.row(b, j) is not None:
+                want[c.row(b, j), :, j % page] = 3
+    owned = torch.zeros(c.pages, page, dtype=torch.bool)   # any place that a sequence's table gives it
+    for b in range(3):
+        for j in range(c.lens[b]):
+            if c.row(b, j) is not None:
+                owned[c.row(b, j), j % page] = True
+    if int(claims.max()) < 2:
+        assert torch.equal(k.cpu(), want)
+    assert torch.equal(k.cpu().transpose(1, 2)[~owned], c.k.transpose(1, 2)[~owned]) and torch.equal(v.cpu().transpose(1, 2)[~owned], c.v.transpose(1, 2)[~owned])
+    free = [p for p in range(c.pages) if not (c.table == p).any()]
+    kept_table = torch.tensor(free[:6], dtype=torch.int32).reshape(3, 2).cuda()
+    kept, *kept_at = guarded((3, hkv, budget), torch.int32, -9)
+    kept_lens, *lens_at = guarded((3,), torch.int32, -9)
+    plan.evict(k, v, scores, table, l, kept_table, budget, 2, 5, kept, kept_lens)
+    assert kept_lens.tolist() == [min(n, budget) for n in c.lens]
+    assert ((kept >= 0).sum(dim=2).cpu() == torch.tensor(c.lens)[:, None].clamp(max=budget)).all()
+    torch.cuda.synchronize()
+    assert all(untouched_outside(*x) for x in places + [out_at, lse_at, kept_at, lens_at])
