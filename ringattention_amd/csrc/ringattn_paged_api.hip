@@ -68,7 +68,8 @@ int check_cache(const ringattn_paged_plan* pl, const ringattn_paged_cache* c, bo
   if (c->batch < 0 || c->batch > pl->p.max_batch) return RINGATTN_ERR_SHAPE;
   if (c->pages < 1 || c->table_pages < 1 || (int64_t)c->table_pages * pl->p.page_size > (int64_t)1 << 30) return RINGATTN_ERR_SHAPE;
   if (c->table_stride < c->table_pages || c->table_stride > (int64_t)1 << 40) return RINGATTN_ERR_SHAPE;
-  const int64_t most = (int64_t)1 << 40;  // (so that no product of a stride and a count overflows 64 bits)
+  const int64_t most = (int64_t)1 << 40;  // (so that a place in the pool, in bytes, is below 2^62)
+  if ((double)c->pages * (double)c->page_stride > (double)((int64_t)1 << 60)) return RINGATTN_ERR_SHAPE;
   if (c->token_stride < pl->p.dim || c->token_stride > 1 << 24 || c->page_stride < pl->p.dim || c->page_stride > most / 2 ||
       c->head_stride < pl->p.dim || c->head_stride > most)
     return RINGATTN_ERR_SHAPE;
