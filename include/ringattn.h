@@ -350,7 +350,8 @@ typedef struct ringattn_paged_cache {
 
 /* Bytes of device workspace a plan needs (sums of rows whose keys are shared out to several workgroups); 0 if the parameters are invalid. */
 size_t ringattn_paged_workspace_bytes(const ringattn_paged_params* params);
-/* As ringattn_plan_create and ringattn_plan_destroy; a workspace of the caller's holds zeros when the plan is made. */
+/* As ringattn_plan_create and ringattn_plan_destroy; a workspace of the caller's holds zeros when the plan is made (workgroups that share a
+ * row count themselves in it and leave the counts at 0: from any other value rows stay unwritten). */
 int ringattn_paged_plan_create(const ringattn_paged_params* params, void* workspace, size_t workspace_bytes, ringattn_paged_plan** plan_out);
 int ringattn_paged_plan_destroy(ringattn_paged_plan* plan);
 

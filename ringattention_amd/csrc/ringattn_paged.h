@@ -15,13 +15,12 @@ namespace paged {
 constexpr int kKeyTile = 32;      // keys of a tile
 constexpr int kFewRows = 32;      // query rows of a workgroup where a sequence's KV head has few of them (ringattn_paged_few.h)
 constexpr int kManyRows = 256;    // ... and where it has many (ringattn_paged_many.h)
-// Up to so many rows of a sequence's KV head are few.  Attention, us as few and as many, 32 heads on 8: one sequence of 32 K, 16 tokens (64 rows) 34
-// and 51, 24 tokens 78 and 51, 32 tokens 41 and 51, over 32800 58 and 50; 16 sequences of 4 K, 16 tokens 53 and 87, 24 tokens 129 and 105, 32
-// tokens 97 and 104.  Weights, the latter: 32 tokens 80 and 105, 48 tokens (192 rows) 112 and 131; one of 32 K, 32 tokens 47 and 54, 48
-// tokens 63 and 67.
+// Up to so many rows of a sequence's KV head are few.  Attention, us as few and as many, 32 heads on 8: 16 sequences of 4 K, 16 tokens each (64
+// rows) 67 and 93, 24 tokens 126 and 96, 32 tokens 99 and 95, 40 tokens 203 and 94.  Weights, the same: 32 tokens 85 and 119, 48 tokens (192
+// rows) 116 and 146; one of 32 K, 32 tokens 49 and 56, 48 tokens 64 and 69.
 constexpr int kFewRowsMost = 64, kWeightFewRowsMost = 192;
-// Of one sequence alone, whose row tiles make even runs: 24 tokens (96 rows) over 32 K 39 as few and 52 as many, over 100 K 121 and 163; 32 tokens 43 and
-// 55, 137 and 148; 40 tokens 53 and 54, 157 and 146.
+// Of one sequence alone, whose row tiles make even runs: 24 tokens (96 rows) over 32 K 39 as few and 52 as many, over 100 K 122 and 122; 32 tokens 42 and
+// 52, 133 and 123; 40 tokens 49 and 53, 155 and 124.
 constexpr int kFewRowsAlone = 128;
 // Of attention where there is little to do for all (ringattn_paged_fwd): us as many and as few, 32 heads on 8: four chunks of 64 over 1 K, 256 rows, 32
 // key tiles a workgroup 26 and 17; one over 8 K, 64 tiles 32 and 27; of 128, 512 rows, 128 tiles 40 and 40; 16 chunks of 24 over 4 K, 96 rows,

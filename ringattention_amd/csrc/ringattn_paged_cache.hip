@@ -4,8 +4,8 @@
 //   paged_append_kernel  : K and V rows of the new tokens to their places.  A copy: 16 bytes a thread.
 //   paged_weights_kernel : score[key] += sum over queries of exp(scale q k - LSE).  The sum runs over queries where attention's runs
 //       over keys, so a workgroup owns keys: K fragments stay in registers, the query rows pass by, S^T = K Q^T on MFMAs, and a
-//       lane adds up the weights of its 16 keys over every 32nd query; lanes meet at the end.  One owner per score: no atomics, the
-//       same bits in every run.
+//       lane adds up the weights of its 16 keys over every 32nd query; lanes meet at the end.  One workgroup adds to a sequence's score, once (an
+//       atomic addition, for pages that sequences share): the same bits in every run where they share none.
 //   paged_select_kernel  : the places of a sequence's KV head that stay.  The budget-th largest score is found by its bits, from the
 //       highest on, in counts of how many scores share the bits so far.
 //   paged_present_kernel : takes those whose page is not there out of them, where they are not to stay.
@@ -140,7 +140,7 @@ template <int DT, int D> struct WeightRows {
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
   }
-  // Every key has one owner, which adds to its score once: no order to go by, and nothing to wait for.
+  // Every key of a sequence has one owner, which adds to its score once: no order to go by.  Atomic, since pages may be several sequences'.
   __device__ __forceinline__ void add_score(int page, int key, float x) const {
     if (page >= 0 && key < s.len)
       unsafeAtomicAdd(a.scores + (((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1)), x);

@@ -56,8 +56,9 @@ class PagedAttention:
     `window` > 0: a token sees the last `window` tokens up to itself and the first `sinks` of the sequence.  `causal=False`:
     it sees every cached token; `partials`: out is float32, a partial (O, LSE) for api.merge -- together, for a sequence whose cache is
     spread over several pools or GPUs.  `keep_present`: evict() keeps no token whose page is not there.  `workspace`: a (device
-    address, bytes) pair the caller owns and keeps alive, instead of an allocation by the plan.  One call at a time, and replays of
-    captured calls in turn: they share the plan's workspace."""
+    address, bytes) pair the caller owns and keeps alive, instead of an allocation by the plan.  It holds zeros when the plan is made
+    (torch.zeros, not torch.empty): workgroups that share a row count themselves in it, and leave it at 0.  One call at a time, and replays
+    of captured calls in turn: they share the plan's workspace."""
 
     def __init__(self, heads, dim, kv_heads=0, dtype="fp16", page_size=64, max_batch=64, max_tokens=8192, causal=True, softmax_scale=0.0,
                  window=0, sinks=0, partials=False, workspace=None, keep_present=False):
