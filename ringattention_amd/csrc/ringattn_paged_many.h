@@ -221,8 +221,9 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   };
   // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where the V of a tile that some row has masked holds such
   // a value, the products of masked tiles are taken key by key from there on, over the visible ones.  A wave looks at what it loaded
-  // itself, when it has arrived and in front of the barrier behind which the others use it.
-  int* odd_seen = (int*)(smem + 2 * NBUF * TILE);
+  // itself, when it has arrived and in front of the barrier behind which the others use it: what it leaves is the pair of tiles that this is the
+  // barrier of, since another wave may still have tiles in front of them, whose products are the same whether it has looked yet or not.
+  volatile int* odd_from = (volatile int*)(smem + 2 * NBUF * TILE);
   auto look_at_v = [&](int t) {
     if ((PIECES < WAVES && wave < PIECES) || t >= n_tiles || !(t >= every.up || t < every.low || any_gone())) return;
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -231,9 +232,9 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     unsigned top = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) top |= (x[e] & kExp) + kOne;  // an exponent of ones carries into the sign's place
-    if (top & 0x80008000u) *odd_seen = 1;
+    if ((top & 0x80008000u) && *odd_from > t) *odd_from = t & ~1;
   };
-  auto odd_values = [&](int t) { return may_be_masked(t) && __builtin_amdgcn_readfirstlane(*(volatile int*)odd_seen) != 0; };
+  auto odd_values = [&](int t) { return may_be_masked(t) && t >= __builtin_amdgcn_readfirstlane(*odd_from); };
   auto pv_by_key = [&](int t, int vslot) {
     const int key0 = first_key(t), gone = gone_of(t);
     const Sight sees = sight();
@@ -388,7 +389,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
 #pragma unroll 1
     for (; t < n_tiles; ++t) masked_block(t);
   };
-  if (tid == 0) *odd_seen = 0;
+  if (tid == 0) *odd_from = INT32_MAX;
   if (n_tiles > 0) {
     hold(0);
     issue_k(0);

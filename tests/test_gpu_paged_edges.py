@@ -392,3 +392,18 @@ def test_lengths_that_are_not_true_write_nothing_else(lens, starts, window, sink
     assert ((kept >= 0).sum(dim=2).cpu() == torch.tensor(c.lens)[:, None].clamp(max=budget)).all()
     torch.cuda.synchronize()
     assert all(untouched_outside(*x) for x in places + [out_at, lse_at, kept_at, lens_at])
+
+
+@pytest.mark.parametrize("dtype,dim,heads,sigma,seed", [("fp16", 128, 99, 3.0, 5113), ("fp16", 128, 99, 1.0, 72), ("bf16", 64, 24, 3.0, 73)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("lens,news,causal,lost", [((469, 235, 358, 455, 473), (120, 43, 90, 187, 79), False, True), ((900, 777), (300, 400), True, False)])
+def test_the_same_bits_whatever_lies_behind_the_last_token(lens, news, causal, lost, value, dtype, dim, heads, sigma, seed):
+    """An infinity or a NaN in a hidden place changes how masked tiles are multiplied, from its own tile on and from no other, in every run."""
+    c = Case(dtype, dim, heads, 3, 256, lens, news, causal=causal, seed=seed, spare=value, sigma=sigma)
+    if lost:
+        c.table[2, 0] = -1
+    plan, out, lse = check_forward(c)
+    q, gpu = c.q.cuda(), on_gpu(c)
+    for _ in range(20):
+        again, lse_again = plan.forward(q, *gpu)
+        assert torch.equal(again, out) and torch.equal(lse_again, lse)
