@@ -766,8 +766,8 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_slices_kernel(con
 }
 
 // Where only tokens whose page is there are to stay: the others out of the list, which is as long for all KV heads, since they rank below everything.
-// A thread a place, 1024 at a time, and written no further than it has been read.  (Two dependent reads a turn, some 0.9 us: of the evictions in the
-// table the batch to 4 K tokens takes 4 us more, the long one to 32 K 29.)
+// A thread a place, 1024 at a time, and written no further than it has been read.  (Two dependent reads a turn, some 0.9 us: 16 sequences of 7.5 K
+// tokens to 4 K, 8 KV heads, take 4 us more by it, one of 128 K to 32 K, 4 KV heads, 29.)
 __global__ __launch_bounds__(kSelectThreads) void paged_present_kernel(const EvictArgs a) {
   __shared__ int counts[2][kSelectThreads / 64];  // in turn, so that one barrier each suffices
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
