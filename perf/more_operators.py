@@ -159,7 +159,7 @@ def _frequencies(c):
     if c["scaling"] == "yarn":   # pairs that turn more than 32 times within what was trained stay, those that turn less than once are stretched
         def pair(turns):
             return half * math.log(TRAINED / (turns * 2 * math.pi)) / math.log(BASE)
-        low, high = max(math.floor(pair(32)), 0), min(math.ceil(pair(1)), half - 1)
+        low, high = max(math.floor(pair(32)), 0), min(math.ceil(pair(1)), 2 * half - 1)
         stays = [1 - min(max((i - low) / max(high - low, 0.001), 0), 1) for i in range(half)]
         return [x / s * (1 - k) + x * k for x, k in zip(f, stays)], 0.1 * math.log(s) + 1
     return f, 1.0
