@@ -401,6 +401,55 @@ int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* 
                          int64_t kept_stride, int budget, int keep_first, int keep_last, int* kept, int* kept_lens, void* stream);
 
 /*
+ * ---- Rotary positions -------------------------------------------------------------------------
+ * Row x of a token at position p becomes y: of every pair of columns (a, b) among the first rotary_dim,
+ *   y_a = factor (x_a cos(p f_i) - x_b sin(p f_i)),   y_b = factor (x_b cos(p f_i) + x_a sin(p f_i)),
+ * the other columns stay.  Pair i is columns i and i + rotary_dim / 2, or, interleaved, 2 i and 2 i + 1.  With `inverse` by the angles' negatives: of
+ * rows that were turned with factor 1 the rows before, and of a gradient by y, with the factor of the forward, the gradient by x.  No counterpart in
+ * the reference, whose Q and K come as they are.
+ */
+typedef struct ringattn_rotary {
+  int rotary_dim;         /* columns that turn: a multiple of 16 up to dim */
+  int interleaved;
+  int inverse;
+  float factor;           /* of the turned columns; 0 stands for 1 */
+  const uint64_t* turns;  /* [rotary_dim / 2] on the device: f_i as ringattn_rotary_turns gives them */
+} ringattn_rotary;
+
+/* Host code: frequencies in radians per position as parts of a full turn, round(2^64 f / 2 pi) mod 2^64: p f_i is then taken exactly, for any
+ * position of 32 bits, however far.  Infinities and NaN are RINGATTN_ERR_SHAPE. */
+int ringattn_rotary_turns(const double* radians, int n, uint64_t* turns);
+
+/* Rows [batch, heads, tokens, dim] by strides (elements, multiples of 8), and where they go: the tensor itself (out == in, with the same
+ * strides) or one that lies elsewhere. */
+typedef struct ringattn_rows {
+  const void* in;
+  void* out;
+  int heads;
+  int64_t in_batch_stride, in_head_stride, in_token_stride;
+  int64_t out_batch_stride, out_head_stride, out_token_stride;
+} ringattn_rows;
+
+/*
+ * Turns the rows of one or two tensors (Q and K) of dim 64 or 128 in one launch, asynchronously on `stream`.  positions: [batch, tokens] on the
+ * device, rows of position_stride ints (0: the same for every batch), of any sign; NULL: a token's number.  A ring's tensors in the zigzag layout have
+ * the positions that their rows have in the sequence.
+ */
+int ringattn_rotary_apply(const ringattn_rotary* rotary, int dim, int dtype, const ringattn_rows* tensors, int count, int batch, int tokens,
+                          const int* positions, int64_t position_stride, void* stream);
+
+/*
+ * ringattn_paged_append with rotary positions on the way: rows q [tokens, heads, dim] are turned into q_out (q itself, with the same strides, or a
+ * tensor that lies elsewhere), those of k_new are turned into the cache, those of v_new go there as they are.  positions: [tokens] on the device;
+ * NULL: a token's place in its sequence (of a sequence that ringattn_paged_evict has shortened, the places count the tokens that are left).
+ * Rows of q_out behind the last sequence are left as they were; a token whose page is not there has its row of q_out all the same.
+ */
+int ringattn_paged_append_rotary(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_rotary* rotary, const int* positions,
+                                 const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t out_token_stride,
+                                 int64_t out_head_stride, const void* k_new, const void* v_new, int tokens, int64_t token_stride, int64_t head_stride,
+                                 float* scores, void* stream);
+
+/*
  * Seeded input generator -- the counterpart of fillWithNum / initQKV
  * (csrc/ring_attention.cu:731-748), which fill a host buffer and copy it to the
  * device.  Writes n values of N(0, sigma^2), rounded to nearest-even into `dtype`,

@@ -56,6 +56,17 @@ class RingattnPagedCache(ctypes.Structure):
                 ("page_table", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("batch", ctypes.c_int)]
 
 
+class RingattnRotary(ctypes.Structure):
+    """struct ringattn_rotary."""
+    _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int), ("factor", ctypes.c_float), ("turns", ctypes.c_void_p)]
+
+
+class RingattnRows(ctypes.Structure):
+    """struct ringattn_rows."""
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("heads", ctypes.c_int)] + [(n, ctypes.c_int64) for n in (
+        "in_batch_stride", "in_head_stride", "in_token_stride", "out_batch_stride", "out_head_stride", "out_token_stride")]
+
+
 _cache_p = ctypes.POINTER(RingattnPagedCache)
 
 SYMBOLS = {
@@ -95,6 +106,12 @@ SYMBOLS = {
                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_paged_evict": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_rotary_turns": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),
+    "ringattn_rotary_apply": (ctypes.c_int, [ctypes.POINTER(RingattnRotary), ctypes.c_int, ctypes.c_int, ctypes.POINTER(RingattnRows), ctypes.c_int,
+                                             ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "ringattn_paged_append_rotary": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.POINTER(RingattnRotary), ctypes.c_void_p] + (
+        [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64] * 2) + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                                                  ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_fill_normal": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64,
                                             ctypes.c_int64, ctypes.c_double]),
     "ringattn_fill_reference_pattern": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int]),

@@ -2,6 +2,7 @@
 // hold is the kernels' to check; everything that the host can see is checked here, before the first HIP call.
 #include "ringattn.h"
 #include "ringattn_paged.h"
+#include "ringattn_rotary.h"
 
 #include <cmath>
 #include <cstring>
@@ -209,6 +210,47 @@ int ringattn_paged_append(ringattn_paged_plan* plan, const ringattn_paged_cache*
   a.scores = scores;
   a.kv_heads = plan->kv_heads;
   RP_HIP(rp::launch_paged_append(a, plan->p.dim, (hipStream_t)stream));
+  return RINGATTN_OK;
+}
+
+int ringattn_paged_append_rotary(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_rotary* rotary, const int* positions,
+                                 const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t out_token_stride,
+                                 int64_t out_head_stride, const void* k_new, const void* v_new, int tokens, int64_t token_stride, int64_t head_stride,
+                                 float* scores, void* stream) {
+  namespace rr = ringattn::rotary;
+  if (!plan_ok(plan)) return RINGATTN_ERR_PLAN;
+  RP_CHECK(check_cache(plan, cache, true, true));
+  rr::AppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  RP_CHECK(rr::check(rotary, plan->p.dim, &a.r));
+  if (!q || !q_out || !k_new || !v_new) return RINGATTN_ERR_NULL;
+  RP_CHECK(check_rows(plan, tokens, plan->p.heads, q_token_stride, q_head_stride, 8, false));
+  RP_CHECK(check_rows(plan, tokens, plan->p.heads, out_token_stride, out_head_stride, 8, true));
+  RP_CHECK(check_rows(plan, tokens, plan->kv_heads, token_stride, head_stride, 8, false));
+  if (!aligned(q, 16) || !aligned(q_out, 16) || !aligned(k_new, 16) || !aligned(v_new, 16) || !aligned(scores, 4) || !aligned(positions, 4))
+    return RINGATTN_ERR_ALIGN;
+  if (tokens == 0 || cache->batch == 0) return RINGATTN_OK;
+  // q_out is q itself, or lies elsewhere
+  auto span = [&](int64_t ts, int64_t hs) { return 2. * ((tokens - 1) * (double)ts + (plan->p.heads - 1) * (double)hs + plan->p.dim); };
+  const bool same = q == q_out && (tokens == 1 || q_token_stride == out_token_stride) && (plan->p.heads == 1 || q_head_stride == out_head_stride);
+  const double from = (double)(uintptr_t)q, to = (double)(uintptr_t)q_out;
+  if (!same && from < to + span(out_token_stride, out_head_stride) && to < from + span(q_token_stride, q_head_stride)) return RINGATTN_ERR_SHAPE;
+  a.c = cache_of(plan, cache, tokens);
+  a.q = (const char*)q;
+  a.k = (const char*)k_new;
+  a.v = (const char*)v_new;
+  a.q_out = (char*)q_out;
+  a.q_ts = q_token_stride * 2;
+  a.q_hs = q_head_stride * 2;
+  a.o_ts = out_token_stride * 2;
+  a.o_hs = out_head_stride * 2;
+  a.ts = token_stride * 2;
+  a.hs = head_stride * 2;
+  a.positions = positions;
+  a.scores = scores;
+  a.heads = plan->p.heads;
+  a.kv_heads = plan->kv_heads;
+  RP_HIP(rr::launch_append(a, plan->p.dtype, plan->p.dim, rotary->interleaved != 0, (hipStream_t)stream));
   return RINGATTN_OK;
 }
 

@@ -1,0 +1,225 @@
+// gfx950 (CDNA4) kernels: rotary positions, of a ring's tensors (ringattn_rotary_apply) and of new tokens on their way into a paged cache
+// (ringattn_paged_append_rotary).  Copies with some arithmetic: memory bounds them where there are many rows, a launch where few.
+//
+//   rotary_kernel        : a thread has sixteen columns of a token, eight pairs, and goes through some of the heads: their angles are
+//       worked out once for all of those.
+//   rotary_append_kernel : a wave has a token, D / 16 lanes a row: Q's heads to their output, K's turned and V's as they are to the page.
+#include "ringattn_rotary.h"
+
+#include <cmath>
+#include <cstring>
+#include <utility>
+
+namespace ringattn {
+namespace rotary {
+
+template <int DT, int D, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(const ApplyArgs a) {
+  constexpr int PIECES = D / 16;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int piece = (int)(item % PIECES);
+  const int64_t t = item / PIECES;
+  if (t >= a.tokens) return;
+  const int b = blockIdx.z, h_begin = blockIdx.y * a.heads_each, h_end = min(h_begin + a.heads_each, a.heads);
+  const Part p = part_of<INTERLEAVED>(a.r, piece);
+  Angles g;
+  if (p.turns) angles_of(g, a.r, piece, a.positions ? (int64_t)a.positions[b * a.position_stride + t] : t);
+  for (int h = h_begin; h < h_end; ++h) {
+    const bool second = h >= a.heads0;
+    const Rows& x = a.x[second ? 1 : 0];
+    const int head = second ? h - a.heads0 : h;
+    const char* from = x.in + b * x.in_bs + head * x.in_hs + t * x.in_ts;
+    char* to = x.out + b * x.out_bs + head * x.out_hs + t * x.out_ts;
+    if (!p.turns && from == to) continue;
+    s16x8 x0 = *(const s16x8*)(from + p.at0), x1 = *(const s16x8*)(from + p.at1);
+    if (p.turns) turn<DT, INTERLEAVED>(x0, x1, g);
+    *(s16x8*)(to + p.at0) = x0;
+    *(s16x8*)(to + p.at1) = x1;
+  }
+}
+
+template <int DT, int D, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) {
+  constexpr int PIECES = D / 16, AT_ONCE = 64 / PIECES;
+  const int lane = threadIdx.x & 63;
+  const int t = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+  if (t >= a.c.tokens) return;
+  // the sequence that token t is of: the last one that begins at or before it; its lengths and starts are held to the same as everywhere
+  int lo = 0, hi = a.c.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.c.starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const paged::Seq s = paged::uniform(paged::seq_of(a.c, lo));
+  const int i = t - s.start, key = s.len - s.n + i;
+  if (i < 0 || i >= s.n) return;  // in front of the first, behind the last
+  int page = key >= 0 ? a.c.table[lo * a.c.table_stride + (key >> a.c.page_shift)] : -1;  // (more new tokens than there are tokens)
+  page = __builtin_amdgcn_readfirstlane(page);
+  const bool there = (unsigned)page < (unsigned)a.c.pages;
+  const int piece = lane % PIECES;
+  const Part p = part_of<INTERLEAVED>(a.r, piece);
+  Angles g;
+  if (p.turns) angles_of(g, a.r, piece, a.positions ? a.positions[t] : key);
+  const int row_begin = blockIdx.y * a.rows_each, rows = min(row_begin + a.rows_each, a.heads + 2 * a.kv_heads);
+  for (int row = row_begin + lane / PIECES; row < rows; row += AT_ONCE) {
+    const bool of_q = row < a.heads, of_v = row >= a.heads + a.kv_heads;
+    const int head = of_q ? row : of_v ? row - a.heads - a.kv_heads : row - a.heads;
+    if (!of_q && !there) continue;
+    const char* from = of_q ? a.q + t * a.q_ts + head * a.q_hs : (of_v ? a.v : a.k) + t * a.ts + head * a.hs;
+    char* to = of_q ? a.q_out + t * a.o_ts + head * a.o_hs : (of_v ? a.c.v : a.c.k) + paged::page_row(a.c, page, head, key);
+    s16x8 x0 = *(const s16x8*)(from + p.at0), x1 = *(const s16x8*)(from + p.at1);
+    if (p.turns && !of_v) turn<DT, INTERLEAVED>(x0, x1, g);
+    *(s16x8*)(to + p.at0) = x0;
+    *(s16x8*)(to + p.at1) = x1;
+    if (of_v && piece == 0 && a.scores) a.scores[(((int64_t)page * a.kv_heads + head) << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))] = 0.f;
+  }
+}
+
+#define RA_ROTARY_FORMS(LAUNCH)                                             \
+  do {                                                                      \
+    if (dtype == 0 && dim == 64 && !interleaved) LAUNCH(0, 64, false);      \
+    else if (dtype == 0 && dim == 64) LAUNCH(0, 64, true);                  \
+    else if (dtype == 1 && dim == 64 && !interleaved) LAUNCH(1, 64, false); \
+    else if (dtype == 1 && dim == 64) LAUNCH(1, 64, true);                  \
+    else if (dtype == 0 && dim == 128 && !interleaved) LAUNCH(0, 128, false); \
+    else if (dtype == 0 && dim == 128) LAUNCH(0, 128, true);                \
+    else if (dtype == 1 && dim == 128 && !interleaved) LAUNCH(1, 128, false); \
+    else if (dtype == 1 && dim == 128) LAUNCH(1, 128, true);                \
+    else return hipErrorInvalidValue;                                       \
+  } while (0)
+
+hipError_t launch_apply(const ApplyArgs& args, int dtype, int dim, bool interleaved, int batch, hipStream_t stream) {
+  ApplyArgs a = args;
+  const int64_t blocks = ((int64_t)a.tokens * (dim / 16) + 255) / 256;
+  a.heads_each = 1;
+  const int groups = (a.heads + a.heads_each - 1) / a.heads_each;
+  if (blocks <= 0 || batch <= 0) return hipSuccess;
+  if (blocks > INT32_MAX || groups > 65535 || batch > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, (unsigned)groups, (unsigned)batch);
+#define RA_LAUNCH(DT_, D_, I_) rotary_kernel<DT_, D_, I_><<<grid, 256, 0, stream>>>(a)
+  RA_ROTARY_FORMS(RA_LAUNCH);
+#undef RA_LAUNCH
+  return hipGetLastError();
+}
+
+hipError_t launch_append(const AppendArgs& args, int dtype, int dim, bool interleaved, hipStream_t stream) {
+  AppendArgs a = args;
+  if (a.c.tokens <= 0 || a.c.batch <= 0) return hipSuccess;
+  const int rows = a.heads + 2 * a.kv_heads;
+  a.rows_each = rows;
+  const dim3 grid((unsigned)((a.c.tokens + 3) / 4), (unsigned)((rows + a.rows_each - 1) / a.rows_each));
+#define RA_LAUNCH(DT_, D_, I_) rotary_append_kernel<DT_, D_, I_><<<grid, 256, 0, stream>>>(a)
+  RA_ROTARY_FORMS(RA_LAUNCH);
+#undef RA_LAUNCH
+  return hipGetLastError();
+}
+
+int check(const ringattn_rotary* r, int dim, Turns* out) {
+  if (!r || !r->turns) return RINGATTN_ERR_NULL;
+  if (r->rotary_dim < 16 || r->rotary_dim > dim || r->rotary_dim % 16 != 0) return RINGATTN_ERR_DIM;
+  if (!std::isfinite(r->factor) || r->factor < 0.f) return RINGATTN_ERR_SHAPE;
+  if ((uintptr_t)r->turns & 7) return RINGATTN_ERR_ALIGN;
+  *out = Turns{r->turns, r->factor > 0.f ? r->factor : 1.f, r->rotary_dim, r->inverse != 0};
+  return RINGATTN_OK;
+}
+
+namespace {
+
+// A tensor's rows: strides of dimensions that have one entry count for nothing.
+struct Extent {
+  int64_t n[3], stride[3];  // elements; batch, head, token
+  int dim;
+  bool in_range() const {
+    for (int i = 0; i < 3; ++i)
+      if (n[i] > 1 && (stride[i] < 0 || stride[i] > (int64_t)1 << 36)) return false;
+    return true;
+  }
+  bool in_pieces() const {
+    for (int i = 0; i < 3; ++i)
+      if (n[i] > 1 && (stride[i] & 7)) return false;
+    return true;
+  }
+  double span() const {  // elements from the first to behind the last (may pass 64 bits)
+    double x = dim;
+    for (int i = 0; i < 3; ++i) x += (double)(n[i] - 1) * (double)(n[i] > 1 ? stride[i] : 0);
+    return x;
+  }
+  // No row on another: each dimension steps over what lies within the smaller ones.
+  bool apart() const {
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+      for (int j = i + 1; j < 3; ++j)
+        if ((n[order[j]] > 1 ? stride[order[j]] : -1) < (n[order[i]] > 1 ? stride[order[i]] : -1)) std::swap(order[i], order[j]);
+    double within = dim;
+    for (int i = 0; i < 3; ++i) {
+      const int d = order[i];
+      if (n[d] < 2) continue;
+      if ((double)stride[d] < within) return false;
+      within += (double)(n[d] - 1) * (double)stride[d];
+    }
+    return true;
+  }
+};
+
+}  // namespace
+
+}  // namespace rotary
+}  // namespace ringattn
+
+extern "C" {
+
+int ringattn_rotary_turns(const double* radians, int n, uint64_t* turns) {
+  if (!radians || !turns) return RINGATTN_ERR_NULL;
+  if (n < 0) return RINGATTN_ERR_SHAPE;
+  for (int i = 0; i < n; ++i)
+    if (!std::isfinite(radians[i])) return RINGATTN_ERR_SHAPE;
+  for (int i = 0; i < n; ++i) {
+    long double t = (long double)radians[i] / 6.283185307179586476925286766559L;
+    t -= floorl(t);  // whole turns are none
+    const long double x = roundl(t * 18446744073709551616.0L);
+    turns[i] = x >= 18446744073709551616.0L ? 0 : (uint64_t)x;
+  }
+  return RINGATTN_OK;
+}
+
+int ringattn_rotary_apply(const ringattn_rotary* rotary, int dim, int dtype, const ringattn_rows* tensors, int count, int batch, int tokens,
+                          const int* positions, int64_t position_stride, void* stream) {
+  namespace rr = ringattn::rotary;
+  if (dim != 64 && dim != 128) return RINGATTN_ERR_DIM;
+  if (dtype != RINGATTN_DTYPE_FP16 && dtype != RINGATTN_DTYPE_BF16) return RINGATTN_ERR_DTYPE;
+  rr::ApplyArgs a;
+  std::memset(&a, 0, sizeof(a));
+  if (const int rc = rr::check(rotary, dim, &a.r)) return rc;
+  if (!tensors) return RINGATTN_ERR_NULL;
+  if (count < 1 || count > 2 || batch < 0 || batch > 65535 || tokens < 0 || tokens > 1 << 30) return RINGATTN_ERR_SHAPE;
+  if (positions && (position_stride < 0 || position_stride > (int64_t)1 << 40)) return RINGATTN_ERR_SHAPE;
+  if ((uintptr_t)positions & 3) return RINGATTN_ERR_ALIGN;
+  for (int i = 0; i < count; ++i) {
+    const ringattn_rows& x = tensors[i];
+    if (x.heads < 1 || x.heads > 65535) return RINGATTN_ERR_SHAPE;
+    if (!x.in || !x.out) return RINGATTN_ERR_NULL;
+    const rr::Extent in{{batch, x.heads, tokens}, {x.in_batch_stride, x.in_head_stride, x.in_token_stride}, dim};
+    const rr::Extent out{{batch, x.heads, tokens}, {x.out_batch_stride, x.out_head_stride, x.out_token_stride}, dim};
+    if (!in.in_range() || !out.in_range()) return RINGATTN_ERR_SHAPE;
+    if (!in.in_pieces() || !out.in_pieces() || (((uintptr_t)x.in | (uintptr_t)x.out) & 15)) return RINGATTN_ERR_ALIGN;
+    if (!out.apart()) return RINGATTN_ERR_SHAPE;
+    // the tensor itself, or one that lies elsewhere
+    bool same = x.in == x.out;
+    for (int d = 0; d < 3; ++d) same = same && (in.n[d] < 2 || in.stride[d] == out.stride[d]);
+    const double from = (double)(uintptr_t)x.in, to = (double)(uintptr_t)x.out;
+    if (!same && batch > 0 && tokens > 0 && from < to + 2 * out.span() && to < from + 2 * in.span()) return RINGATTN_ERR_SHAPE;
+    rr::Rows& r = a.x[i];
+    auto bytes = [](const rr::Extent& e, int d) { return e.n[d] > 1 ? e.stride[d] * 2 : 0; };
+    r = rr::Rows{(const char*)x.in, (char*)x.out, bytes(in, 0), bytes(in, 1), bytes(in, 2), bytes(out, 0), bytes(out, 1), bytes(out, 2)};
+    a.heads += x.heads;
+  }
+  a.heads0 = tensors[0].heads;
+  a.tokens = tokens;
+  a.positions = positions;
+  a.position_stride = position_stride;
+  const hipError_t e = rr::launch_apply(a, dtype, dim, rotary->interleaved != 0, batch, (hipStream_t)stream);
+  return e == hipSuccess ? RINGATTN_OK : ringattn::hip_failed(e);
+}
+
+}  // extern "C"

@@ -168,6 +168,14 @@ class PagedAttention:
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=device)
 
+    @staticmethod
+    def _like(t, stream):
+        """A tensor that lies in memory as t does, of a call on `stream`."""
+        if stream is None:
+            return torch.empty_like(t)
+        with torch.cuda.stream(stream):
+            return torch.empty_like(t)
+
     def append(self, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores=None, stream=None):
         """Rows k, v [tokens, kv_heads, dim] of the new tokens into the cache, as the last of each sequence's kv_lens tokens; their scores to 0."""
         if self._call_type:
@@ -186,6 +194,32 @@ class PagedAttention:
             return
         self._call("ringattn_paged_append", k.device, stream, ctypes.byref(cache), k.data_ptr(), v.data_ptr(), shape[0], *_strides(k),
                    scores.data_ptr() if scores is not None else None)
+
+    def append_rotary(self, rotary, q, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores=None, positions=None, q_out=None, stream=None):
+        """append() with rotary positions on the way (rotary.Rotary): K turned and V as it is into the cache, q [tokens, heads, dim] turned into q_out
+        (q itself for in place).  `positions` int32 [tokens]; None: a token's place in its sequence.  Returns q_out."""
+        shape, kv_shape = self._tokens(q, "q", self.heads), self._tokens(k, "k", self.kv_heads)
+        if kv_shape[0] != shape[0]:
+            raise ValueError("q and k must have as many tokens")
+        rotary.check(self.dim, self.torch_dtype)
+        cache = self._cache(k_cache, v_cache, page_table, kv_lens, q_starts)
+        _check_rows((q, "q", self.torch_dtype, shape), (k, "k", self.torch_dtype, kv_shape), (v, "v", self.torch_dtype, kv_shape))
+        if _strides(k) != _strides(v):
+            raise ValueError("k and v must have the same strides")
+        if q_out is None:
+            q_out = self._like(q, stream)
+        _check_rows((q_out, "q_out", self.torch_dtype, shape))
+        if scores is not None:
+            _check_tensors((scores, "scores", torch.float32, k_cache.shape[:3]))
+        if positions is not None:
+            _check_tensors((positions, "positions", torch.int32, (shape[0],)))
+        self._same_device(k_cache, q, q_out, k, v, scores, positions, rotary.turns)
+        if shape[0] == 0 or cache.batch == 0:
+            return q_out
+        self._call("ringattn_paged_append_rotary", k.device, stream, ctypes.byref(cache), ctypes.byref(rotary.params(False)),
+                   positions.data_ptr() if positions is not None else None, q.data_ptr(), *_strides(q), q_out.data_ptr(), *_strides(q_out), k.data_ptr(),
+                   v.data_ptr(), shape[0], *_strides(k), scores.data_ptr() if scores is not None else None)
+        return q_out
 
     def forward(self, q, k_cache, v_cache, page_table, kv_lens, q_starts, out=None, lse=None, stream=None):
         """Attention of the new tokens q [tokens, heads, dim] over the cache (their own rows are in it).  Returns (out, lse)."""
