@@ -385,6 +385,28 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
                            int64_t q_head_stride, const float* lse, float* scores, void* stream);
 
 /*
+ * Scores that are not the plain products, for models that have them so.  In this order: x = scale q k; softcap > 0: x = softcap tanh(x / softcap);
+ * slopes: x -= slopes[head] |p - j| for the query at place p and the key at place j of the sequence.  And which keys a query sees: those in front of
+ * prefix_lens[b], whatever else is said; else j <= p, where also j < sinks, or j >= first_keys[token] and, with a window, j > p - window.
+ * With first_keys the tokens of several documents that lie one behind the other in a sequence see their own document's alone (the places of
+ * their documents' first tokens: in any order, of any value).  Members that are 0 or NULL change nothing.  Places count the tokens that are in the cache, after
+ * an eviction those that are left.  Slopes, prefixes and first keys are for causal plans.
+ */
+typedef struct ringattn_paged_scoring {
+  float softcap;
+  const float* slopes;      /* [heads], on the device */
+  const int* prefix_lens;   /* [batch], on the device; held to the sequence's length */
+  const int* first_keys;    /* [tokens], on the device: a row for every row of q */
+} ringattn_paged_scoring;
+
+/* ringattn_paged_fwd and ringattn_paged_weights with such scores; scoring may be NULL. */
+int ringattn_paged_fwd_scored(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q,
+                              int tokens, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              float* lse, void* stream);
+int ringattn_paged_weights_scored(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q,
+                                  int tokens, int64_t q_token_stride, int64_t q_head_stride, const float* lse, float* scores, void* stream);
+
+/*
  * Keeps `budget` tokens of every sequence, for each KV head its own: the first keep_first, the last keep_last, and of those between
  * them the ones with the largest scores (of equal ones the earliest; a NaN, and a token whose page is not there, counts as -inf).  Their K and V rows and scores are copied, in
  * their order, to the pages of kept_table ([batch, kept_pages] by rows of kept_stride ints, entries of the same pools; kept_pages *

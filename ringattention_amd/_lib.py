@@ -56,6 +56,11 @@ class RingattnPagedCache(ctypes.Structure):
                 ("page_table", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("batch", ctypes.c_int)]
 
 
+class RingattnPagedScoring(ctypes.Structure):
+    """struct ringattn_paged_scoring."""
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p), ("first_keys", ctypes.c_void_p)]
+
+
 class RingattnRotary(ctypes.Structure):
     """struct ringattn_rotary."""
     _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int), ("factor", ctypes.c_float), ("turns", ctypes.c_void_p)]
@@ -104,6 +109,11 @@ SYMBOLS = {
                                           ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_paged_weights": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_paged_fwd_scored": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.POINTER(RingattnPagedScoring), ctypes.c_void_p, ctypes.c_int,
+                                                 ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                                 ctypes.c_void_p]),
+    "ringattn_paged_weights_scored": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.POINTER(RingattnPagedScoring), ctypes.c_void_p, ctypes.c_int,
+                                                     ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_paged_evict": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_rotary_turns": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),

@@ -54,8 +54,40 @@ struct Parts {
   int* arrived;   // few rows: how many parts of a row tile are there, [2 kFewWorkgroups]; 0 between launches
 };
 
+// Scores that are not the plain products (ringattn_paged_fwd_scored): a template parameter SC of the programs says which of these there are,
+// 0 being plain scores; the masks of any scored call are data.
+constexpr int kCapped = 1, kSloped = 2, kScored = 4;
+struct Scoring {
+  float cap_in, cap_out;  // x = scale q k log2(e) becomes c tanh(x / c), c = cap_out = cap log2(e): cap_in takes q k to 2 log2(e) x / c
+  const float* slopes;    // [heads]
+  const int* prefix;      // [batch]
+  const int* first;       // [tokens]
+};
+// Scores of a 32 x 32 tile, as the products give them (lane (n, h): row n, keys key0 + 4 h + [0, 4) of every eight), in units of log2: what the
+// exponentials take.  tanh y = 1 - 2 / (e^2y + 1): an exponential and a reciprocal, each off by 2^-23 of itself, so that a capped score is off by
+// some 2^-22 of the cap; an infinite one is the cap.  dist: key0 + 4 h less the row's place in the sequence.
+template <int SC> static __device__ __forceinline__ void shape_scores(f32x16& s, const Scoring& x, float scale_log2, float slope, int dist) {
+  if constexpr ((SC & kCapped) != 0) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * x.cap_in) + 1.f);
+      s[e] = __builtin_fmaf(r, -2.f * x.cap_out, x.cap_out);
+    }
+  }
+  if constexpr ((SC & kSloped) != 0) {
+    const float d0 = (float)dist;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float far = __builtin_fabsf(d0 + (float)(8 * (e >> 2) + (e & 3)));
+      if constexpr ((SC & kCapped) != 0) s[e] = __builtin_fmaf(far, -slope, s[e]);
+      else s[e] = __builtin_fmaf(s[e], scale_log2, far * -slope);
+    }
+  }
+}
+
 struct AttendArgs {
   Cache c;
+  Scoring x;
   const char* q;
   char* out;
   float* lse;             // [heads, tokens]
@@ -74,36 +106,39 @@ struct AttendArgs {
 
 struct Seq {
   int len, start, n;
+  int prefix;  // tokens at the beginning that every new one sees (0 but for scored calls)
 };
 static __device__ __forceinline__ int clamped(int x, int lo, int hi) { return min(max(x, lo), hi); }
 // Lengths are data: whatever they hold, nothing outside the tensors is touched.  (A sequence's own are held to its table and to the call's tokens
 // here; few_rows looks at what starts that do not ascend make of them all together.)
-static __device__ __forceinline__ Seq seq_of(const Cache& c, int b) {
+static __device__ __forceinline__ Seq seq_of(const Cache& c, int b, const int* prefix = nullptr) {
   Seq s;
   s.len = clamped(c.lens[b], 0, c.table_pages << c.page_shift);
   s.start = clamped(c.starts[b], 0, c.tokens);
   s.n = clamped(c.starts[b + 1], s.start, c.tokens) - s.start;
+  s.prefix = prefix ? clamped(prefix[b], 0, s.len) : 0;
   return s;
 }
 
 static __device__ __forceinline__ Seq uniform(const Seq& s) {
-  return Seq{__builtin_amdgcn_readfirstlane(s.len), __builtin_amdgcn_readfirstlane(s.start), __builtin_amdgcn_readfirstlane(s.n)};
+  return Seq{__builtin_amdgcn_readfirstlane(s.len), __builtin_amdgcn_readfirstlane(s.start), __builtin_amdgcn_readfirstlane(s.n),
+             __builtin_amdgcn_readfirstlane(s.prefix)};
 }
 
 // The key tiles that rows of the new tokens [i0, i1] of a sequence see: `sink_tiles` first ones and those from `sink_tiles + skip` on, `count`
-// in all.  Tile u of them is tile u or u + skip of the sequence.
+// in all.  Tile u of them is tile u or u + skip of the sequence.  `first`: what none of the rows sees lies in front of it, but for a prefix and sinks.
 struct Keys {
   int sink_tiles, skip, count;
 };
-static __device__ __forceinline__ Keys keys_of(const Seq& s, int i0, int i1, int causal, int window, int sinks) {
+static __device__ __forceinline__ Keys keys_of(const Seq& s, int i0, int i1, int causal, int window, int sinks, int first = 0) {
   const int before = s.len - s.n;  // tokens that were there (negative: queries that see nothing)
-  const int end = causal ? min(s.len, before + i1 + 1) : s.len;
+  const int end = max(causal ? min(s.len, before + i1 + 1) : s.len, s.prefix);
   Keys k{0, 0, 0};
   if (end <= 0) return k;
   const int tiles = (end + kKeyTile - 1) / kKeyTile;
-  if (window > 0) {
-    const int low = max(0, before + i0 + 1 - window);
-    k.sink_tiles = (min(sinks, end) + kKeyTile - 1) / kKeyTile;
+  if (window > 0 || first > 0) {
+    const int low = max(first, window > 0 ? before + i0 + 1 - window : 0);
+    k.sink_tiles = (max(min(sinks, end), s.prefix) + kKeyTile - 1) / kKeyTile;
     k.skip = max(0, min(low / kKeyTile, tiles) - k.sink_tiles);
   }
   k.count = tiles - k.skip;
@@ -117,7 +152,7 @@ template <bool MANY> static __device__ __forceinline__ void load_of(const Attend
   tiles = (rows > a.few_most) == MANY ? (rows + ROWS - 1) / ROWS : 0;
   keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks).count;
   if (a.window > 0) {  // a row tile sees no more than its own window, wherever that begins, and the first tokens
-    const int most = (a.window + ROWS - 1 + kKeyTile - 1) / kKeyTile + 1 + (a.sinks + kKeyTile - 1) / kKeyTile;
+    const int most = (a.window + ROWS - 1 + kKeyTile - 1) / kKeyTile + 1 + (max(a.sinks, s.prefix) + kKeyTile - 1) / kKeyTile;
     keys = min(keys, most);
   }
   keys = max(keys, 1);  // rows that see nothing are written too
@@ -150,6 +185,29 @@ static __device__ __forceinline__ float wave_sum(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
+// The least and the largest first key of the new tokens [i0, i1] of a sequence (a.x.first), of a whole wave.
+struct Firsts {
+  int least, most;
+};
+static __device__ __forceinline__ Firsts firsts_of_lanes(int least, int most) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    least = min(least, __shfl_xor(least, m));
+    most = max(most, __shfl_xor(most, m));
+  }
+  return Firsts{__builtin_amdgcn_readfirstlane(least), __builtin_amdgcn_readfirstlane(most)};
+}
+static __device__ __forceinline__ Firsts firsts_of(const Scoring& x, const Seq& s, int i0, int i1) {
+  if (!x.first) return Firsts{0, 0};
+  int least = INT32_MAX, most = 0;
+  for (int i = i0 + (int)(threadIdx.x & 63); i <= i1; i += 64) {
+    const int f = clamped(x.first[s.start + i], 0, s.len);
+    least = min(least, f);
+    most = max(most, f);
+  }
+  return firsts_of_lanes(least, most);
+}
+
 // Many rows: the key tiles of a row tile are cut into even shares, so many that the whole launch makes about kManyWorkgroups workgroups,
 // each of kManyLeast tiles at least.  (A chunk of 512 over 2 K, 8 heads, us with 8, 12, 16 and 32 tiles: 28, 31, 35, 45.)
 struct Place {
@@ -160,14 +218,14 @@ struct Place {
 };
 // The place-th share of a KV head; MERGE: the place-th row tile that was cut.  Every wave works it out for itself, a lane a sequence, so that
 // there is no barrier.  False beyond the last.
-template <bool MERGE> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
+template <bool MERGE, int SC> static __device__ __forceinline__ bool find_place(const AttendArgs& a, int place, Place& p) {
   const int lane = threadIdx.x & 63;
   float total = 0.f;
   for (int b0 = 0; a.many_cut && b0 < a.c.batch; b0 += 64) {
     float work = 0.f;
     if (b0 + lane < a.c.batch) {
       int tiles, keys;
-      load_of<true>(a, seq_of(a.c, b0 + lane), tiles, keys);
+      load_of<true>(a, seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr), tiles, keys);
       work = (float)tiles * (float)keys;
     }
     total += wave_sum(work);
@@ -175,11 +233,11 @@ template <bool MERGE> static __device__ __forceinline__ bool find_place(const At
   const float share = fmaxf(total * a.kv_heads / kManyWorkgroups, (float)kManyLeast);
   int before = 0, slots_before = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
-    Seq s{0, 0, 0};
+    Seq s{0, 0, 0, 0};
     int tiles = 0, splits = 1;
     if (b0 + lane < a.c.batch) {
       int keys;
-      s = seq_of(a.c, b0 + lane);
+      s = seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr);
       load_of<true>(a, s, tiles, keys);
       splits = a.many_cut ? max(1, (int)ceilf(keys / share)) : 1;
     }
@@ -189,7 +247,7 @@ template <bool MERGE> static __device__ __forceinline__ bool find_place(const At
     if (beyond) {
       const int l = __builtin_ctzll(beyond);
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      p.s = Seq{of(s.len), of(s.start), of(s.n)};
+      p.s = Seq{of(s.len), of(s.start), of(s.n), SC ? of(s.prefix) : 0};
       p.b = b0 + l;
       p.splits = of(splits);
       const int r = place - (before + of(upto) - of(units));
@@ -350,6 +408,9 @@ template <bool ONCE, int HALF> static __device__ __forceinline__ void load_half_
 #undef RA_LOAD
 }
 
+// The same with scores that are shaped; which: SC.
+hipError_t launch_paged_scored(const AttendArgs& a, int sc, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream);
+
 // A launch of kFewWorkgroups workgroups and `many_places` more for each KV head; a.many_cut: and one that puts together the row tiles
 // whose keys were shared out, of which there are up to `cut_tiles`.
 hipError_t launch_paged_attend(const AttendArgs& a, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream);
@@ -366,6 +427,7 @@ hipError_t launch_paged_append(const AppendArgs& a, int dim, hipStream_t stream)
 
 struct WeightsArgs {
   Cache c;
+  Scoring x;
   const char* q;
   const float* lse;  // [heads, tokens]
   float* scores;     // [pages, kv_heads, page]
@@ -379,7 +441,7 @@ struct WeightsArgs {
   float* parts;  // many rows: sums of the parts of a block of keys, kManyKeys each
   int* arrived;  // ... and how many of them are there; 0 between launches
 };
-hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream);
+hipError_t launch_paged_weights(const WeightsArgs& a, int sc, int dtype, int dim, hipStream_t stream);
 
 struct EvictArgs {
   Cache c;

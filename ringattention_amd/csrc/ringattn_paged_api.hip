@@ -124,6 +124,29 @@ rp::Cache cache_of(const ringattn_paged_plan* pl, const ringattn_paged_cache* c,
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// What a call does with its scores; sc stays 0 where that is nothing.  Places in the sequence, which slopes and masks go by, a plan without
+// causality does not know.
+int check_scoring(const ringattn_paged_plan* pl, const ringattn_paged_scoring* s, int* sc, rp::Scoring* out) {
+  std::memset(out, 0, sizeof(*out));
+  if (!s) return RINGATTN_OK;
+  if (!std::isfinite(s->softcap) || s->softcap < 0.f) return RINGATTN_ERR_SHAPE;
+  if (!pl->p.causal && (s->slopes || s->prefix_lens || s->first_keys)) return RINGATTN_ERR_SHAPE;
+  if (!aligned(s->slopes, 4) || !aligned(s->prefix_lens, 4) || !aligned(s->first_keys, 4)) return RINGATTN_ERR_ALIGN;
+  if (s->softcap > 0.f) {
+    const double in = 2. * 1.4426950408889634 * pl->scale / s->softcap, outer = s->softcap * 1.4426950408889634;
+    // (a cap that leaves nothing of any score, or that 32 bits do not tell from none)
+    if (!(in < 1e30 && in > 1e-30 && outer < 1e30 && outer > 1e-30)) return RINGATTN_ERR_SHAPE;
+    out->cap_in = (float)in;
+    out->cap_out = (float)outer;
+  }
+  out->slopes = s->slopes;
+  out->prefix = s->prefix_lens;
+  out->first = s->first_keys;
+  if (s->softcap > 0.f || s->slopes || s->prefix_lens || s->first_keys)
+    *sc = rp::kScored | (s->softcap > 0.f ? rp::kCapped : 0) | (s->slopes ? rp::kSloped : 0);
+  return RINGATTN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -254,10 +277,13 @@ int ringattn_paged_append_rotary(ringattn_paged_plan* plan, const ringattn_paged
   return RINGATTN_OK;
 }
 
-int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
-                       int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* stream_) {
+static int attend(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q, int tokens,
+                  int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* stream_) {
   if (!plan_ok(plan)) return RINGATTN_ERR_PLAN;
   RP_CHECK(check_cache(plan, cache, true, true));
+  int sc = 0;
+  rp::Scoring x;
+  RP_CHECK(check_scoring(plan, scoring, &sc, &x));
   if (!q || !out || !lse) return RINGATTN_ERR_NULL;
   const bool fp32 = (plan->p.flags & RINGATTN_FLAG_PAGED_PARTIALS) != 0;
   RP_CHECK(check_rows(plan, tokens, plan->p.heads, q_token_stride, q_head_stride, 8, false));
@@ -269,6 +295,7 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   rp::AttendArgs a;
   std::memset(&a, 0, sizeof(a));
   a.c = cache_of(plan, cache, tokens);
+  a.x = x;
   a.q = (const char*)q;
   a.out = (char*)out;
   a.lse = lse;
@@ -295,7 +322,8 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   // What sequences see at most, in key tiles, and their row tiles if all have few rows; in units so large that 2^30 suffice for both.
   const int64_t few_tiles = rows / rp::kFewRows + sequences;
   const int64_t see = ((int64_t)cache->table_pages * plan->p.page_size + rp::kKeyTile - 1) / rp::kKeyTile + rp::kFewSmall;
-  const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see, most = see < in_window ? see : in_window;
+  const int64_t in_window = a.window > 0 ? (a.window + rp::kManyRows + (int64_t)a.sinks) / rp::kKeyTile + 3 : see;
+  const int64_t most = see < in_window || x.prefix ? see : in_window;  // (prefixes are of any length)
   // More rows are few where that cannot make more work than kFewMore key tiles a workgroup, whose parts are fewer and smaller.
   const bool little = few_tiles * kv * most <= (int64_t)rp::kFewMore * rp::kFewWorkgroups;
   a.few_most = few_most(tokens, cache->batch, little ? rp::kFewRowsMore : cache->batch == 1 ? rp::kFewRowsAlone : rp::kFewRowsMost);
@@ -312,14 +340,29 @@ int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* ca
   // Workgroups of few rows first; of a sequence alone, whose rows are many if q is full, last, where they cost a full one next to nothing (us
   // with and without them: 4096 tokens over 32 K, 32 heads 1867 and 1867; with a window of 1024, 8 KV heads 94.9 and 94.2).
   a.few_begin = sequences == 1 ? (int)(places * kv) : 0;
-  RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, places, tiles < due ? tiles : due, stream));
+  const int64_t cut_tiles = tiles < due ? tiles : due;
+  if (sc) RP_HIP(rp::launch_paged_scored(a, sc, plan->p.dtype, plan->p.dim, places, cut_tiles, stream));
+  else RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, places, cut_tiles, stream));
   return RINGATTN_OK;
 }
 
-int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
-                           int64_t q_head_stride, const float* lse, float* scores, void* stream) {
+int ringattn_paged_fwd(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
+                       int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* stream) {
+  return attend(plan, cache, nullptr, q, tokens, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, lse, stream);
+}
+int ringattn_paged_fwd_scored(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q,
+                              int tokens, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              float* lse, void* stream) {
+  return attend(plan, cache, scoring, q, tokens, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, lse, stream);
+}
+
+static int weigh(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q, int tokens,
+                 int64_t q_token_stride, int64_t q_head_stride, const float* lse, float* scores, void* stream) {
   if (!plan_ok(plan)) return RINGATTN_ERR_PLAN;
   RP_CHECK(check_cache(plan, cache, false, true));
+  int sc = 0;
+  rp::Scoring x;
+  RP_CHECK(check_scoring(plan, scoring, &sc, &x));
   if (!q || !lse || !scores) return RINGATTN_ERR_NULL;
   RP_CHECK(check_rows(plan, tokens, plan->p.heads, q_token_stride, q_head_stride, 8, false));
   if (!aligned(q, 16) || !aligned(lse, 4) || !aligned(scores, 4)) return RINGATTN_ERR_ALIGN;
@@ -327,6 +370,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   rp::WeightsArgs a;
   std::memset(&a, 0, sizeof(a));
   a.c = cache_of(plan, cache, tokens);
+  a.x = x;
   a.q = (const char*)q;
   a.lse = lse;
   a.scores = scores;
@@ -346,8 +390,17 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
   a.arrived = (int*)plan->ws;
   a.parts = (float*)((char*)plan->ws + kCounterBytes);
   a.q_even = 32 % a.group == 0 && a.q_ts < 1 << 25 && a.q_hs < 1 << 25 && (int64_t)a.group * tokens < 1 << 29;
-  RP_HIP(rp::launch_paged_weights(a, plan->p.dtype, plan->p.dim, (hipStream_t)stream));
+  RP_HIP(rp::launch_paged_weights(a, sc, plan->p.dtype, plan->p.dim, (hipStream_t)stream));
   return RINGATTN_OK;
+}
+
+int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const void* q, int tokens, int64_t q_token_stride,
+                           int64_t q_head_stride, const float* lse, float* scores, void* stream) {
+  return weigh(plan, cache, nullptr, q, tokens, q_token_stride, q_head_stride, lse, scores, stream);
+}
+int ringattn_paged_weights_scored(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, const ringattn_paged_scoring* scoring, const void* q,
+                                  int tokens, int64_t q_token_stride, int64_t q_head_stride, const float* lse, float* scores, void* stream) {
+  return weigh(plan, cache, scoring, q, tokens, q_token_stride, q_head_stride, lse, scores, stream);
 }
 
 int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, float* scores, const int* kept_table, int kept_pages,

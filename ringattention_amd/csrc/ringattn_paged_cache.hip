@@ -84,7 +84,7 @@ static __device__ __forceinline__ float sum_lanes(float (&w)[16]) {
 
 
 // What both kernels know of their sequence and KV head.
-template <int DT, int D> struct WeightRows {
+template <int DT, int D, int SC> struct WeightRows {
   const WeightsArgs& a;
   const Seq s;
   const int head, rows, before;
@@ -116,9 +116,9 @@ template <int DT, int D> struct WeightRows {
   }
   // the new tokens [i0, i1) that see any of the keys [key0, key0 + keys)
   __device__ __forceinline__ void tokens_of(int key0, int keys, int& i0, int& i1) const {
-    i0 = a.causal ? max(0, key0 - before) : 0;
+    i0 = a.causal && key0 >= s.prefix ? max(0, key0 - before) : 0;
     i1 = s.n;
-    if (a.window > 0 && key0 >= a.sinks) i1 = max(i0, (int)min((int64_t)s.n, (int64_t)key0 + keys - 1 + a.window - before));
+    if (a.window > 0 && key0 >= (SC ? max(a.sinks, s.prefix) : a.sinks)) i1 = max(i0, (int)min((int64_t)s.n, (int64_t)key0 + keys - 1 + a.window - before));
   }
   // scores that weigh nothing: of row r, of the 16 keys that a lane has from key0 on.  z: its log2(e) LSE.  One that is no number makes no
   // number of -inf either, so that there the scores of the keys that the row sees are none, and z is 0.
@@ -126,9 +126,13 @@ template <int DT, int D> struct WeightRows {
     const float none = z == z ? 0.f : z;
     z = z == z ? z : 0.f;
     const int token = quotient(min(r, rows - 1), a.by_group);
-    const int lim = r >= rows ? 0 : a.causal ? min(s.len, before + token + 1) : s.len;
-    const int low = a.window > 0 ? before + token - a.window : -1;
-    int first = key0 + 4 * h, sinks = a.sinks;
+    int lim = r >= rows ? 0 : a.causal ? min(s.len, before + token + 1) : s.len;
+    int low = a.window > 0 ? before + token - a.window : -1;
+    if constexpr (SC != 0) {
+      lim = r >= rows ? 0 : max(lim, s.prefix);
+      if (a.x.first) low = max(low, clamped(a.x.first[s.start + token], 0, s.len) - 1);
+    }
+    int first = key0 + 4 * h, sinks = SC ? max(a.sinks, s.prefix) : a.sinks;
     asm volatile("" : "+v"(first), "+v"(sinks));  // (nothing of these comparisons is kept from tile to tile: it took 100 registers)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -136,9 +140,18 @@ template <int DT, int D> struct WeightRows {
       sacc[e] = bool((k >= lim) | ((k <= low) & (k >= sinks))) ? -INFINITY : sacc[e] + none;  // (no branches)
     }
   }
+  // Scores to what attention takes the exponentials of, but for a factor k2.
+  __device__ __forceinline__ float k2() const { return (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2; }
+  __device__ __forceinline__ void shape(f32x16& sacc, int key0, int r) const {
+    if constexpr ((SC & (kCapped | kSloped)) != 0) {
+      int token, q_head;
+      row_of(r, token, q_head);
+      shape_scores<SC>(sacc, a.x, a.scale_log2, (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f, key0 + 4 * h - before - token);
+    }
+  }
   __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse) const {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], a.scale_log2, -lse));
+    for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], k2(), -lse));
   }
   // Every key of a sequence has one owner, which adds to its score once: no order to go by.  Atomic, since pages may be several sequences'.
   __device__ __forceinline__ void add_score(int page, int key, float x) const {
@@ -150,15 +163,15 @@ template <int DT, int D> struct WeightRows {
 // Few rows: a wave has 32 keys at a time, all rows.  Bound by the read of K: tiles come HBM -> LDS one ahead, and every compute unit has eight
 // waves of them.
 constexpr int kFewWaves = 4;
-template <int DT, int D>
+template <int DT, int D, int SC>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(const WeightsArgs a) {
   using E = Elem<DT>;
   constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, HALF = D / 32;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kFewWaves * 2 * TILE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.x, b = blockIdx.z;
-  const Seq s = uniform(seq_of(a.c, b));
-  const WeightRows<DT, D> x(a, s, b, head);
+  const Seq s = uniform(seq_of(a.c, b, SC ? a.x.prefix : nullptr));
+  const WeightRows<DT, D, SC> x(a, s, b, head);
   if (x.rows == 0 || s.len == 0 || x.rows > a.few_most) return;
   const int n = x.n, h = x.h;
   const Keys keys = keys_of(s, 0, s.n - 1, a.causal, a.window, a.sinks);  // that any row sees
@@ -223,6 +236,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
       float z = lse_first;
+      x.shape(sacc, key0, n);
       x.hide(sacc, key0, n, z);
       x.weigh(w, sacc, z);
     }
@@ -235,6 +249,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(q + ks * 32), sacc);
+      x.shape(sacc, key0, r0 + n);
       x.hide(sacc, key0, r0 + n, z);
       x.weigh(w, sacc, z);
     }
@@ -252,7 +267,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
 // a Q tile for each wave and nothing on the way while it has the exponentials, 180 with no equal shares of the triangle).  Bound by power as much as
 // by the order of things: with queries and keys of 0 the same launch takes 140 us.  Workgroups of four waves, two to a compute unit, take
 // 162: of two waves of a SIMD that wait for nothing together the older one gets most of its issue, and when it is done the younger is alone.
-template <int DT, int D>
+template <int DT, int D, int SC>
 __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(const WeightsArgs a) {
   using E = Elem<DT>;
   constexpr int KS = D / 16, ROWB = D * 2, TILE = 32 * ROWB, CPR = D / 8, PIECES = TILE / 2048;  // (pieces of 1 KB that a wave brings of its tile)
@@ -268,19 +283,20 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
   Seq s{};
   for (int b0 = 0, before = 0; b0 < a.c.batch && b < 0; b0 += 64) {
     Seq mine{};
-    if (b0 + lane < a.c.batch) mine = seq_of(a.c, b0 + lane);
+    if (b0 + lane < a.c.batch) mine = seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr);
     const uint64_t many = __builtin_amdgcn_ballot_w64(mine.n * a.group > a.few_most);
     const int wanted = (int)blockIdx.z - before, count = __builtin_popcountll(many);
     if (wanted < count) {
       const bool it = (many >> lane & 1) && __builtin_popcountll(many & (((uint64_t)1 << lane) - 1)) == wanted;
       const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(it));
-      s = Seq{__builtin_amdgcn_readlane(mine.len, l), __builtin_amdgcn_readlane(mine.start, l), __builtin_amdgcn_readlane(mine.n, l)};
+      s = Seq{__builtin_amdgcn_readlane(mine.len, l), __builtin_amdgcn_readlane(mine.start, l), __builtin_amdgcn_readlane(mine.n, l),
+              SC ? __builtin_amdgcn_readlane(mine.prefix, l) : 0};
       b = b0 + l;
     }
     before += count;
   }
   if (b < 0) return;
-  const WeightRows<DT, D> x(a, s, b, head);
+  const WeightRows<DT, D, SC> x(a, s, b, head);
   const int n = x.n, h = x.h, before = x.before;
   auto page_of = [&](int key) {  // -1: not there, or behind the end
     const int page = key < s.len ? x.table[key >> a.c.page_shift] : -1;
@@ -347,7 +363,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
     // the steps all of whose rows see all of the keys
     int seen_from = 0, seen_to = (x.rows - r_begin) / STEP;
     if (a.causal) seen_from = (max(0, key0 + kManyKeys - 1 - before - i0) * a.group + STEP - 1) / STEP;
-    if (key0 + kManyKeys > s.len) seen_to = 0;
+    if (key0 + kManyKeys > s.len || (SC && a.x.first)) seen_to = 0;
     if (a.window > 0 && key0 + kManyKeys > a.sinks) seen_to = min(seen_to, (int)max((int64_t)0, min((int64_t)s.n, (int64_t)key0 + a.window - before - i0)) * a.group / STEP);
     const unsigned seen = max(0, seen_to - seen_from);
     s16x8 kfr[2][KS];
@@ -396,6 +412,8 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
         for (int c = 0; c < 2; ++c) sacc[c] = E::mma(kfr[c][ks], qfr[ks], sacc[c]);
     };
     auto hide = [&](f32x16 (&sacc)[2], int step, float& z) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x.shape(sacc[c], my_key0 + 32 * c, r_begin + step * STEP + 32 * pair + n);
       if ((unsigned)(step - seen_from) >= seen) {
         const float from = z;
 #pragma unroll
@@ -410,7 +428,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          w[c][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c][e], a.scale_log2, -z));
+          w[c][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c][e], x.k2(), -z));
           asm volatile("" : "+v"(w[c][e]));  // (here, not where the sums are used next)
         }
     };
@@ -485,7 +503,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
   }
 }
 
-hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream) {
+template <int SC> static hipError_t launch_weights(const WeightsArgs& a, int dtype, int dim, hipStream_t stream) {
   const int64_t keys = (int64_t)a.c.table_pages << a.c.page_shift;
   const int64_t pairs = (int64_t)a.c.batch * a.kv_heads;
   if (pairs <= 0 || keys <= 0) return hipSuccess;
@@ -504,9 +522,9 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
 #define RA_LAUNCH_WEIGHTS(DT_, D_)                                                                                                      \
   do {                                                                                                                                 \
     if (a.c.batch > 1 || with_many == 0)                                                                                               \
-      paged_weights_few_kernel<DT_, D_><<<grid(kFewWaves * kKeyTile, a.c.batch, 2048), 64 * kFewWaves, 0, stream>>>(a);                 \
+      paged_weights_few_kernel<DT_, D_, SC><<<grid(kFewWaves * kKeyTile, a.c.batch, 2048), 64 * kFewWaves, 0, stream>>>(a);                 \
     if (with_many > 0)                                                                                                                 \
-      paged_weights_kernel<DT_, D_>                                                                                                    \
+      paged_weights_kernel<DT_, D_, SC>                                                                                                \
           <<<grid(kManyKeys / kWeightParts, with_many, with_many > 1 ? kWeightUnits / kWeightLaps : 256), 64 * kWeightWaves, 0, stream>>>(a); \
   } while (0)
   if (dtype == 0 && dim == 64) RA_LAUNCH_WEIGHTS(0, 64);
@@ -516,6 +534,17 @@ hipError_t launch_paged_weights(const WeightsArgs& a, int dtype, int dim, hipStr
 #undef RA_LAUNCH_WEIGHTS
   else return hipErrorInvalidValue;
   return hipGetLastError();
+}
+
+hipError_t launch_paged_weights(const WeightsArgs& a, int sc, int dtype, int dim, hipStream_t stream) {
+  switch (sc) {
+    case 0: return launch_weights<0>(a, dtype, dim, stream);
+    case kScored: return launch_weights<kScored>(a, dtype, dim, stream);
+    case kScored | kCapped: return launch_weights<kScored | kCapped>(a, dtype, dim, stream);
+    case kScored | kSloped: return launch_weights<kScored | kSloped>(a, dtype, dim, stream);
+    case kScored | kCapped | kSloped: return launch_weights<kScored | kCapped | kSloped>(a, dtype, dim, stream);
+  }
+  return hipErrorInvalidValue;
 }
 
 // ---- eviction ----------------------------------------------------------------------

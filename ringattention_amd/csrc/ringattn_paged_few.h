@@ -23,13 +23,13 @@ struct Lanes {
   int most = 0, fewest = INT32_MAX;  // key tiles that a row tile of any sequence sees
   float news = 0.f;                  // new tokens of this lane's sequences
   // round: to multiples of kFewLeast; else kFewSmall at least, or `fixed` of them
-  __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round, int fixed) {
+  template <int SC> __device__ __forceinline__ int add(const AttendArgs& a, int b0, int before, bool round, int fixed) {
     const int lane = threadIdx.x & 63;
-    s = Seq{0, 0, 0};
+    s = Seq{0, 0, 0, 0};
     tiles = 0;
     keys = 1;
     if (b0 + lane < a.c.batch) {
-      s = seq_of(a.c, b0 + lane);
+      s = seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr);
       news += (float)s.n;
       load_of<false>(a, s, tiles, keys);
       if (tiles > 0) {
@@ -48,12 +48,12 @@ struct Piece {
   Seq s;
   int b, tile, head;
   int from, keys;   // unit of the row tile, of how many
-  __device__ __forceinline__ bool find(const AttendArgs& a, const Lanes& x, int b0, int pos) {
+  template <int SC> __device__ __forceinline__ bool find(const AttendArgs& a, const Lanes& x, int b0, int pos) {
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(x.upto > pos);
     if (beyond == 0) return false;
     const int l = __builtin_ctzll(beyond);
     auto of = [&](int y) { return __builtin_amdgcn_readlane(y, l); };
-    s = Seq{of(x.s.len), of(x.s.start), of(x.s.n)};
+    s = Seq{of(x.s.len), of(x.s.start), of(x.s.n), SC ? of(x.s.prefix) : 0};
     b = b0 + l;
     keys = of(x.keys);
     const int at = pos - (of(x.upto) - of(x.tiles) * keys * a.kv_heads), unit = at / keys;
@@ -149,7 +149,7 @@ struct Left {
 };
 template <int D> constexpr int kFewLds = 8 * kFewWaveLds<D> + 8 * kFewRows * (int)sizeof(float2) + 2 * (int)sizeof(Left) + 16 * (int)sizeof(int);
 
-template <int DT, int D> static __device__ __forceinline__ void few_rows(const AttendArgs& a, unsigned char* smem, int block) {
+template <int DT, int D, int SC = 0> static __device__ __forceinline__ void few_rows(const AttendArgs& a, unsigned char* smem, int block) {
   using E = Elem<DT>;
   constexpr int WAVES = 8, BM = kFewRows, BN = kKeyTile;
   constexpr int ROWB = D * 2, TILE = BN * ROWB;
@@ -175,7 +175,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   // heads takes 15 instead of 14, and one of 16 K has half as many workgroups.)
   const int least = max(1, kFewLeast >> a.few_shift), small = max(1, kFewSmall >> a.few_shift);  // units
   int total = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, true, 0);
+  for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.template add<SC>(a, b0, total, true, 0);
   // Starts that go down and up again have sequences share the call's tokens, and a.few_shift lets 32 bits suffice for sequences that do not: with
   // as many new tokens in all as the call has, 2^30.  Where they have more than a few shared ones, nothing is done for those of few rows.
   if (wave_sum(lanes.news) > 1.75f * a.c.tokens) return;
@@ -183,7 +183,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   const bool some_small = !round && __builtin_amdgcn_ballot_w64(lanes.fewest <= kFewSmall) != 0;
   if (!round) {
     total = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.add(a, b0, total, false, 0);
+    for (int b0 = 0; b0 < a.c.batch; b0 += 64) total = lanes.template add<SC>(a, b0, total, false, 0);
   }
   int each = round ? least : max((total + kFewWorkgroups - 1) / kFewWorkgroups, least);
   if (!round && all_small) each = (each + small - 1) / small * small;
@@ -218,17 +218,18 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
   for (int pos = w * each, turn = 0; pos < end; turn ^= 1) {
     auto find = [&](Piece& p, int at) {
       if (a.c.batch <= 64) {
-        p.find(a, lanes, 0, at);
+        p.template find<SC>(a, lanes, 0, at);
       } else {
         for (int b0 = 0, before = 0; b0 < a.c.batch; b0 += 64) {
-          before = lanes.add(a, b0, before, round, fixed);
-          if (p.find(a, lanes, b0, at)) break;
+          before = lanes.template add<SC>(a, b0, before, round, fixed);
+          if (p.template find<SC>(a, lanes, b0, at)) break;
         }
       }
     };
     auto keys_at = [&](const Piece& p) {
       const int first = p.tile * BM, last = min(first + BM, p.s.n * a.group) - 1;
-      return keys_of(p.s, quotient(first, a.by_group), quotient(last, a.by_group), a.causal, a.window, a.sinks);
+      const int i0 = quotient(first, a.by_group), i1 = quotient(last, a.by_group);
+      return keys_of(p.s, i0, i1, a.causal, a.window, a.sinks, SC ? firsts_of(a.x, p.s, i0, i1).least : 0);
     };
     // Where some of the next eight row tiles see little, each is a wave's own: they begin and end beside each other, and do not meet.  Against eight
     // waves a row tile one after the other, that is `most` tiles in a wave instead of `in_row` beginnings and ends.  (Us alone and not: 94
@@ -276,10 +277,15 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
     // this lane's row: its token, its head, its position; rows beyond the range read the last valid one
     const int row = min(r0 + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
     const int before = p.s.len - p.s.n;
-    const int lim = a.causal ? min(p.s.len, before + token + 1) : p.s.len;           // keys below it are visible ...
-    const int low = a.window > 0 ? before + token - a.window : -1;                   // ... if they are above this one, or sinks
+    const int first = SC && a.x.first ? clamped(a.x.first[p.s.start + token], 0, p.s.len) : 0;  // of a scored call: the first key that the row sees
+    const int lim = max(a.causal ? min(p.s.len, before + token + 1) : p.s.len, p.s.prefix);  // keys below it are visible ...
+    const int low = max(a.window > 0 ? before + token - a.window : -1, first - 1);   // ... if they are above this one, or sinks or of the prefix
+    const int keep = SC ? max(a.sinks, p.s.prefix) : a.sinks;
     // of all rows of the tile
-    const int lim_all = a.causal ? min(p.s.len, before + i0 + 1) : p.s.len, low_any = a.window > 0 ? before + i1 - a.window : -1;
+    const int lim_all = max(a.causal ? min(p.s.len, before + i0 + 1) : p.s.len, p.s.prefix);
+    const int low_any = max(a.window > 0 ? before + i1 - a.window : -1, SC && a.x.first ? firsts_of_lanes(first, first).most - 1 : -1);
+    const float slope = (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f;
+    const float k2 = (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2;  // scores to units of log2, where they are not in these already
 
     s16x8 qf[KS];
     {
@@ -367,7 +373,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
         typename E::vec8 pv;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], a.scale_log2, -ms));
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], k2, -ms));
           sums[e & 3] = t2 == 0 && e < 4 ? x : sums[e & 3] + x;
           pv[e] = (typename E::type)x;
         }
@@ -382,7 +388,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
         m1 = fmaxf(fmaxf(m1, sacc[e + 2]), sacc[e + 3]);
       }
       m = cross_half_max(fmaxf(m0, m1));
-      const float cs = (m == -INFINITY) ? kNoReference : m * a.scale_log2;
+      const float cs = (m == -INFINITY) ? kNoReference : m * k2;
       const float alpha = __builtin_amdgcn_exp2f(ms - cs);
 #pragma unroll
       for (int i = 0; i < 4; ++i) ls[i] *= alpha;
@@ -392,7 +398,7 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
     };
     auto hidden = [&](const Tile& x, int e, int hh) {  // of accumulator e of a lane of half hh: is its key hidden from this lane's row?
       const int key = x.key + 8 * (e >> 2) + (e & 3) + 4 * hh;
-      return bool((key >= lim) | ((key <= low) & (key >= a.sinks)) | (x.gone >> (e >> 3) & 1));  // (no branches)
+      return bool((key >= lim) | ((key <= low) & (key >= keep)) | (x.gone >> (e >> 3) & 1));  // (no branches)
     };
 
     int u = u_begin + (alone ? 0 : wave);
@@ -424,7 +430,8 @@ template <int DT, int D> static __device__ __forceinline__ void few_rows(const A
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
       }
-      const bool masked = cur.key + BN > lim_all || (cur.key <= low_any && cur.key + BN > a.sinks) || cur.gone;
+      if constexpr (SC != 0) shape_scores<SC>(sacc, a.x, a.scale_log2, slope, cur.key + 4 * h - before - token);
+      const bool masked = cur.key + BN > lim_all || (cur.key <= low_any && cur.key + BN > keep) || cur.gone;
       if (masked) {
         asm volatile("");  // (a branch, not sixteen selections in every tile)
 #pragma unroll

@@ -14,7 +14,7 @@ namespace paged {
 
 template <int D> constexpr int kManyLds = 8 * kKeyTile * D * 2 + 16;
 
-template <int DT, int D> static __device__ __forceinline__ void many_rows(const AttendArgs& a, unsigned char* smem, int block) {
+template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many_rows(const AttendArgs& a, unsigned char* smem, int block) {
   using E = Elem<DT>;
   constexpr int WAVES = 8, BM = kManyRows, BN = kKeyTile, NBUF = 4;
   constexpr int CPR = D / 8, ROWB = D * 2, TILE = BN * ROWB, KS = D / 16, DB = D / 32;
@@ -31,16 +31,23 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   Place p;
   const int unit = quotient(block, a.by_kv_heads);
   const int head = block - unit * a.kv_heads;
-  if (!find_place<false>(a, unit, p)) return;
+  if (!find_place<false, SC>(a, unit, p)) return;
   const int rows = p.s.n * a.group;
   const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
-  const Keys keys = keys_of(p.s, quotient(r0, a.by_group), quotient(r_last, a.by_group), a.causal, a.window, a.sinks);
+  const int i_first = quotient(r0, a.by_group), i_last = quotient(r_last, a.by_group);
+  const Firsts firsts = SC ? firsts_of(a.x, p.s, i_first, i_last) : Firsts{0, 0};
+  const Keys keys = keys_of(p.s, i_first, i_last, a.causal, a.window, a.sinks, firsts.least);
   const int u_begin = (int)((int64_t)p.split * keys.count / p.splits);
   const int n_tiles = (int)((int64_t)(p.split + 1) * keys.count / p.splits) - u_begin;  // of this share: tile t is tile u_begin + t
 
   // this lane's row; rows beyond the range read the last valid one
   const int row = min(r0 + 32 * wave + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
   const int before = p.s.len - p.s.n;
+  // of a scored call: the first key that this lane's row sees, its head's slope; keys in front of `keep` are seen by rows that come behind them, whatever window and documents say
+  const int first = SC && a.x.first ? clamped(a.x.first[p.s.start + token], 0, p.s.len) : 0;
+  const float slope = (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f;
+  const int keep = SC ? max(a.sinks, p.s.prefix) : a.sinks;
+  const float k2 = (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2;  // scores to units of log2, where they are not in these already
   // What the masks and other seldom taken paths are worked out from: the compiler would keep all of it in registers through every tile.
   auto fresh = [](int x) {
     asm volatile("" : "+v"(x));
@@ -52,14 +59,15 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   struct Clear {
     int up, low;
   };
-  auto clear_of = [&](int first, int last) {
+  auto clear_of = [&](int first, int last, int most_first) {
     const int i0 = quotient(min(first, r_last), a.by_group), i1 = quotient(min(last, r_last), a.by_group);
+    const int low = max(a.window > 0 ? before + i1 - a.window : -1, most_first - 1);
     Clear x;
-    x.up = __builtin_amdgcn_readfirstlane(tile_of(max(0, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
-    x.low = a.window > 0 && before + i1 - a.window >= 0 ? __builtin_amdgcn_readfirstlane(tile_of((before + i1 - a.window) / BN + 1)) : 0;
+    x.up = __builtin_amdgcn_readfirstlane(tile_of(max(p.s.prefix, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
+    x.low = low >= 0 ? __builtin_amdgcn_readfirstlane(tile_of(low / BN + 1)) : 0;
     return x;
   };
-  const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31), every = clear_of(r0, r_last);
+  const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31, SC && a.x.first ? firsts_of_lanes(first, first).most : 0), every = clear_of(r0, r_last, firsts.most);
   const int t_up = mine.up, t_low = mine.low;
 
   s16x8 qf[KS];
@@ -145,11 +153,12 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   };
   auto sight = [&]() {
     const int t = fresh(token);
-    return Sight{a.causal ? min(p.s.len, before + t + 1) : p.s.len, a.window > 0 ? before + t - a.window : -1};
+    const Sight x{a.causal ? min(p.s.len, before + t + 1) : p.s.len, a.window > 0 ? before + t - a.window : -1};
+    return SC ? Sight{max(x.lim, p.s.prefix), max(x.low, fresh(first) - 1)} : x;
   };
   auto hidden = [&](const Sight& x, int key0, int gone, int e, int hh) {  // is the key of accumulator e of a lane of half hh hidden?
     const int key = key0 + 8 * (e >> 2) + (e & 3) + 4 * hh;
-    return bool((key >= x.lim) | ((key <= x.low) & (key >= a.sinks)) | (gone >> (e >> 3) & 1));  // (no branches)
+    return bool((key >= x.lim) | ((key <= x.low) & (key >= keep)) | (gone >> (e >> 3) & 1));  // (no branches)
   };
 
   float m = -INFINITY;  // reference max (raw score units)
@@ -173,7 +182,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
     if (!may_be_masked(t)) return;
     const int key0 = first_key(t), gone = gone_of(t), half = fresh(lane) >> 5;
     const Sight x = sight();
-    if (gone == 0 && key0 >= a.sinks) {  // the keys between `low` and `lim`, as one comparison each
+    if (gone == 0 && key0 >= keep) {  // the keys between `low` and `lim`, as one comparison each
       const unsigned from = key0 + 4 * half - x.low - 1, count = max(0, x.lim - x.low - 1);
 #pragma unroll
       for (int e = 0; e < 16; ++e) sacc[e] = from + (8 * (e >> 2) + (e & 3)) < count ? sacc[e] : -INFINITY;
@@ -192,9 +201,9 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
       m1 = fmaxf(fmaxf(m1, sacc[e + 2]), sacc[e + 3]);
     }
     const float cand = cross_half_max(fmaxf(m0, m1));
-    if (__builtin_amdgcn_ballot_w64((cand - m) * a.scale_log2 > kLazyLog2) != 0) {
-      const float cs = (cand == -INFINITY) ? 0.f : cand * a.scale_log2;
-      const float alpha = __builtin_amdgcn_exp2f(m * a.scale_log2 - cs);
+    if (__builtin_amdgcn_ballot_w64((cand - m) * k2 > kLazyLog2) != 0) {
+      const float cs = (cand == -INFINITY) ? 0.f : cand * k2;
+      const float alpha = __builtin_amdgcn_exp2f(m * k2 - cs);
 #pragma unroll
       for (int i = 0; i < 2; ++i) ls[i] *= alpha;
 #pragma unroll
@@ -205,14 +214,19 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
   };
   // P = exp2(S k2 - m k2); the sums from the unrounded values, the operands of the next product rounded to the storage type: no more than
   // the output's own rounding
-  auto softmax_phase = [&]() {
+  // Scored: the scores of tile t are shaped first, and then masked, so that a hidden one is -inf and not minus the cap.
+  auto softmax_phase = [&](int t, bool may_hide) {
+    if constexpr (SC != 0) {
+      shape_scores<SC>(sacc, a.x, a.scale_log2, slope, first_key(t) + 4 * h - before - token);
+      if (may_hide) mask_tile(t);
+    }
     move_reference();
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
       typename E::vec8 pv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], a.scale_log2, -ms));
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * t2 + e], k2, -ms));
         ls[e & 1] += x;
         pv[e] = (typename E::type)x;
       }
@@ -338,11 +352,11 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
       if (SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
       if (!SECOND) mfma_phase(SLOT, (SLOT + 1) & 3);
-      else softmax_phase();
+      else softmax_phase(t, false);
       phase_fence();
       if (!SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
-      if (!SECOND) softmax_phase();
+      if (!SECOND) softmax_phase(t + 1, false);
       else mfma_phase(SLOT, (SLOT + 1) & 3);
       phase_fence();
     };
@@ -351,7 +365,7 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
       if ((t & 1) == 0) looking_barrier(t);
       if (SECOND) {
         issue_loads(t, (t & 1) == 0);
-        softmax_phase();
+        softmax_phase(t, true);
       }
       phase_fence();
       if (odd_values(t)) {
@@ -361,15 +375,15 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
         mfma_phase(t & 3, (t + 1) & 3);
       }
       phase_fence();
-      mask_tile(t + 1);
+      if (SC == 0) mask_tile(t + 1);
       if (!SECOND) {
         issue_loads(t, (t & 1) == 0);
-        if (t + 1 < n_tiles) softmax_phase();  // (the scores past the last tile are of nothing)
+        if (t + 1 < n_tiles) softmax_phase(t + 1, true);  // (the scores past the last tile are of nothing)
       }
       phase_fence();
     };
-    mask_tile(0);
-    if (!SECOND) softmax_phase();
+    if (SC == 0) mask_tile(0);
+    if (!SECOND) softmax_phase(0, true);
     // block t has the products of tile t and the scores of tile t + 1.  Three loops one after the other, not one with two ways through it:
     // where two meet again the compiler has two sets of accumulators (64 moves a group, and registers in scratch)
     int t = 0;
@@ -422,12 +436,12 @@ template <int DT, int D> static __device__ __forceinline__ void many_rows(const 
 // share.  (A chunk of 16 tokens, 128 K cached, 16 heads on one, 256 shares: 97 us with one wave for all shares and the four column blocks in a
 // workgroup, 69, 52 and 51 with two, four and eight waves and a workgroup for each; four sequences of 4 K, 64 tokens each, 8 shares:
 // 41, 40, 40 and 47.)  One barrier a call, whatever there is to do.  False behind the last.
-template <int DT, int D> static __device__ __forceinline__ bool merge_many(const AttendArgs& a, int block, float (*sums)[18][64]) {
+template <int DT, int D, int SC = 0> static __device__ __forceinline__ bool merge_many(const AttendArgs& a, int block, float (*sums)[18][64]) {
   constexpr int BLOCKS = kManyRows / 32, DB = D / 32;
   const int lane = threadIdx.x & 63, n = lane & 31, sharer = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Place p;
   const int unit = quotient(block, a.by_kv_heads), head = block - unit * a.kv_heads, rows_of = unit / DB % BLOCKS, db = unit % DB;
-  if (!find_place<true>(a, unit / (DB * BLOCKS), p)) return false;
+  if (!find_place<true, SC>(a, unit / (DB * BLOCKS), p)) return false;
   const int r0 = p.tile * kManyRows, r_last = min(r0 + kManyRows, p.s.n * a.group) - 1;
   if (r0 + 32 * rows_of > r_last) {  // (rows of no token: the same for all waves)
     __syncthreads();

@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import RingattnPagedCache, RingattnPagedParams, check
+from ._lib import RingattnPagedCache, RingattnPagedParams, RingattnPagedScoring, check
 from .api import DTYPE_CODE, TORCH_DTYPE, _check_tensors, _stream_ptr
 
 FLAG_PAGED_PARTIALS = 1
@@ -55,13 +55,14 @@ class PagedAttention:
 
     `window` > 0: a token sees the last `window` tokens up to itself and the first `sinks` of the sequence.  `causal=False`:
     it sees every cached token; `partials`: out is float32, a partial (O, LSE) for api.merge -- together, for a sequence whose cache is
-    spread over several pools or GPUs.  `keep_present`: evict() keeps no token whose page is not there.  `workspace`: a (device
+    spread over several pools or GPUs.  `softcap` > 0: a score x becomes softcap tanh(x / softcap); `slopes`, float32 [heads] on the device: less
+    slopes[head] times the distance of query and key (causal plans); for forward() and weights().  `keep_present`: evict() keeps no token whose page is not there.  `workspace`: a (device
     address, bytes) pair the caller owns and keeps alive, instead of an allocation by the plan.  It holds zeros when the plan is made
     (torch.zeros, not torch.empty): workgroups that share a row count themselves in it, and leave it at 0.  One call at a time, and replays
     of captured calls in turn: they share the plan's workspace."""
 
     def __init__(self, heads, dim, kv_heads=0, dtype="fp16", page_size=64, max_batch=64, max_tokens=8192, causal=True, softmax_scale=0.0,
-                 window=0, sinks=0, partials=False, workspace=None, keep_present=False):
+                 window=0, sinks=0, partials=False, workspace=None, keep_present=False, softcap=0.0, slopes=None):
         self.lib = _lib.load()
         self.heads, self.dim, self.kv_heads, self.page_size = int(heads), int(dim), int(kv_heads) or int(heads), int(page_size)
         self.max_batch, self.max_tokens = int(max_batch), int(max_tokens)
@@ -75,6 +76,13 @@ class PagedAttention:
         self.params = RingattnPagedParams(self.dim, self.heads, int(kv_heads), code, float(softmax_scale), self.page_size, self.max_batch,
                                           self.max_tokens, int(bool(causal)), int(window), int(sinks),
                                           (FLAG_PAGED_PARTIALS if partials else 0) | (FLAG_PAGED_KEEP_PRESENT if keep_present else 0))
+        self.softcap, self.slopes = float(softcap), slopes
+        if not (0 <= self.softcap < float("inf")):
+            raise ValueError("softcap must be 0 or a positive number")
+        if slopes is not None:
+            if not causal:
+                raise ValueError("slopes are for causal plans")
+            _check_tensors((slopes, "slopes", torch.float32, (self.heads,)))
         self.handle = ctypes.c_void_p()
         self.device = torch.cuda.current_device() if workspace is None and torch.cuda.is_available() else None
         ws_ptr, ws_bytes = (None, 0) if workspace is None else (ctypes.c_void_p(int(workspace[0])), int(workspace[1]))
@@ -144,6 +152,16 @@ class PagedAttention:
                 raise ValueError("the tensors of a call must be on one device")
         if self.device is not None and first.device.index != self.device:
             raise ValueError(f"the plan's workspace is on device {self.device}")
+
+    def _scoring(self, prefix_lens, first_keys, batch, tokens):
+        """What a call does with its scores as struct ringattn_paged_scoring."""
+        if (prefix_lens is not None or first_keys is not None) and not self.params.causal:
+            raise ValueError("prefixes and first keys are for causal plans")
+        if prefix_lens is not None:
+            _check_tensors((prefix_lens, "prefix_lens", torch.int32, (batch,)))
+        if first_keys is not None:
+            _check_tensors((first_keys, "first_keys", torch.int32, (tokens,)))
+        return RingattnPagedScoring(self.softcap, *(t.data_ptr() if t is not None else None for t in (self.slopes, prefix_lens, first_keys)))
 
     def _tokens(self, t, name, heads):
         if t.dim() != 3:
@@ -221,9 +239,13 @@ class PagedAttention:
                    v.data_ptr(), shape[0], *_strides(k), scores.data_ptr() if scores is not None else None)
         return q_out
 
-    def forward(self, q, k_cache, v_cache, page_table, kv_lens, q_starts, out=None, lse=None, stream=None):
-        """Attention of the new tokens q [tokens, heads, dim] over the cache (their own rows are in it).  Returns (out, lse)."""
-        if out is not None and lse is not None and self._call_type:
+    def forward(self, q, k_cache, v_cache, page_table, kv_lens, q_starts, out=None, lse=None, stream=None, prefix_lens=None, first_keys=None):
+        """Attention of the new tokens q [tokens, heads, dim] over the cache (their own rows are in it).  Returns (out, lse).
+
+        `prefix_lens`, int32 [batch]: all new tokens of a sequence see so many first tokens, also those that come behind them.  `first_keys`, int32
+        [tokens]: a token sees no key in front of this place (the first token of its document), but for the prefix and the sinks."""
+        plain = prefix_lens is None and first_keys is None and self.slopes is None and not self.softcap
+        if plain and out is not None and lse is not None and self._call_type:
             rc = (self._native.get(1) or self._made(1))(q, k_cache, v_cache, page_table, kv_lens, q_starts, out, lse, stream)
             if rc is not None:
                 check(rc, "ringattn_paged_fwd")
@@ -239,17 +261,19 @@ class PagedAttention:
             lse = self._new((self.heads, shape[0]), torch.float32, q.device, stream)
         _check_rows((out, "out", self.out_dtype, shape))
         _check_tensors((lse, "lse", torch.float32, (self.heads, shape[0])))
-        self._same_device(k_cache, q, out, lse)
+        scoring = self._scoring(prefix_lens, first_keys, cache.batch, shape[0])
+        self._same_device(k_cache, q, out, lse, prefix_lens, first_keys, self.slopes)
         if shape[0] == 0 or cache.batch == 0:
             return out, lse
-        self._call("ringattn_paged_fwd", q.device, stream, ctypes.byref(cache), q.data_ptr(), shape[0], *_strides(q), out.data_ptr(), *_strides(out),
+        self._call("ringattn_paged_fwd_scored", q.device, stream, ctypes.byref(cache), ctypes.byref(scoring), q.data_ptr(), shape[0], *_strides(q), out.data_ptr(), *_strides(out),
                    lse.data_ptr())
         return out, lse
 
-    def weights(self, q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream=None):
+    def weights(self, q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream=None, prefix_lens=None, first_keys=None):
         """Adds to scores what forward(q, ...) that returned `lse` gave to every cached token: the sum of its attention weights over the
-        new tokens and the query heads of each KV head.  Returns scores."""
-        if self._call_type:
+        new tokens and the query heads of each KV head.  prefix_lens and first_keys as forward() had them.  Returns scores."""
+        plain = prefix_lens is None and first_keys is None and self.slopes is None and not self.softcap
+        if plain and self._call_type:
             rc = (self._native.get(2) or self._made(2))(q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream)
             if rc is not None:
                 check(rc, "ringattn_paged_weights")
@@ -258,10 +282,11 @@ class PagedAttention:
         cache = self._cache(k_cache, None, page_table, kv_lens, q_starts)
         _check_rows((q, "q", self.torch_dtype, shape))
         _check_tensors((lse, "lse", torch.float32, (self.heads, shape[0])), (scores, "scores", torch.float32, k_cache.shape[:3]))
-        self._same_device(k_cache, q, lse, scores)
+        scoring = self._scoring(prefix_lens, first_keys, cache.batch, shape[0])
+        self._same_device(k_cache, q, lse, scores, prefix_lens, first_keys, self.slopes)
         if shape[0] == 0 or cache.batch == 0:
             return scores
-        self._call("ringattn_paged_weights", q.device, stream, ctypes.byref(cache), q.data_ptr(), shape[0], *_strides(q), lse.data_ptr(),
+        self._call("ringattn_paged_weights_scored", q.device, stream, ctypes.byref(cache), ctypes.byref(scoring), q.data_ptr(), shape[0], *_strides(q), lse.data_ptr(),
                    scores.data_ptr())
         return scores
 

@@ -1,0 +1,40 @@
+"""Scored attention over the paged cache without a GPU: what the C entry points refuse before any HIP call."""
+import ctypes
+
+import numpy as np
+
+from ringattention_amd._lib import RingattnPagedCache, RingattnPagedScoring
+from test_paged import params
+
+OK, E_NULL, E_NPES, E_DIM, E_DTYPE, E_SEQLEN, E_SHAPE, E_WS, E_RANK, E_PLAN, E_HIP, E_ALLOC, E_ALIGN = range(13)
+
+
+def test_scoring_refusals(ralib):
+    memory = np.zeros(160 << 20, dtype=np.uint8)
+    x = memory.ctypes.data + (-memory.ctypes.data % 16)
+    plans = {}
+    for causal in (1, 0):
+        h = ctypes.c_void_p()
+        assert ralib.ringattn_paged_plan_create(ctypes.byref(params(causal=causal)), ctypes.c_void_p(x), (160 << 20) - 16, ctypes.byref(h)) == OK
+        plans[causal] = h
+    cache = RingattnPagedCache(k=x, v=x, page_stride=2 * 16 * 64, head_stride=16 * 64, token_stride=64, pages=8, table_pages=4, table_stride=4, page_table=x,
+                               kv_lens=x, q_starts=x, batch=2)
+
+    def both(causal=1, tokens=0, q=x, plan=None, **scoring):
+        s = RingattnPagedScoring(**dict(dict(softcap=0.0, slopes=None, prefix_lens=None, first_keys=None), **scoring))
+        h = plan or plans[causal]
+        a = ralib.ringattn_paged_fwd_scored(h, ctypes.byref(cache), ctypes.byref(s), q, tokens, 512, 64, x, 512, 64, x, None)
+        b = ralib.ringattn_paged_weights_scored(h, ctypes.byref(cache), ctypes.byref(s), q, tokens, 512, 64, x, x, None)
+        assert a == b, (a, b)
+        return a
+
+    assert both() == OK and both(softcap=30.0, slopes=x, prefix_lens=x, first_keys=x) == OK and both(causal=0, softcap=30.0) == OK
+    for bad in (float("nan"), float("inf"), -1.0, 1e-38, 3e38):
+        assert both(softcap=bad) == E_SHAPE, bad
+    for bad in ("slopes", "prefix_lens", "first_keys"):
+        assert both(causal=0, **{bad: x}) == E_SHAPE and both(**{bad: x + 2}) == E_ALIGN
+    assert both(plan=ctypes.c_void_p(x)) == E_PLAN and both(q=None) == E_NULL and both(tokens=65) == E_SHAPE
+    assert ralib.ringattn_paged_fwd_scored(plans[1], ctypes.byref(cache), None, x, 0, 512, 64, x, 512, 64, x, None) == OK
+    assert ralib.ringattn_paged_weights_scored(plans[1], None, None, x, 0, 512, 64, x, x, None) == E_NULL
+    for h in plans.values():
+        assert ralib.ringattn_paged_plan_destroy(h) == OK
