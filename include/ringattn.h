@@ -423,6 +423,66 @@ int ringattn_paged_evict(ringattn_paged_plan* plan, const ringattn_paged_cache* 
                          int64_t kept_stride, int budget, int keep_first, int keep_last, int* kept, int* kept_lens, void* stream);
 
 /*
+ * ---- Pages of a paged K/V cache -----------------------------------------------------------------
+ * Which rows of a page table own and share which pages of a pool, on the device: no call waits for the host or tells it anything, all may be recorded
+ * into graphs, and whole numbers are taken in the order of rows and pages, so that every run gives the same table.  The calls above take the table
+ * and lengths as they are.  No counterpart in the reference, which has no cache.
+ *
+ * refs[page] counts the entries of the table that name a page; 0: free.  A caller may count entries of his own besides (a prompt that is kept): such
+ * pages are never given out, and never written on.  lens[row]: tokens of the row's sequence; the first ceil(lens / page_size) entries
+ * are its pages, those behind them -1.  Entries outside the pool are pages that are not there, as above: they are not counted, and stay what they are.
+ * Calls on one table are ordered by the caller (a stream does); they share the scratch memory, which holds nothing between calls.
+ */
+typedef struct ringattn_pages {
+  int* refs;              /* [pages], 16-byte aligned */
+  int* page_table;        /* [rows, table_pages], rows of table_stride ints */
+  int* lens;              /* [rows] */
+  int64_t table_stride;
+  int pages, rows, table_pages, page_size;   /* up to 4096 rows; page_size as in ringattn_paged_params */
+  void* scratch;          /* device memory of the caller's */
+  size_t scratch_bytes;   /* at least ringattn_pages_scratch_bytes(pages, rows, table_pages) */
+} ringattn_pages;
+
+/* The pool that the pages are of: rows of dim 16-bit values, strides in elements as in ringattn_paged_cache.  scores: [pages, kv_heads, page_size]
+ * (ringattn_paged_weights), or NULL. */
+typedef struct ringattn_paged_pool {
+  void* k;
+  void* v;
+  float* scores;
+  int64_t page_stride, head_stride, token_stride;
+  int kv_heads, dim;
+} ringattn_paged_pool;
+
+/* 0 if the sizes are invalid. */
+size_t ringattn_pages_scratch_bytes(int pages, int rows, int table_pages);
+
+/*
+ * A step of a serving loop: all rows at once, from what they are before the call.
+ *   parents : [rows], NULL: every row its own.  Row b begins with the tokens of row parents[b] as they are before the call, whose pages it shares (beams,
+ *             samples of one prompt); outside [0, rows): with none, so that its pages are free for others where nothing else names them
+ *   add     : [rows], NULL: 0.  Tokens more, for which pages are made ready (ringattn_paged_append writes them); negative: fewer, to none
+ *   missing : [rows], may be NULL: 1 where a row was to grow and did not, else 0
+ * Rows that grow take free pages, lowest first, in the order of the rows as long as there are enough; behind a row that finds too few none
+ * grows.  A row that would grow past its entries of the table does not, and takes none.  A row that does not grow has what it began with.  Where a row grows from within a page that something
+ * else names too, the page is copied (K, V, scores) and the copy is the row's alone.
+ */
+int ringattn_pages_update(const ringattn_pages* pages, const ringattn_paged_pool* pool, const int* parents, const int* add, int* missing, void* stream);
+
+/*
+ * Of the n pages with a count, those at places from n on move (K, V, scores, counts) to the free ones in front of it, the i-th to the i-th, and the table's
+ * entries go with them: pages [n, pages) are free afterwards.  used: [1], n.  moved: [pages], may be NULL: the place that the page of a
+ * place has now, -1 for free ones (for entries that the caller counts besides).
+ */
+int ringattn_pages_compact(const ringattn_pages* pages, const ringattn_paged_pool* pool, int* used, int* moved, void* stream);
+
+/*
+ * K, V and scores of pages from one pool to another of as many heads, or within one: pairs [n, 2] on the device, from which page to which.  A page that is written
+ * to is in no other pair.  Pairs outside the pools are left out.
+ */
+int ringattn_pages_copy(const ringattn_paged_pool* from, int from_pages, const ringattn_paged_pool* to, int to_pages, int page_size, const int* pairs, int n,
+                        void* stream);
+
+/*
  * ---- Rotary positions -------------------------------------------------------------------------
  * Row x of a token at position p becomes y: of every pair of columns (a, b) among the first rotary_dim,
  *   y_a = factor (x_a cos(p f_i) - x_b sin(p f_i)),   y_b = factor (x_b cos(p f_i) + x_a sin(p f_i)),

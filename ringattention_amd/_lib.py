@@ -61,6 +61,18 @@ class RingattnPagedScoring(ctypes.Structure):
     _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p), ("first_keys", ctypes.c_void_p)]
 
 
+class RingattnPages(ctypes.Structure):
+    """struct ringattn_pages."""
+    _fields_ = [("refs", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("table_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_int) for n in ("pages", "rows", "table_pages", "page_size")] + [("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
+
+
+class RingattnPagedPool(ctypes.Structure):
+    """struct ringattn_paged_pool."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("scores", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("page_stride", "head_stride", "token_stride")] + [("kv_heads", ctypes.c_int), ("dim", ctypes.c_int)]
+
+
 class RingattnRotary(ctypes.Structure):
     """struct ringattn_rotary."""
     _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int), ("factor", ctypes.c_float), ("turns", ctypes.c_void_p)]
@@ -116,6 +128,11 @@ SYMBOLS = {
                                                      ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_paged_evict": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "ringattn_pages_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "ringattn_pages_update": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 4),
+    "ringattn_pages_compact": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 3),
+    "ringattn_pages_copy": (ctypes.c_int, [ctypes.POINTER(RingattnPagedPool), ctypes.c_int, ctypes.POINTER(RingattnPagedPool), ctypes.c_int, ctypes.c_int,
+                                           ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "ringattn_rotary_turns": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),
     "ringattn_rotary_apply": (ctypes.c_int, [ctypes.POINTER(RingattnRotary), ctypes.c_int, ctypes.c_int, ctypes.POINTER(RingattnRows), ctypes.c_int,
                                              ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),

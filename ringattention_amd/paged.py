@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import RingattnPagedCache, RingattnPagedParams, RingattnPagedScoring, check
+from ._lib import RingattnPagedCache, RingattnPagedParams, RingattnPagedPool, RingattnPagedScoring, RingattnPages, check
 from .api import DTYPE_CODE, TORCH_DTYPE, _check_tensors, _stream_ptr
 
 FLAG_PAGED_PARTIALS = 1
@@ -324,3 +324,113 @@ class PagedAttention:
         self._call("ringattn_paged_evict", k_cache.device, stream, ctypes.byref(cache), scores.data_ptr(), kept_table.data_ptr(), kept_table.shape[1],
                    kept_table.shape[1], budget, int(keep_first), int(keep_last), kept.data_ptr(), kept_lens.data_ptr())
         return kept, kept_lens
+
+
+def _pool(k_cache, v_cache, scores, page_size):
+    """The checked pool of a call as struct ringattn_paged_pool."""
+    if k_cache.dim() != 4 or k_cache.dtype not in TORCH_DTYPE.values():
+        raise ValueError("k_cache must be [pages, kv_heads, page_size, dim] of 16-bit floats")
+    if k_cache.shape[2] != page_size:
+        raise ValueError(f"k_cache must have pages of {page_size} tokens")
+    _check_rows((k_cache, "k_cache", k_cache.dtype, k_cache.shape), (v_cache, "v_cache", k_cache.dtype, k_cache.shape))
+    strides = _strides(k_cache)
+    if _strides(v_cache) != strides:
+        raise ValueError("k_cache and v_cache must have the same strides")
+    if scores is not None:
+        _check_tensors((scores, "scores", torch.float32, k_cache.shape[:3]))
+    for t in (v_cache, scores):
+        if t is not None and t.device != k_cache.device:
+            raise ValueError("the tensors of a call must be on one device")
+    return RingattnPagedPool(k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr() if scores is not None else None, *strides, k_cache.shape[1], k_cache.shape[3])
+
+
+def _on(device, stream, fn, *args):
+    """A launch on the tensors' own device, whichever is the current one."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, _stream_ptr(stream))
+    with torch.cuda.device(device):
+        return fn(*args, _stream_ptr(stream))
+
+
+def copy_pages(k_from, v_from, k_to, v_to, pairs, scores_from=None, scores_to=None, stream=None):
+    """K, V (and scores) of pages from one pool to another of as many heads, or within one: pairs int32 [n, 2], from which page to which.  A page that
+    is written to is in no other pair; pairs outside the pools are left out."""
+    page = k_from.shape[2] if k_from.dim() == 4 else 0
+    source, target = _pool(k_from, v_from, scores_from, page), _pool(k_to, v_to, scores_to, page)
+    if k_from.dtype != k_to.dtype or k_from.shape[1:] != k_to.shape[1:]:
+        raise ValueError("the two pools must have pages of the same shape and dtype")
+    if (scores_from is None) != (scores_to is None):
+        raise ValueError("scores of both pools, or of none")
+    if pairs.dim() != 2:
+        raise ValueError("pairs must be [n, 2]")
+    _check_tensors((pairs, "pairs", torch.int32, (pairs.shape[0], 2)))
+    for t in (k_to, pairs):
+        if t.device != k_from.device:
+            raise ValueError("the tensors of a call must be on one device")
+    if pairs.shape[0]:
+        check(_on(k_from.device, stream, _lib.load().ringattn_pages_copy, ctypes.byref(source), k_from.shape[0], ctypes.byref(target), k_to.shape[0], page,
+                  pairs.data_ptr(), pairs.shape[0]), "ringattn_pages_copy")
+
+
+class PagePool:
+    """Which rows of a page table own and share which of `pages` pages, on the device: `page_table` int32 [rows, table_pages], `lens` int32 [rows],
+    `refs` int32 [pages], how many entries of the table name a page (0: free).  They are a PagedAttention call's page_table and kv_lens as
+    they are, or rows of theirs.  A caller may count entries of its own in refs (a prompt that is kept): those pages are not given out, and not written on.
+
+        pool.update(k_cache, v_cache, parents, add)      rows become forks of others, or begin anew, and grow: before a step's append()
+        pool.compact(k_cache, v_cache)                   the pages in use to the front of the pool
+
+    The same calls give the same tables in every run.  Nothing waits for the host; calls may be captured.  One call at a time."""
+
+    def __init__(self, pages, rows, table_pages, page_size=64, device=None):
+        self.lib = _lib.load()
+        self.pages, self.rows, self.table_pages, self.page_size = int(pages), int(rows), int(table_pages), int(page_size)
+        for name, x in (("pages", self.pages), ("rows", self.rows), ("table_pages", self.table_pages)):
+            if not 0 < x < 2 ** 31:
+                raise ValueError(f"{name} must be positive and fit 32 bits")
+        if self.page_size not in (16, 32, 64, 128, 256, 512, 1024) or self.table_pages * self.page_size > 2 ** 30:
+            raise ValueError("page_size must be 16, 32, ... 1024, and a row of the table have room for 2^30 tokens at most")
+        bytes_ = self.lib.ringattn_pages_scratch_bytes(self.pages, self.rows, self.table_pages)
+        if bytes_ == 0:
+            raise ValueError("up to 4096 rows, and 2^30 entries of the table")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        ints = dict(dtype=torch.int32, device=device)
+        self.refs, self.lens = torch.zeros(self.pages, **ints), torch.zeros(self.rows, **ints)
+        self.page_table = torch.full((self.rows, self.table_pages), -1, **ints)
+        self._scratch = torch.empty(bytes_, dtype=torch.uint8, device=device)
+        self._struct = RingattnPages(self.refs.data_ptr(), self.page_table.data_ptr(), self.lens.data_ptr(), self.table_pages, self.pages, self.rows,
+                                     self.table_pages, self.page_size, self._scratch.data_ptr(), bytes_)
+
+    def _checked(self, k_cache, v_cache, scores, *ints):
+        pool = _pool(k_cache, v_cache, scores, self.page_size)
+        if k_cache.shape[0] != self.pages:
+            raise ValueError(f"k_cache must have {self.pages} pages")
+        for t, name, n in ints:
+            if t is not None:
+                _check_tensors((t, name, torch.int32, (n,)))
+        for t in (k_cache,) + tuple(t for t, _, _ in ints):
+            if t is not None and t.device != self.refs.device:
+                raise ValueError(f"the tensors of a call must be on {self.refs.device}, where the table is")
+        return pool
+
+    def update(self, k_cache, v_cache, parents=None, add=None, scores=None, short=None, stream=None):
+        """All rows at once, from what they are before the call: row b begins with the tokens of row parents[b] (int32 [rows]; outside of [0, rows): with
+        none), sharing their pages, and has add[b] more (int32 [rows]; negative: fewer).  Rows that grow take free pages, lowest first, in the order of
+        the rows while there are enough; a page that is written on from within and that others name too is copied (K, V and `scores`).
+        Returns short, int32 [rows]: 1 where a row was to grow and did not -- it then has what it began with."""
+        pool = self._checked(k_cache, v_cache, scores, (parents, "parents", self.rows), (add, "add", self.rows), (short, "short", self.rows))
+        if short is None:
+            short = PagedAttention._new((self.rows,), torch.int32, self.refs.device, stream)
+        check(_on(self.refs.device, stream, self.lib.ringattn_pages_update, ctypes.byref(self._struct), ctypes.byref(pool),
+                  parents.data_ptr() if parents is not None else None, add.data_ptr() if add is not None else None, short.data_ptr()), "ringattn_pages_update")
+        return short
+
+    def compact(self, k_cache, v_cache, scores=None, used=None, moved=None, stream=None):
+        """The n pages that something names to the first n places of the pool, their counts and the table with them; the others are free.  `moved`,
+        int32 [pages]: where the page of a place is now, -1 for free ones.  Returns used, int32 [1]: n."""
+        pool = self._checked(k_cache, v_cache, scores, (used, "used", 1), (moved, "moved", self.pages))
+        if used is None:
+            used = PagedAttention._new((1,), torch.int32, self.refs.device, stream)
+        check(_on(self.refs.device, stream, self.lib.ringattn_pages_compact, ctypes.byref(self._struct), ctypes.byref(pool), used.data_ptr(),
+                  moved.data_ptr() if moved is not None else None), "ringattn_pages_compact")
+        return used
