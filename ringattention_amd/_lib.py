@@ -163,7 +163,9 @@ def load():
         fn.argtypes = argtypes
     # where the entry points lie that ringattn_calls calls
     lib.addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-        "ringattn_fwd", "ringattn_rank_step_fwd", "ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict")}
+        "ringattn_fwd", "ringattn_rank_step_fwd", "ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict",
+        "ringattn_paged_fwd_scored", "ringattn_paged_weights_scored", "ringattn_paged_append_rotary", "ringattn_rotary_apply", "ringattn_pages_update",
+        "ringattn_pages_compact")}
     _lib = lib
     return lib
 

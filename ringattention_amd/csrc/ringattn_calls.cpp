@@ -5,7 +5,8 @@
 // 0.2 (4.4).  A Call holds one entry point of the C ABI with its plan and the shapes and types it expects.  Called with five tensors and a stream it
 // returns the entry point's code, or None, without having done anything, where the arguments are not plainly what it
 // expects: the caller then goes the general way, which says what is wrong, or serves what is merely unusual (tensor subclasses).
-// Only addresses of this call's tensors are handed on; nothing of a tensor is kept.  A Paged is the same for the paged cache's calls.
+// Only addresses of this call's tensors are handed on; nothing of a tensor is kept.  A Paged is the same for the paged cache's calls, a Turn for rotary positions, a
+// Pages for the bookkeeping of a cache's pages.
 #include <Python.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -128,29 +129,40 @@ struct Paged {
   vectorcallfunc vectorcall;
   void* entry;
   void* plan;
-  int kind;  // 0 append, 1 forward, 2 weights, 3 evict
+  int kind;  // 0 append, 1 forward, 2 weights, 3 evict; 4, 5: 1 and 2 with scores that are shaped; 6: 0 with rotary positions
   int heads, kv_heads, dim, page, max_batch, device;
   long max_tokens;
   at::ScalarType type, out_type;
+  float softcap;
 };
 
-// A tensor on the plan's device, or nothing.
-const at::Tensor* tensor_of(PyObject* o, const Paged& p, at::ScalarType type, int64_t dims) {
+// A tensor on a device, or nothing.
+const at::Tensor* tensor_on(PyObject* o, int device, at::ScalarType type, int64_t dims) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.device().index() != p.device || t.scalar_type() != type || t.dim() != dims) return nullptr;
+  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.device().index() != device || t.scalar_type() != type || t.dim() != dims) return nullptr;
   return &t;
 }
+const at::Tensor* tensor_of(PyObject* o, const Paged& p, at::ScalarType type, int64_t dims) { return tensor_on(o, p.device, type, dims); }
 // Whole, of these sizes.
 bool whole(const at::Tensor& t, std::initializer_list<int64_t> sizes) {
   return t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size()) && t.is_contiguous();
 }
+// None, or a whole tensor of n entries: whether it is one of the two, and its address.
+bool whole_or_none(PyObject* o, int device, at::ScalarType type, int64_t n, void** at) {
+  *at = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = tensor_on(o, device, type, 1);
+  if (!t || !whole(*t, {n})) return false;
+  *at = t->data_ptr();
+  return true;
+}
 // Rows of p.dim that begin at multiples of 16 bytes; the strides of the other dimensions, those of length one as if it were contiguous.
-bool rows_of(const at::Tensor& t, const Paged& p, int64_t* strides) {
+bool rows_of(const at::Tensor& t, int dim, int64_t* strides) {
   const int dims = (int)t.dim();
   const int64_t unit = 16 / (int64_t)t.element_size();
-  if (t.size(dims - 1) != p.dim || t.stride(dims - 1) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
-  int64_t step = p.dim;
+  if (t.size(dims - 1) != dim || t.stride(dims - 1) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
+  int64_t step = dim;
   for (int i = dims - 2; i >= 0; --i) {
     const int64_t n = t.size(i), s = n > 1 ? t.stride(i) : step;
     if (n < 1 || s < 0 || s % unit) return false;
@@ -159,21 +171,34 @@ bool rows_of(const at::Tensor& t, const Paged& p, int64_t* strides) {
   }
   return true;
 }
+bool rows_of(const at::Tensor& t, const Paged& p, int64_t* strides) { return rows_of(t, p.dim, strides); }
+// The stream that a call is to go to; false with a Python error set.
+bool stream_of(PyObject* given, hipStream_t* stream) {
+  if (given == Py_None) return true;
+  PyObject* handle = PyObject_GetAttrString(given, "cuda_stream");
+  if (!handle) return false;
+  *stream = static_cast<hipStream_t>(PyLong_AsVoidPtr(handle));
+  Py_DECREF(handle);
+  return !PyErr_Occurred();
+}
 
 PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyObject* kwnames) {
   Paged& p = *reinterpret_cast<Paged*>(self_);
-  static constexpr Py_ssize_t kArgs[4] = {9, 9, 8, 12};
+  static constexpr Py_ssize_t kArgs[7] = {9, 9, 8, 12, 12, 11, 14};
   if (PyVectorcall_NARGS(nargsf) != kArgs[p.kind] || kwnames) {
     PyErr_SetString(PyExc_TypeError, "the tensors of the call and a stream (or None)");
     return nullptr;
   }
   PyObject* stream_arg = args[kArgs[p.kind] - 1];
   // where the sequences' tensors are among the arguments
-  static constexpr int kCache[4] = {2, 1, 2, 0}, kTable[4] = {4, 3, 3, 3};
+  static constexpr int kCache[7] = {2, 1, 2, 0, 1, 2, 3}, kTable[7] = {4, 3, 3, 3, 3, 3, 5};
   ringattn_paged_cache c{};
   hipStream_t stream = nullptr;
+  const bool forward = p.kind == 1 || p.kind == 4, weights = p.kind == 2 || p.kind == 5;
   void* x[6] = {};
-  int64_t a[2] = {}, b[2] = {};
+  void* masks[3] = {};  // slopes, prefix lengths, first keys
+  const ringattn_rotary* rotary = nullptr;
+  int64_t a[2] = {}, b[2] = {}, kv[2] = {};
   int tokens = 0, budget = 0, first = 0, last = 0, kept_pages = 0;
   try {
     const at::Tensor* k = tensor_of(args[kCache[p.kind]], p, p.type, 4);
@@ -185,7 +210,7 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
     if (batch < 1 || batch > p.max_batch || table->size(1) < 1 || table->size(1) > INT32_MAX || !whole(*lens, {batch})) Py_RETURN_NONE;
     if ((table->size(1) > 1 && table->stride(1) != 1) || (batch > 1 && table->stride(0) < table->size(1))) Py_RETURN_NONE;
     c.k = k->data_ptr();
-    if (p.kind != 2) {
+    if (!weights) {
       const at::Tensor* v = tensor_of(args[kCache[p.kind] + 1], p, p.type, 4);
       if (!v || v->sizes() != k->sizes() || !rows_of(*v, p, v_strides)) Py_RETURN_NONE;
       for (int i = 0; i < 3; ++i)
@@ -218,7 +243,25 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
           if (!scores || !whole(*scores, {pages, p.kv_heads, p.page})) Py_RETURN_NONE;
           x[2] = scores->data_ptr();
         }
-      } else if (p.kind == 1) {
+      } else if (p.kind == 6) {
+        const at::Tensor* k_new = tensor_of(args[1], p, p.type, 3);
+        const at::Tensor* v_new = tensor_of(args[2], p, p.type, 3);
+        const at::Tensor* out = tensor_of(args[10], p, p.type, 3);
+        int64_t of_v[2];
+        if (!k_new || !v_new || k_new->size(0) != tokens || k_new->size(1) != p.kv_heads || k_new->sizes() != v_new->sizes() || !rows_of(*k_new, p, kv) ||
+            !rows_of(*v_new, p, of_v) || kv[0] != of_v[0] || kv[1] != of_v[1] || !out || out->sizes() != rows->sizes() || !rows_of(*out, p, b))
+          Py_RETURN_NONE;
+        x[1] = k_new->data_ptr();
+        x[2] = v_new->data_ptr();
+        x[3] = out->data_ptr();
+        if (args[8] != Py_None) {
+          const at::Tensor* scores = tensor_of(args[8], p, at::kFloat, 3);
+          if (!scores || !whole(*scores, {pages, p.kv_heads, p.page})) Py_RETURN_NONE;
+          x[4] = scores->data_ptr();
+        }
+        if (!whole_or_none(args[9], p.device, at::kInt, tokens, &x[5]) || !PyLong_CheckExact(args[11]) || !tensor_of(args[12], p, at::kLong, 1)) Py_RETURN_NONE;
+        rotary = static_cast<const ringattn_rotary*>(PyLong_AsVoidPtr(args[11]));
+      } else if (forward) {
         const at::Tensor* out = tensor_of(args[6], p, p.out_type, 3);
         const at::Tensor* lse = tensor_of(args[7], p, at::kFloat, 2);
         if (!out || out->sizes() != rows->sizes() || !rows_of(*out, p, b) || !lse || !whole(*lse, {p.heads, tokens})) Py_RETURN_NONE;
@@ -230,6 +273,12 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
         if (!lse || !whole(*lse, {p.heads, tokens}) || !scores || !whole(*scores, {pages, p.kv_heads, p.page})) Py_RETURN_NONE;
         x[1] = lse->data_ptr();
         x[2] = scores->data_ptr();
+      }
+      if (p.kind == 4 || p.kind == 5) {
+        PyObject* const* m = args + kArgs[p.kind] - 4;
+        if (!whole_or_none(m[0], p.device, at::kFloat, p.heads, &masks[0]) || !whole_or_none(m[1], p.device, at::kInt, batch, &masks[1]) ||
+            !whole_or_none(m[2], p.device, at::kInt, tokens, &masks[2]))
+          Py_RETURN_NONE;
       }
     } else {
       const at::Tensor* scores = tensor_of(args[2], p, at::kFloat, 3);
@@ -259,13 +308,7 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
   } catch (...) {  // a tensor without storage, or whose sizes are symbols
     Py_RETURN_NONE;
   }
-  if (stream_arg != Py_None) {
-    PyObject* handle = PyObject_GetAttrString(stream_arg, "cuda_stream");
-    if (!handle) return nullptr;
-    stream = static_cast<hipStream_t>(PyLong_AsVoidPtr(handle));
-    Py_DECREF(handle);
-    if (PyErr_Occurred()) return nullptr;
-  }
+  if (!stream_of(stream_arg, &stream)) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
   auto* plan = static_cast<ringattn_paged_plan*>(p.plan);
@@ -275,6 +318,15 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
     rc = reinterpret_cast<decltype(&ringattn_paged_fwd)>(p.entry)(plan, &c, x[0], tokens, a[0], a[1], x[1], b[0], b[1], (float*)x[2], stream);
   else if (p.kind == 2)
     rc = reinterpret_cast<decltype(&ringattn_paged_weights)>(p.entry)(plan, &c, x[0], tokens, a[0], a[1], (const float*)x[1], (float*)x[2], stream);
+  else if (p.kind == 4 || p.kind == 5) {
+    const ringattn_paged_scoring scoring{p.softcap, (const float*)masks[0], (const int*)masks[1], (const int*)masks[2]};
+    if (p.kind == 4)
+      rc = reinterpret_cast<decltype(&ringattn_paged_fwd_scored)>(p.entry)(plan, &c, &scoring, x[0], tokens, a[0], a[1], x[1], b[0], b[1], (float*)x[2], stream);
+    else
+      rc = reinterpret_cast<decltype(&ringattn_paged_weights_scored)>(p.entry)(plan, &c, &scoring, x[0], tokens, a[0], a[1], (const float*)x[1], (float*)x[2], stream);
+  } else if (p.kind == 6)
+    rc = reinterpret_cast<decltype(&ringattn_paged_append_rotary)>(p.entry)(plan, &c, rotary, (const int*)x[5], x[0], a[0], a[1], x[3], b[0], b[1], x[1], x[2],
+                                                                          tokens, kv[0], kv[1], (float*)x[4], stream);
   else
     rc = reinterpret_cast<decltype(&ringattn_paged_evict)>(p.entry)(plan, &c, (float*)x[0], (const int*)x[1], kept_pages, kept_pages, budget, first, last,
                                                                    (int*)x[2], (int*)x[3], stream);
@@ -282,19 +334,20 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
   return PyLong_FromLong(rc);
 }
 
-// Paged(address of the entry point, of the plan, kind, heads, kv_heads, dim, page_size, max_batch, max_tokens, device, dtype, dtype of out)
+// Paged(address of the entry point, of the plan, kind, heads, kv_heads, dim, page_size, max_batch, max_tokens, device, dtype, dtype of out[, softcap])
 PyObject* paged_create(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   unsigned long long entry, plan;
   int kind, heads, kv_heads, dim, page, max_batch, max_tokens, device;
   PyObject *dtype, *out_dtype;
+  float softcap = 0.f;
   if (kwargs && PyDict_Size(kwargs) > 0) {
     PyErr_SetString(PyExc_TypeError, "positional arguments only");
     return nullptr;
   }
-  if (!PyArg_ParseTuple(args, "KKiiiiiiiiOO", &entry, &plan, &kind, &heads, &kv_heads, &dim, &page, &max_batch, &max_tokens, &device, &dtype, &out_dtype))
+  if (!PyArg_ParseTuple(args, "KKiiiiiiiiOO|f", &entry, &plan, &kind, &heads, &kv_heads, &dim, &page, &max_batch, &max_tokens, &device, &dtype, &out_dtype, &softcap))
     return nullptr;
-  if (!entry || kind < 0 || kind > 3 || !THPDtype_Check(dtype) || !THPDtype_Check(out_dtype)) {
-    PyErr_SetString(PyExc_ValueError, "an entry point, which of the four it is, and two torch.dtypes");
+  if (!entry || kind < 0 || kind > 6 || !THPDtype_Check(dtype) || !THPDtype_Check(out_dtype)) {
+    PyErr_SetString(PyExc_ValueError, "an entry point, which of the seven it is, and two torch.dtypes");
     return nullptr;
   }
   Paged* self = reinterpret_cast<Paged*>(type->tp_alloc(type, 0));
@@ -312,46 +365,214 @@ PyObject* paged_create(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   self->device = device;
   self->type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
   self->out_type = reinterpret_cast<THPDtype*>(out_dtype)->scalar_type;
+  self->softcap = softcap;
   return reinterpret_cast<PyObject*>(self);
 }
 
-void paged_destroy(PyObject* self) { Py_TYPE(self)->tp_free(self); }
+void plain_destroy(PyObject* self) { Py_TYPE(self)->tp_free(self); }
+
+// ---- rotary positions (rotary.py): Turn(q, k or None, positions or None, q_out, k_out or None, inverse, stream or None)
+struct Turn {
+  PyObject_HEAD
+  vectorcallfunc vectorcall;
+  void* entry;
+  const ringattn_rotary* params[2];  // forth and back: the caller keeps them
+  int dim, dtype, device;
+  at::ScalarType type;
+};
+
+PyObject* turn_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyObject* kwnames) {
+  const Turn& p = *reinterpret_cast<Turn*>(self_);
+  if (PyVectorcall_NARGS(nargsf) != 7 || kwnames) {
+    PyErr_SetString(PyExc_TypeError, "the tensors of the call, whether back, and a stream (or None)");
+    return nullptr;
+  }
+  ringattn_rows rows[2];
+  int count = 0;
+  int64_t batch = 0, tokens = 0, position_stride = 0;
+  void* positions = nullptr;
+  hipStream_t stream = nullptr;
+  try {
+    const int dims = THPVariable_CheckExact(args[0]) ? (int)THPVariable_Unpack(args[0]).dim() : 0;
+    if (dims != 3 && dims != 4) Py_RETURN_NONE;
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && args[1] == Py_None) {
+        if (args[4] != Py_None) Py_RETURN_NONE;
+        break;
+      }
+      const at::Tensor* in = tensor_on(args[i], p.device, p.type, dims);
+      const at::Tensor* out = tensor_on(args[3 + i], p.device, p.type, dims);
+      int64_t s[3], o[3];
+      if (!in || !out || in->sizes() != out->sizes() || !rows_of(*in, p.dim, s) || !rows_of(*out, p.dim, o)) Py_RETURN_NONE;
+      const int64_t b = dims == 4 ? in->size(0) : 1, t = in->size(dims == 4 ? 2 : 0), heads = in->size(1);
+      if (b > 65535 || t > 1 << 30 || heads > 65535 || (i == 1 && (b != batch || t != tokens))) Py_RETURN_NONE;
+      batch = b;
+      tokens = t;
+      if (dims == 4) rows[i] = ringattn_rows{in->data_ptr(), out->data_ptr(), (int)heads, s[0], s[1], s[2], o[0], o[1], o[2]};
+      else rows[i] = ringattn_rows{in->data_ptr(), out->data_ptr(), (int)heads, 0, s[1], s[0], 0, o[1], o[0]};
+      ++count;
+    }
+    if (args[2] != Py_None) {
+      if (dims == 4 && THPVariable_CheckExact(args[2]) && THPVariable_Unpack(args[2]).dim() == 2) {
+        const at::Tensor* x = tensor_on(args[2], p.device, at::kInt, 2);
+        if (!x || !whole(*x, {batch, tokens})) Py_RETURN_NONE;
+        positions = x->data_ptr();
+        position_stride = tokens;
+      } else if (!whole_or_none(args[2], p.device, at::kInt, tokens, &positions)) Py_RETURN_NONE;
+    }
+    const auto current = c10::hip::getCurrentHIPStream();
+    if (current.device_index() != p.device) Py_RETURN_NONE;
+    stream = current.stream();
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  const int back = PyObject_IsTrue(args[5]);
+  if (back < 0 || !stream_of(args[6], &stream)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = reinterpret_cast<decltype(&ringattn_rotary_apply)>(p.entry)(p.params[back], p.dim, p.dtype, rows, count, (int)batch, (int)tokens, (const int*)positions,
+                                                                 position_stride, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// Turn(address of the entry point, of the parameters forth, back, dim, RINGATTN_DTYPE_*, device, dtype)
+PyObject* turn_create(PyTypeObject* type, PyObject* args, PyObject*) {
+  unsigned long long entry, forth, back;
+  int dim, code, device;
+  PyObject* dtype;
+  if (!PyArg_ParseTuple(args, "KKKiiiO", &entry, &forth, &back, &dim, &code, &device, &dtype)) return nullptr;
+  if (!entry || !forth || !back || !THPDtype_Check(dtype)) {
+    PyErr_SetString(PyExc_ValueError, "an entry point, its parameters, and a torch.dtype");
+    return nullptr;
+  }
+  Turn* self = reinterpret_cast<Turn*>(type->tp_alloc(type, 0));
+  if (!self) return nullptr;
+  self->vectorcall = turn_call;
+  self->entry = reinterpret_cast<void*>(static_cast<uintptr_t>(entry));
+  self->params[0] = reinterpret_cast<const ringattn_rotary*>(static_cast<uintptr_t>(forth));
+  self->params[1] = reinterpret_cast<const ringattn_rotary*>(static_cast<uintptr_t>(back));
+  self->dim = dim;
+  self->dtype = code;
+  self->device = device;
+  self->type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+  return reinterpret_cast<PyObject*>(self);
+}
+
+// ---- pages (paged.PagePool): Pages(k, v, scores or None, parents or None, add or None, short, stream or None), or with kind 1
+// Pages(k, v, scores or None, moved or None, None, used, stream or None)
+struct Pages {
+  PyObject_HEAD
+  vectorcallfunc vectorcall;
+  void* entry;
+  const ringattn_pages* pages;  // the caller keeps it
+  int kind, device;
+};
+
+PyObject* pages_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyObject* kwnames) {
+  const Pages& p = *reinterpret_cast<Pages*>(self_);
+  if (PyVectorcall_NARGS(nargsf) != 7 || kwnames) {
+    PyErr_SetString(PyExc_TypeError, "the tensors of the call and a stream (or None)");
+    return nullptr;
+  }
+  ringattn_paged_pool pool{};
+  void* x[3] = {};
+  hipStream_t stream = nullptr;
+  try {
+    if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+    const at::ScalarType type = THPVariable_Unpack(args[0]).scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16) Py_RETURN_NONE;
+    const at::Tensor* k = tensor_on(args[0], p.device, type, 4);
+    const at::Tensor* v = tensor_on(args[1], p.device, type, 4);
+    int64_t s[3], of_v[3];
+    if (!k || !v || k->sizes() != v->sizes() || k->size(0) != p.pages->pages || k->size(2) != p.pages->page_size || k->size(1) > 65535 || k->size(3) > 128 ||
+        !rows_of(*k, (int)k->size(3), s) || !rows_of(*v, (int)k->size(3), of_v) || s[0] != of_v[0] || s[1] != of_v[1] || s[2] != of_v[2])
+      Py_RETURN_NONE;
+    pool = ringattn_paged_pool{k->data_ptr(), v->data_ptr(), nullptr, s[0], s[1], s[2], (int)k->size(1), (int)k->size(3)};
+    if (args[2] != Py_None) {
+      const at::Tensor* scores = tensor_on(args[2], p.device, at::kFloat, 3);
+      if (!scores || !whole(*scores, {k->size(0), k->size(1), k->size(2)})) Py_RETURN_NONE;
+      pool.scores = scores->data_ptr<float>();
+    }
+    const int64_t rows = p.pages->rows, n[2][3] = {{rows, rows, rows}, {p.pages->pages, 0, 1}};
+    for (int i = 0; i < 3; ++i)
+      if (!whole_or_none(args[3 + i], p.device, at::kInt, n[p.kind][i], &x[i])) Py_RETURN_NONE;
+    if (!x[2]) Py_RETURN_NONE;
+    const auto current = c10::hip::getCurrentHIPStream();
+    if (current.device_index() != p.device) Py_RETURN_NONE;
+    stream = current.stream();
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  if (!stream_of(args[6], &stream)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  if (p.kind == 0)
+    rc = reinterpret_cast<decltype(&ringattn_pages_update)>(p.entry)(p.pages, &pool, (const int*)x[0], (const int*)x[1], (int*)x[2], stream);
+  else
+    rc = reinterpret_cast<decltype(&ringattn_pages_compact)>(p.entry)(p.pages, &pool, (int*)x[2], (int*)x[0], stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// Pages(address of the entry point, of the ringattn_pages, 0: update or 1: compact, device)
+PyObject* pages_create(PyTypeObject* type, PyObject* args, PyObject*) {
+  unsigned long long entry, pages;
+  int kind, device;
+  if (!PyArg_ParseTuple(args, "KKii", &entry, &pages, &kind, &device)) return nullptr;
+  if (!entry || !pages || kind < 0 || kind > 1) {
+    PyErr_SetString(PyExc_ValueError, "an entry point, which of the two it is, and its pages");
+    return nullptr;
+  }
+  Pages* self = reinterpret_cast<Pages*>(type->tp_alloc(type, 0));
+  if (!self) return nullptr;
+  self->vectorcall = pages_call;
+  self->entry = reinterpret_cast<void*>(static_cast<uintptr_t>(entry));
+  self->pages = reinterpret_cast<const ringattn_pages*>(static_cast<uintptr_t>(pages));
+  self->kind = kind;
+  self->device = device;
+  return reinterpret_cast<PyObject*>(self);
+}
 
 PyTypeObject call_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 PyTypeObject paged_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+PyTypeObject turn_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+PyTypeObject pages_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ringattn_calls", "checks and launch of a call", -1};
 
 }  // namespace
 
 PyMODINIT_FUNC PyInit_ringattn_calls() {
-  call_type.tp_name = "ringattn_calls.Call";
-  call_type.tp_basicsize = sizeof(Call);
-  call_type.tp_dealloc = destroy;
-  call_type.tp_vectorcall_offset = offsetof(Call, vectorcall);
-  call_type.tp_call = PyVectorcall_Call;
-  call_type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL;
-  call_type.tp_new = create;
-  paged_type.tp_name = "ringattn_calls.Paged";
-  paged_type.tp_basicsize = sizeof(Paged);
-  paged_type.tp_dealloc = paged_destroy;
-  paged_type.tp_vectorcall_offset = offsetof(Paged, vectorcall);
-  paged_type.tp_call = PyVectorcall_Call;
-  paged_type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL;
-  paged_type.tp_new = paged_create;
-  if (PyType_Ready(&call_type) < 0 || PyType_Ready(&paged_type) < 0) return nullptr;
-  PyObject* m = PyModule_Create(&module);
-  if (!m) return nullptr;
-  Py_INCREF(&paged_type);
-  if (PyModule_AddObject(m, "Paged", reinterpret_cast<PyObject*>(&paged_type)) < 0) {
-    Py_DECREF(&paged_type);
-    Py_DECREF(m);
-    return nullptr;
+  struct Made {
+    PyTypeObject& type;
+    const char *name, *in_module;
+    Py_ssize_t size, vectorcall;
+    destructor destroy;
+    newfunc create;
+  };
+  const Made made[] = {{call_type, "ringattn_calls.Call", "Call", sizeof(Call), offsetof(Call, vectorcall), destroy, create},
+                       {paged_type, "ringattn_calls.Paged", "Paged", sizeof(Paged), offsetof(Paged, vectorcall), plain_destroy, paged_create},
+                       {turn_type, "ringattn_calls.Turn", "Turn", sizeof(Turn), offsetof(Turn, vectorcall), plain_destroy, turn_create},
+                       {pages_type, "ringattn_calls.Pages", "Pages", sizeof(Pages), offsetof(Pages, vectorcall), plain_destroy, pages_create}};
+  for (const Made& m : made) {
+    m.type.tp_name = m.name;
+    m.type.tp_basicsize = m.size;
+    m.type.tp_dealloc = m.destroy;
+    m.type.tp_vectorcall_offset = m.vectorcall;
+    m.type.tp_call = PyVectorcall_Call;
+    m.type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL;
+    m.type.tp_new = m.create;
+    if (PyType_Ready(&m.type) < 0) return nullptr;
   }
-  Py_INCREF(&call_type);
-  if (PyModule_AddObject(m, "Call", reinterpret_cast<PyObject*>(&call_type)) < 0) {
-    Py_DECREF(&call_type);
-    Py_DECREF(m);
-    return nullptr;
+  PyObject* module_ = PyModule_Create(&module);
+  if (!module_) return nullptr;
+  for (const Made& m : made) {
+    Py_INCREF(&m.type);
+    if (PyModule_AddObject(module_, m.in_module, reinterpret_cast<PyObject*>(&m.type)) < 0) {
+      Py_DECREF(&m.type);
+      Py_DECREF(module_);
+      return nullptr;
+    }
   }
-  return m;
+  return module_;
 }

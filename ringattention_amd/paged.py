@@ -95,9 +95,10 @@ class PagedAttention:
         self._native = {}
 
     def _made(self, kind):
-        entry = self.lib.addresses[("ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict")[kind]]
+        entry = self.lib.addresses[("ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict",
+                                    "ringattn_paged_fwd_scored", "ringattn_paged_weights_scored", "ringattn_paged_append_rotary")[kind]]
         self._native[kind] = call = self._call_type(entry, self.handle.value, kind, self.heads, self.kv_heads, self.dim, self.page_size,
-                                                    self.max_batch, self.max_tokens, self.device, self.torch_dtype, self.out_dtype)
+                                                    self.max_batch, self.max_tokens, self.device, self.torch_dtype, self.out_dtype, self.softcap)
         return call
 
     def close(self):
@@ -216,10 +217,16 @@ class PagedAttention:
     def append_rotary(self, rotary, q, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores=None, positions=None, q_out=None, stream=None):
         """append() with rotary positions on the way (rotary.Rotary): K turned and V as it is into the cache, q [tokens, heads, dim] turned into q_out
         (q itself for in place).  `positions` int32 [tokens]; None: a token's place in its sequence.  Returns q_out."""
+        rotary.check(self.dim, self.torch_dtype)
+        if q_out is not None and self._call_type:
+            rc = (self._native.get(6) or self._made(6))(q, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores, positions, q_out, rotary.address,
+                                                        rotary.turns, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_append_rotary")
+                return q_out
         shape, kv_shape = self._tokens(q, "q", self.heads), self._tokens(k, "k", self.kv_heads)
         if kv_shape[0] != shape[0]:
             raise ValueError("q and k must have as many tokens")
-        rotary.check(self.dim, self.torch_dtype)
         cache = self._cache(k_cache, v_cache, page_table, kv_lens, q_starts)
         _check_rows((q, "q", self.torch_dtype, shape), (k, "k", self.torch_dtype, kv_shape), (v, "v", self.torch_dtype, kv_shape))
         if _strides(k) != _strides(v):
@@ -250,6 +257,11 @@ class PagedAttention:
             if rc is not None:
                 check(rc, "ringattn_paged_fwd")
                 return out, lse
+        elif out is not None and lse is not None and self._call_type and self.params.causal:
+            rc = (self._native.get(4) or self._made(4))(q, k_cache, v_cache, page_table, kv_lens, q_starts, out, lse, self.slopes, prefix_lens, first_keys, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_fwd_scored")
+                return out, lse
         shape = self._tokens(q, "q", self.heads)
         cache = self._cache(k_cache, v_cache, page_table, kv_lens, q_starts)
         _check_rows((q, "q", self.torch_dtype, shape))
@@ -277,6 +289,11 @@ class PagedAttention:
             rc = (self._native.get(2) or self._made(2))(q, lse, k_cache, page_table, kv_lens, q_starts, scores, stream)
             if rc is not None:
                 check(rc, "ringattn_paged_weights")
+                return scores
+        elif self._call_type and self.params.causal:
+            rc = (self._native.get(5) or self._made(5))(q, lse, k_cache, page_table, kv_lens, q_starts, scores, self.slopes, prefix_lens, first_keys, stream)
+            if rc is not None:
+                check(rc, "ringattn_paged_weights_scored")
                 return scores
         shape = self._tokens(q, "q", self.heads)
         cache = self._cache(k_cache, None, page_table, kv_lens, q_starts)
@@ -398,8 +415,13 @@ class PagePool:
         self.refs, self.lens = torch.zeros(self.pages, **ints), torch.zeros(self.rows, **ints)
         self.page_table = torch.full((self.rows, self.table_pages), -1, **ints)
         self._scratch = torch.empty(bytes_, dtype=torch.uint8, device=device)
+        calls = _lib.load_calls()
+        self._native = None
         self._struct = RingattnPages(self.refs.data_ptr(), self.page_table.data_ptr(), self.lens.data_ptr(), self.table_pages, self.pages, self.rows,
                                      self.table_pages, self.page_size, self._scratch.data_ptr(), bytes_)
+        if calls and device.type == "cuda":   # checks and launches in native code, as PagedAttention's
+            self._native = [calls.Pages(self.lib.addresses[name], ctypes.addressof(self._struct), kind, self.refs.device.index)
+                            for kind, name in enumerate(("ringattn_pages_update", "ringattn_pages_compact"))]
 
     def _checked(self, k_cache, v_cache, scores, *ints):
         pool = _pool(k_cache, v_cache, scores, self.page_size)
@@ -418,6 +440,11 @@ class PagePool:
         none), sharing their pages, and has add[b] more (int32 [rows]; negative: fewer).  Rows that grow take free pages, lowest first, in the order of
         the rows while there are enough; a page that is written on from within and that others name too is copied (K, V and `scores`).
         Returns short, int32 [rows]: 1 where a row was to grow and did not -- it then has what it began with."""
+        if short is not None and self._native:
+            rc = self._native[0](k_cache, v_cache, scores, parents, add, short, stream)
+            if rc is not None:
+                check(rc, "ringattn_pages_update")
+                return short
         pool = self._checked(k_cache, v_cache, scores, (parents, "parents", self.rows), (add, "add", self.rows), (short, "short", self.rows))
         if short is None:
             short = PagedAttention._new((self.rows,), torch.int32, self.refs.device, stream)
@@ -428,6 +455,11 @@ class PagePool:
     def compact(self, k_cache, v_cache, scores=None, used=None, moved=None, stream=None):
         """The n pages that something names to the first n places of the pool, their counts and the table with them; the others are free.  `moved`,
         int32 [pages]: where the page of a place is now, -1 for free ones.  Returns used, int32 [1]: n."""
+        if used is not None and self._native:
+            rc = self._native[1](k_cache, v_cache, scores, moved, None, used, stream)
+            if rc is not None:
+                check(rc, "ringattn_pages_compact")
+                return used
         pool = self._checked(k_cache, v_cache, scores, (used, "used", 1), (moved, "moved", self.pages))
         if used is None:
             used = PagedAttention._new((1,), torch.int32, self.refs.device, stream)

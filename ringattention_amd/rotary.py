@@ -98,6 +98,12 @@ class Rotary:
             device = f"cuda:{torch.cuda.current_device()}" if torch.cuda.is_available() else "cpu"
         self.turns = turns.to(device)
         self._params = [RingattnRotary(self.rotary_dim, int(self.interleaved), back, self.scale, self.turns.data_ptr()) for back in (0, 1)]
+        self.address = ctypes.addressof(self._params[0])   # for calls that are made in native code
+        calls = _lib.load_calls()
+        self._native = None
+        if calls and self.turns.is_cuda:
+            self._native = calls.Turn(self.lib.addresses["ringattn_rotary_apply"], self.address, ctypes.addressof(self._params[1]), self.dim, self.dtype_code,
+                                      self.turns.device.index, self.torch_dtype)
 
     def params(self, inverse):
         """struct ringattn_rotary."""
@@ -113,6 +119,11 @@ class Rotary:
         """q, k: [batch, heads, tokens, dim] or both [tokens, heads, dim], of any strides that keep a row together.  `positions`: int32 [tokens] or
         [batch, tokens], of any sign; None: a token's number.  q_out, k_out: the tensor itself for in place.  `inverse`: turned back -- of
         gradients by the outputs the gradients by the inputs.  Returns (q_out, k_out), k_out None without k."""
+        if q_out is not None and (k is None or k_out is not None) and self._native:
+            rc = self._native(q, k, positions, q_out, k_out, inverse, stream)
+            if rc is not None:
+                check(rc, "ringattn_rotary_apply")
+                return q_out, k_out
         given = [(q, "q", q_out)] + ([(k, "k", k_out)] if k is not None else [])
         if k is None and k_out is not None:
             raise ValueError("k_out without k")
