@@ -63,27 +63,46 @@ struct Scoring {
   const int* prefix;      // [batch]
   const int* first;       // [tokens]
 };
-// Scores of a 32 x 32 tile, as the products give them (lane (n, h): row n, keys key0 + 4 h + [0, 4) of every eight), in units of log2: what the
-// exponentials take.  tanh y = 1 - 2 / (e^2y + 1): an exponential and a reciprocal, each off by 2^-23 of itself, so that a capped score is off by
-// some 2^-22 of the cap; an infinite one is the cap.  dist: key0 + 4 h less the row's place in the sequence.
-template <int SC> static __device__ __forceinline__ void shape_scores(f32x16& s, const Scoring& x, float scale_log2, float slope, int dist) {
+// Scores of a 32 x 32 tile, as the products give them (lane (n, h): row n, keys key0 + 4 h + [0, 4) of every eight), to what the exponentials take
+// a multiple of (score_unit), less a constant of all scores (score_base).  tanh y = 1 - 2 / (e^2y + 1): an exponential and a reciprocal, each off by
+// 2^-23 of itself; the softmax takes -1 / (e^2y + 1) as it is, 2 c times that being the capped score less c, so that a cap costs four instructions
+// a score.  An infinite score is the cap.
+// In steps, so that none waits for the one before: each takes one score as far as the next stage (left to itself the compiler has each score's
+// instructions one behind the other).  `at`: slope times dist.  Of a key that lies in front of its row a slope takes slope |dist| = -slope dist, so that
+// what is added is at + slope (0, 1, 2, 3, 8, ...): no absolute values; keys behind their rows, which prefixes show, are put right after (turn_slopes).
+template <int SC> constexpr int kShapeSteps = (SC & kCapped) ? ((SC & kSloped) ? 25 : 22) : (SC & kSloped) ? 16 : 0;
+template <int SC> static __device__ __forceinline__ void shape_step(f32x16& s, int i, const Scoring& x, float unit, float slope, float at) {
+  constexpr int kSlopeAt = (SC & kCapped) ? 9 : 0;
   if constexpr ((SC & kCapped) != 0) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * x.cap_in) + 1.f);
-      s[e] = __builtin_fmaf(r, -2.f * x.cap_out, x.cap_out);
-    }
+    if (i < 16) s[i] *= x.cap_in;
+    if (i >= 2 && i < 18) s[i - 2] = __builtin_amdgcn_exp2f(s[i - 2]);
+    if (i >= 5 && i < 21) s[i - 5] = -1.f - s[i - 5];
+    if (i >= 6 && i < 22) s[i - 6] = __builtin_amdgcn_rcpf(s[i - 6]);
   }
   if constexpr ((SC & kSloped) != 0) {
-    const float d0 = (float)dist;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float far = __builtin_fabsf(d0 + (float)(8 * (e >> 2) + (e & 3)));
-      if constexpr ((SC & kCapped) != 0) s[e] = __builtin_fmaf(far, -slope, s[e]);
-      else s[e] = __builtin_fmaf(s[e], scale_log2, far * -slope);
-    }
+    const int e = i - kSlopeAt;
+    if (e >= 0 && e < 16) s[e] = __builtin_fmaf(s[e], unit, __builtin_fmaf(slope, (float)(8 * (e >> 2) + (e & 3)), at));
   }
 }
+// Scores of keys that lie behind their rows: slope dist has been added where it was to be taken.  per: of a score's own units.
+static __device__ __forceinline__ void turn_slopes(f32x16& s, float slope, int dist, float per) {
+  const float twice = -2.f * slope * per;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf((float)max(dist + 8 * (e >> 2) + (e & 3), 0), twice, s[e]);
+}
+template <int SC> static __device__ __forceinline__ float shape_unit(const Scoring& x, float scale_log2) { return (SC & kCapped) ? 2.f * x.cap_out : scale_log2; }
+// dist: key0 + 4 h less the row's place in the sequence.
+template <int SC> static __device__ __forceinline__ void shape_scores(f32x16& s, const Scoring& x, float scale_log2, float slope, int dist) {
+#pragma unroll
+  for (int i = 0; i < kShapeSteps<SC>; ++i) {
+    shape_step<SC>(s, i, x, shape_unit<SC>(x, scale_log2), slope, slope * (float)dist);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <int SC> static __device__ __forceinline__ float score_unit(const Scoring& x, float scale_log2) {
+  return (SC & kSloped) ? 1.f : shape_unit<SC>(x, scale_log2);
+}
+template <int SC> static __device__ __forceinline__ float score_base(const Scoring& x) { return (SC & kCapped) ? x.cap_out : 0.f; }
 
 struct AttendArgs {
   Cache c;

@@ -111,7 +111,7 @@ template <int DT, int D, int SC> struct WeightRows {
   }
   // log2(e) LSE of a row; +inf, against which every weight is 0, for a row that is not there or saw nothing
   __device__ __forceinline__ float lse_of(int r) const {
-    const float x = *lse_place(r) * 1.4426950408889634f;
+    const float x = *lse_place(r) * 1.4426950408889634f - score_base<SC>(a.x);
     return r >= rows || x == -INFINITY ? INFINITY : x;
   }
   // the new tokens [i0, i1) that see any of the keys [key0, key0 + keys)
@@ -132,6 +132,10 @@ template <int DT, int D, int SC> struct WeightRows {
       lim = r >= rows ? 0 : max(lim, s.prefix);
       if (a.x.first) low = max(low, clamped(a.x.first[s.start + token], 0, s.len) - 1);
     }
+    if ((SC & kSloped) && s.prefix > 0 && key0 + 31 > before) {
+      const int q_head = head * a.group + min(r, rows - 1) - token * a.group;
+      turn_slopes(sacc, a.x.slopes[q_head] * 1.4426950408889634f, key0 + 4 * h - before - token, 1.f / unit());
+    }
     int first = key0 + 4 * h, sinks = SC ? max(a.sinks, s.prefix) : a.sinks;
     asm volatile("" : "+v"(first), "+v"(sinks));  // (nothing of these comparisons is kept from tile to tile: it took 100 registers)
 #pragma unroll
@@ -140,18 +144,33 @@ template <int DT, int D, int SC> struct WeightRows {
       sacc[e] = bool((k >= lim) | ((k <= low) & (k >= sinks))) ? -INFINITY : sacc[e] + none;  // (no branches)
     }
   }
-  // Scores to what attention takes the exponentials of, but for a factor k2.
-  __device__ __forceinline__ float k2() const { return (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2; }
-  __device__ __forceinline__ void shape(f32x16& sacc, int key0, int r) const {
-    if constexpr ((SC & (kCapped | kSloped)) != 0) {
-      int token, q_head;
-      row_of(r, token, q_head);
-      shape_scores<SC>(sacc, a.x, a.scale_log2, (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f, key0 + 4 * h - before - token);
+  // What becomes of scores, as in attention, but that a slope goes into what the exponentials take of each (exponent): `at` is slope times the distance of
+  // key0 + 4 h, less log2(e) LSE.  A cap first, then masks.
+  struct Slope {
+    float slope, at;
+  };
+  __device__ __forceinline__ float unit() const { return shape_unit<SC>(a.x, a.scale_log2); }
+  __device__ __forceinline__ void cap(f32x16& sacc) const {
+    if constexpr ((SC & kCapped) != 0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sacc[e] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(sacc[e] * a.x.cap_in));
     }
   }
-  __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, float lse) const {
+  __device__ __forceinline__ float slope_of_row(int r) const {
+    int token, q_head;
+    row_of(r, token, q_head);
+    return a.x.slopes[q_head] * 1.4426950408889634f;
+  }
+  __device__ __forceinline__ Slope slope_of(int key0, int r, float slope, float z) const {
+    if constexpr ((SC & kSloped) == 0) return Slope{0.f, -z};
+    return Slope{slope, __builtin_fmaf(slope, (float)(key0 + 4 * h - before - quotient(min(r, rows - 1), a.by_group)), -z)};
+  }
+  __device__ __forceinline__ float exponent(float s, int e, const Slope& g) const {
+    return __builtin_fmaf(s, unit(), (SC & kSloped) ? __builtin_fmaf(g.slope, (float)(8 * (e >> 2) + (e & 3)), g.at) : g.at);
+  }
+  __device__ __forceinline__ void weigh(float (&w)[16], const f32x16& sacc, const Slope& g) const {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], k2(), -lse));
+    for (int e = 0; e < 16; ++e) w[e] += __builtin_amdgcn_exp2f(exponent(sacc[e], e, g));
   }
   // Every key of a sequence has one owner, which adds to its score once: no order to go by.  Atomic, since pages may be several sequences'.
   __device__ __forceinline__ void add_score(int page, int key, float x) const {
@@ -186,7 +205,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(q + ks * 32);
   }
-  const float lse_first = x.lse_of(n);
+  const float lse_first = x.lse_of(n), slope_first = (SC & kSloped) ? x.slope_of_row(n) : 0.f;
   unsigned char* my = smem + wave * 2 * TILE;
   const unsigned my_lds = lds_offset(smem) + wave * 2 * TILE;
   int koff[KS], goff[HALF];
@@ -236,9 +255,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
       float z = lse_first;
-      x.shape(sacc, key0, n);
+      x.cap(sacc);
       x.hide(sacc, key0, n, z);
-      x.weigh(w, sacc, z);
+      x.weigh(w, sacc, x.slope_of(key0, n, slope_first, z));
     }
 #pragma unroll 1
     for (int r0 = 32; r0 < x.rows; r0 += 32) {
@@ -249,9 +268,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_weights_few_kernel(co
       for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], *(const s16x8*)(q + ks * 32), sacc);
-      x.shape(sacc, key0, r0 + n);
+      x.cap(sacc);
       x.hide(sacc, key0, r0 + n, z);
-      x.weigh(w, sacc, z);
+      x.weigh(w, sacc, x.slope_of(key0, r0 + n, (SC & kSloped) ? x.slope_of_row(r0 + n) : 0.f, z));
     }
     const float sum = sum_lanes(w);
     const int e = n >> 1;
@@ -307,6 +326,8 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
   // A tile of Q, 1 KB a piece, half of them by each of the two waves.  Where 32 rows are whole tokens (a.q_even) a piece's rows lie at
   // fixed offsets from the tile's first, and so do the rows of their LSEs; elsewhere, and where the last rows are not there, every row's
   // place is worked out.  (Worked out for every tile it cost as much as the exponentials: a prompt of 8 K tokens, 16/4 heads 250 us.)
+  // (Rows of a lane are then of one head, whose slope stays in a register.)
+  const float even_slope = (SC & kSloped) && a.q_even ? x.slope_of_row(n) : 0.f;
   int at_piece[PIECES], lse_at = 0;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j) at_piece[j] = 0;
@@ -393,7 +414,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
         if (ks > 0) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(o) : "n"(32 * ks), "v"(from));
         qfr[ks] = *(const s16x8*)(smem + o);
       }
-      const float raw = *(const float*)(smem + here + LSES + threadIdx.x * 4) * 1.4426950408889634f;
+      const float raw = *(const float*)(smem + here + LSES + threadIdx.x * 4) * 1.4426950408889634f - score_base<SC>(a.x);
       z = raw == -INFINITY ? INFINITY : raw;
       if (t + 2 < t_end) fetch(t + 2, free);
       const int last = free;
@@ -413,7 +434,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
     };
     auto hide = [&](f32x16 (&sacc)[2], int step, float& z) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) x.shape(sacc[c], my_key0 + 32 * c, r_begin + step * STEP + 32 * pair + n);
+      for (int c = 0; c < 2; ++c) x.cap(sacc[c]);
       if ((unsigned)(step - seen_from) >= seen) {
         const float from = z;
 #pragma unroll
@@ -423,28 +444,45 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
         }
       }
     };
-    auto weigh = [&](const f32x16 (&sacc)[2], float z) {
+    using Slope = typename WeightRows<DT, D, SC>::Slope;
+    // of a step that has been through hide()
+    auto weigh = [&](const f32x16 (&sacc)[2], const Slope (&g)[2]) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          w[c][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[c][e], x.k2(), -z));
+          w[c][e] += __builtin_amdgcn_exp2f(x.exponent(sacc[c][e], e, g[c]));
           asm volatile("" : "+v"(w[c][e]));  // (here, not where the sums are used next)
         }
+    };
+    auto slopes = [&](Slope (&g)[2], int step, float z) {
+      const int r = r_begin + step * STEP + 32 * pair + n;
+      float slope = even_slope;
+      if ((SC & kSloped) && !a.q_even) slope = x.slope_of_row(r);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) g[c] = x.slope_of(my_key0 + 32 * c, r, slope, z);
     };
     auto both = [&](f32x16 (&next)[2], float& z_next, f32x16 (&sacc)[2], float z) {
       receive(z_next);
       hide(sacc, t - 1, z);
+      Slope g[2];
+      slopes(g, t - 1, z);
       __builtin_amdgcn_sched_barrier(0);
       multiply(next);
-      weigh(sacc, z);
+      weigh(sacc, g);
 #pragma unroll
       for (int i = 0; i < 2 * KS; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 32 / KS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, ((SC & kSloped) ? 48 : 32) / KS, 0);
         __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
+    };
+    auto last_one = [&](f32x16 (&sacc)[2], int step, float z) {
+      hide(sacc, step, z);
+      Slope g[2];
+      slopes(g, step, z);
+      weigh(sacc, g);
     };
     if (t < t_end) {
       fetch(t, here);
@@ -461,11 +499,9 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void paged_weights_kernel(con
       }
       if (t < t_end) {
         both(odd, z_odd, even, z_even);
-        hide(odd, t, z_odd);
-        weigh(odd, z_odd);
+        last_one(odd, t, z_odd);
       } else {
-        hide(even, t - 1, z_even);
-        weigh(even, z_even);
+        last_one(even, t - 1, z_even);
       }
     }
 #pragma unroll

@@ -285,7 +285,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void few_
     const int lim_all = max(a.causal ? min(p.s.len, before + i0 + 1) : p.s.len, p.s.prefix);
     const int low_any = max(a.window > 0 ? before + i1 - a.window : -1, SC && a.x.first ? firsts_of_lanes(first, first).most - 1 : -1);
     const float slope = (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f;
-    const float k2 = (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2;  // scores to units of log2, where they are not in these already
+    const float k2 = score_unit<SC>(a.x, a.scale_log2);  // scores, as the softmax has them, to units of log2
 
     s16x8 qf[KS];
     {
@@ -431,6 +431,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void few_
         for (int ks = 0; ks < KS; ++ks) sacc = E::mma(kfr[ks], qf[ks], sacc);
       }
       if constexpr (SC != 0) shape_scores<SC>(sacc, a.x, a.scale_log2, slope, cur.key + 4 * h - before - token);
+      if ((SC & kSloped) && p.s.prefix > 0 && cur.key + BN - 1 > before + i0) turn_slopes(sacc, slope, cur.key + 4 * h - before - token, 1.f);
       const bool masked = cur.key + BN > lim_all || (cur.key <= low_any && cur.key + BN > keep) || cur.gone;
       if (masked) {
         asm volatile("");  // (a branch, not sixteen selections in every tile)
@@ -518,13 +519,13 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void few_
     }
 
     if (alone) {
-      store_rows<DT, DB>(a, p.s, head, r0, r_last, oacc, 0, cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3])), ms);
+      store_rows<DT, DB>(a, p.s, head, r0, r_last, oacc, 0, cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3])), ms + score_base<SC>(a.x));
       continue;
     }
     // This wave's state where the workgroup can read it: acc-O as fp32 over its own tiles, 16-byte chunk c of row n at chunk c ^ n.
     {
       const float l = cross_half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
-      if (h == 0) stat[wave][n] = float2{l == 0.f ? -INFINITY : ms, l};  // (0: nothing seen; a NaN stays one)
+      if (h == 0) stat[wave][n] = float2{l == 0.f ? -INFINITY : ms + score_base<SC>(a.x), l};  // (0: nothing seen; a NaN stays one)
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll

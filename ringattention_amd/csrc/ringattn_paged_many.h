@@ -47,7 +47,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   const int first = SC && a.x.first ? clamped(a.x.first[p.s.start + token], 0, p.s.len) : 0;
   const float slope = (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f;
   const int keep = SC ? max(a.sinks, p.s.prefix) : a.sinks;
-  const float k2 = (SC & (kCapped | kSloped)) ? 1.f : a.scale_log2;  // scores to units of log2, where they are not in these already
+  const float k2 = score_unit<SC>(a.x, a.scale_log2);  // scores, as the softmax has them, to units of log2
   // What the masks and other seldom taken paths are worked out from: the compiler would keep all of it in registers through every tile.
   auto fresh = [](int x) {
     asm volatile("" : "+v"(x));
@@ -63,12 +63,26 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
     const int i0 = quotient(min(first, r_last), a.by_group), i1 = quotient(min(last, r_last), a.by_group);
     const int low = max(a.window > 0 ? before + i1 - a.window : -1, most_first - 1);
     Clear x;
-    x.up = __builtin_amdgcn_readfirstlane(tile_of(max(p.s.prefix, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len) / BN));
+    const int clear = max((SC & kSloped) ? 0 : p.s.prefix, a.causal ? min(p.s.len, before + i0 + 1) : p.s.len);  // (slopes look at keys behind their rows)
+    x.up = __builtin_amdgcn_readfirstlane(tile_of(clear / BN));
     x.low = low >= 0 ? __builtin_amdgcn_readfirstlane(tile_of(low / BN + 1)) : 0;
     return x;
   };
   const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31, SC && a.x.first ? firsts_of_lanes(first, first).most : 0), every = clear_of(r0, r_last, firsts.most);
   const int t_up = mine.up, t_low = mine.low;
+  // Of a scored call: tiles that no row of this wave sees -- those of the documents that other rows of the workgroup are of -- are passed over.
+  struct Seen {
+    int from, to;
+  };
+  auto seen_of = [&]() {
+    if constexpr (SC == 0) return Seen{0, 0};
+    const int i0 = quotient(min(r0 + 32 * wave, r_last), a.by_group), i1 = quotient(min(r0 + 32 * wave + 31, r_last), a.by_group);
+    const int low = max(a.window > 0 ? before + i0 + 1 - a.window : 0, a.x.first ? firsts_of_lanes(first, first).least : 0);
+    const int lim = max(p.s.prefix, a.causal ? min(p.s.len, before + i1 + 1) : p.s.len);
+    return Seen{__builtin_amdgcn_readfirstlane(tile_of(low / BN)), __builtin_amdgcn_readfirstlane(tile_of((lim + BN - 1) / BN))};
+  };
+  const Seen seen_tiles = seen_of();
+  auto passed_over = [&](int t) { return SC != 0 && ((t < seen_tiles.from && first_key(t) >= keep) || t >= seen_tiles.to); };
 
   s16x8 qf[KS];
   {
@@ -214,11 +228,14 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   };
   // P = exp2(S k2 - m k2); the sums from the unrounded values, the operands of the next product rounded to the storage type: no more than
   // the output's own rounding
-  // Scored: the scores of tile t are shaped first, and then masked, so that a hidden one is -inf and not minus the cap.
+  // Scored: the scores of tile t have been shaped, and are masked now, so that a hidden one is -inf and not minus the cap.
   auto softmax_phase = [&](int t, bool may_hide) {
     if constexpr (SC != 0) {
-      shape_scores<SC>(sacc, a.x, a.scale_log2, slope, first_key(t) + 4 * h - before - token);
-      if (may_hide) mask_tile(t);
+      if (may_hide) {
+        // (of a prefix, rows may see keys that come behind them)
+        if ((SC & kSloped) && p.s.prefix > 0 && t >= t_up) turn_slopes(sacc, slope, first_key(t) + 4 * h - before - fresh(token), 1.f);
+        mask_tile(t);
+      }
     }
     move_reference();
 #pragma unroll
@@ -232,6 +249,10 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       }
       pf[t2] = __builtin_bit_cast(s16x8, pv);
     }
+  };
+  auto weights_of = [&](int t) {  // of a tile that may be hidden from all rows of the wave
+    if (passed_over(t)) pf[0] = pf[1] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    else softmax_phase(t, true);
   };
   // A hidden key's probability is 0, and 0 times an infinity or a NaN is not: where the V of a tile that some row has masked holds such
   // a value, the products of masked tiles are taken key by key from there on, over the visible ones.  A wave looks at what it loaded
@@ -282,7 +303,55 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   };
   auto phase_fence = [&]() { __builtin_amdgcn_sched_barrier(0); };  // keeps the compiler from mixing the phases
   // The MFMA phase of a tile: O += P(t) V(t), then S(t+1) = K(t+1) Q^T, eight fragment reads ahead of the MFMAs that consume them.
-  auto mfma_phase = [&](int vslot, int kslot) __attribute__((always_inline)) {
+  auto shape = [&](int t) {
+    if constexpr (kShapeSteps<SC> > 0) shape_scores<SC>(sacc, a.x, a.scale_log2, slope, first_key(t) + 4 * h - before - token);
+  };
+  // Where scores are shaped, the products go the other way round, S(t+1) first, which is shaped in place while O += P(t) V(t) is on the matrix cores.
+  auto shaping_phase = [&](int t, int vslot, int kslot) __attribute__((always_inline)) {
+    constexpr int AHEAD = 4, STEPS = kShapeSteps<SC>, EACH = (STEPS + 2 * DB - 1) / (2 * DB);
+    const float unit = shape_unit<SC>(a.x, a.scale_log2), at = slope * (float)(first_key(t + 1) + 4 * h - before - token);
+    phase_fence();
+    const unsigned char* vs_lds = smem + (NBUF + vslot) * TILE;
+    const unsigned char* ks_lds = smem + kslot * TILE;
+    s16x8 vfr[2 * DB], kfr[KS];
+    auto read_k = [&](int ks) { kfr[ks] = *(const s16x8*)(ks_lds + koff(ks)); };
+    auto read_v = [&](int f) {
+      const unsigned char* src = vs_lds + 16 * (f / DB) * ROWB + voff[f % DB];
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src + 8 * ROWB));
+      vfr[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto read = [&](int i) {  // fragments in the order of their MFMAs
+      if (i < KS) read_k(i);
+      else if (i < KS + 2 * DB) read_v(i - KS);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) read(i);
+    phase_fence();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      sacc = E::mma(kfr[ks], qf[ks], sacc);
+      phase_fence();
+      read(AHEAD + ks);
+      phase_fence();
+    }
+#pragma unroll
+    for (int f = 0; f < 2 * DB; ++f) {
+      oacc[f % DB] = E::mma(vfr[f], pf[f / DB], oacc[f % DB]);
+      phase_fence();
+      read(AHEAD + KS + f);
+      phase_fence();
+#pragma unroll
+      for (int i = f * EACH; i < (f + 1) * EACH && i < STEPS; ++i) {
+        shape_step<SC>(sacc, i, a.x, unit, slope, at);
+        phase_fence();
+      }
+    }
+  };
+  auto mfma_phase = [&](int t, int vslot, int kslot) __attribute__((always_inline)) {
+    if constexpr (kShapeSteps<SC> > 0) return shaping_phase(t, vslot, kslot);
     phase_fence();
     const unsigned char* vs_lds = smem + (NBUF + vslot) * TILE;
     const unsigned char* ks_lds = smem + kslot * TILE;
@@ -351,13 +420,13 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       if ((SLOT & 1) == 0) ring_barrier();
       if (SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
-      if (!SECOND) mfma_phase(SLOT, (SLOT + 1) & 3);
+      if (!SECOND) mfma_phase(t, SLOT, (SLOT + 1) & 3);
       else softmax_phase(t, false);
       phase_fence();
       if (!SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
       if (!SECOND) softmax_phase(t + 1, false);
-      else mfma_phase(SLOT, (SLOT + 1) & 3);
+      else mfma_phase(t, SLOT, (SLOT + 1) & 3);
       phase_fence();
     };
     auto masked_block = [&](int t) __attribute__((always_inline)) {
@@ -365,46 +434,114 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       if ((t & 1) == 0) looking_barrier(t);
       if (SECOND) {
         issue_loads(t, (t & 1) == 0);
-        softmax_phase(t, true);
+        weights_of(t);
       }
       phase_fence();
       if (odd_values(t)) {
         pv_by_key(t, t & 3);
         qk((t + 1) & 3);
+        shape(t + 1);
       } else {
-        mfma_phase(t & 3, (t + 1) & 3);
+        mfma_phase(t, t & 3, (t + 1) & 3);
       }
       phase_fence();
       if (SC == 0) mask_tile(t + 1);
       if (!SECOND) {
         issue_loads(t, (t & 1) == 0);
-        if (t + 1 < n_tiles) softmax_phase(t + 1, true);  // (the scores past the last tile are of nothing)
+        if (t + 1 < n_tiles) weights_of(t + 1);  // (the scores past the last tile are of nothing)
       }
       phase_fence();
     };
     if (SC == 0) mask_tile(0);
-    if (!SECOND) softmax_phase(0, true);
+    if (!SECOND) weights_of(0);
     // block t has the products of tile t and the scores of tile t + 1.  Three loops one after the other, not one with two ways through it:
     // where two meet again the compiler has two sets of accumulators (64 moves a group, and registers in scratch)
     int t = 0;
-    // (by the rows of the workgroup: what a wave does not mask itself it may have to look at for another)
-    const int masked_first = min((max(every.low, 0) + 3) & ~3, n_tiles);
+    if constexpr (SC == 0) {
+      // (by the rows of the workgroup: what a wave does not mask itself it may have to look at for another)
+      const int masked_first = min((max(every.low, 0) + 3) & ~3, n_tiles);
 #pragma unroll 1
-    for (; t < masked_first; ++t) masked_block(t);
+      for (; t < masked_first; ++t) masked_block(t);
 #pragma unroll 1
-    for (; t + 4 < min(n_tiles, every.up); t += 4) {
-      hold_for(t + 6);
-      if (any_gone()) break;
-      plain_block(std::integral_constant<int, 0>{}, t);
-      plain_block(std::integral_constant<int, 1>{}, t + 1);
-      plain_block(std::integral_constant<int, 2>{}, t + 2);
-      plain_block(std::integral_constant<int, 3>{}, t + 3);
+      for (; t + 4 < min(n_tiles, every.up); t += 4) {
+        hold_for(t + 6);
+        if (any_gone()) break;
+        plain_block(std::integral_constant<int, 0>{}, t);
+        plain_block(std::integral_constant<int, 1>{}, t + 1);
+        plain_block(std::integral_constant<int, 2>{}, t + 2);
+        plain_block(std::integral_constant<int, 3>{}, t + 3);
+      }
     }
 #pragma unroll 1
     for (; t < n_tiles; ++t) masked_block(t);
   };
-  if (tid == 0) *odd_from = INT32_MAX;
-  if (n_tiles > 0) {
+  // The walk of a scored call, whose tiles may be masked anywhere: those that may be in front, those that are not, and the others, all of them four at a
+  // time with their slots at compile time.  Nothing is looked at on the way: a V that is no number where some row does not see it makes that row's sums no numbers, which is looked
+  // for at the end, and then the workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, every token with a document of its own: TIME us; 545
+  // with a look at each tile, its slots worked out and both ways of the products in the loop; plain causal 267.)
+  auto scored_walk = [&](auto second_c) __attribute__((always_inline)) {
+    constexpr bool SECOND = decltype(second_c)::value;
+    auto block = [&](int t, int slot, bool plain, bool last) __attribute__((always_inline)) {
+      auto issue_loads = [&]() __attribute__((always_inline)) {
+        if ((slot & 1) == 0) {
+          issue_k(t + 3);
+          issue_k(t + 4);
+        } else {
+          issue_v(t + 1);
+          issue_v(t + 2);
+        }
+      };
+      if ((slot & 1) == 0) ring_barrier();
+      if (SECOND) {
+        issue_loads();
+        phase_fence();
+        if (plain) softmax_phase(t, false);
+        else weights_of(t);
+      }
+      phase_fence();
+      if (plain || !(passed_over(t) && passed_over(t + 1))) mfma_phase(t, slot, (slot + 1) & 3);
+      phase_fence();
+      if (!SECOND) {
+        issue_loads();
+        phase_fence();
+        if (plain) softmax_phase(t + 1, false);
+        else if (!last || t + 1 < n_tiles) weights_of(t + 1);
+      }
+      phase_fence();
+    };
+    auto four = [&](int t, auto plain_c) __attribute__((always_inline)) {
+      constexpr bool PLAIN = decltype(plain_c)::value;
+      block(t, 0, PLAIN, false);
+      block(t + 1, 1, PLAIN, false);
+      block(t + 2, 2, PLAIN, false);
+      block(t + 3, 3, PLAIN, !PLAIN);
+    };
+    if (!SECOND) weights_of(0);
+    int t = 0;
+    const int masked_first = min((max(t_low, 0) + 3) & ~3, n_tiles & ~3);
+#pragma unroll 1
+    for (; t < masked_first; t += 4) {
+      hold_for(t + 6);
+      four(t, std::false_type{});
+    }
+#pragma unroll 1
+    for (; t + 4 < min(n_tiles, t_up); t += 4) {
+      hold_for(t + 6);
+      if (any_gone()) break;
+      four(t, std::true_type{});
+    }
+#pragma unroll 1
+    for (; t + 4 <= n_tiles; t += 4) {
+      hold_for(t + 6);
+      four(t, std::false_type{});
+    }
+#pragma unroll 1
+    for (; t < n_tiles; ++t) {
+      hold_for(t + 4);
+      block(t, t & 3, false, true);
+    }
+  };
+  auto begin = [&]() {
     hold(0);
     issue_k(0);
     issue_k(1);
@@ -414,9 +551,43 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
     __builtin_amdgcn_s_waitcnt(0);  // retire the Q loads with a wait the compiler can see (and the tiles)
     ring_barrier();
     qk(0);
-    if (wave < WAVES / 2) walk(std::false_type{});
-    else walk(std::true_type{});
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // re-reads of the last tile
+    shape(0);
+  };
+  auto end = []() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };  // re-reads of the last tile
+  if (tid == 0) *odd_from = INT32_MAX;
+  if (n_tiles > 0) {
+    begin();
+    if constexpr (SC == 0) {
+      if (wave < WAVES / 2) walk(std::false_type{});
+      else walk(std::true_type{});
+      end();
+    } else {
+      if (wave < WAVES / 2) scored_walk(std::false_type{});
+      else scored_walk(std::true_type{});
+      end();
+      float none[4] = {0.f, 0.f, 0.f, 0.f};  // not 0 where a sum is no number
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) none[e & 3] = __builtin_fmaf(oacc[db][e], 0.f, none[e & 3]);
+      const float any = (none[0] + none[1]) + (none[2] + none[3]);
+      if (any != any) *odd_from = 0;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(*odd_from) != INT32_MAX) {
+        __syncthreads();
+        if (tid == 0) *odd_from = INT32_MAX;
+        m = -INFINITY;
+        ms = ls[0] = ls[1] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+        begin();
+        if (wave < WAVES / 2) walk(std::false_type{});
+        else walk(std::true_type{});
+        end();
+      }
+    }
   }
 
   const float l = cross_half_sum(ls[0] + ls[1]);
@@ -426,10 +597,10 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
 #pragma unroll
     for (int i = 0; i < DB * 4; ++i)
       *(f32x4*)(to + 256 * i) = f32x4{oacc[i / 4][i % 4 * 4], oacc[i / 4][i % 4 * 4 + 1], oacc[i / 4][i % 4 * 4 + 2], oacc[i / 4][i % 4 * 4 + 3]};
-    if (h == 0) a.many.stat[slot * BM + 32 * wave + n] = float2{l == 0.f ? -INFINITY : ms, l};
+    if (h == 0) a.many.stat[slot * BM + 32 * wave + n] = float2{l == 0.f ? -INFINITY : ms + score_base<SC>(a.x), l};
     return;
   }
-  store_rows<DT, DB>(a, p.s, head, r0 + 32 * wave, r_last, oacc, 0, l, ms);
+  store_rows<DT, DB>(a, p.s, head, r0 + 32 * wave, r_last, oacc, 0, l, ms + score_base<SC>(a.x));
 }
 
 // The shares of a row tile added up in an order of their own: a workgroup has 32 columns of the 32 rows of a wave, its waves every so-many-th

@@ -1,50 +1,15 @@
-// gfx950 (CDNA4) kernel: attention of new tokens over a paged cache with scores that are capped, biased by distance, or masked by documents and
-// prefixes (the programs of ringattn_paged_few.h and ringattn_paged_many.h; ringattn_paged_attend.hip has those of plain scores).
-//
-//   paged_scored_kernel : SC says what becomes of a score between the products and the softmax (shape_scores), in registers, where the
-//       vector pipes have what the matrix cores leave them: a cap is an exponential and a reciprocal more, a slope an addition and a fused
-//       multiply-add.  Masks cost what those of a window cost: only tiles that some row of a wave may not see are compared.
-#include "ringattn_paged_few.h"
-#include "ringattn_paged_many.h"
+// gfx950 (CDNA4): attention with shaped scores over a paged cache, dim 128 (ringattn_paged_scored.h).
+#include "ringattn_paged_scored.h"
 
 namespace ringattn {
 namespace paged {
 
-template <int DT, int D, int SC>
-__global__ __launch_bounds__(512, 2) void paged_scored_kernel(const AttendArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kFewLds<D> > kManyLds<D> ? kFewLds<D> : kManyLds<D>];
-  const int few = (int)blockIdx.x - a.few_begin;
-  if ((unsigned)few < (unsigned)kFewWorkgroups) few_rows<DT, D, SC>(a, smem, few);
-  else many_rows<DT, D, SC>(a, smem, few < 0 ? (int)blockIdx.x : few - kFewWorkgroups);
-}
-
-// As paged_merge_kernel: which row tiles were cut goes by the prefixes too.
-template <int DT, int D> __global__ __launch_bounds__(64 * kMergeSharers) void paged_scored_merge_kernel(const AttendArgs a) {
-  __shared__ float sums[2][kMergeSharers - 1][18][64];
-  for (int64_t block = blockIdx.x, turn = 0; block < INT32_MAX && merge_many<DT, D, kScored>(a, (int)block, sums[turn]); block += gridDim.x, turn ^= 1) {}
-}
+hipError_t launch_paged_scored64(const AttendArgs& a, int sc, int dtype, int64_t many_places, int64_t cut_tiles, hipStream_t stream);
 
 hipError_t launch_paged_scored(const AttendArgs& a, int sc, int dtype, int dim, int64_t many_places, int64_t cut_tiles, hipStream_t stream) {
-  const int64_t blocks = kFewWorkgroups + many_places * a.kv_heads, merges = a.many_cut ? cut_tiles * a.kv_heads * (kManyRows / 32) * (dim / 32) : 0;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-#define RA_LAUNCH_SCORED(DT_, D_)                                                                                              \
-  do {                                                                                                                         \
-    if (sc == kScored) paged_scored_kernel<DT_, D_, kScored><<<(unsigned)blocks, 512, 0, stream>>>(a);                           \
-    else if (sc == (kScored | kCapped)) paged_scored_kernel<DT_, D_, kScored | kCapped><<<(unsigned)blocks, 512, 0, stream>>>(a); \
-    else if (sc == (kScored | kSloped)) paged_scored_kernel<DT_, D_, kScored | kSloped><<<(unsigned)blocks, 512, 0, stream>>>(a); \
-    else if (sc == (kScored | kCapped | kSloped))                                                                              \
-      paged_scored_kernel<DT_, D_, kScored | kCapped | kSloped><<<(unsigned)blocks, 512, 0, stream>>>(a);                       \
-    else return hipErrorInvalidValue;                                                                                          \
-    if (merges > 0)                                                                                                            \
-      paged_scored_merge_kernel<DT_, D_><<<(unsigned)(merges < 1024 ? merges : 1024), 64 * kMergeSharers, 0, stream>>>(a);      \
-  } while (0)
-  if (dtype == 0 && dim == 64) RA_LAUNCH_SCORED(0, 64);
-  else if (dtype == 1 && dim == 64) RA_LAUNCH_SCORED(1, 64);
-  else if (dtype == 0 && dim == 128) RA_LAUNCH_SCORED(0, 128);
-  else if (dtype == 1 && dim == 128) RA_LAUNCH_SCORED(1, 128);
-#undef RA_LAUNCH_SCORED
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+  if (dim == 64) return launch_paged_scored64(a, sc, dtype, many_places, cut_tiles, stream);
+  if (dtype == 0) return launch_scored<0, 128>(a, sc, many_places, cut_tiles, stream);
+  return launch_scored<1, 128>(a, sc, many_places, cut_tiles, stream);
 }
 
 }  // namespace paged

@@ -412,8 +412,8 @@ class PagePool:
             raise ValueError("up to 4096 rows, and 2^30 entries of the table")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         ints = dict(dtype=torch.int32, device=device)
-        self.refs, self.lens = torch.zeros(self.pages, **ints), torch.zeros(self.rows, **ints)
-        self.page_table = torch.full((self.rows, self.table_pages), -1, **ints)
+        self._refs, self._lens = torch.zeros(self.pages, **ints), torch.zeros(self.rows, **ints)
+        self._table = torch.full((self.rows, self.table_pages), -1, **ints)
         self._scratch = torch.empty(bytes_, dtype=torch.uint8, device=device)
         calls = _lib.load_calls()
         self._native = None
@@ -422,6 +422,11 @@ class PagePool:
         if calls and device.type == "cuda":   # checks and launches in native code, as PagedAttention's
             self._native = [calls.Pages(self.lib.addresses[name], ctypes.addressof(self._struct), kind, self.refs.device.index)
                             for kind, name in enumerate(("ringattn_pages_update", "ringattn_pages_compact"))]
+
+    # (tensors of the pool's own, whose addresses its calls hold: written in place, not replaced)
+    refs = property(lambda self: self._refs)
+    lens = property(lambda self: self._lens)
+    page_table = property(lambda self: self._table)
 
     def _checked(self, k_cache, v_cache, scores, *ints):
         pool = _pool(k_cache, v_cache, scores, self.page_size)

@@ -96,7 +96,7 @@ class Rotary:
         turns = torch.tensor([x - 2 ** 64 if x >= 2 ** 63 else x for x in made], dtype=torch.int64)
         if device is None:
             device = f"cuda:{torch.cuda.current_device()}" if torch.cuda.is_available() else "cpu"
-        self.turns = turns.to(device)
+        self._turns = turns.to(device)
         self._params = [RingattnRotary(self.rotary_dim, int(self.interleaved), back, self.scale, self.turns.data_ptr()) for back in (0, 1)]
         self.address = ctypes.addressof(self._params[0])   # for calls that are made in native code
         calls = _lib.load_calls()
@@ -104,6 +104,8 @@ class Rotary:
         if calls and self.turns.is_cuda:
             self._native = calls.Turn(self.lib.addresses["ringattn_rotary_apply"], self.address, ctypes.addressof(self._params[1]), self.dim, self.dtype_code,
                                       self.turns.device.index, self.torch_dtype)
+
+    turns = property(lambda self: self._turns)   # (its address is the structs')
 
     def params(self, inverse):
         """struct ringattn_rotary."""

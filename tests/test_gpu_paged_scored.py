@@ -171,6 +171,38 @@ def test_hidden_places_may_hold_anything():
                 compare(lse[:, t], want_lse[:, t], tol_lse[:, t], t)
 
 
+@pytest.mark.parametrize("scores", ["documents", "cap and slopes", "window and prefix"])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_long_chunks_walk_again_where_a_hidden_v_is_odd(scores, value):
+    """Many rows: a V that is no number, in places that some rows of a workgroup see and others do not, and in places that none sees."""
+    lens, news = [700], [420]
+    more = SCORES[scores](dict(lens=lens, news=news, heads=4))
+    c = ref.Case(lens=lens, news=news, heads=4, kv_heads=2, page=32, seed=12, **more)
+    places = [5, 300, 431, 699]
+    for j in places:
+        c.v[c.row(0, j), :, j % 32, 7] = value
+    c.k[c.row(0, 40), :, 40 % 32] = value if scores == "documents" else 0.5
+    c.table[0, 4] = -1 if scores == "documents" else c.table[0, 4]
+    plan = plan_of(c)
+    slopes, prefix, first = c.given()
+    out, lse = plan.forward(c.q.cuda(), c.k.cuda(), c.v.cuda(), *sequences(c), prefix_lens=prefix, first_keys=first)
+    want, want_lse, tol, tol_lse = ref.attend(c)
+    compare(lse, want_lse, tol_lse, "lse")
+    # (place 5 is seen by all rows but those of later documents: as one of the keys before, or of the prefix)
+    assert torch.isfinite(want[:, :, 8:]).all() and not torch.isfinite(want[:, :, 7]).all() and (scores != "documents" or torch.isfinite(want[:, :, 7]).any())
+    # A weight below 2^-126 is 0 in 32 bits, and 0 times an infinity is no number, where the definition has an infinity: under slopes that of a far key.
+    faint = torch.zeros(420, 4, dtype=torch.bool)
+    for h in range(4):
+        k, there = c.rows(c.k, 0, h // 2)
+        ok, x, _ = c.scores(0, h, k, there)
+        faint[:, h] = (ok & (x - want_lse[h][:, None] < -125 * math.log(2)))[:, places].any(dim=1)
+    assert scores != "documents" or not faint.any()
+    assert not torch.isfinite(out[:, :, 7].cpu()[faint]).any()
+    got = out.double().cpu()
+    got[:, :, 7] = torch.where(faint, want[:, :, 7], got[:, :, 7])
+    compare(got, want, tol, "out")
+
+
 def test_a_cap_holds_infinite_scores():
     """Products past the range of 32 bits: the cap, of either sign."""
     c = ref.Case(lens=[64], news=[2], heads=2, kv_heads=2, cap=30.0, dtype="bf16", seed=3)
