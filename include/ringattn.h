@@ -463,17 +463,21 @@ size_t ringattn_pages_scratch_bytes(int pages, int rows, int table_pages);
  *   add     : [rows], NULL: 0.  Tokens more, for which pages are made ready (ringattn_paged_append writes them); negative: fewer, to none
  *   missing : [rows], may be NULL: 1 where a row was to grow and did not, else 0
  * Rows that grow take free pages, lowest first, in the order of the rows as long as there are enough; behind a row that finds too few none
- * grows.  A row that would grow past its entries of the table does not, and takes none.  A row that does not grow has what it began with.  Where a row grows from within a page that something
- * else names too, the page is copied (K, V, scores) and the copy is the row's alone.
+ * grows.  A row that would grow past its entries of the table does not, and takes none.  A row that does not grow has what it began with.  Where a
+ * row grows from within a page that something else names too, the page is copied (K, V, scores) and the copy is the row's alone.
+ *   copies  : [rows, 2], 8-byte aligned, may be NULL: from which page to which a row's was copied, or -1, -1.  Where several pools (a model's
+ *             layers) go by one table: ringattn_pages_copy of these pairs in the others.  With pool NULL nothing is copied but by the caller
  */
-int ringattn_pages_update(const ringattn_pages* pages, const ringattn_paged_pool* pool, const int* parents, const int* add, int* missing, void* stream);
+int ringattn_pages_update(const ringattn_pages* pages, const ringattn_paged_pool* pool, const int* parents, const int* add, int* missing, int* copies,
+                          void* stream);
 
 /*
  * Of the n pages with a count, those at places from n on move (K, V, scores, counts) to the free ones in front of it, the i-th to the i-th, and the table's
  * entries go with them: pages [n, pages) are free afterwards.  used: [1], n.  moved: [pages], may be NULL: the place that the page of a
- * place has now, -1 for free ones (for entries that the caller counts besides).
+ * place has now, -1 for free ones (for entries that the caller counts besides).  moves: [pages, 2], 8-byte aligned, may be NULL: from where to where, -1, -1
+ * behind the last; pool may be NULL as above.
  */
-int ringattn_pages_compact(const ringattn_pages* pages, const ringattn_paged_pool* pool, int* used, int* moved, void* stream);
+int ringattn_pages_compact(const ringattn_pages* pages, const ringattn_paged_pool* pool, int* used, int* moved, int* moves, void* stream);
 
 /*
  * K, V and scores of pages from one pool to another of as many heads, or within one: pairs [n, 2] on the device, from which page to which.  A page that is written

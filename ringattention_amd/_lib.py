@@ -129,8 +129,8 @@ SYMBOLS = {
     "ringattn_paged_evict": (ctypes.c_int, [ctypes.c_void_p, _cache_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "ringattn_pages_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
-    "ringattn_pages_update": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 4),
-    "ringattn_pages_compact": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 3),
+    "ringattn_pages_update": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 5),
+    "ringattn_pages_compact": (ctypes.c_int, [ctypes.POINTER(RingattnPages), ctypes.POINTER(RingattnPagedPool)] + [ctypes.c_void_p] * 4),
     "ringattn_pages_copy": (ctypes.c_int, [ctypes.POINTER(RingattnPagedPool), ctypes.c_int, ctypes.POINTER(RingattnPagedPool), ctypes.c_int, ctypes.c_int,
                                            ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "ringattn_rotary_turns": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),

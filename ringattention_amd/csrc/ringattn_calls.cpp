@@ -334,7 +334,7 @@ PyObject* paged_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
   return PyLong_FromLong(rc);
 }
 
-// Paged(address of the entry point, of the plan, kind, heads, kv_heads, dim, page_size, max_batch, max_tokens, device, dtype, dtype of out[, softcap])
+// Paged(address of the entry point, of the plan, kind (0 to 3; 16, 17, 18 for 4, 5, 6), heads, kv_heads, dim, page_size, max_batch, max_tokens, device, dtype, dtype of out[, softcap])
 PyObject* paged_create(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   unsigned long long entry, plan;
   int kind, heads, kv_heads, dim, page, max_batch, max_tokens, device;
@@ -346,7 +346,8 @@ PyObject* paged_create(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   }
   if (!PyArg_ParseTuple(args, "KKiiiiiiiiOO|f", &entry, &plan, &kind, &heads, &kv_heads, &dim, &page, &max_batch, &max_tokens, &device, &dtype, &out_dtype, &softcap))
     return nullptr;
-  if (!entry || kind < 0 || kind > 6 || !THPDtype_Check(dtype) || !THPDtype_Check(out_dtype)) {
+  const bool known = (kind >= 0 && kind < 4) || (kind >= 16 && kind < 19);
+  if (!entry || !known || !THPDtype_Check(dtype) || !THPDtype_Check(out_dtype)) {
     PyErr_SetString(PyExc_ValueError, "an entry point, which of the seven it is, and two torch.dtypes");
     return nullptr;
   }
@@ -355,7 +356,7 @@ PyObject* paged_create(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   self->vectorcall = paged_call;
   self->entry = reinterpret_cast<void*>(static_cast<uintptr_t>(entry));
   self->plan = reinterpret_cast<void*>(static_cast<uintptr_t>(plan));
-  self->kind = kind;
+  self->kind = kind < 4 ? kind : kind - 12;
   self->heads = heads;
   self->kv_heads = kv_heads;
   self->dim = dim;
@@ -460,7 +461,7 @@ PyObject* turn_create(PyTypeObject* type, PyObject* args, PyObject*) {
 }
 
 // ---- pages (paged.PagePool): Pages(k, v, scores or None, parents or None, add or None, short, stream or None), or with kind 1
-// Pages(k, v, scores or None, moved or None, None, used, stream or None)
+// Pages(k, v, scores or None, moved or None, None, used, stream or None); calls that ask for pairs go the general way
 struct Pages {
   PyObject_HEAD
   vectorcallfunc vectorcall;
@@ -508,9 +509,9 @@ PyObject* pages_call(PyObject* self_, PyObject* const* args, size_t nargsf, PyOb
   int rc;
   Py_BEGIN_ALLOW_THREADS
   if (p.kind == 0)
-    rc = reinterpret_cast<decltype(&ringattn_pages_update)>(p.entry)(p.pages, &pool, (const int*)x[0], (const int*)x[1], (int*)x[2], stream);
+    rc = reinterpret_cast<decltype(&ringattn_pages_update)>(p.entry)(p.pages, &pool, (const int*)x[0], (const int*)x[1], (int*)x[2], nullptr, stream);
   else
-    rc = reinterpret_cast<decltype(&ringattn_pages_compact)>(p.entry)(p.pages, &pool, (int*)x[2], (int*)x[0], stream);
+    rc = reinterpret_cast<decltype(&ringattn_pages_compact)>(p.entry)(p.pages, &pool, (int*)x[2], (int*)x[0], nullptr, stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
 }

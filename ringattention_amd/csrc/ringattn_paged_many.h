@@ -477,8 +477,8 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   };
   // The walk of a scored call, whose tiles may be masked anywhere: those that may be in front, those that are not, and the others, all of them four at a
   // time with their slots at compile time.  Nothing is looked at on the way: a V that is no number where some row does not see it makes that row's sums no numbers, which is looked
-  // for at the end, and then the workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, every token with a document of its own: TIME us; 545
-  // with a look at each tile, its slots worked out and both ways of the products in the loop; plain causal 267.)
+  // for at the end, and then the workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, in every 64 one that sees itself
+  // alone, which masks all tiles: 409 us; 545 with a look at each tile, its slots worked out and both ways of the products in the loop; with no masks 278.)
   auto scored_walk = [&](auto second_c) __attribute__((always_inline)) {
     constexpr bool SECOND = decltype(second_c)::value;
     auto block = [&](int t, int slot, bool plain, bool last) __attribute__((always_inline)) {

@@ -76,9 +76,12 @@ struct Args {
   const int* parents;  // [rows] or NULL
   const int* add;      // [rows] or NULL
   int* missing;        // [rows] or NULL
+  int2* pairs;         // copies of an update [rows], moves of a compaction [pages]: from, to, or -1; or NULL
   // scratch
   int* made;           // [rows, table_pages]: rows that others were made of
-  int4* told;          // [rows]: the row's entries end in `made`; the page that is copied, to which page (-1: none); where its entries begin
+  int2* told;          // [rows]: where the row's entries of `made` begin and end; of a compaction [0]: pages in use, and how many move
+  int2* copies;        // [rows]: pages that are copied, from, to; [0, copied[0])
+  int* copied;         // [1]
   int* list;           // [pages]: free pages; of a compaction: pages that move
   int* slots;          // [pages]: where they go
   int* counts;         // [pages / kBlock + 1] pages in use
@@ -218,6 +221,7 @@ __global__ __launch_bounds__(kThreads) void pages_grow_kernel(const Args a) {
   found = min(found, total);
   __syncthreads();  // (all waves see the list and the rows of this workgroup's own)
   // all lengths have been read: they may be written
+  int copies = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int b = EACH * tid + i;
@@ -226,20 +230,22 @@ __global__ __launch_bounds__(kThreads) void pages_grow_kernel(const Args a) {
     const int now = grows && !granted ? had[i] : want[i];
     a.lens[b] = now;
     if (a.missing) a.missing[b] = grows && !granted;
-    int4 t{0, -1, -1, 0};
+    int2 copy{-1, -1};
     if (granted && torn[i] >= 0) {
-      t.y = torn[i];
-      t.z = a.list[upto[b] - need[i]];
+      copy = int2{torn[i], a.list[upto[b] - need[i]]};
       atomicAdd(a.refs + torn[i], -1);
+      ++copies;
     }
-    if (a.parents) {
-      t.x = max((now + page - 1) >> a.page_shift, old[i]);
-      t.w = itself[i] ? kept[i] - (granted && torn[i] >= 0 ? 1 : 0) : 0;
-    }
-    a.told[b] = t;
+    torn[i] = copy.x;
+    if (a.pairs) a.pairs[b] = copy;
+    if (a.parents) a.told[b] = int2{itself[i] ? kept[i] - (copy.x >= 0 ? 1 : 0) : 0, max((now + page - 1) >> a.page_shift, old[i])};
     if (!granted) first[b] = -1;
   }
-  __syncthreads();
+  int all_copies, at_copy = scan_all(copies, sums[0], all_copies) - copies;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (torn[i] >= 0) a.copies[at_copy++] = int2{torn[i], a.list[upto[EACH * tid + i] - need[i]]};
+  if (tid == 0) a.copied[0] = all_copies;
   for (int j = tid; j < found; j += kThreads) {
     int lo = 0, hi = kMaxRows - 1;  // the first row whose pages end behind j
     while (lo < hi) {
@@ -255,16 +261,21 @@ __global__ __launch_bounds__(kThreads) void pages_grow_kernel(const Args a) {
   }
 }
 
-__global__ __launch_bounds__(256) void pages_settle_kernel(const Args a, const Pool pool, int pieces) {
-  const int b = blockIdx.x;
-  const int4 t = a.told[b];
-  if ((int)blockIdx.y < pieces) {
-    if (t.y >= 0) copy_units(pool, pool, t.y, t.z, (int64_t)blockIdx.y * kUnits);
+// Workgroups [0, entry_blocks): entries of the table, with parents.  The others: pages, piece by piece.
+__global__ __launch_bounds__(256) void pages_settle_kernel(const Args a, const Pool pool, int pieces, int entry_blocks, int each) {
+  if ((int)blockIdx.x < entry_blocks) {
+    const int b = blockIdx.x / each;
+    const int2 t = a.told[b];
+    for (int e = t.x + (int)((blockIdx.x - b * each) * 256 + threadIdx.x); e < t.y; e += each * 256)
+      a.table[b * a.table_stride + e] = a.made[(int64_t)b * a.table_pages + e];
     return;
   }
-  // (with parents) entries of the table: of a row that was made of itself, those that it did not have
-  for (int e = t.w + (int)((blockIdx.y - pieces) * 256 + threadIdx.x); e < t.x; e += (gridDim.y - pieces) * 256)
-    a.table[b * a.table_stride + e] = a.made[(int64_t)b * a.table_pages + e];
+  const int64_t items = (int64_t)a.copied[0] * pieces;
+  for (int64_t i = blockIdx.x - entry_blocks; i < items; i += gridDim.x - entry_blocks) {
+    const int64_t j = i / pieces;
+    const int2 copy = a.copies[j];
+    copy_units(pool, pool, copy.x, copy.y, (i - j * pieces) * kUnits);
+  }
 }
 
 // ---- compaction
@@ -331,15 +342,17 @@ __global__ __launch_bounds__(kThreads) void pages_rank_kernel(const Args a) {
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.used[0] = n;
-    a.told[0] = int4{n, n - in_front, 0, 0};  // for the next launch: how many there are, how many move
+    a.told[0] = int2{n, n - in_front};  // for the next launch
   }
 }
 
-// Workgroups [0, table_blocks): entries of the table.  The others: pages, piece by piece.
+// Workgroups [0, table_blocks): entries of the table.  The others: pages, piece by piece (one piece that copies nothing where the caller does that).
 __global__ __launch_bounds__(256) void pages_move_kernel(const Args a, const Pool pool, int pieces, int table_blocks) {
-  const int4 t = a.told[0];
+  const int2 t = a.told[0];
   const int n = t.x, m = t.y;
   if ((int)blockIdx.x < table_blocks) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; a.pairs && i < a.pages; i += (int64_t)table_blocks * 256)
+      a.pairs[i] = i < m ? int2{a.list[i], a.slots[i]} : int2{-1, -1};
     if (m == 0) return;
     const int64_t entries = (int64_t)a.rows * a.table_pages;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)table_blocks * 256) {
@@ -364,7 +377,7 @@ __global__ __launch_bounds__(256) void pages_move_kernel(const Args a, const Poo
       a.refs[from] = 0;
       if (a.moved) a.moved[from] = to;
     }
-    copy_units(pool, pool, from, to, (int64_t)piece * kUnits);
+    if (pool.k) copy_units(pool, pool, from, to, (int64_t)piece * kUnits);
   }
 }
 
@@ -389,7 +402,7 @@ inline bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (byt
 
 // Scratch: told, then the lists, then rows that others were made of.
 struct Scratch {
-  size_t told, list, slots, counts, made, bytes;
+  size_t told, copies, copied, list, slots, counts, made, bytes;
 };
 bool sizes_ok(int pages, int rows, int table_pages, int page_size) {
   return pages >= 1 && rows >= 1 && rows <= kMaxRows && table_pages >= 1 && page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 &&
@@ -399,7 +412,9 @@ Scratch scratch_of(int pages, int rows, int table_pages) {
   Scratch s;
   auto up = [](size_t x) { return (x + 15) & ~(size_t)15; };
   s.told = 0;
-  s.list = s.told + up((size_t)rows * sizeof(int4));
+  s.copies = s.told + up((size_t)rows * sizeof(int2));
+  s.copied = s.copies + up((size_t)rows * sizeof(int2));
+  s.list = s.copied + up(sizeof(int));
   s.slots = s.list + up((size_t)pages * sizeof(int));
   s.counts = s.slots + up((size_t)pages * sizeof(int));
   s.made = s.counts + up(((size_t)pages / kBlock + 1) * sizeof(int));
@@ -429,6 +444,13 @@ int check_pool(const ringattn_paged_pool* p, int pages, int page_size, Pool* out
   out->unit_shift = p->dim == 64 ? 3 : 4;
   return RINGATTN_OK;
 }
+// A pool, or none: then the caller makes the copies, for which it needs the pairs.
+int check_pool_or_pairs(const ringattn_paged_pool* p, const ringattn_pages* pages, const int* pairs, Pool* out) {
+  if (!aligned(pairs, 8)) return RINGATTN_ERR_ALIGN;
+  std::memset(out, 0, sizeof(*out));
+  if (!p) return pairs ? RINGATTN_OK : RINGATTN_ERR_NULL;
+  return check_pool(p, pages->pages, pages->page_size, out);
+}
 int pieces_of(const Pool& p) { return (int)((((int64_t)p.kv_heads << (p.page_shift + p.unit_shift)) + kUnits - 1) / kUnits); }
 
 int check_pages(const ringattn_pages* p, Args* a) {
@@ -450,7 +472,9 @@ int check_pages(const ringattn_pages* p, Args* a) {
   a->table_pages = p->table_pages;
   a->page_shift = __builtin_ctz((unsigned)p->page_size);
   char* w = (char*)p->scratch;
-  a->told = (int4*)(w + s.told);
+  a->told = (int2*)(w + s.told);
+  a->copies = (int2*)(w + s.copies);
+  a->copied = (int*)(w + s.copied);
   a->list = (int*)(w + s.list);
   a->slots = (int*)(w + s.slots);
   a->counts = (int*)(w + s.counts);
@@ -475,44 +499,48 @@ size_t ringattn_pages_scratch_bytes(int pages, int rows, int table_pages) {
   return pg::sizes_ok(pages, rows, table_pages, 16) ? pg::scratch_of(pages, rows, table_pages).bytes : 0;
 }
 
-int ringattn_pages_update(const ringattn_pages* pages, const ringattn_paged_pool* pool, const int* parents, const int* add, int* missing, void* stream_) {
+int ringattn_pages_update(const ringattn_pages* pages, const ringattn_paged_pool* pool, const int* parents, const int* add, int* missing, int* copies,
+                          void* stream_) {
   pg::Args a;
   pg::Pool p;
   PG_CHECK(pg::check_pages(pages, &a));
-  PG_CHECK(pg::check_pool(pool, pages->pages, pages->page_size, &p));
+  PG_CHECK(pg::check_pool_or_pairs(pool, pages, copies, &p));
   if (!pg::aligned(parents, 4) || !pg::aligned(add, 4) || !pg::aligned(missing, 4)) return RINGATTN_ERR_ALIGN;
   a.parents = parents;
   a.add = add;
   a.missing = missing;
+  a.pairs = (int2*)copies;
   hipStream_t stream = (hipStream_t)stream_;
   // workgroups of a row: all of its entries, 256 at a time, but no more than 4096 workgroups in all
   int each = (a.table_pages + 255) / 256;
   const int most = 4096 / a.rows > 1 ? 4096 / a.rows : 1;
   each = each < most ? each : most;
-  const int pieces = pg::pieces_of(p);
-  if (pieces + each > 65535) return RINGATTN_ERR_SHAPE;
+  const int pieces = pool ? pg::pieces_of(p) : 0, entry_blocks = parents ? a.rows * each : 0;
+  const int64_t items = (int64_t)a.rows * pieces, copy_blocks = items < 4096 ? items : 4096;  // (a copy for every row at most)
   pg::pages_share_kernel<<<dim3((unsigned)a.rows, (unsigned)each), 256, 0, stream>>>(a);
   pg::pages_grow_kernel<<<1, pg::kThreads, 0, stream>>>(a);
-  pg::pages_settle_kernel<<<dim3((unsigned)a.rows, (unsigned)(pieces + (parents ? each : 0))), 256, 0, stream>>>(a, p, pieces);
+  if (entry_blocks + copy_blocks > 0) pg::pages_settle_kernel<<<(unsigned)(entry_blocks + copy_blocks), 256, 0, stream>>>(a, p, pieces, entry_blocks, each);
   return pg::launched();
 }
 
-int ringattn_pages_compact(const ringattn_pages* pages, const ringattn_paged_pool* pool, int* used, int* moved, void* stream_) {
+int ringattn_pages_compact(const ringattn_pages* pages, const ringattn_paged_pool* pool, int* used, int* moved, int* moves, void* stream_) {
   pg::Args a;
   pg::Pool p;
   PG_CHECK(pg::check_pages(pages, &a));
-  PG_CHECK(pg::check_pool(pool, pages->pages, pages->page_size, &p));
+  PG_CHECK(pg::check_pool_or_pairs(pool, pages, moves, &p));
   if (!used) return RINGATTN_ERR_NULL;
   if (!pg::aligned(used, 4) || !pg::aligned(moved, 4)) return RINGATTN_ERR_ALIGN;
   a.used = used;
   a.moved = moved;
+  a.pairs = (int2*)moves;
   hipStream_t stream = (hipStream_t)stream_;
   const unsigned blocks = (unsigned)((a.pages + (int64_t)pg::kBlock - 1) / pg::kBlock);
   const int64_t entries = ((int64_t)a.rows * a.table_pages + 1023) / 1024;
-  const int table_blocks = (int)(entries < 512 ? entries : 512);
+  const int table_blocks = (int)(entries < 512 ? entries : 512), pieces = pool ? pg::pieces_of(p) : 1;
+  const int64_t items = (int64_t)(a.pages / 2) * pieces, move_blocks = items < 4096 ? items : 4096;  // (no more than half of the pages move)
   pg::pages_count_kernel<<<blocks, 256, 0, stream>>>(a);
   pg::pages_rank_kernel<<<blocks, pg::kThreads, 0, stream>>>(a);
-  pg::pages_move_kernel<<<table_blocks + 4096, 256, 0, stream>>>(a, p, pg::pieces_of(p), table_blocks);
+  pg::pages_move_kernel<<<(unsigned)(table_blocks + move_blocks), 256, 0, stream>>>(a, p, pieces, table_blocks);
   return pg::launched();
 }
 

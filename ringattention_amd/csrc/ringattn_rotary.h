@@ -29,7 +29,6 @@ struct ApplyArgs {
   Turns r;
   Rows x[2];
   int heads0, heads;       // of the first tensor, of both
-  int heads_each;          // heads of a thread
   int tokens;
   const int* positions;    // NULL: a row's number
   int64_t position_stride; // between batches

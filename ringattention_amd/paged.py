@@ -97,7 +97,7 @@ class PagedAttention:
     def _made(self, kind):
         entry = self.lib.addresses[("ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict",
                                     "ringattn_paged_fwd_scored", "ringattn_paged_weights_scored", "ringattn_paged_append_rotary")[kind]]
-        self._native[kind] = call = self._call_type(entry, self.handle.value, kind, self.heads, self.kv_heads, self.dim, self.page_size,
+        self._native[kind] = call = self._call_type(entry, self.handle.value, kind if kind < 4 else 12 + kind, self.heads, self.kv_heads, self.dim, self.page_size,
                                                     self.max_batch, self.max_tokens, self.device, self.torch_dtype, self.out_dtype, self.softcap)
         return call
 
@@ -392,7 +392,7 @@ def copy_pages(k_from, v_from, k_to, v_to, pairs, scores_from=None, scores_to=No
 class PagePool:
     """Which rows of a page table own and share which of `pages` pages, on the device: `page_table` int32 [rows, table_pages], `lens` int32 [rows],
     `refs` int32 [pages], how many entries of the table name a page (0: free).  They are a PagedAttention call's page_table and kv_lens as
-    they are, or rows of theirs.  A caller may count entries of its own in refs (a prompt that is kept): those pages are not given out, and not written on.
+    they are, or rows of theirs.  They are written in place, not replaced.  A caller may count entries of its own in refs (a prompt that is kept): those pages are not given out, and not written on.
 
         pool.update(k_cache, v_cache, parents, add)      rows become forks of others, or begin anew, and grow: before a step's append()
         pool.compact(k_cache, v_cache)                   the pages in use to the front of the pool
@@ -428,46 +428,56 @@ class PagePool:
     lens = property(lambda self: self._lens)
     page_table = property(lambda self: self._table)
 
-    def _checked(self, k_cache, v_cache, scores, *ints):
-        pool = _pool(k_cache, v_cache, scores, self.page_size)
-        if k_cache.shape[0] != self.pages:
-            raise ValueError(f"k_cache must have {self.pages} pages")
-        for t, name, n in ints:
+    def _checked(self, k_cache, v_cache, scores, pairs, *ints):
+        """The checked pool of a call, None where there is none and the caller copies by `pairs`, (tensor, name, shape)."""
+        pool = None
+        if k_cache is not None:
+            pool = _pool(k_cache, v_cache, scores, self.page_size)
+            if k_cache.shape[0] != self.pages:
+                raise ValueError(f"k_cache must have {self.pages} pages")
+        elif pairs[0] is None or v_cache is not None or scores is not None:
+            raise ValueError(f"without a cache, {pairs[1]} are needed")
+        for t, name, shape in (pairs,) + ints:
             if t is not None:
-                _check_tensors((t, name, torch.int32, (n,)))
-        for t in (k_cache,) + tuple(t for t, _, _ in ints):
+                _check_tensors((t, name, torch.int32, shape))
+        for t in (k_cache, pairs[0]) + tuple(t for t, _, _ in ints):
             if t is not None and t.device != self.refs.device:
                 raise ValueError(f"the tensors of a call must be on {self.refs.device}, where the table is")
-        return pool
+        return ctypes.byref(pool) if pool is not None else None
 
-    def update(self, k_cache, v_cache, parents=None, add=None, scores=None, short=None, stream=None):
+    def update(self, k_cache, v_cache, parents=None, add=None, scores=None, short=None, copies=None, stream=None):
         """All rows at once, from what they are before the call: row b begins with the tokens of row parents[b] (int32 [rows]; outside of [0, rows): with
         none), sharing their pages, and has add[b] more (int32 [rows]; negative: fewer).  Rows that grow take free pages, lowest first, in the order of
         the rows while there are enough; a page that is written on from within and that others name too is copied (K, V and `scores`).
-        Returns short, int32 [rows]: 1 where a row was to grow and did not -- it then has what it began with."""
-        if short is not None and self._native:
+        Returns short, int32 [rows]: 1 where a row was to grow and did not -- it then has what it began with.
+
+        Several caches (a model's layers) go by one table: `copies`, int32 [rows, 2], gets the pairs for copy_pages in the others; with None for k_cache and
+        v_cache nothing is copied here."""
+        if short is not None and copies is None and self._native:
             rc = self._native[0](k_cache, v_cache, scores, parents, add, short, stream)
             if rc is not None:
                 check(rc, "ringattn_pages_update")
                 return short
-        pool = self._checked(k_cache, v_cache, scores, (parents, "parents", self.rows), (add, "add", self.rows), (short, "short", self.rows))
+        rows = (self.rows,)
+        pool = self._checked(k_cache, v_cache, scores, (copies, "copies", (self.rows, 2)), (parents, "parents", rows), (add, "add", rows), (short, "short", rows))
         if short is None:
-            short = PagedAttention._new((self.rows,), torch.int32, self.refs.device, stream)
-        check(_on(self.refs.device, stream, self.lib.ringattn_pages_update, ctypes.byref(self._struct), ctypes.byref(pool),
-                  parents.data_ptr() if parents is not None else None, add.data_ptr() if add is not None else None, short.data_ptr()), "ringattn_pages_update")
+            short = PagedAttention._new(rows, torch.int32, self.refs.device, stream)
+        check(_on(self.refs.device, stream, self.lib.ringattn_pages_update, ctypes.byref(self._struct), pool,
+                  *(t.data_ptr() if t is not None else None for t in (parents, add, short, copies))), "ringattn_pages_update")
         return short
 
-    def compact(self, k_cache, v_cache, scores=None, used=None, moved=None, stream=None):
+    def compact(self, k_cache, v_cache, scores=None, used=None, moved=None, moves=None, stream=None):
         """The n pages that something names to the first n places of the pool, their counts and the table with them; the others are free.  `moved`,
-        int32 [pages]: where the page of a place is now, -1 for free ones.  Returns used, int32 [1]: n."""
-        if used is not None and self._native:
+        int32 [pages]: where the page of a place is now, -1 for free ones.  `moves`, int32 [pages, 2]: the pairs for copy_pages in other caches that go by
+        this table, as update()'s copies.  Returns used, int32 [1]: n."""
+        if used is not None and moves is None and self._native:
             rc = self._native[1](k_cache, v_cache, scores, moved, None, used, stream)
             if rc is not None:
                 check(rc, "ringattn_pages_compact")
                 return used
-        pool = self._checked(k_cache, v_cache, scores, (used, "used", 1), (moved, "moved", self.pages))
+        pool = self._checked(k_cache, v_cache, scores, (moves, "moves", (self.pages, 2)), (used, "used", (1,)), (moved, "moved", (self.pages,)))
         if used is None:
             used = PagedAttention._new((1,), torch.int32, self.refs.device, stream)
-        check(_on(self.refs.device, stream, self.lib.ringattn_pages_compact, ctypes.byref(self._struct), ctypes.byref(pool), used.data_ptr(),
-                  moved.data_ptr() if moved is not None else None), "ringattn_pages_compact")
+        check(_on(self.refs.device, stream, self.lib.ringattn_pages_compact, ctypes.byref(self._struct), pool,
+                  *(t.data_ptr() if t is not None else None for t in (used, moved, moves))), "ringattn_pages_compact")
         return used

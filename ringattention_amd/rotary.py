@@ -143,8 +143,8 @@ class Rotary:
         batch, tokens = (q.shape[0], q.shape[2]) if four else (1, q.shape[0])
         if k is not None and (k.dim() != q.dim() or ((k.shape[0], k.shape[2]) if four else (1, k.shape[0])) != (batch, tokens)):
             raise ValueError("q and k must have the same batch and as many tokens")
-        if tokens > MAX_POSITIONS or batch > 65535:
-            raise ValueError("a call takes up to 2^30 tokens and 65535 batches")
+        if tokens > MAX_POSITIONS or batch > 65535 or sum(t.shape[1] for t, _, _ in given) > 65535:
+            raise ValueError("a call takes up to 2^30 tokens, 65535 heads of q and k together, and 65535 batches")
         stride = 0
         if positions is not None:
             shape = (batch, tokens) if positions.dim() == 2 and four else (tokens,)

@@ -167,6 +167,49 @@ def test_the_same_as_torch_in_any_stream_and_captured():
         assert short.tolist() == want and used.tolist() == [n]
 
 
+def test_layers_that_go_by_one_table():
+    """Pairs of an update and of a compaction, for the caches of other layers and for all of them."""
+    b = Both(40, 5, 6, heads=2)
+    other = [(torch.randn_like(b.k), torch.randn_like(b.v)) for _ in range(2)]
+    want = [(k.clone(), v.clone()) for k, v in other]
+    copies, moves = torch.empty(5, 2, dtype=torch.int32, device="cuda"), torch.empty(40, 2, dtype=torch.int32, device="cuda")
+
+    def follow(pairs):
+        for k, v in other:
+            paged.copy_pages(k, v, k, v, pairs)
+        made = [p for p in pairs.tolist() if p != [-1, -1]]
+        for k, v in want:
+            for x in (k, v):
+                if made:
+                    s, t = (torch.tensor(y, device="cuda") for y in zip(*made))
+                    x[t] = x[s]
+        assert all(torch.equal(x, y) for a, c in zip(other, want) for x, y in zip(a, c))
+        return made
+
+    b.update(None, [20, 33, 0, 7, 0])
+    for parents, add in (([0, 0, 1, 0, 1], [1, 2, 3, 0, -4]), ([0, 1, 4, 4, 4], [5, 0, 1, 1, 1]), ([0, 1, -1, 2, 3], [0, 0, 90, 0, 0])):
+        _, pairs = b.want.update(parents, add)
+        b.moved(pairs)
+        b.pool.update(b.k, b.v, ints(parents), ints(add), scores=b.scores, copies=copies)
+        b.check(parents)
+        assert [tuple(p) for p in follow(copies)] == pairs
+        before = [x.clone() for x in (b.k, b.v)]
+        n, pairs, _ = b.want.compact()
+        assert b.pool.compact(None, None, moves=moves).tolist() == [n]    # this layer too by the pairs
+        assert torch.equal(b.k, before[0]) and torch.equal(b.v, before[1])
+        assert [tuple(p) for p in follow(moves)] == pairs
+        paged.copy_pages(b.k, b.v, b.k, b.v, moves, b.scores, b.scores)
+        b.moved(pairs)
+        b.check("compact")
+    b.want.update([0, 0, 0, 0, 0], [1, 1, 1, 1, 1])
+    short = b.pool.update(None, None, ints([0, 0, 0, 0, 0]), ints([1, 1, 1, 1, 1]), copies=copies)
+    assert b.pool.page_table.tolist() == b.want.table and not short.any()
+    for call in (lambda: b.pool.update(None, None), lambda: b.pool.compact(None, None), lambda: b.pool.update(None, b.v, copies=copies),
+                 lambda: b.pool.update(None, None, copies=copies[:4]), lambda: b.pool.update(b.k, b.v, copies=copies.float())):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_copy_pages():
     g = torch.Generator(device="cuda").manual_seed(1)
     k, v = (torch.randn(9, 3, 32, 128, generator=g, device="cuda").half() for _ in range(2))

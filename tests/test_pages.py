@@ -51,13 +51,13 @@ def test_refusals(ralib):
     table = dict(refs=x, page_table=x, lens=x, table_stride=4, pages=8, rows=3, table_pages=4, page_size=16, scratch=x, scratch_bytes=need)
     pool = dict(k=x, v=x, scores=None, page_stride=2 * 16 * 64, head_stride=16 * 64, token_stride=64, kv_heads=2, dim=64)
 
-    def update(t=None, p=None, parents=None, add=None, missing=None):
+    def update(t=None, p=None, parents=None, add=None, missing=None, copies=None, none=False):
         t, p = RingattnPages(**dict(table, **(t or {}))), RingattnPagedPool(**dict(pool, **(p or {})))
-        return ralib.ringattn_pages_update(ctypes.byref(t), ctypes.byref(p), parents, add, missing, None)
+        return ralib.ringattn_pages_update(ctypes.byref(t), None if none else ctypes.byref(p), parents, add, missing, copies, None)
 
-    def compact(t=None, p=None, used=x, moved=None):
+    def compact(t=None, p=None, used=x, moved=None, moves=None, none=False):
         t, p = RingattnPages(**dict(table, **(t or {}))), RingattnPagedPool(**dict(pool, **(p or {})))
-        return ralib.ringattn_pages_compact(ctypes.byref(t), ctypes.byref(p), used, moved, None)
+        return ralib.ringattn_pages_compact(ctypes.byref(t), None if none else ctypes.byref(p), used, moved, moves, None)
 
     for call in (update, compact):
         for bad, code in ((dict(refs=None), E_NULL), (dict(page_table=None), E_NULL), (dict(lens=None), E_NULL), (dict(refs=x + 4), E_ALIGN), (dict(lens=x + 2), E_ALIGN),
@@ -70,7 +70,7 @@ def test_refusals(ralib):
                           (dict(page_stride=2 ** 39, kv_heads=65536), E_SHAPE)):
             assert call(p=bad) == code, bad
     assert update(parents=x + 1) == E_ALIGN and update(add=x + 2) == E_ALIGN and update(missing=x + 3) == E_ALIGN
-    assert update(t=dict(page_size=1024, table_pages=1), p=dict(kv_heads=65535)) == E_SHAPE   # more pieces of a page than a launch has places
+    assert update(none=True) == E_NULL and compact(none=True) == E_NULL and update(copies=x + 4) == E_ALIGN and compact(moves=x + 4) == E_ALIGN
     assert compact(used=None) == E_NULL and compact(used=x + 2) == E_ALIGN and compact(moved=x + 2) == E_ALIGN
 
     def copy(f=None, t=None, from_pages=8, to_pages=8, page=16, pairs=x, n=0):

@@ -103,7 +103,7 @@ def test_apply_refusals(ralib):
                       (dict(in_head_stride=60), E_ALIGN), (dict(out_token_stride=132), E_ALIGN), (dict(in_token_stride=-128), E_SHAPE),
                       (dict(in_token_stride=2 ** 37), E_SHAPE), (dict(out=far, out_head_stride=32), E_SHAPE), (dict(out=far, out_token_stride=64), E_SHAPE),
                       (dict(out=far, out_head_stride=0), E_SHAPE), (dict(batch=2, out=far, out_batch_stride=64), E_SHAPE), (dict(out=far, batch=2), E_SHAPE),
-                      (dict(out=x + 64 * 2), E_SHAPE), (dict(out_token_stride=256), E_SHAPE), (dict(count=2, second=dict(heads=0)), E_SHAPE),
+                      (dict(out=x + 64 * 2), E_SHAPE), (dict(out_token_stride=256), E_SHAPE), (dict(count=2, second=dict(heads=0)), E_SHAPE), (dict(heads=40000, tokens=0, count=2, second=dict(heads=40000)), E_SHAPE),
                       (dict(count=2, second=dict(out=x + 256)), E_SHAPE)):
         assert call(**bad) == code, bad
     # nothing to do is no error, and strides of dimensions of one entry count for nothing
@@ -134,3 +134,34 @@ def test_append_rotary_refusals(ralib):
         assert call(**bad) == code, bad
     assert call(tokens=0) == OK and call(c=dict(batch=0)) == OK
     assert ralib.ringattn_paged_plan_destroy(h) == OK
+
+
+def test_native_calls_leave_what_is_unusual_to_the_general_way(ralib):
+    """Rotary positions, pages, and the paged calls with scores that are shaped or rows that turn (csrc/ringattn_calls.cpp): what is no device tensor of the
+    expected kind gives None, a wrong number of arguments is refused."""
+    from ringattention_amd import paged
+    calls = _lib.load_calls()
+    half = torch.float16
+    x = torch.zeros(1, 2, 16, 64, dtype=half)
+    r = rotary.Rotary(64, device="cpu")
+    for kind, n in ((16, 12), (17, 11), (18, 14)):
+        call = calls.Paged(1, 1, kind, 8, 2, 64, 16, 4, 64, 0, half, half, 30.0)
+        for wrong in (n - 1, n + 1):
+            with pytest.raises(TypeError):
+                call(*(None,) * wrong)
+        assert call(*(None,) * n) is None and call(*(x,) * (n - 1), None) is None
+    for bad in (19, 15, -1):
+        with pytest.raises(ValueError):
+            calls.Paged(1, 1, bad, 8, 2, 64, 16, 4, 64, 0, half, half)
+    turn = calls.Turn(1, r.address, r.address, 64, 0, 0, half)
+    pool = paged.PagePool(1, 2, 3, 16, device="cpu")
+    pages = calls.Pages(1, ctypes.addressof(pool._struct), 0, 0)
+    for call in (turn, pages):
+        for wrong in (6, 8):
+            with pytest.raises(TypeError):
+                call(*(None,) * wrong)
+        assert call(*(None,) * 7) is None and call(x, x, None, None, None, x, None) is None and call(*(x,) * 6, None) is None
+    for make, bad in ((calls.Turn, (0, 1, 1, 64, 0, 0, half)), (calls.Turn, (1, 0, 1, 64, 0, 0, half)), (calls.Turn, (1, 1, 1, 64, 0, 0, 1)), (calls.Turn, (1,)),
+                      (calls.Pages, (1, 1, 2, 0)), (calls.Pages, (0, 1, 0, 0)), (calls.Pages, (1, 0, 0, 0)), (calls.Pages, (1, 1))):
+        with pytest.raises((ValueError, TypeError)):
+            make(*bad)
