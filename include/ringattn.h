@@ -385,7 +385,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
                            int64_t q_head_stride, const float* lse, float* scores, void* stream);
 
 /*
- * Scores that are not the plain products, for models that have them so.  In this order: x = scale q k; softcap > 0: x = softcap tanh(x / softcap);
+ * Scores that are not the plain products, for models that have them so.  In this order: x = scale q k; softcap > 0, up to 1024: x = softcap tanh(x / softcap);
  * slopes: x -= slopes[head] |p - j| for the query at place p and the key at place j of the sequence.  And which keys a query sees: those in front of
  * prefix_lens[b], whatever else is said; else j <= p, where also j < sinks, or j >= first_keys[token] and, with a window, j > p - window.
  * With first_keys the tokens of several documents that lie one behind the other in a sequence see their own document's alone (the places of

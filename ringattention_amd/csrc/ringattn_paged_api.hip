@@ -133,9 +133,10 @@ int check_scoring(const ringattn_paged_plan* pl, const ringattn_paged_scoring* s
   if (!pl->p.causal && (s->slopes || s->prefix_lens || s->first_keys)) return RINGATTN_ERR_SHAPE;
   if (!aligned(s->slopes, 4) || !aligned(s->prefix_lens, 4) || !aligned(s->first_keys, 4)) return RINGATTN_ERR_ALIGN;
   if (s->softcap > 0.f) {
+    // A capped score is off by some 2^-22 of the cap, which is to stay below the roundings of a 16-bit output; and what leaves nothing of any score, or
+    // takes 32 bits past their range, is no cap.
     const double in = 2. * 1.4426950408889634 * pl->scale / s->softcap, outer = s->softcap * 1.4426950408889634;
-    // (a cap that leaves nothing of any score, or that 32 bits do not tell from none)
-    if (!(in < 1e30 && in > 1e-30 && outer < 1e30 && outer > 1e-30)) return RINGATTN_ERR_SHAPE;
+    if (!(s->softcap <= 1024.f && in < 1e30 && in > 1e-30 && outer > 1e-30)) return RINGATTN_ERR_SHAPE;
     out->cap_in = (float)in;
     out->cap_out = (float)outer;
   }

@@ -55,7 +55,7 @@ class PagedAttention:
 
     `window` > 0: a token sees the last `window` tokens up to itself and the first `sinks` of the sequence.  `causal=False`:
     it sees every cached token; `partials`: out is float32, a partial (O, LSE) for api.merge -- together, for a sequence whose cache is
-    spread over several pools or GPUs.  `softcap` > 0: a score x becomes softcap tanh(x / softcap); `slopes`, float32 [heads] on the device: less
+    spread over several pools or GPUs.  `softcap` > 0, up to 1024: a score x becomes softcap tanh(x / softcap); `slopes`, float32 [heads] on the device: less
     slopes[head] times the distance of query and key (causal plans); for forward() and weights().  `keep_present`: evict() keeps no token whose page is not there.  `workspace`: a (device
     address, bytes) pair the caller owns and keeps alive, instead of an allocation by the plan.  It holds zeros when the plan is made
     (torch.zeros, not torch.empty): workgroups that share a row count themselves in it, and leave it at 0.  One call at a time, and replays
@@ -77,8 +77,8 @@ class PagedAttention:
                                           self.max_tokens, int(bool(causal)), int(window), int(sinks),
                                           (FLAG_PAGED_PARTIALS if partials else 0) | (FLAG_PAGED_KEEP_PRESENT if keep_present else 0))
         self.softcap, self.slopes = float(softcap), slopes
-        if not (0 <= self.softcap < float("inf")):
-            raise ValueError("softcap must be 0 or a positive number")
+        if not 0 <= self.softcap <= 1024:
+            raise ValueError("softcap must be 0 or a positive number up to 1024")
         if slopes is not None:
             if not causal:
                 raise ValueError("slopes are for causal plans")

@@ -88,6 +88,19 @@ def test_the_other_types(dtype, dim):
             check(ref.Case(**SCORES[scores](b), **b, dtype=dtype, dim=dim, sigma=1.5, seed=9))
 
 
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 200.0, 1024.0])
+def test_caps_small_and_large(cap):
+    for b in ("tokens", "many"):
+        check(ref.Case(cap=cap, **BATCHES[b], dtype="fp16", dim=64, sigma=3.0, seed=11))
+
+
+def test_slopes_of_either_sign():
+    """And of a size at which a few keys are all that counts."""
+    for b in ("few", "many"):
+        check(ref.Case(slopes=[-0.25, 8.0, 0.0, -1e-3], **dict(BATCHES[b], heads=4), seed=13))
+        check(ref.Case(slopes=[-0.25, 8.0, 0.0, -1e-3], prefix=[40] * len(BATCHES[b]["lens"]), **dict(BATCHES[b], heads=4), seed=14))
+
+
 @pytest.mark.parametrize("n", range(6))
 def test_first_keys_of_any_kind(n):
     """Out of order, negative, behind the token itself (which then sees nothing but a prefix), behind the end."""
@@ -316,7 +329,7 @@ def test_refusals():
     for bad in (dict(prefix_lens=ints[:1]), dict(first_keys=ints[:4])):
         with pytest.raises(ValueError, match="causal"):
             open_plan.forward(q, k, v, *seqs, **bad)
-    for bad in (dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(slopes=torch.zeros(3, device="cuda")),
+    for bad in (dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=2000.0), dict(slopes=torch.zeros(3, device="cuda")),
                 dict(slopes=torch.zeros(4)), dict(slopes=torch.zeros(4, device="cuda"), causal=False)):
         with pytest.raises(ValueError):
             paged.PagedAttention(4, 128, kv_heads=2, dtype="bf16", page_size=16, **bad)

@@ -29,7 +29,8 @@ def test_scoring_refusals(ralib):
         return a
 
     assert both() == OK and both(softcap=30.0, slopes=x, prefix_lens=x, first_keys=x) == OK and both(causal=0, softcap=30.0) == OK
-    for bad in (float("nan"), float("inf"), -1.0, 1e-38, 3e38):
+    assert both(softcap=1024.0) == OK and both(softcap=1e-6) == OK
+    for bad in (float("nan"), float("inf"), -1.0, 1e-38, 3e38, 1025.0):
         assert both(softcap=bad) == E_SHAPE, bad
     for bad in ("slopes", "prefix_lens", "first_keys"):
         assert both(causal=0, **{bad: x}) == E_SHAPE and both(**{bad: x + 2}) == E_ALIGN
