@@ -192,7 +192,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) sacc = E::mma(*(const s16x8*)(ks_lds + koff(ks)), qf[ks], sacc);
   };
-  auto mask_tile = [&](int t) {
+  auto mask_scores = [&](f32x16& sacc, int t) {
     if (!may_be_masked(t)) return;
     const int key0 = first_key(t), gone = gone_of(t), half = fresh(lane) >> 5;
     const Sight x = sight();
@@ -206,8 +206,15 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
     for (int e = 0; e < 16; ++e)
       sacc[e] = hidden(x, key0, gone, e, half) ? -INFINITY : sacc[e];
   };
+  auto mask_tile = [&](int t) { mask_scores(sacc, t); };
+  // ... of a scored call, shaped first, so that a hidden one is -inf and not minus the cap
+  auto mask_scored = [&](f32x16& sacc, int t) {
+    // (of a prefix, rows may see keys that come behind them)
+    if ((SC & kSloped) && p.s.prefix > 0 && t >= t_up) turn_slopes(sacc, slope, first_key(t) + 4 * h - before - fresh(token), 1.f);
+    mask_scores(sacc, t);
+  };
   // The reference moves when some row's tile maximum is far above it (or it is unset): until then exponentials may exceed 1, by 2^kLazyLog2.
-  auto move_reference = [&]() {
+  auto move_reference_of = [&](const f32x16& sacc) {
     float m0 = m, m1 = m;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
@@ -228,16 +235,9 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   };
   // P = exp2(S k2 - m k2); the sums from the unrounded values, the operands of the next product rounded to the storage type: no more than
   // the output's own rounding
-  // Scored: the scores of tile t have been shaped, and are masked now, so that a hidden one is -inf and not minus the cap.
   auto softmax_phase = [&](int t, bool may_hide) {
-    if constexpr (SC != 0) {
-      if (may_hide) {
-        // (of a prefix, rows may see keys that come behind them)
-        if ((SC & kSloped) && p.s.prefix > 0 && t >= t_up) turn_slopes(sacc, slope, first_key(t) + 4 * h - before - fresh(token), 1.f);
-        mask_tile(t);
-      }
-    }
-    move_reference();
+    if (SC != 0 && may_hide) mask_scored(sacc, t);
+    move_reference_of(sacc);
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
       typename E::vec8 pv;
@@ -306,52 +306,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   auto shape = [&](int t) {
     if constexpr (kShapeSteps<SC> > 0) shape_scores<SC>(sacc, a.x, a.scale_log2, slope, first_key(t) + 4 * h - before - token);
   };
-  // Where scores are shaped, the products go the other way round, S(t+1) first, which is shaped in place while O += P(t) V(t) is on the matrix cores.
-  auto shaping_phase = [&](int t, int vslot, int kslot) __attribute__((always_inline)) {
-    constexpr int AHEAD = 4, STEPS = kShapeSteps<SC>, EACH = (STEPS + 2 * DB - 1) / (2 * DB);
-    const float unit = shape_unit<SC>(a.x, a.scale_log2), at = slope * (float)(first_key(t + 1) + 4 * h - before - token);
-    phase_fence();
-    const unsigned char* vs_lds = smem + (NBUF + vslot) * TILE;
-    const unsigned char* ks_lds = smem + kslot * TILE;
-    s16x8 vfr[2 * DB], kfr[KS];
-    auto read_k = [&](int ks) { kfr[ks] = *(const s16x8*)(ks_lds + koff(ks)); };
-    auto read_v = [&](int f) {
-      const unsigned char* src = vs_lds + 16 * (f / DB) * ROWB + voff[f % DB];
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src + 8 * ROWB));
-      vfr[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    auto read = [&](int i) {  // fragments in the order of their MFMAs
-      if (i < KS) read_k(i);
-      else if (i < KS + 2 * DB) read_v(i - KS);
-    };
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) read(i);
-    phase_fence();
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      sacc = E::mma(kfr[ks], qf[ks], sacc);
-      phase_fence();
-      read(AHEAD + ks);
-      phase_fence();
-    }
-#pragma unroll
-    for (int f = 0; f < 2 * DB; ++f) {
-      oacc[f % DB] = E::mma(vfr[f], pf[f / DB], oacc[f % DB]);
-      phase_fence();
-      read(AHEAD + KS + f);
-      phase_fence();
-#pragma unroll
-      for (int i = f * EACH; i < (f + 1) * EACH && i < STEPS; ++i) {
-        shape_step<SC>(sacc, i, a.x, unit, slope, at);
-        phase_fence();
-      }
-    }
-  };
-  auto mfma_phase = [&](int t, int vslot, int kslot) __attribute__((always_inline)) {
-    if constexpr (kShapeSteps<SC> > 0) return shaping_phase(t, vslot, kslot);
+  auto mfma_phase = [&](int vslot, int kslot) __attribute__((always_inline)) {
     phase_fence();
     const unsigned char* vs_lds = smem + (NBUF + vslot) * TILE;
     const unsigned char* ks_lds = smem + kslot * TILE;
@@ -420,13 +375,13 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       if ((SLOT & 1) == 0) ring_barrier();
       if (SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
-      if (!SECOND) mfma_phase(t, SLOT, (SLOT + 1) & 3);
+      if (!SECOND) mfma_phase(SLOT, (SLOT + 1) & 3);
       else softmax_phase(t, false);
       phase_fence();
       if (!SECOND) issue_loads(t, (SLOT & 1) == 0);
       phase_fence();
       if (!SECOND) softmax_phase(t + 1, false);
-      else mfma_phase(t, SLOT, (SLOT + 1) & 3);
+      else mfma_phase(SLOT, (SLOT + 1) & 3);
       phase_fence();
     };
     auto masked_block = [&](int t) __attribute__((always_inline)) {
@@ -440,12 +395,12 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       if (odd_values(t)) {
         pv_by_key(t, t & 3);
         qk((t + 1) & 3);
-        shape(t + 1);
       } else {
-        mfma_phase(t, t & 3, (t + 1) & 3);
+        mfma_phase(t & 3, (t + 1) & 3);
       }
       phase_fence();
       if (SC == 0) mask_tile(t + 1);
+      else shape(t + 1);
       if (!SECOND) {
         issue_loads(t, (t & 1) == 0);
         if (t + 1 < n_tiles) weights_of(t + 1);  // (the scores past the last tile are of nothing)
@@ -475,48 +430,107 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
 #pragma unroll 1
     for (; t < n_tiles; ++t) masked_block(t);
   };
-  // The walk of a scored call, whose tiles may be masked anywhere: those that may be in front, those that are not, and the others, all of them four at a
-  // time with their slots at compile time.  Nothing is looked at on the way: a V that is no number where some row does not see it makes that row's sums no numbers, which is looked
-  // for at the end, and then the workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, in every 64 one that sees itself
-  // alone, which masks all tiles: 409 us; 545 with a look at each tile, its slots worked out and both ways of the products in the loop; with no masks 278.)
-  auto scored_walk = [&](auto second_c) __attribute__((always_inline)) {
-    constexpr bool SECOND = decltype(second_c)::value;
-    auto block = [&](int t, int slot, bool plain, bool last) __attribute__((always_inline)) {
-      auto issue_loads = [&]() __attribute__((always_inline)) {
-        if ((slot & 1) == 0) {
-          issue_k(t + 3);
-          issue_k(t + 4);
-        } else {
-          issue_v(t + 1);
-          issue_v(t + 2);
-        }
-      };
-      if ((slot & 1) == 0) ring_barrier();
-      if (SECOND) {
-        issue_loads();
-        phase_fence();
-        if (plain) softmax_phase(t, false);
-        else weights_of(t);
+  // The walk of a scored call.  A wave alone issues a vector instruction every eight cycles or so, an exponential every sixteen -- half of what its SIMD
+  // can --, and what it does beside its own matrix products is for nothing: so block t has the exponentials of tile t beside S(t+1) = K(t+1) Q^T, and
+  // what shapes those scores beside O += P(t) V(t); then the reference.  (In two phases against each other, as above, and so: 4096 tokens over 32 K, 32/8
+  // heads x 128, sloped 1.11 and 1.08 of the plain call's time, capped 1.31 and 1.32, of which power is the bound: 1.9 GHz, vector pipe at work 67 % of the time,
+  // matrix cores 39; a ragged batch with slopes 240 us and 227; documents of 1365 in 16 K tokens 159 and 153; and half the code.)
+  // Tiles that may be masked are in front and at the end, those between are not looked at; all four at a time, their slots at compile time.  Nor is V looked
+  // at on the way: one that is no number where some row does not see it makes that row's sums no numbers, which is looked for at the end, and then the
+  // workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, in every 64 one that sees itself alone, which masks all tiles: 381 us; 545 with a
+  // look at each tile, its slots worked out and both ways of the products in the loop; with no masks 271.)
+  auto scored_walk = [&]() __attribute__((always_inline)) {
+    f32x16 spare;  // the other tile's scores
+    auto weigh_step = [&](f32x16& s, int i) __attribute__((always_inline)) {
+      if (i < 16) s[i] = __builtin_fmaf(s[i], k2, -ms);
+      if (i >= 2 && i < 18) s[i - 2] = __builtin_amdgcn_exp2f(s[i - 2]);
+      if (i >= 5 && i < 21) ls[(i - 5) & 1] += s[i - 5];
+      if (i >= 6 && i < 22 && (i & 1)) {
+        const int e = i - 7;
+        typename E::vec8 v = __builtin_bit_cast(typename E::vec8, pf[e >> 3]);
+        v[e & 7] = (typename E::type)s[e];
+        v[(e + 1) & 7] = (typename E::type)s[e + 1];
+        pf[e >> 3] = __builtin_bit_cast(s16x8, v);
+      }
+    };
+    constexpr int kWeighSteps = 23;  // (the last pair is packed in step 22)
+    // block t: `now` has the scores of tile t, `next` gets those of tile t + 1
+    auto block = [&](int t, int slot, f32x16& now, f32x16& next, bool plain, bool last) __attribute__((always_inline)) {
+      constexpr int AHEAD = 4, STEPS = kShapeSteps<SC>, EACH_K = (kWeighSteps + KS - 1) / KS, EACH_V = (STEPS + 2 * DB - 1) / (2 * DB);
+      const int kslot = (slot + 1) & 3;
+      if ((slot & 1) == 0) {
+        ring_barrier();
+        issue_k(t + 3);
+        issue_k(t + 4);
+      } else {
+        issue_v(t + 1);
+        issue_v(t + 2);
       }
       phase_fence();
-      if (plain || !(passed_over(t) && passed_over(t + 1))) mfma_phase(t, slot, (slot + 1) & 3);
-      phase_fence();
-      if (!SECOND) {
-        issue_loads();
+      if (!plain && passed_over(t) && passed_over(t + 1)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) next[e] = -INFINITY;
+      } else {
+        const float unit = shape_unit<SC>(a.x, a.scale_log2), at = slope * (float)(first_key(t + 1) + 4 * h - before - token);
+        const unsigned char* vs_lds = smem + (NBUF + slot) * TILE;
+        const unsigned char* ks_lds = smem + kslot * TILE;
+        s16x8 vfr[2 * DB], kfr[KS];
+        auto read = [&](int i) {  // fragments in the order of their MFMAs
+          if (i < KS) {
+            kfr[i] = *(const s16x8*)(ks_lds + koff(i));
+          } else if (i < KS + 2 * DB) {
+            const int f = i - KS;
+            const unsigned char* src = vs_lds + 16 * (f / DB) * ROWB + voff[f % DB];
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src + 8 * ROWB));
+            vfr[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) read(i);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) next[e] = 0.f;
         phase_fence();
-        if (plain) softmax_phase(t + 1, false);
-        else if (!last || t + 1 < n_tiles) weights_of(t + 1);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          next = E::mma(kfr[ks], qf[ks], next);
+          phase_fence();
+          read(AHEAD + ks);
+          phase_fence();
+#pragma unroll
+          for (int i = ks * EACH_K; i < (ks + 1) * EACH_K && i < kWeighSteps; ++i) {
+            weigh_step(now, i);
+            phase_fence();
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < 2 * DB; ++f) {
+          oacc[f % DB] = E::mma(vfr[f], pf[f / DB], oacc[f % DB]);
+          phase_fence();
+          read(AHEAD + KS + f);
+          phase_fence();
+#pragma unroll
+          for (int i = f * EACH_V; i < (f + 1) * EACH_V && i < STEPS; ++i) {
+            shape_step<SC>(next, i, a.x, unit, slope, at);
+            phase_fence();
+          }
+        }
+      }
+      if (plain || !last || t + 1 < n_tiles) {
+        if (!plain) mask_scored(next, t + 1);
+        move_reference_of(next);
       }
       phase_fence();
     };
     auto four = [&](int t, auto plain_c) __attribute__((always_inline)) {
       constexpr bool PLAIN = decltype(plain_c)::value;
-      block(t, 0, PLAIN, false);
-      block(t + 1, 1, PLAIN, false);
-      block(t + 2, 2, PLAIN, false);
-      block(t + 3, 3, PLAIN, !PLAIN);
+      block(t, 0, sacc, spare, PLAIN, false);
+      block(t + 1, 1, spare, sacc, PLAIN, false);
+      block(t + 2, 2, sacc, spare, PLAIN, false);
+      block(t + 3, 3, spare, sacc, PLAIN, !PLAIN);
     };
-    if (!SECOND) weights_of(0);
+    mask_scored(sacc, 0);
+    move_reference_of(sacc);
     int t = 0;
     const int masked_first = min((max(t_low, 0) + 3) & ~3, n_tiles & ~3);
 #pragma unroll 1
@@ -538,7 +552,8 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
 #pragma unroll 1
     for (; t < n_tiles; ++t) {
       hold_for(t + 4);
-      block(t, t & 3, false, true);
+      block(t, t & 3, sacc, spare, false, true);
+      sacc = spare;
     }
   };
   auto begin = [&]() {
@@ -562,8 +577,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
       else walk(std::true_type{});
       end();
     } else {
-      if (wave < WAVES / 2) scored_walk(std::false_type{});
-      else scored_walk(std::true_type{});
+      scored_walk();
       end();
       float none[4] = {0.f, 0.f, 0.f, 0.f};  // not 0 where a sum is no number
 #pragma unroll
