@@ -209,12 +209,18 @@ struct Firsts {
   int least, most;
 };
 static __device__ __forceinline__ Firsts firsts_of_lanes(int least, int most) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    least = min(least, __shfl_xor(least, m));
-    most = max(most, __shfl_xor(most, m));
-  }
-  return Firsts{__builtin_amdgcn_readfirstlane(least), __builtin_amdgcn_readfirstlane(most)};
+  auto meet = [&](auto ctrl, auto rows) {  // (as wave_scan; a lane without a partner meets itself)
+    least = min(least, __builtin_amdgcn_update_dpp(least, least, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    most = max(most, __builtin_amdgcn_update_dpp(most, most, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using all = std::integral_constant<int, 0xf>;
+  meet(std::integral_constant<int, 0x111>{}, all{});
+  meet(std::integral_constant<int, 0x112>{}, all{});
+  meet(std::integral_constant<int, 0x114>{}, all{});
+  meet(std::integral_constant<int, 0x118>{}, all{});
+  meet(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  meet(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return Firsts{__builtin_amdgcn_readlane(least, 63), __builtin_amdgcn_readlane(most, 63)};
 }
 static __device__ __forceinline__ Firsts firsts_of(const Scoring& x, const Seq& s, int i0, int i1) {
   if (!x.first) return Firsts{0, 0};
@@ -260,6 +266,24 @@ template <bool MERGE, int SC> static __device__ __forceinline__ bool find_place(
       load_of<true>(a, s, tiles, keys);
       splits = a.many_cut ? max(1, (int)ceilf(keys / share)) : 1;
     }
+    int b = b0 + lane;
+    // Of a scored call of up to 64 sequences, those first whose shortest row tile sees most: rows of long contexts that start when all others are done
+    // are waited for.  (Prompts of 4 K and 1 K beside 1 K over 4 K and single tokens, 16 heads x 128, slopes: 232 us in the sequences' order, and 212.)
+    if constexpr (SC != 0) {
+      if (a.c.batch <= 64 && a.c.batch > 1) {
+        const int sees = tiles > 0 ? max(s.len - s.n, 0) : -1;
+        int rank = 0;
+        for (int l = 0; l < 64; ++l) {
+          const int other = __builtin_amdgcn_readlane(sees, l);
+          rank += other > sees || (other == sees && l < lane);
+        }
+        auto to_rank = [&](int x) { return __builtin_amdgcn_ds_permute(4 * rank, x); };
+        s = Seq{to_rank(s.len), to_rank(s.start), to_rank(s.n), to_rank(s.prefix)};
+        tiles = to_rank(tiles);
+        splits = to_rank(splits);
+        b = to_rank(b);
+      }
+    }
     const int shares = tiles * splits, slots = splits > 1 ? shares : 0, units = !MERGE ? shares : splits > 1 ? tiles : 0;
     const int upto = wave_scan(units), slots_upto = wave_scan(slots);
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(before + upto > place);
@@ -267,7 +291,7 @@ template <bool MERGE, int SC> static __device__ __forceinline__ bool find_place(
       const int l = __builtin_ctzll(beyond);
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
       p.s = Seq{of(s.len), of(s.start), of(s.n), SC ? of(s.prefix) : 0};
-      p.b = b0 + l;
+      p.b = of(b);
       p.splits = of(splits);
       const int r = place - (before + of(upto) - of(units));
       const int first = slots_before + of(slots_upto) - of(slots);

@@ -34,15 +34,22 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   if (!find_place<false, SC>(a, unit, p)) return;
   const int rows = p.s.n * a.group;
   const int r0 = p.tile * BM, r_last = min(r0 + BM, rows) - 1;
+  // this lane's row; rows beyond the range read the last valid one
+  const int row = min(r0 + 32 * wave + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
+  const int before = p.s.len - p.s.n;
+  s16x8 qf[KS];
+  auto load_q = [&]() {
+    const char* qrow = a.q + (p.s.start + token) * a.q_ts + q_head * a.q_hs + h * 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(qrow + ks * 32);
+  };
+  if (SC != 0) load_q();  // (on its way while documents are looked up)
   const int i_first = quotient(r0, a.by_group), i_last = quotient(r_last, a.by_group);
   const Firsts firsts = SC ? firsts_of(a.x, p.s, i_first, i_last) : Firsts{0, 0};
   const Keys keys = keys_of(p.s, i_first, i_last, a.causal, a.window, a.sinks, firsts.least);
   const int u_begin = (int)((int64_t)p.split * keys.count / p.splits);
   const int n_tiles = (int)((int64_t)(p.split + 1) * keys.count / p.splits) - u_begin;  // of this share: tile t is tile u_begin + t
 
-  // this lane's row; rows beyond the range read the last valid one
-  const int row = min(r0 + 32 * wave + n, r_last), token = quotient(row, a.by_group), q_head = head * a.group + row - token * a.group;
-  const int before = p.s.len - p.s.n;
   // of a scored call: the first key that this lane's row sees, its head's slope; keys in front of `keep` are seen by rows that come behind them, whatever window and documents say
   const int first = SC && a.x.first ? clamped(a.x.first[p.s.start + token], 0, p.s.len) : 0;
   const float slope = (SC & kSloped) ? a.x.slopes[q_head] * 1.4426950408889634f : 0.f;
@@ -68,28 +75,26 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
     x.low = low >= 0 ? __builtin_amdgcn_readfirstlane(tile_of(low / BN + 1)) : 0;
     return x;
   };
-  const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31, SC && a.x.first ? firsts_of_lanes(first, first).most : 0), every = clear_of(r0, r_last, firsts.most);
-  const int t_up = mine.up, t_low = mine.low;
+  const Firsts of_wave = SC && a.x.first ? firsts_of_lanes(first, first) : Firsts{0, 0};
+  const Clear mine = clear_of(r0 + 32 * wave, r0 + 32 * wave + 31, of_wave.most), every = clear_of(r0, r_last, firsts.most);
+  // (a wave without rows, at the end of a sequence, only brings its part of the tiles in a scored call)
+  const bool idle = SC != 0 && r0 + 32 * wave > r_last;
+  const int t_up = idle ? 0 : mine.up, t_low = idle ? 0 : mine.low;
   // Of a scored call: tiles that no row of this wave sees -- those of the documents that other rows of the workgroup are of -- are passed over.
   struct Seen {
     int from, to;
   };
   auto seen_of = [&]() {
-    if constexpr (SC == 0) return Seen{0, 0};
+    if (SC == 0 || idle) return Seen{0, 0};
     const int i0 = quotient(min(r0 + 32 * wave, r_last), a.by_group), i1 = quotient(min(r0 + 32 * wave + 31, r_last), a.by_group);
-    const int low = max(a.window > 0 ? before + i0 + 1 - a.window : 0, a.x.first ? firsts_of_lanes(first, first).least : 0);
+    const int low = max(a.window > 0 ? before + i0 + 1 - a.window : 0, of_wave.least);
     const int lim = max(p.s.prefix, a.causal ? min(p.s.len, before + i1 + 1) : p.s.len);
     return Seen{__builtin_amdgcn_readfirstlane(tile_of(low / BN)), __builtin_amdgcn_readfirstlane(tile_of((lim + BN - 1) / BN))};
   };
   const Seen seen_tiles = seen_of();
   auto passed_over = [&](int t) { return SC != 0 && ((t < seen_tiles.from && first_key(t) >= keep) || t >= seen_tiles.to); };
 
-  s16x8 qf[KS];
-  {
-    const char* qrow = a.q + (p.s.start + token) * a.q_ts + q_head * a.q_hs + h * 16;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const s16x8*)(qrow + ks * 32);
-  }
+  if (SC == 0) load_q();
   // the 1 KB piece of a tile this wave loads: all waves a piece of K and of V each (d = 128), or waves 0-3 the K tile and waves 4-7 the V
   // tile (d = 64)
   const int piece = PIECES == WAVES ? wave : wave & (PIECES - 1);
@@ -467,10 +472,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
         issue_v(t + 2);
       }
       phase_fence();
-      if (!plain && passed_over(t) && passed_over(t + 1)) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) next[e] = -INFINITY;
-      } else {
+      if (plain || !(passed_over(t) && passed_over(t + 1))) {
         const float unit = shape_unit<SC>(a.x, a.scale_log2), at = slope * (float)(first_key(t + 1) + 4 * h - before - token);
         const unsigned char* vs_lds = smem + (NBUF + slot) * TILE;
         const unsigned char* ks_lds = smem + kslot * TILE;
@@ -516,7 +518,10 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
           }
         }
       }
-      if (plain || !last || t + 1 < n_tiles) {
+      if (!plain && passed_over(t + 1)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) next[e] = -INFINITY;
+      } else if (plain || !last || t + 1 < n_tiles) {
         if (!plain) mask_scored(next, t + 1);
         move_reference_of(next);
       }
