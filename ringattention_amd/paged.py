@@ -76,8 +76,8 @@ class PagedAttention:
         self.params = RingattnPagedParams(self.dim, self.heads, int(kv_heads), code, float(softmax_scale), self.page_size, self.max_batch,
                                           self.max_tokens, int(bool(causal)), int(window), int(sinks),
                                           (FLAG_PAGED_PARTIALS if partials else 0) | (FLAG_PAGED_KEEP_PRESENT if keep_present else 0))
-        self.softcap, self.slopes = float(softcap), slopes
-        if not 0 <= self.softcap <= 1024:
+        self._softcap, self._slopes = ctypes.c_float(softcap).value, slopes
+        if not 0 <= float(softcap) <= 1024 or (softcap and not self._softcap):   # (what is nothing in 32 bits would be no cap)
             raise ValueError("softcap must be 0 or a positive number up to 1024")
         if slopes is not None:
             if not causal:
@@ -93,6 +93,10 @@ class PagedAttention:
         calls = _lib.load_calls()
         self._call_type = calls.Paged if calls and self.device is not None else None
         self._native = {}
+
+    # (calls that are made in native code hold the one, and the other has been checked: a plan's own, not to be replaced)
+    softcap = property(lambda self: self._softcap)
+    slopes = property(lambda self: self._slopes)
 
     def _made(self, kind):
         entry = self.lib.addresses[("ringattn_paged_append", "ringattn_paged_fwd", "ringattn_paged_weights", "ringattn_paged_evict",
@@ -257,7 +261,7 @@ class PagedAttention:
             if rc is not None:
                 check(rc, "ringattn_paged_fwd")
                 return out, lse
-        elif out is not None and lse is not None and self._call_type and self.params.causal:
+        elif out is not None and lse is not None and self._call_type and (self.params.causal or prefix_lens is None and first_keys is None):
             rc = (self._native.get(4) or self._made(4))(q, k_cache, v_cache, page_table, kv_lens, q_starts, out, lse, self.slopes, prefix_lens, first_keys, stream)
             if rc is not None:
                 check(rc, "ringattn_paged_fwd_scored")
@@ -290,7 +294,7 @@ class PagedAttention:
             if rc is not None:
                 check(rc, "ringattn_paged_weights")
                 return scores
-        elif self._call_type and self.params.causal:
+        elif self._call_type and (self.params.causal or prefix_lens is None and first_keys is None):
             rc = (self._native.get(5) or self._made(5))(q, lse, k_cache, page_table, kv_lens, q_starts, scores, self.slopes, prefix_lens, first_keys, stream)
             if rc is not None:
                 check(rc, "ringattn_paged_weights_scored")

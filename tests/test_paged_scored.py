@@ -2,7 +2,10 @@
 import ctypes
 
 import numpy as np
+import pytest
+import torch
 
+from ringattention_amd import paged
 from ringattention_amd._lib import RingattnPagedCache, RingattnPagedScoring
 from test_paged import params
 
@@ -39,3 +42,20 @@ def test_scoring_refusals(ralib):
     assert ralib.ringattn_paged_weights_scored(plans[1], None, None, x, 0, 512, 64, x, x, None) == E_NULL
     for h in plans.values():
         assert ralib.ringattn_paged_plan_destroy(h) == OK
+
+
+def test_a_plan_keeps_its_scoring():
+    """A cap that 32 bits do not hold is refused, not left out; what a plan was made with is not replaced under its calls."""
+    memory = np.zeros(160 << 20, dtype=np.uint8)
+    x = memory.ctypes.data + (-memory.ctypes.data % 16)
+    make = lambda cap: paged.PagedAttention(8, 64, kv_heads=2, page_size=16, max_batch=4, max_tokens=64, softcap=cap, workspace=(x, (160 << 20) - 16))   # noqa: E731
+    for bad in (1e-50, -1e-50, -1.0, 1024.5, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            make(bad)
+    plan = make(30.0)
+    assert plan.softcap == 30.0 and plan.slopes is None
+    with pytest.raises(AttributeError):
+        plan.softcap = 50.0
+    with pytest.raises(AttributeError):
+        plan.slopes = torch.zeros(8)
+    plan.close()
