@@ -221,6 +221,9 @@ int ringattn_rotary_apply(const ringattn_rotary* rotary, int dim, int dtype, con
     a.heads += x.heads;
     if (a.heads > 65535) return RINGATTN_ERR_SHAPE;
   }
+  // Of two, neither's output has the other's rows.  (Which rows of two that lie between each other meet, strides of any kind would have to tell: what is in the
+  // same place is refused, the rest is the caller's.)
+  if (count == 2 && batch > 0 && tokens > 0 && (tensors[0].out == tensors[1].out || tensors[0].out == tensors[1].in || tensors[1].out == tensors[0].in)) return RINGATTN_ERR_SHAPE;
   a.heads0 = tensors[0].heads;
   a.tokens = tokens;
   a.positions = positions;

@@ -111,6 +111,22 @@ def test_apply_refusals(ralib):
     assert call(tokens=0, heads=1, in_head_stride=3) == OK
 
 
+def test_outputs_in_the_other_tensor_are_refused(ralib):
+    memory = np.zeros(1 << 20, dtype=np.uint8)
+    x = memory.ctypes.data + (-memory.ctypes.data % 16)
+    far, further = x + (1 << 18), x + (1 << 19)
+    r = RingattnRotary(64, 0, 0, 1.0, x)
+
+    def call(first, second):
+        rows = (RingattnRows * 2)(*(RingattnRows(i, o, 2, 2 * 5 * 64, 5 * 64, 64, 2 * 5 * 64, 5 * 64, 64) for i, o in (first, second)))
+        return ralib.ringattn_rotary_apply(ctypes.byref(r), 64, 0, rows, 2, 1, 5, None, 0, None)
+
+    assert call((x, far), (further, far)) == E_SHAPE        # one output for both
+    assert call((x, far), (far, further)) == E_SHAPE        # Q turned over K
+    assert call((x, far), (further, x)) == E_SHAPE          # K turned over Q
+    assert call((x, x), (x, x)) == E_SHAPE and call((x, x), (x, far)) == E_SHAPE
+
+
 def test_append_rotary_refusals(ralib):
     memory = np.zeros(160 << 20, dtype=np.uint8)
     x = memory.ctypes.data + (-memory.ctypes.data % 16)
