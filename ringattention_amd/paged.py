@@ -7,6 +7,10 @@ The calls of a step of a serving loop, for a ragged batch of sequences with some
     plan.weights(q, lse, k_cache, page_table, kv_lens, q_starts, scores)            what they gave to each cached token
     plan.evict(k_cache, v_cache, scores, page_table, kv_lens, kept_table, budget)   now and then: the tokens that drew most stay
 
+Of models with rotary positions, plan.append_rotary(rotary, q, k, v, ...) in place of append().  Capped scores and slopes of distance are a plan's
+(softcap, slopes), prefixes that all tokens see and documents one behind the other a call's (prefix_lens, first_keys).  PagePool keeps the page table
+on the device: forks, growth, releases, compaction.
+
 Tensors (device): k_cache, v_cache [pages, kv_heads, page_size, dim] (any strides that keep a row together, both alike); page_table int32
 [batch, pages of a sequence], -1 where there is none; kv_lens int32 [batch], tokens in the cache, the new ones among them; q_starts int32
 [batch + 1], where a sequence's new tokens begin; q, out [tokens, heads, dim], k, v [tokens, kv_heads, dim] (any strides that
