@@ -339,8 +339,10 @@ static int attend(ringattn_paged_plan* plan, const ringattn_paged_cache* cache, 
   a.many_cut = tiles > 0 && rows / rp::kManyRows * kv < (most >= 512 ? 4 * rp::kManyWorkgroups : rp::kManyWorkgroups);
   const int64_t places = tiles + (a.many_cut ? due : 0);
   // Workgroups of few rows first; of a sequence alone, whose rows are many if q is full, last, where they cost a full one next to nothing (us
-  // with and without them: 4096 tokens over 32 K, 32 heads 1867 and 1867; with a window of 1024, 8 KV heads 94.9 and 94.2).
-  a.few_begin = sequences == 1 ? (int)(places * kv) : 0;
+  // with and without them: 4096 tokens over 32 K, 32 heads 1867 and 1867; with a window of 1024, 8 KV heads 94.9 and 94.2).  Last in scored calls, too: the
+  // longest row tiles begin at once, and what is small fills the gaps at the end.  (Slopes, 16 heads, us with few rows first and last: prompts of 4 K
+  // and 1.3 K beside 1 K over 4 K and single tokens 195 and 183; two chunks over 4 K and single tokens 113 and 110; a chunk over 8 K beside 40 tokens over 3 K 128 and 130.)
+  a.few_begin = sequences == 1 || sc ? (int)(places * kv) : 0;
   const int64_t cut_tiles = tiles < due ? tiles : due;
   if (sc) RP_HIP(rp::launch_paged_scored(a, sc, plan->p.dtype, plan->p.dim, places, cut_tiles, stream));
   else RP_HIP(rp::launch_paged_attend(a, plan->p.dtype, plan->p.dim, places, cut_tiles, stream));
