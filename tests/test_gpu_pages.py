@@ -96,6 +96,18 @@ def test_large():
     c.compact()
 
 
+@pytest.mark.parametrize("pages", [4095, 4096, 4097, 20001, 32768, 32769, 36865])
+def test_compaction_of_one_to_ten_blocks(pages):
+    """Pools that every workgroup counts for itself, and those of a count beforehand; rows that are freed in front, between and at the end."""
+    b = Both(pages, 5, pages, heads=1, seed=pages, scores=False)
+    each = pages // 5
+    for gone in ([0], [2, 4], [1, 2, 3]):
+        b.update(None, [each * 16 - n for n in b.want.lens])
+        b.update([-1 if i in gone else i for i in range(5)], [-16 * 77 if i == 3 else 0 for i in range(5)])
+        b.compact()
+    b.compact()
+
+
 def test_edges():
     # the whole pool, to the last page, and one page too few
     b = Both(8, 3, 8)
