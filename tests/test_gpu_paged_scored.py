@@ -314,6 +314,22 @@ def test_streams_and_layouts():
     compare(lse, want_lse, tol_lse, "lse")
 
 
+def test_pages_past_32_bits():
+    """Pages behind the first 2^32 elements of a pool: the same bits as in a small one."""
+    c = ref.Case(lens=[300, 40, 90], news=[130, 1, 5], heads=4, kv_heads=2, dim=64, cap=8.0, slopes=slopes_of(4), prefix=[10, 0, 90], first=docs_of([300, 40, 90], [130, 1, 5], 64), seed=4, spare=0.0)
+    plan = plan_of(c)
+    slopes, prefix, first = c.given()
+    table, lens, starts = sequences(c)
+    out, lse = plan.forward(c.q.cuda(), c.k.cuda(), c.v.cuda(), table, lens, starts, prefix_lens=prefix, first_keys=first)
+    scores = plan.weights(c.q.cuda(), lse, c.k.cuda(), table, lens, starts, torch.zeros(c.pages, 2, 16, device="cuda"), prefix_lens=prefix, first_keys=first)
+    more = 2 ** 21 + 5    # pages of 2 x 16 x 64 in front
+    k, v = (torch.cat((torch.zeros(more, *x.shape[1:], dtype=x.dtype, device="cuda"), x.cuda())) for x in (c.k, c.v))
+    far = torch.where(table >= 0, table + more, table)
+    out2, lse2 = plan.forward(c.q.cuda(), k, v, far, lens, starts, prefix_lens=prefix, first_keys=first)
+    scores2 = plan.weights(c.q.cuda(), lse2, k, far, lens, starts, torch.zeros(more + c.pages, 2, 16, device="cuda"), prefix_lens=prefix, first_keys=first)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2) and torch.equal(scores, scores2[more:]) and not scores2[:more].any()
+
+
 def test_refusals():
     c = ref.Case(lens=[40], news=[4], heads=4, kv_heads=2)
     q, k, v, seqs = c.q.cuda(), c.k.cuda(), c.v.cuda(), sequences(c)

@@ -222,6 +222,29 @@ def test_layers_that_go_by_one_table():
             call()
 
 
+def test_offsets_past_32_bits():
+    """Pages behind the first 2^32 elements: forks that are copied there and back, compaction to the front."""
+    pages = 2 ** 22 + 6    # of 16 x 64, one head
+    k, v = (torch.zeros(pages, 1, 16, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    scores = torch.zeros(pages, 1, 16, device="cuda")
+    pool = paged.PagePool(pages, 2, 4, 16)
+    pool.refs[:-4] = 1    # of the caller's own
+    pool.update(k, v, add=ints([20, 0]), scores=scores)
+    assert pool.page_table.tolist()[0] == [pages - 4, pages - 3, -1, -1]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for x in (k, v, scores):
+        x[-4:-2].copy_(torch.randn(x[-4:-2].shape, generator=g, device="cuda"))
+    kept = [x[-4:-2].clone() for x in (k, v, scores)]
+    pool.update(k, v, ints([0, 0]), ints([0, 3]), scores=scores)
+    assert pool.page_table.tolist()[1] == [pages - 4, pages - 2, -1, -1] and pool.refs[-4:].tolist() == [2, 1, 1, 0]
+    for x, want in zip((k, v, scores), kept):
+        assert torch.equal(x[-2], want[1]) and not x[-1].any()
+    pool.refs[5:-4] = 0
+    assert pool.compact(k, v, scores=scores).tolist() == [8] and pool.page_table.tolist() == [[5, 6, -1, -1], [5, 7, -1, -1]]
+    for x, want in zip((k, v, scores), kept):
+        assert torch.equal(x[5:7], want) and torch.equal(x[7], want[1])
+
+
 def test_copy_pages():
     g = torch.Generator(device="cuda").manual_seed(1)
     k, v = (torch.randn(9, 3, 32, 128, generator=g, device="cuda").half() for _ in range(2))

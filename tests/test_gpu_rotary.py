@@ -257,3 +257,28 @@ def test_append_pages_that_are_not_there_and_odd_starts():
             written = {(c.row(b, p), p % c.page) for b, p in places(c) if (b, p // c.page) not in table_fix}
             touched = (big[1][1:-1] != 3).any(dim=3).any(dim=1).cpu()
             assert {(i, j) for i in range(c.pages) for j in range(c.page) if touched[i, j]} <= written
+
+
+def test_offsets_past_32_bits():
+    """Rows behind the first 2^32 elements, and pages behind them: the same bits as near the beginning."""
+    r = Rotary(64, dtype="bf16")
+    n = 2 ** 26 + 5
+    x = torch.empty(n, 1, 64, dtype=torch.bfloat16, device="cuda")
+    x[-70:] = normal((70, 1, 64), torch.bfloat16, 50)
+    last, want = x[-70:].clone(), torch.arange(n - 70, n, dtype=torch.int32).cuda()
+    got = r.apply(last, positions=want)[0]
+    r.apply(x, q_out=x)
+    assert torch.equal(x[-70:], got)
+    del x
+    c = ref.Case(lens=[40], news=[40], heads=2, kv_heads=1, dim=64, seed=9)
+    pages = 2 ** 22 + 3    # of 16 x 64
+    k_cache, v_cache = (torch.zeros(pages, 1, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k, v = (normal((40, 1, 64), torch.bfloat16, 51 + i) for i in range(2))
+    plan = paged.PagedAttention(2, 64, kv_heads=1, dtype="bf16", page_size=16, max_batch=1, max_tokens=40)
+    table = torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32).cuda()
+    lens, starts = torch.tensor([40], dtype=torch.int32).cuda(), torch.tensor([0, 40], dtype=torch.int32).cuda()
+    plan.append_rotary(r, c.q.cuda(), k, v, k_cache, v_cache, table, lens, starts)
+    want = r.apply(k)[0]
+    at = torch.cat([torch.arange(16) + 16 * p for p in table[0].tolist()])[:40].cuda()
+    assert torch.equal(k_cache.view(-1, 64)[at], want[:, 0]) and torch.equal(v_cache.view(-1, 64)[at], v[:, 0])
+    assert not k_cache[:-3].any() and not v_cache[:-3].any()
