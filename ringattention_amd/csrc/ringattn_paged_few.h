@@ -31,7 +31,7 @@ struct Lanes {
     if (b0 + lane < a.c.batch) {
       s = seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr);
       news += (float)s.n;
-      load_of<false>(a, s, tiles, keys);
+      load_of<false, SC>(a, s, tiles, keys);
       if (tiles > 0) {
         most = max(most, keys);
         fewest = min(fewest, keys);

@@ -132,6 +132,17 @@ def test_long(lens, news):
     check(ref.Case(lens=lens, news=news, heads=4, kv_heads=1, first=docs_of(lens, news, 701), prefix=[100] * len(lens), page=128, seed=5))
 
 
+@pytest.mark.parametrize("more", [dict(window=200, sinks=40, prefix=[130, 0, 900]), dict(prefix=[0, 700, 3]), dict(window=33, prefix=[1100, 0, 0]), dict(sinks=0, window=500), {}])
+@pytest.mark.parametrize("docs", [0, 40, 333])
+def test_keys_that_no_row_sees(more, docs):
+    """Long contexts of which windows and documents leave little, of few rows and of many: what lies between the first keys and them is passed over."""
+    lens, news = [2600, 1900, 1300], [300, 140, 5]
+    first = docs_of(lens, news, docs) if docs else None
+    check(ref.Case(lens=lens, news=news, heads=4, kv_heads=2, dim=64, first=first, cap=9.0, slopes=[0.2, 0.01, -0.001, 0.0] if docs != 40 else None, page=32, seed=docs, **more))
+    first = [first[(7 * i) % len(first)] for i in range(len(first))] if docs else None    # in no order
+    check(ref.Case(lens=lens, news=news, heads=4, kv_heads=2, dim=64, first=first, cap=9.0, page=32, seed=docs + 1, **more))
+
+
 def test_packed_documents_are_sequences_of_their_own():
     """Documents one behind the other in one sequence and as sequences of a batch: the same, to the rounding of what is summed in which order."""
     sizes = [100, 33, 1, 257, 64, 130, 32, 7]
