@@ -27,7 +27,7 @@ constexpr int kFewRowsAlone = 128;
 // 187 tiles 109 and 127; four of 256 over 1 K, 1024 rows, 128 tiles 45 and 56.  8 heads, two chunks of 512 over 2 K, 64 tiles 34 and 23.
 constexpr int kFewRowsMore = 512, kFewMore = 96;
 constexpr int kFewWorkgroups = 256, kFewLeast = 16, kFewSmall = 32, kFewMerge = 16;     // see few_rows
-constexpr int kManyWorkgroups = 256, kManyLeast = 8, kMergeSharers = 4;  // see find_place, merge_many
+constexpr int kManyWorkgroups = 256, kManyLeast = 8, kManySaved = 12, kMergeSharers = 4;  // see find_place, merge_many
 constexpr int kFewSlots = 2 * kFewWorkgroups, kManySlots = 2 * kManyWorkgroups + 16;  // parts that there can be
 constexpr int kManyKeys = 128;      // keys of a workgroup of paged_weights_kernel
 constexpr int kWeightUnits = 2048;   // parts of rows that there can be, where it shares them out
@@ -272,6 +272,12 @@ template <bool MERGE, int SC> static __device__ __forceinline__ bool find_place(
       s = seq_of(a.c, b0 + lane, SC ? a.x.prefix : nullptr);
       load_of<true, SC>(a, s, tiles, keys);
       splits = a.many_cut ? max(1, (int)ceilf(keys / share)) : 1;
+      // Of a scored call no more shares than run at once, where there is that much to do, and none that leave a row tile less than kManySaved shorter: a part's
+      // way through memory and the putting together cost as much.  (Us with shares as those of plain calls and so, 32 heads on 4 x 128: chunks of 147 to 315 tokens
+      // in a window of 78 59 and 33, five sequences of some 1 K in documents of 50 65 and 29; prompts of 90 to 1000 tokens, 16 heads on 8, 73 and 59; four
+      // chunks of some 300 over 500 to 900, 16 heads on 4, 49 and 51; a prompt of 700 31 and 31.)
+      if (SC != 0 && share > (float)kManyLeast) splits = max(1, (int)(keys / share + 0.01f));
+      if (SC != 0 && (!a.many_cut || keys - (keys + splits - 1) / splits < kManySaved)) splits = 1;
     }
     int b = b0 + lane;
     // Of a scored call of up to 64 sequences, those first whose shortest row tile sees most: rows of long contexts that start when all others are done
