@@ -274,19 +274,20 @@ template <bool MERGE, int SC> static __device__ __forceinline__ bool find_place(
       splits = a.many_cut ? max(1, (int)ceilf(keys / share)) : 1;
       // Of a scored call no more shares than run at once, where there is that much to do, and none that leave a row tile less than kManySaved shorter: a part's
       // way through memory and the putting together cost as much.  (Us with shares as those of plain calls and so, 32 heads on 4 x 128: chunks of 147 to 315 tokens
-      // in a window of 78 59 and 33, five sequences of some 1 K in documents of 50 65 and 29; prompts of 90 to 1000 tokens, 16 heads on 8, 73 and 59; four
-      // chunks of some 300 over 500 to 900, 16 heads on 4, 49 and 51; a prompt of 700 31 and 31.)
+      // in a window of 78 41 and 29, five sequences of some 1 K in documents of 50 49 and 25; prompts of 90 to 1000 tokens, 16 heads on 8, 56 and 50; four
+      // chunks of some 300 over 500 to 900, 16 heads on 4, 37 and 43; a prompt of 700 31 and 31.)
       if (SC != 0 && share > (float)kManyLeast) splits = max(1, (int)(keys / share + 0.01f));
       if (SC != 0 && (!a.many_cut || keys - (keys + splits - 1) / splits < kManySaved)) splits = 1;
     }
     int b = b0 + lane;
     // Of a scored call of up to 64 sequences, those first whose shortest row tile sees most: rows of long contexts that start when all others are done
-    // are waited for.  (Prompts of 4 K and 1 K beside 1 K over 4 K and single tokens, 16 heads x 128, slopes: 232 us in the sequences' order, and 212.)
+    // are waited for.  (Prompts of 4 K and 1.3 K beside 1 K over 4 K and single tokens, 16 heads x 128, slopes: 198 us in the sequences' order, and 184; two
+    // chunks over 4 K, 16 heads on 4, 91 and 92, and 105 where every wave looks at 64 lanes in place of the sequences there are.)
     if constexpr (SC != 0) {
       if (a.c.batch <= 64 && a.c.batch > 1) {
         const int sees = tiles > 0 ? max(s.len - s.n, 0) : -1;
-        int rank = 0;
-        for (int l = 0; l < 64; ++l) {
+        int rank = max(lane - a.c.batch, 0);  // (lanes without a sequence stay behind)
+        for (int l = 0; l < a.c.batch; ++l) {
           const int other = __builtin_amdgcn_readlane(sees, l);
           rank += other > sees || (other == sees && l < lane);
         }

@@ -439,7 +439,7 @@ template <int DT, int D, int SC = 0> static __device__ __forceinline__ void many
   // can --, and what it does beside its own matrix products is for nothing: so block t has the exponentials of tile t beside S(t+1) = K(t+1) Q^T, and
   // what shapes those scores beside O += P(t) V(t); then the reference.  (In two phases against each other, as above, and so: 4096 tokens over 32 K, 32/8
   // heads x 128, sloped 1.11 and 1.08 of the plain call's time, capped 1.31 and 1.32, of which power is the bound: 1.9 GHz, vector pipe at work 67 % of the time,
-  // matrix cores 39; a ragged batch with slopes 240 us and 227; documents of 1365 in 16 K tokens 159 and 153; and half the code.)
+  // matrix cores 39; documents of 1365 in 16 K tokens 159 and 153; and half the code.)
   // Tiles that may be masked are in front and at the end, those between are not looked at; all four at a time, their slots at compile time.  Nor is V looked
   // at on the way: one that is no number where some row does not see it makes that row's sums no numbers, which is looked for at the end, and then the
   // workgroup walks again, looking.  (16 heads on 4, 8 K of 8 K tokens, in every 64 one that sees itself alone, which masks all tiles: 381 us; 545 with a
