@@ -527,7 +527,9 @@ int ringattn_rotary_apply(const ringattn_rotary* rotary, int dim, int dtype, con
 
 /*
  * ringattn_paged_append with rotary positions on the way: rows q [tokens, heads, dim] are turned into q_out (q itself, with the same strides, or a
- * tensor that lies elsewhere), those of k_new are turned into the cache, those of v_new go there as they are.  positions: [tokens] on the device;
+ * tensor that lies elsewhere), those of k_new are turned into the cache, those of v_new go there as they are.  Rows of q_out may lie between those of
+ * k_new and v_new, as a fused product's do, but not on them: where neither equal distances of tokens with room for all heads of both, nor equal
+ * distances of tokens and heads show that they do not, that is RINGATTN_ERR_SHAPE.  positions: [tokens] on the device;
  * NULL: a token's place in its sequence (of a sequence that ringattn_paged_evict has shortened, the places count the tokens that are left).
  * Rows of q_out behind the last sequence are left as they were; a token whose page is not there has its row of q_out all the same.
  */

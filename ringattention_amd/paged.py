@@ -224,7 +224,8 @@ class PagedAttention:
 
     def append_rotary(self, rotary, q, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores=None, positions=None, q_out=None, stream=None):
         """append() with rotary positions on the way (rotary.Rotary): K turned and V as it is into the cache, q [tokens, heads, dim] turned into q_out
-        (q itself for in place).  `positions` int32 [tokens]; None: a token's place in its sequence.  Returns q_out."""
+        (q itself for in place; not on rows of k or v, between which it may lie).  `positions` int32 [tokens]; None: a token's place in its sequence.
+        Returns q_out."""
         rotary.check(self.dim, self.torch_dtype)
         if q_out is not None and self._call_type:
             rc = (self._native.get(6) or self._made(6))(q, k, v, k_cache, v_cache, page_table, kv_lens, q_starts, scores, positions, q_out, rotary.address,
