@@ -137,7 +137,8 @@ class Rotary:
             if out.shape != t.shape:
                 raise ValueError(f"{name}_out must have shape {tuple(t.shape)}")
             out_strides = _rows(out, f"{name}_out", self.torch_dtype, self.dim)
-            made.append(RingattnRows(t.data_ptr(), out.data_ptr(), t.shape[1], *strides, *out_strides))
+            if t.shape[1]:   # (a tensor of no heads has no rows; the other one's turn all the same)
+                made.append(RingattnRows(t.data_ptr(), out.data_ptr(), t.shape[1], *strides, *out_strides))
             outs.append(out)
         four = q.dim() == 4
         batch, tokens = (q.shape[0], q.shape[2]) if four else (1, q.shape[0])
@@ -154,7 +155,7 @@ class Rotary:
         for t in outs + [k, positions, self.turns]:
             if t is not None and t.device != q.device:
                 raise ValueError("the tensors of a call must be on one device")
-        if batch and tokens and all(t.shape[1] for t, _, _ in given):
+        if batch and tokens and made:
             self._call(q.device, stream, made, batch, tokens, positions.data_ptr() if positions is not None else None, stride, inverse)
         return outs[0], outs[1] if len(outs) > 1 else None
 
