@@ -55,3 +55,26 @@ def test_on_each_other_is_refused():
     for out in (k, v):
         with pytest.raises(RuntimeError):
             plan.append_rotary(r, c.q.cuda(), k, v, c.k.cuda(), c.v.cuda(), c.table.cuda(), c.kv_lens().cuda(), c.starts.cuda(), q_out=out)
+
+
+@pytest.mark.parametrize("batch", [65, 1000, 4096])
+def test_as_many_sequences_as_a_plan_takes(batch):
+    """Single tokens, sequences without any and some with several, on a stream: the same bits as turning first and appending then."""
+    news = [(0, 1, 1, 1, 3, 1, 0)[i % 7] for i in range(batch)]
+    lens = [max(1, n) + (i * 29) % 40 for i, n in enumerate(news)]
+    c = ref.Case(dtype="fp16", dim=64, heads=2, kv_heads=1, lens=lens, news=news, spare=0.0, extra_rows=2)
+    r = Rotary(64, dtype="fp16", interleaved=True)
+    plan = paged.PagedAttention(2, 64, kv_heads=1, dtype="fp16", page_size=16, max_batch=batch, max_tokens=c.tokens)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn((c.tokens, 1, 64), generator=g, device="cuda").half() for _ in range(2))
+    q, seqs = c.q.cuda(), (c.table.cuda(), c.kv_lens().cuda(), c.starts.cuda())
+    pos = torch.tensor([n - m + i for n, m in zip(lens, news) for i in range(m)] + [0, 0], dtype=torch.int32).cuda()
+    want = [c.k.cuda(), c.v.cuda()]
+    want_q, turned = r.apply(q, k, pos)
+    plan.append(turned, v, *want, *seqs)
+    got, out = [c.k.cuda(), c.v.cuda()], torch.full_like(q, 3.0)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    plan.append_rotary(r, q, k, v, *got, *seqs, q_out=out, stream=stream)
+    stream.synchronize()
+    assert torch.equal(out[:-2], want_q[:-2]) and (out[-2:] == 3).all() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
