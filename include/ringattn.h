@@ -390,7 +390,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
  * prefix_lens[b], whatever else is said; else j <= p, where also j < sinks, or j >= first_keys[token] and, with a window, j > p - window.
  * With first_keys the tokens of several documents that lie one behind the other in a sequence see their own document's alone (the places of
  * their documents' first tokens: in any order, of any value).  Members that are 0 or NULL change nothing.  Places count the tokens that are in the cache, after
- * an eviction those that are left.  Slopes, prefixes and first keys are for causal plans.
+ * an eviction those that are left.  Slopes, prefixes and first keys are for causal plans.  A weight below 2^-126, the least normal number of 32 bits, counts as 0.
  */
 typedef struct ringattn_paged_scoring {
   float softcap;

@@ -167,8 +167,9 @@ int check_scoring(const ringattn_paged_plan* pl, const ringattn_paged_scoring* s
   if (!pl->p.causal && (s->slopes || s->prefix_lens || s->first_keys)) return RINGATTN_ERR_SHAPE;
   if (!aligned(s->slopes, 4) || !aligned(s->prefix_lens, 4) || !aligned(s->first_keys, 4)) return RINGATTN_ERR_ALIGN;
   if (s->softcap > 0.f) {
-    // A capped score is off by some 2^-22 of the cap, which is to stay below the roundings of a 16-bit output; and what leaves nothing of any score, or
-    // takes 32 bits past their range, is no cap.
+    // A capped score is off by up to 1.5 x 2^-22 of the cap (2^-22 for the last bits of exponential and reciprocal and the sum between them, the rest
+    // for the argument and the cap in 32 bits), and 2 x 2^-22 under slopes, whose sum is rounded where it is as large as two caps: up to 1024 no more than
+    // the rounding of an output of 16 bits, 2^-11.  And what leaves nothing of any score, or takes 32 bits past their range, is no cap.
     const double in = 2. * 1.4426950408889634 * pl->scale / s->softcap, outer = s->softcap * 1.4426950408889634;
     if (!(s->softcap <= 1024.f && in < 1e30 && in > 1e-30 && outer > 1e-30)) return RINGATTN_ERR_SHAPE;
     out->cap_in = (float)in;

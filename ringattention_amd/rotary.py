@@ -1,5 +1,6 @@
 """Rotary positions on top of the C ABI (ringattn_rotary_* in include/ringattn.h): Rotary, for the Q and K of a ring
-(apply), their gradients (apply with inverse=True), and the new tokens of a paged cache (paged.PagedAttention.append_rotary).
+(apply), gradients by what apply() returned to those by what it was given (apply with inverse=True, called by hand: no call here is part of autograd's
+graph), and the new tokens of a paged cache (paged.PagedAttention.append_rotary).
 
     rotary = Rotary(128, scaling="yarn", factor=8, trained=4096, dtype="bf16")
     q, k = rotary.apply(q, k, positions)                                    [batch, heads, tokens, dim], or [tokens, heads, dim]
@@ -120,7 +121,8 @@ class Rotary:
     def apply(self, q, k=None, positions=None, q_out=None, k_out=None, inverse=False, stream=None):
         """q, k: [batch, heads, tokens, dim] or both [tokens, heads, dim], of any strides that keep a row together.  `positions`: int32 [tokens] or
         [batch, tokens], of any sign; None: a token's number.  q_out, k_out: the tensor itself for in place.  `inverse`: turned back -- of
-        gradients by the outputs the gradients by the inputs.  Returns (q_out, k_out), k_out None without k."""
+        gradients by the outputs the gradients by the inputs.  Returns (q_out, k_out), k_out None without k.  Autograd does not see the call: what it
+        returns has no history, also where q and k require gradients, and tensors that it writes count no new version."""
         if q_out is not None and (k is None or k_out is not None) and self._native:
             rc = self._native(q, k, positions, q_out, k_out, inverse, stream)
             if rc is not None:
