@@ -508,7 +508,7 @@ int ringattn_rotary_turns(const double* radians, int n, uint64_t* turns);
 
 /* Rows [batch, heads, tokens, dim] by strides (elements, multiples of 8), and where they go: the tensor itself (out == in, with the same
  * strides) or one that lies elsewhere.  Of two tensors the output of neither has rows of the other: Q and K may lie between each other, as a fused
- * product's do, but not in the same place. */
+ * product's do, but not on each other, which is RINGATTN_ERR_SHAPE where they begin in the same place or equal strides show it. */
 typedef struct ringattn_rows {
   const void* in;
   void* out;

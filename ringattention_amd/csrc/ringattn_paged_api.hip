@@ -4,9 +4,7 @@
 #include "ringattn_paged.h"
 #include "ringattn_rotary.h"
 
-#include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <new>
@@ -92,38 +90,6 @@ int check_rows(const ringattn_paged_plan* pl, int tokens, int heads, int64_t ts,
   if (written && ((tokens > 1 && ts < dim) || (heads > 1 && hs < dim) || (tokens > 1 && heads > 1 && ts < heads_span && (double)hs < tokens_span)))
     return RINGATTN_ERR_SHAPE;
   return RINGATTN_OK;
-}
-// Rows of a call's own tensors: bytes from the first, elements between tokens and heads.
-struct RowsAt {
-  const void* at;
-  int64_t ts, hs;
-  int heads;
-};
-// Whether no row of the one tensor lies on a row of the other, as far as that can be told: they lie apart; or a token's rows do, modulo the distance of
-// tokens, which is the same for both (a fused projection's Q, K and V); or both distances are the same and no two rows come within dim of each other.
-bool rows_apart(const RowsAt& a, const RowsAt& b, int tokens, int dim) {
-  const double fa = (double)(uintptr_t)a.at, fb = (double)(uintptr_t)b.at;
-  auto bytes = [&](const RowsAt& x) { return 2. * ((double)(tokens - 1) * (double)x.ts + (double)(x.heads - 1) * (double)x.hs + dim); };
-  if (fa + bytes(a) <= fb || fb + bytes(b) <= fa) return true;
-  const int64_t d = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at) / 2;  // elements from a's first row to b's
-  const int64_t none = INT64_MAX / 4;                                  // the distance of what there is one of
-  if (tokens > 1 && (a.ts != b.ts || a.ts == 0)) return false;
-  const int64_t ts = tokens > 1 ? a.ts : none, hs = a.heads > 1 ? a.hs : b.heads > 1 ? b.hs : none;
-  auto block = [&](const RowsAt& x) { return x.heads > 1 ? (x.heads - 1) * x.hs + dim : dim; };  // of a token
-  const int64_t from = (d % ts + ts) % ts;                                                        // where b's begins in a's distance of tokens
-  if (from >= block(a) && from + block(b) <= ts) return true;
-  if ((a.heads > 1 && b.heads > 1 && a.hs != b.hs) || hs == 0) return false;
-  // the rows that come nearest: so many tokens and heads of a's further on, the larger distance first
-  const bool by_token = ts > hs;
-  const int64_t large = by_token ? ts : hs, small = by_token ? hs : ts;
-  auto in_range = [&](int64_t n, bool of_tokens) { return of_tokens ? n > -tokens && n < tokens : n > -b.heads && n < a.heads; };
-  for (int64_t i = d / large - 2; i <= d / large + 2; ++i) {
-    if (!in_range(i, by_token)) continue;
-    const int64_t left = d - i * large;
-    for (int64_t j = left / small - 1; j <= left / small + 1; ++j)
-      if (in_range(j, !by_token) && std::llabs(left - j * small) < dim) return false;
-  }
-  return true;
 }
 #define RP_CHECK(expr)                            \
   do {                                            \
@@ -295,9 +261,9 @@ int ringattn_paged_append_rotary(ringattn_paged_plan* plan, const ringattn_paged
   const double from = (double)(uintptr_t)q, to = (double)(uintptr_t)q_out;
   if (!same && from < to + span(out_token_stride, out_head_stride) && to < from + span(q_token_stride, q_head_stride)) return RINGATTN_ERR_SHAPE;
   // ... and none of its rows is one of K's or V's, which other waves read
-  const RowsAt to_rows{q_out, out_token_stride, out_head_stride, plan->p.heads};
+  const rr::RowsAt to_rows{q_out, out_token_stride, out_head_stride, plan->p.heads};
   for (const void* other : {k_new, v_new})
-    if (!rows_apart(to_rows, RowsAt{other, token_stride, head_stride, plan->kv_heads}, tokens, plan->p.dim)) return RINGATTN_ERR_SHAPE;
+    if (rr::rows_meet(to_rows, rr::RowsAt{other, token_stride, head_stride, plan->kv_heads}, tokens, plan->p.dim) != rr::Meet::kApart) return RINGATTN_ERR_SHAPE;
   a.c = cache_of(plan, cache, tokens);
   a.q = (const char*)q;
   a.k = (const char*)k_new;

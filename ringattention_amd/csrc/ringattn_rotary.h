@@ -4,6 +4,8 @@
 // integer, and pos * f_i mod 2^64 is the part of a turn, exactly, for any position of 32 bits; its upper half, as a number in [-1/2, 1/2), is off
 // by 2^-26 (32 bits of fp32 in its place are off by pos * f_i * 2^-24: 0.06 of a radian at a million tokens).
 #pragma once
+#include <cstdlib>
+
 #include "ringattn.h"
 #include "ringattn_paged.h"
 
@@ -19,6 +21,42 @@ struct Turns {
 
 // What is wrong with a caller's rotary, or what the kernels are told of it.
 int check(const ringattn_rotary* r, int dim, Turns* out);
+
+// Rows [tokens, heads, dim] of 16-bit values: the first one, and elements between tokens and heads.
+struct RowsAt {
+  const void* at;
+  int64_t ts, hs;
+  int heads;
+};
+// Whether a row of the one tensor, none of whose own lie on each other, lies on a row of the other, as far as that can be told: they lie apart; or a
+// token's rows do, modulo the distance of tokens, which is the same for both (a fused projection's Q, K and V); or both distances are the same and two
+// rows come within dim of each other, or none do.
+enum class Meet { kApart, kMeet, kUnknown };
+inline Meet rows_meet(const RowsAt& a, const RowsAt& b, int tokens, int dim) {
+  const double fa = (double)(uintptr_t)a.at, fb = (double)(uintptr_t)b.at;
+  auto bytes = [&](const RowsAt& x) { return 2. * ((double)(tokens - 1) * (double)x.ts + (double)(x.heads - 1) * (double)x.hs + dim); };
+  if (fa + bytes(a) <= fb || fb + bytes(b) <= fa) return Meet::kApart;
+  const int64_t d = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at) / 2;  // elements from a's first row to b's
+  if (d > -dim && d < dim) return Meet::kMeet;                         // (the first rows themselves)
+  const int64_t none = INT64_MAX / 4;                                  // the distance of what there is one of
+  if (tokens > 1 && (a.ts != b.ts || a.ts == 0)) return Meet::kUnknown;
+  const int64_t ts = tokens > 1 ? a.ts : none, hs = a.heads > 1 ? a.hs : b.heads > 1 ? b.hs : none;
+  auto block = [&](const RowsAt& x) { return x.heads > 1 ? (x.heads - 1) * x.hs + dim : dim; };  // of a token
+  const int64_t from = (d % ts + ts) % ts;                                                        // where b's begins in a's distance of tokens
+  if (from >= block(a) && from + block(b) <= ts) return Meet::kApart;
+  if ((a.heads > 1 && b.heads > 1 && a.hs != b.hs) || hs == 0) return Meet::kUnknown;
+  // the rows that come nearest: so many tokens and heads of a's further on, the larger distance first
+  const bool by_token = ts > hs;
+  const int64_t large = by_token ? ts : hs, small = by_token ? hs : ts;
+  auto in_range = [&](int64_t n, bool of_tokens) { return of_tokens ? n > -tokens && n < tokens : n > -b.heads && n < a.heads; };
+  for (int64_t i = d / large - 2; i <= d / large + 2; ++i) {
+    if (!in_range(i, by_token)) continue;
+    const int64_t left = d - i * large;
+    for (int64_t j = left / small - 1; j <= left / small + 1; ++j)
+      if (in_range(j, !by_token) && std::llabs(left - j * small) < dim) return Meet::kMeet;
+  }
+  return a.heads >= b.heads ? Meet::kApart : Meet::kUnknown;  // (b's heads may reach past a's distance of tokens)
+}
 
 struct Rows {
   const char* in;

@@ -168,6 +168,24 @@ struct Extent {
   }
 };
 
+// Whether the output of one tensor of a call can be shown to lie on rows of the other one, by what lies in each batch (rows_meet).
+struct Tensor {
+  const void* at;
+  int64_t bs, hs, ts;
+  int heads;
+};
+bool lies_on(const Tensor& out, const Tensor& other, int batch, int tokens, int dim) {
+  if (batch > 1 && (out.bs != other.bs || out.bs == 0)) return false;
+  const RowsAt rows{out.at, out.ts, out.hs, out.heads};
+  const int64_t d = (int64_t)((uintptr_t)other.at - (uintptr_t)out.at) / 2, near = batch > 1 ? d / out.bs : 0;
+  for (int64_t i = near - 2; i <= near + 2; ++i) {
+    if (i <= -batch || i >= batch) continue;
+    const uintptr_t at = (uintptr_t)other.at - (uintptr_t)(batch > 1 ? i * out.bs * 2 : 0);  // as it lies to the output i batches on
+    if (rows_meet(rows, RowsAt{(const void*)at, other.ts, other.hs, other.heads}, tokens, dim) == Meet::kMeet) return true;
+  }
+  return false;
+}
+
 }  // namespace
 
 }  // namespace rotary
@@ -221,9 +239,15 @@ int ringattn_rotary_apply(const ringattn_rotary* rotary, int dim, int dtype, con
     a.heads += x.heads;
     if (a.heads > 65535) return RINGATTN_ERR_SHAPE;
   }
-  // Of two, neither's output has the other's rows.  (Which rows of two that lie between each other meet, strides of any kind would have to tell: what is in the
-  // same place is refused, the rest is the caller's.)
-  if (count == 2 && batch > 0 && tokens > 0 && (tensors[0].out == tensors[1].out || tensors[0].out == tensors[1].in || tensors[1].out == tensors[0].in)) return RINGATTN_ERR_SHAPE;
+  // Of two, neither's output has the other's rows: what is in the same place, and what equal strides show, is refused; of other strides it is the caller's to see.
+  if (count == 2 && batch > 0 && tokens > 0) {
+    if (tensors[0].out == tensors[1].out || tensors[0].out == tensors[1].in || tensors[1].out == tensors[0].in) return RINGATTN_ERR_SHAPE;
+    auto in = [](const ringattn_rows& x) { return rr::Tensor{x.in, x.in_batch_stride, x.in_head_stride, x.in_token_stride, x.heads}; };
+    auto out = [](const ringattn_rows& x) { return rr::Tensor{x.out, x.out_batch_stride, x.out_head_stride, x.out_token_stride, x.heads}; };
+    if (rr::lies_on(out(tensors[0]), out(tensors[1]), batch, tokens, dim) || rr::lies_on(out(tensors[0]), in(tensors[1]), batch, tokens, dim) ||
+        rr::lies_on(out(tensors[1]), in(tensors[0]), batch, tokens, dim))
+      return RINGATTN_ERR_SHAPE;
+  }
   a.heads0 = tensors[0].heads;
   a.tokens = tokens;
   a.positions = positions;

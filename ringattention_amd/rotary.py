@@ -120,7 +120,8 @@ class Rotary:
 
     def apply(self, q, k=None, positions=None, q_out=None, k_out=None, inverse=False, stream=None):
         """q, k: [batch, heads, tokens, dim] or both [tokens, heads, dim], of any strides that keep a row together.  `positions`: int32 [tokens] or
-        [batch, tokens], of any sign; None: a token's number.  q_out, k_out: the tensor itself for in place.  `inverse`: turned back -- of
+        [batch, tokens], of any sign; None: a token's number.  q_out, k_out: the tensor itself for in place; neither
+        has rows of the other tensor, between whose rows it may lie.  `inverse`: turned back -- of
         gradients by the outputs the gradients by the inputs.  Returns (q_out, k_out), k_out None without k.  Autograd does not see the call: what it
         returns has no history, also where q and k require gradients, and tensors that it writes count no new version."""
         if q_out is not None and (k is None or k_out is not None) and self._native:
