@@ -391,6 +391,7 @@ int ringattn_paged_weights(ringattn_paged_plan* plan, const ringattn_paged_cache
  * With first_keys the tokens of several documents that lie one behind the other in a sequence see their own document's alone (the places of
  * their documents' first tokens: in any order, of any value).  Members that are 0 or NULL change nothing.  Places count the tokens that are in the cache, after
  * an eviction those that are left.  Slopes, prefixes and first keys are for causal plans.  A weight below 2^-126, the least normal number of 32 bits, counts as 0.
+ * Slopes are finite, of either sign, up to 2^64: in 32 bits a sloped score is off by up to 2^-19 of its slope and 2^-21 of slope times distance.
  */
 typedef struct ringattn_paged_scoring {
   float softcap;

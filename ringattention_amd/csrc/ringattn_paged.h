@@ -69,7 +69,8 @@ struct Scoring {
 // a score.  An infinite score is the cap.
 // In steps, so that none waits for the one before: each takes one score as far as the next stage (left to itself the compiler has each score's
 // instructions one behind the other).  `at`: slope times dist.  Of a key that lies in front of its row a slope takes slope |dist| = -slope dist, so that
-// what is added is at + slope (0, 1, 2, 3, 8, ...): no absolute values; keys behind their rows, which prefixes show, are put right after (turn_slopes).
+// what is added is at + slope (0, 1, 2, 3, 8, ...): no absolute values; keys behind their rows, which prefixes show, are put right after (turn_slopes).  The
+// rounding of `at` is 2^-24 of slope times up to 27 more than the distance, also of the row's own key, whose sum is 0: 2^-19 of a slope.
 template <int SC> constexpr int kShapeSteps = (SC & kCapped) ? ((SC & kSloped) ? 25 : 22) : (SC & kSloped) ? 16 : 0;
 template <int SC> static __device__ __forceinline__ void shape_step(f32x16& s, int i, const Scoring& x, float unit, float slope, float at) {
   constexpr int kSlopeAt = (SC & kCapped) ? 9 : 0;

@@ -120,3 +120,21 @@ def test_masks_that_hide_nothing_are_the_plain_definition():
     want, want_lse, tol, tol_lse = paged_reference.attend(plain)
     compare(out, want, 2 * tol, "out")
     compare(lse, want_lse, 2 * tol_lse, "lse")
+
+
+class Steep(ref.Case):
+    """With what the product of a slope and a place is off by besides: the place is that of a lane's first key of a tile, up to 27 further from the row than
+    the key itself, and 2^-24 of the product is rounded away, also where the key is the row's own."""
+
+    def scores(self, b, h, k, there):
+        ok, s, off = super().scores(b, h, k, there)
+        return ok, s, torch.where(ok, off + 28 * abs(self.slopes[h]) * 2.0 ** -24, 0.0)
+
+
+@pytest.mark.parametrize("prefix,cap", [(False, 0.0), (True, 0.0), (False, 6.0)])
+@pytest.mark.parametrize("lens,news", [([50, 301, 64], [1, 1, 1]), ([200, 40], [17, 40]), ([600], [420])])
+def test_slopes_of_thousands(lens, news, prefix, cap):
+    """One key takes a row: its own, or of negative slopes the farthest."""
+    c = Steep(lens=lens, news=news, heads=4, kv_heads=2, dim=64, dtype="fp16", page=32, slopes=[1000.0, -300.0, 37.5, 4096.0], cap=cap,
+              prefix=[45, 30, 64][:len(lens)] if prefix else None, seed=21)
+    check_all(c)
