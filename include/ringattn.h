@@ -367,6 +367,8 @@ int ringattn_paged_append(ringattn_paged_plan* plan, const ringattn_paged_cache*
  * Attention of the new tokens over the cache (which holds their own K and V rows already).  New token i of n of a sequence of L tokens
  * is its token p = L - n + i and sees token j iff 0 <= j <= p (causal; else j < L), and, with a window, j > p - window or
  * j < sinks.  A query that sees nothing gets O = 0 and LSE = -inf.
+ * Weights are rounded to the storage type for the product with V: an infinity in a V row that the query sees is one of the output, or no number where
+ * the row's weight is nothing in that type (below 2^-126, in fp16 2^-25, of the largest).
  *   q   : [tokens, heads, dim] by strides (elements, multiples of 8)
  *   out : the same shape, by strides of its own (token by token or head by head, with or without room between); fp32 with
  *         RINGATTN_FLAG_PAGED_PARTIALS (strides multiples of 4)
